@@ -123,6 +123,11 @@ SIGNATURES = {
     "mi355_rope_bf16_dev": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i]),
     "mi355_qknorm_rope_fwd_bf16_dev": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _f]),
     "mi355_qknorm_rope_bwd_bf16_dev": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _f, _i]),
+    "mi355_attn_plan_dev": (_i, [_p, _p, _i, _i, _i]),
+    "mi355_attn_fwd_dev": (_i, [_p] * 6 + [_i] * 5 + [_f]),
+    "mi355_attn_fwd_bf16_dev": (_i, [_p] * 6 + [_i] * 5 + [_f]),
+    "mi355_attn_bwd_dev": (_i, [_p] * 10 + [_i] * 5 + [_f]),
+    "mi355_attn_bwd_bf16_dev": (_i, [_p] * 10 + [_i] * 5 + [_f]),
     "mi355_workspace_size": (_z, []),
     "mi355_graph_begin": (_i, []),
     "mi355_graph_end": (_p, []),

@@ -1,0 +1,153 @@
+// attn_bwd.hip — causal attention, backward: dq and delta, then the entry points (attention.h has the mathematics, attn_dkv.hip dk and dv).
+#include "attention.h"
+
+namespace {
+
+// ---- backward: dq and delta -----------------------------------------------------------------------------------------------------
+
+template <typename T, int HDB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                             const int *__restrict__ bounds, int S, int heads, int kv_heads, int hd,
+                                                             float scale, const T *__restrict__ o, const T *__restrict__ d_o,
+                                                             const float *__restrict__ lse, T *__restrict__ dq, float *__restrict__ delta,
+                                                             int batch, int blocks) {
+    typedef Mma<T> M;
+    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP, THREADS = WAVES * 64;
+    __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
+    __shared__ int firsts[WAVES];
+    const Place at = place(blocks, heads, batch, true);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+    const int q0 = at.block * QT, wq = q0 + wave * 32, mine = wq + (lane & 31);
+    int start = S;
+    if (mine < S) start = bounds ? max(bounds[(size_t)at.b * 2 * S + mine], 0) : 0;
+    const bool active = mine < S && start <= mine;
+    int wfrom = 0, wfull = 0;
+    if (bounds) {
+        wfrom = uniform(wave_min_int(active ? start : S));
+        wfull = uniform(wave_max_int(active ? start : 0));
+    } else if (wq >= S) wfrom = S;
+    int from = wfrom;
+    if constexpr (WAVES > 1) {
+        if (lane == 0) firsts[wave] = wfrom;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) from = min(from, uniform(firsts[w]));
+    }
+    if (from >= S) return;
+    const int to = min(q0 + QT, S);
+    const int kvh = at.h / (heads / kv_heads);
+    const T *kb = k + ((size_t)at.b * kv_heads + kvh) * hd * S, *vb = v + ((size_t)at.b * kv_heads + kvh) * hd * S;
+    const size_t slab = ((size_t)at.b * heads + at.h) * hd * S, row = ((size_t)at.b * heads + at.h) * S;
+
+    typename M::Frag qf[STEPS], gf[STEPS];
+    own_columns<T, HDB, WAVES, STEPS>(qf, lds, q + slab, S, hd, q0, S);
+    own_columns<T, HDB, WAVES, STEPS>(gf, lds, d_o + slab, S, hd, q0, S);
+    // delta: two lanes share a query, each takes every other channel
+    float dlt = 0.f, lse2 = 0.f;
+    if (active) {
+        for (int d = h; d < hd; d += 2)
+            dlt += M::widen(o[slab + (size_t)d * S + mine]) * M::widen(d_o[slab + (size_t)d * S + mine]);
+        lse2 = lse[row + mine] * LOG2E;
+    }
+    dlt += lane_xor<32>(dlt);
+    if (active && h == 0) delta[row + mine] = dlt;
+    const float scale2 = scale * LOG2E;
+
+    v16f acc[HDB];
+    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
+    auto walk = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+        for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
+        PanelLoad<T, HDB * 32, THREADS> lk, lv;
+        lk.load(kb, S, hd, t0 * M::COLS, from, to);
+        lv.load(vb, S, hd, t0 * M::COLS, from, to);
+        __syncthreads();
+        lk.store(lds);
+        lv.store(lds + BYTES);
+        __syncthreads();
+        for (int t = t0; t <= t1; t++) {
+            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES;
+            if (t < t1) {
+                lk.load(kb, S, hd, (t + 1) * M::COLS, from, to);
+                lv.load(vb, S, hd, (t + 1) * M::COLS, from, to);
+            }
+            const int c0 = t * M::COLS;
+            if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+                const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
+                unsigned long long odd = 0;
+                if constexpr (CAREFUL) odd = masked ? odd_columns<T, HDB * 32>(kp) : 0;
+#pragma unroll
+                for (int u = 0; u < M::SUBS; u++) {
+                    v16f s = v16_zero(), g = v16_zero();
+#pragma unroll
+                    for (int i = 0; i < STEPS; i++) s = M::mul(M::columns(kp, u, i), qf[i], s);
+#pragma unroll
+                    for (int i = 0; i < STEPS; i++) g = M::mul(M::columns(vp, u, i), gf[i], g);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -lse2));
+                        s[r] = p * (g[r] - dlt);
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int key = c0 + u * 32 + acc_row(r) + 4 * h;
+                            s[r] = key <= mine && key >= start ? s[r] : 0.f;
+                        }
+                    }
+                    const typename M::Packed p = M::pack(s);
+#pragma unroll
+                    for (int d = 0; d < HDB; d++) {
+                        if (CAREFUL && odd) acc[d] = M::template rows<true>(kp, d, u, p, acc[d]);
+                        else acc[d] = M::template rows<false>(kp, d, u, p, acc[d]);
+                    }
+                    if (CAREFUL && odd) add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                }
+            }
+            if (t < t1) {
+                char *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
+                lk.store(next);
+                lv.store(next + BYTES);
+            }
+            __syncthreads();
+        }
+    };
+    walk(std::false_type());
+    if (__syncthreads_or(active && has_nan<HDB>(acc))) walk(std::true_type());
+    if (active) store_columns<T, HDB>(dq + slab + mine, S, hd, acc, scale);
+}
+
+template <typename T>
+int attn_bwd(const char *who, T *dq, T *dk, T *dv, const T *d_o, const T *q, const T *k, const T *v, const T *o, const float *lse,
+             const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale) {
+    if (!mi355_ready(who)) return -1;
+    if (!dq || !dk || !dv || !d_o || !q || !k || !v || !o || !lse) return mi355_fail("%s: NULL pointer", who);
+    if (!shape_ok(who, heads, kv_heads, hd, S, batch, scale)) return -1;
+    const size_t n = (size_t)heads * batch;
+    float *delta = (float *)mi355_ws(n * S * sizeof(float));
+    if (!delta) return -1;
+    int rc = dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
+        constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
+        const int blocks = (int)ceil_div(S, 32 * W);
+        attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, heads, kv_heads, hd, scale, o, d_o,
+                                                                                       lse, dq, delta, batch, blocks);
+        LAUNCH_OK(who);
+        return 0;
+    });
+    if (rc) return rc;
+    return mi355_attn_dkv(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, batch, scale);
+}
+
+}  // namespace
+
+MI355_API int mi355_attn_bwd_dev(float *dq, float *dk, float *dv, const float *d_o, const float *q, const float *k, const float *v,
+                                 const float *o, const float *lse, const int32_t *bounds, int heads, int kv_heads, int hd, int S,
+                                 int batch, float scale) {
+    return attn_bwd<float>("attn_bwd", dq, dk, dv, d_o, q, k, v, o, lse, bounds, heads, kv_heads, hd, S, batch, scale);
+}
+MI355_API int mi355_attn_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, uint16_t *dv, const uint16_t *d_o, const uint16_t *q, const uint16_t *k,
+                                      const uint16_t *v, const uint16_t *o, const float *lse, const int32_t *bounds, int heads,
+                                      int kv_heads, int hd, int S, int batch, float scale) {
+    return attn_bwd<bf16_t>("attn_bwd_bf16", dq, dk, dv, d_o, q, k, v, o, lse, bounds, heads, kv_heads, hd, S, batch, scale);
+}

@@ -1,0 +1,191 @@
+// attn_fwd.hip — causal attention, forward, and the plan of packed rows (attention.h has the mathematics).
+#include "attention.h"
+
+namespace {
+
+// ---- forward --------------------------------------------------------------------------------------------------------------------
+
+template <typename T, int HDB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                              const int *__restrict__ bounds, int S, int heads, int kv_heads, int hd,
+                                                              float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
+    typedef Mma<T> M;
+    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP, THREADS = WAVES * 64;
+    __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
+    __shared__ int firsts[WAVES];
+    const Place at = place(blocks, heads, batch, true);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+    const int q0 = at.block * QT, wq = q0 + wave * 32, mine = wq + (lane & 31);
+    int start = S;
+    if (mine < S) start = bounds ? max(bounds[(size_t)at.b * 2 * S + mine], 0) : 0;
+    const bool active = mine < S && start <= mine;
+    int wfrom = 0, wfull = 0;               // keys below wfrom meet none of the wave's queries, from wfull on all that are not behind
+    if (bounds) {
+        wfrom = uniform(wave_min_int(active ? start : S));
+        wfull = uniform(wave_max_int(active ? start : 0));
+    } else if (wq >= S) wfrom = S;
+    int from = wfrom;
+    if constexpr (WAVES > 1) {
+        if (lane == 0) firsts[wave] = wfrom;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) from = min(from, uniform(firsts[w]));
+    }
+    if (from >= S) return;
+    const int to = min(q0 + QT, S);
+    const int kvh = at.h / (heads / kv_heads);
+    const T *kb = k + ((size_t)at.b * kv_heads + kvh) * hd * S, *vb = v + ((size_t)at.b * kv_heads + kvh) * hd * S;
+    const size_t slab = ((size_t)at.b * heads + at.h) * hd * S;
+
+    typename M::Frag qf[STEPS];
+    own_columns<T, HDB, WAVES, STEPS>(qf, lds, q + slab, S, hd, q0, S);
+
+    v16f acc[HDB];
+    float m, l;
+    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
+    auto walk = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
+        PanelLoad<T, HDB * 32, THREADS> lk, lv;
+        lk.load(kb, S, hd, t0 * M::COLS, from, to);
+        lv.load(vb, S, hd, t0 * M::COLS, from, to);
+        __syncthreads();                    // nobody reads the panels of an earlier walk any more
+        lk.store(lds);
+        lv.store(lds + BYTES);
+        __syncthreads();
+        for (int t = t0; t <= t1; t++) {
+            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES;
+            if (t < t1) {
+                lk.load(kb, S, hd, (t + 1) * M::COLS, from, to);
+                lv.load(vb, S, hd, (t + 1) * M::COLS, from, to);
+            }
+            const int c0 = t * M::COLS;
+            if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+                const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
+                unsigned long long odd = 0;
+                if constexpr (CAREFUL) odd = masked ? odd_columns<T, HDB * 32>(vp) : 0;
+                v16f s[M::SUBS];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < M::SUBS; u++) {
+                    s[u] = v16_zero();
+#pragma unroll
+                    for (int i = 0; i < STEPS; i++) s[u] = M::mul(M::columns(kp, u, i), qf[i], s[u]);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int u = 0; u < M::SUBS; u++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int key = c0 + u * 32 + acc_row(r) + 4 * h;
+                            s[u][r] = key <= mine && key >= start ? s[u][r] : -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < M::SUBS; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
+                mx = fmaxf(mx, lane_xor<32>(mx)) * scale2;
+                if (__any(mx > m)) {        // the running maximum moves: what is there is brought to the new one
+                    const float to_m = fmaxf(m, mx), f = to_m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to_m);
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < HDB; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[d][r] *= f;
+                    m = to_m;
+                }
+                const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int u = 0; u < M::SUBS; u++) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, -base));
+                        l += s[u][r];
+                    }
+                    const typename M::Packed p = M::pack(s[u]);
+#pragma unroll
+                    for (int d = 0; d < HDB; d++) {
+                        if (CAREFUL && odd) acc[d] = M::template rows<true>(vp, d, u, p, acc[d]);
+                        else acc[d] = M::template rows<false>(vp, d, u, p, acc[d]);
+                    }
+                    if (CAREFUL && odd)
+                        add_odd<T, HDB>(acc, vp, u, s[u], odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                }
+            }
+            if (t < t1) {
+                char *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
+                lk.store(next);
+                lv.store(next + BYTES);
+            }
+            __syncthreads();
+        }
+        l += lane_xor<32>(l);
+    };
+    walk(std::false_type());
+    // An infinity or a NaN among the values of keys that the mask hides makes 0 * inf of their weights: such rows are computed again,
+    // with those values taken out of the product and added for the pairs that count.
+    if (__syncthreads_or(active && has_nan<HDB>(acc))) walk(std::true_type());
+    if (!active) return;
+    store_columns<T, HDB>(o + slab + mine, S, hd, acc, 1.f / l);
+    if (lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---- the plan of packed rows ----------------------------------------------------------------------------------------------------
+
+// One thread to a position: the last offset at or below it, by bisection.
+__global__ void attn_plan_kernel(int *__restrict__ bounds, const int *__restrict__ cu, int n_seqs, int S) {
+    const int s = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    if (s >= S) return;
+    const int *c = cu + (size_t)b * (n_seqs + 1);
+    int lo = 0, hi = n_seqs + 1;            // offsets below lo are <= s, from hi on > s
+    while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (c[mid] <= s) lo = mid + 1;
+        else hi = mid;
+    }
+    const bool in = lo > 0 && lo <= n_seqs;
+    bounds[(size_t)b * 2 * S + s] = in ? max(c[lo - 1], 0) : S;
+    bounds[((size_t)b * 2 + 1) * S + s] = in ? min(c[lo], S) : 0;
+}
+
+template <typename T>
+int attn_fwd(const char *who, T *o, float *lse, const T *q, const T *k, const T *v, const int32_t *bounds, int heads, int kv_heads, int hd,
+             int S, int batch, float scale) {
+    if (!mi355_ready(who)) return -1;
+    if (!o || !q || !k || !v) return mi355_fail("%s: NULL pointer", who);
+    if (!shape_ok(who, heads, kv_heads, hd, S, batch, scale)) return -1;
+    const size_t n = (size_t)heads * batch;
+    return dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
+        constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
+        const int blocks = (int)ceil_div(S, 32 * W);
+        attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, heads, kv_heads, hd, scale * LOG2E,
+                                                                                        o, lse, batch, blocks);
+        LAUNCH_OK(who);
+        return 0;
+    });
+}
+
+}  // namespace
+
+MI355_API int mi355_attn_plan_dev(int32_t *bounds, const int32_t *cu, int n_seqs, int S, int batch) {
+    if (!mi355_ready("attn_plan")) return -1;
+    if (!bounds || !cu) return mi355_fail("attn_plan: NULL pointer");
+    if (n_seqs <= 0 || S <= 0 || batch <= 0 || S > 1 << 30 || n_seqs > 1 << 30 || batch > 65535)
+        return mi355_fail("attn_plan: bad shape n_seqs=%d S=%d batch=%d", n_seqs, S, batch);
+    attn_plan_kernel<<<dim3((unsigned)ceil_div(S, 256), (unsigned)batch), 256, 0, g_ctx.stream>>>(bounds, cu, n_seqs, S);
+    LAUNCH_OK("attn_plan");
+    return 0;
+}
+
+MI355_API int mi355_attn_fwd_dev(float *o, float *lse, const float *q, const float *k, const float *v, const int32_t *bounds, int heads,
+                                 int kv_heads, int hd, int S, int batch, float scale) {
+    return attn_fwd<float>("attn_fwd", o, lse, q, k, v, bounds, heads, kv_heads, hd, S, batch, scale);
+}
+MI355_API int mi355_attn_fwd_bf16_dev(uint16_t *o, float *lse, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                                      const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale) {
+    return attn_fwd<bf16_t>("attn_fwd_bf16", o, lse, q, k, v, bounds, heads, kv_heads, hd, S, batch, scale);
+}

@@ -1,0 +1,177 @@
+// mma.h — operand tiles of the matrix instructions, for the kernels that multiply channel-first tensors.
+//
+// An operand lies in LDS as a panel: rows of 128 bytes (64 bfloat16 or 32 fp32 values), the positions of a tensor [channel][position]
+// along the row, one channel to a row.  A panel is read in two ways:
+//   columns: a lane takes one position and the values of several channels (products over the channels: scores from Q and K).  In
+//            bfloat16 that is gfx950's transposing LDS read, which hands 4 rows x 16 columns around among 16 lanes; fp32 needs one
+//            value per lane and instruction.
+//   rows:    a lane takes one channel and several positions (products over the positions: P V, dS K, and the gradients).
+// The result of a 32 x 32 product, C[i][j], has column j = lane % 32 in every lane and rows i = 8 * (r / 4) + 4 * (lane / 32) + r % 4
+// in its 16 registers r.  A product over those rows takes the registers as they are for its second operand when the first one is
+// read in the same order of positions: no score and no gradient of one ever passes through LDS.
+//
+// Chunk c (16 bytes) of row r is kept in place c ^ panel_swz(r).  Of the 64 banks (256 bytes: two rows) a transposing read then
+// touches each at most twice with 512 bytes, a row read of 8 bytes per lane all of them with 16 rows, one of 16 bytes no bank twice
+// with 8 rows.
+#pragma once
+#include "tile.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+constexpr int PANEL_ROW = 128;      // bytes
+
+__device__ __forceinline__ int panel_swz(int row) { return (row >> 1 & 1) << 2 | (row >> 2 & 1) | (row >> 3 & 1) << 1; }
+__device__ __forceinline__ int panel_at(int row, int chunk) { return row * PANEL_ROW + ((chunk ^ panel_swz(row)) << 4); }
+
+// row of register r of a 32 x 32 product, less the 4 that lanes 32..63 add
+__device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+__device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ v16f v16_zero() {
+    v16f z;
+#pragma unroll
+    for (int r = 0; r < 16; r++) z[r] = 0.f;
+    return z;
+}
+
+template <typename T> struct Mma;
+
+template <> struct Mma<bf16_t> {
+    static constexpr int COLS = 64, SUBS = 2, EPC = 8;      // columns of a panel, groups of 32 of them, values per 16 bytes
+    static constexpr int STEP = 16;                         // rows of a panel that one product over the channels takes
+    typedef bf16x8 Frag;
+    typedef v4u_any Any16;                                  // 16 bytes of global memory at any value
+    // Values of rows step*16 + 8*(lane/32) .. +7 at column sub*32 + lane%32.
+    static __device__ __forceinline__ Frag columns(const char *panel, int sub, int step) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4 & 1, h = lane >> 5;
+        const int row = 8 * h + (i >> 2), chunk = sub * 4 + 2 * g + (i >> 1 & 1);
+        const char *at = panel + step * (16 * PANEL_ROW) + ((i & 1) << 3);
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + panel_at(row, chunk)));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + panel_at(row + 4, chunk)));
+        const v8s v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return __builtin_bit_cast(Frag, v);
+    }
+    static __device__ __forceinline__ v16f mul(Frag a, Frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+    // A product's registers as the second operand of a product over its rows.
+    struct Packed { Frag f[2]; };
+    static __device__ __forceinline__ Packed pack(const v16f &p) {
+        Packed out;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const v4u w = {f2_to_bf2(p[8 * j], p[8 * j + 1]), f2_to_bf2(p[8 * j + 2], p[8 * j + 3]), f2_to_bf2(p[8 * j + 4], p[8 * j + 5]),
+                           f2_to_bf2(p[8 * j + 6], p[8 * j + 7])};
+            out.f[j] = __builtin_bit_cast(Frag, w);
+        }
+        return out;
+    }
+    // acc[row block][column] += sum over the panel's 32 columns `sub` of panel[row][.] * p[.][column]; FINITE: infinities and NaNs
+    // of the panel count as zero.
+    template <bool FINITE>
+    static __device__ __forceinline__ v16f rows(const char *panel, int block, int sub, const Packed &p, v16f acc) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+        const char *at = panel + block * (32 * PANEL_ROW) + (h << 3);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const v4s lo = *reinterpret_cast<const v4s *>(at + panel_at(row, sub * 4 + 2 * j));
+            const v4s hi = *reinterpret_cast<const v4s *>(at + panel_at(row, sub * 4 + 2 * j + 1));
+            v8s v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if constexpr (FINITE) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
+            }
+            acc = mul(__builtin_bit_cast(Frag, v), p.f[j], acc);
+        }
+        return acc;
+    }
+    static __device__ __forceinline__ float value(const char *panel, int row, int col) {
+        return bf_to_f(*reinterpret_cast<const bf16_t *>(panel + panel_at(row, col >> 3) + ((col & 7) << 1)));
+    }
+    static __device__ __forceinline__ float widen(bf16_t v) { return bf_to_f(v); }
+    static __device__ __forceinline__ bf16_t narrow(float v) { return (bf16_t)f_to_bf(v); }
+};
+
+template <> struct Mma<float> {
+    static constexpr int COLS = 32, SUBS = 1, EPC = 4;
+    static constexpr int STEP = 2;
+    typedef float Frag;
+    typedef unsigned Any16 __attribute__((ext_vector_type(4), aligned(4)));
+    static __device__ __forceinline__ Frag columns(const char *panel, int, int step) {
+        const int lane = threadIdx.x & 63, col = lane & 31;
+        return *reinterpret_cast<const float *>(panel + panel_at(2 * step + (lane >> 5), col >> 2) + ((col & 3) << 2));
+    }
+    static __device__ __forceinline__ v16f mul(Frag a, Frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+    typedef v16f Packed;
+    static __device__ __forceinline__ Packed pack(const v16f &p) { return p; }
+    template <bool FINITE>
+    static __device__ __forceinline__ v16f rows(const char *panel, int block, int, const Packed &p, v16f acc) {
+        const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+        const char *at = panel + block * (32 * PANEL_ROW);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const v4f v = *reinterpret_cast<const v4f *>(at + panel_at(row, 2 * j + h));
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc = mul(FINITE && !is_finite(v[e]) ? 0.f : v[e], p[4 * j + e], acc);
+        }
+        return acc;
+    }
+    static __device__ __forceinline__ float value(const char *panel, int row, int col) {
+        return *reinterpret_cast<const float *>(panel + panel_at(row, col >> 2) + ((col & 3) << 2));
+    }
+    static __device__ __forceinline__ float widen(float v) { return v; }
+    static __device__ __forceinline__ float narrow(float v) { return v; }
+};
+
+// A panel of ROWS rows on its way from memory to LDS: the chunks of one thread.  src: row 0, column 0 of a tensor with `pitch` values
+// between rows; columns [lo, hi) and rows below `rows` are read, the others become zero.
+template <typename T, int ROWS, int THREADS>
+struct PanelLoad {
+    static constexpr int N = ROWS * 8 / THREADS;
+    static_assert(N * THREADS == ROWS * 8, "whole chunks per thread");
+    v4u w[N];
+    __device__ __forceinline__ void load(const T *src, size_t pitch, int rows, int col0, int lo, int hi) {
+        typedef Mma<T> M;
+        const bool whole = rows >= ROWS && col0 >= lo && col0 + M::COLS <= hi;       // the same for every thread
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int t = threadIdx.x + i * THREADS;
+                const T *p = src + (size_t)(t >> 3) * pitch + col0 + (t & 7) * M::EPC;
+                w[i] = *reinterpret_cast<const typename M::Any16 *>(p);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int t = threadIdx.x + i * THREADS, row = t >> 3, col = col0 + (t & 7) * M::EPC;
+                v4u v = {0u, 0u, 0u, 0u};
+                if (row < rows) {
+                    const T *p = src + (size_t)row * pitch + col;
+                    if (col >= lo && col + M::EPC <= hi) v = *reinterpret_cast<const typename M::Any16 *>(p);
+                    else if (col < hi && col + M::EPC > lo) {
+                        unsigned e[M::EPC];
+#pragma unroll
+                        for (int j = 0; j < M::EPC; j++) e[j] = col + j >= lo && col + j < hi ? bits(p[j]) : 0u;
+                        if constexpr (M::EPC == 4) v = v4u{e[0], e[1], e[2], e[3]};
+                        else v = v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+                    }
+                }
+                w[i] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *panel) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int t = threadIdx.x + i * THREADS;
+            *reinterpret_cast<v4u *>(panel + panel_at(t >> 3, t & 7)) = w[i];
+        }
+    }
+
+private:
+    static __device__ __forceinline__ unsigned bits(bf16_t v) { return v; }
+    static __device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
+};

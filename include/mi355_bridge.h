@@ -145,6 +145,36 @@ int mi355_qknorm_rope_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, float *dwq, float
                                    const float *wk, int heads, int kv_heads, int hd, int S, int batch,
                                    const float *cos_dev, const float *sin_dev, float eps, int variant);
 
+/* Causal attention over whole prompts.  Not among the reference's CPU ops (its attention is a part of the MIL kernels,
+ * training/training_dynamic/mil_dynamic.h:131-168 on); it takes q and k as mi355_qknorm_rope_fwd_dev / mi355_rope_dev leave them.
+ *   p[s][t] = exp(scale q_s.k_t - lse_s) for first_s <= t <= s, o_s = sum_t p[s][t] v_t, lse_s = log sum_t exp(scale q_s.k_t)
+ * q, o: [batch][heads*hd][S]; k, v: [batch][kv_heads*hd][S], heads a multiple of kv_heads (query heads h*heads/kv_heads .. share KV
+ * head h); lse: [batch][heads][S] fp32, may be NULL when no gradient follows.  hd <= 128, scale > 0.
+ * bounds: NULL when every row is one sequence of S positions, else the plan of rows into which sequences of different lengths are
+ * packed, from mi355_attn_plan_dev, kept for all layers and both directions: bounds[b][0][s] is the first position of the sequence that
+ * s belongs to (S if it is in none), bounds[b][1][s] one past its last (0).  Columns of no sequence are neither read for another
+ * position's result nor written, in either direction.  What a sequence's results are does not depend on what the others hold, nor a
+ * position's on what later ones hold, infinities and NaNs included (a row whose own values hold one is NaN, as the formula gives).
+ * Sums and the softmax are fp32; with bfloat16 storage p and the score gradients are rounded to bfloat16 where they are multiplied again.
+ * Outputs must not overlap inputs.  Deterministic: no atomics. */
+int mi355_attn_fwd_dev(float *o, float *lse, const float *q, const float *k, const float *v, const int32_t *bounds, int heads,
+                       int kv_heads, int hd, int S, int batch, float scale);
+int mi355_attn_fwd_bf16_dev(uint16_t *o, float *lse, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                            const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale);
+/* Its gradients: dq, dk and dv are assigned (dk and dv summed over the query heads that share them).  o and lse: what the forward call
+ * gave.  delta_s = do_s.o_s, ds[s][t] = p[s][t] (do_s.v_t - delta_s); dv_t = sum_s p[s][t] do_s, dq_s = scale sum_t ds[s][t] k_t,
+ * dk_t = scale sum_s ds[s][t] q_s.  The workspace holds delta (4 * batch * heads * S bytes). */
+int mi355_attn_bwd_dev(float *dq, float *dk, float *dv, const float *d_o, const float *q, const float *k, const float *v,
+                       const float *o, const float *lse, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch,
+                       float scale);
+int mi355_attn_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, uint16_t *dv, const uint16_t *d_o, const uint16_t *q, const uint16_t *k,
+                            const uint16_t *v, const uint16_t *o, const float *lse, const int32_t *bounds, int heads, int kv_heads,
+                            int hd, int S, int batch, float scale);
+/* The plan of packed rows: cu[batch][n_seqs + 1], ascending offsets (device memory): sequence i of row b is cu[b][i] .. cu[b][i+1]-1,
+ * of any length, zero included; positions before cu[b][0] and from cu[b][n_seqs] on are in no sequence (a batch padded to S is
+ * {0, length}, n_seqs = 1).  bounds: [batch][2][S]. */
+int mi355_attn_plan_dev(int32_t *bounds, const int32_t *cu, int n_seqs, int S, int batch);
+
 /* Graphs: record a launch-bound sequence of device-resident ops once, replay it as one submission.  No
  * counterpart in the reference (its ops are synchronous CPU calls).  Between begin and end the *_dev ops are
  * recorded instead of run; calls that allocate, wait or touch the host (buf_alloc/free/read/write, sync,
