@@ -123,6 +123,9 @@ SIGNATURES = {
     "mi355_rope_bf16_dev": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i]),
     "mi355_qknorm_rope_fwd_bf16_dev": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _f]),
     "mi355_qknorm_rope_bwd_bf16_dev": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _f, _i]),
+    "mi355_linear_fwd_bf16_dev": (_i, [_p] * 5 + [_i, _p, _f] + [_i] * 4),
+    "mi355_linear_bwd_bf16_dev": (_i, [_p] * 6 + [_f, _i, _p, _i] + [_i] * 4),
+    "mi355_act_bwd_bf16_dev": (_i, [_p] * 3 + [_f, _i, _z]),
     "mi355_attn_plan_dev": (_i, [_p, _p, _i, _i, _i]),
     "mi355_attn_fwd_dev": (_i, [_p] * 6 + [_i] * 5 + [_f]),
     "mi355_attn_fwd_bf16_dev": (_i, [_p] * 6 + [_i] * 5 + [_f]),

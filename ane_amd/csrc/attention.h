@@ -148,8 +148,9 @@ bool shape_ok(const char *who, int heads, int kv_heads, int hd, int S, int batch
         mi355_fail("%s: scale must be positive and finite", who);
         return false;
     }
-    if (S > 1 << 30 || (double)S * heads * batch > 2e9) {
-        mi355_fail("%s: heads * batch * S = %.0f rows (at most 2e9), S at most 2^30", who, (double)S * heads * batch);
+    // what a launch can number (2^32 threads, two waves to 64 positions), and 32-bit positions
+    if (S > 1 << 30 || (double)heads * batch * ceil_div(S, 64) > (double)((1 << 25) - 1)) {
+        mi355_fail("%s: heads * batch * ceil(S / 64) = %.0f (at most 2^25 - 1), S = %d (at most 2^30)", who, (double)heads * batch * ceil_div(S, 64), S);
         return false;
     }
     return true;

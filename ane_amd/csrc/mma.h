@@ -56,6 +56,11 @@ template <> struct Mma<bf16_t> {
         return __builtin_bit_cast(Frag, v);
     }
     static __device__ __forceinline__ v16f mul(Frag a, Frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    // For products over the positions whose result rows are the panel's: columns step*16 + 8*(lane/32) .. +7 of row block*32 + lane%32.
+    static __device__ __forceinline__ Frag along(const char *panel, int block, int step) {
+        const int lane = threadIdx.x & 63;
+        return *reinterpret_cast<const Frag *>(panel + block * (32 * PANEL_ROW) + panel_at(lane & 31, step * 2 + (lane >> 5)));
+    }
 
     // A product's registers as the second operand of a product over its rows.
     struct Packed { Frag f[2]; };

@@ -145,6 +145,27 @@ int mi355_qknorm_rope_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, float *dwq, float
                                    const float *wk, int heads, int kv_heads, int hd, int S, int batch,
                                    const float *cos_dev, const float *sin_dev, float eps, int variant);
 
+/* The products of a layer on bfloat16 storage, with what stands around them in one pass.  No counterpart among the reference's CPU ops
+ * (its projections run in MIL kernels; the fp32 product is mi355_sgemm_dev).  x [batch][K][S], w [M][K], y [batch][M][S].
+ *   forward: z = w x + bias[m] (bias fp32, NULL = none), y = res + alpha * act(z) (res [batch][M][S], NULL = 0); pre, if not NULL,
+ *            receives z [batch][M][S].  act is applied to the sum itself, not to its rounding.  y may be res.
+ *   act: MI355_ACT_NONE, MI355_ACT_RELU, MI355_ACT_SILU, MI355_ACT_GELU (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))))
+ * Sums are fp32; y, pre and dx are rounded once.  Deterministic (slices of a long sum are added in a fixed order, through the
+ * workspace).  Outputs must not overlap inputs otherwise. */
+enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_SILU = 2, MI355_ACT_GELU = 3 };
+int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16_t *x, const uint16_t *w, const float *bias, int act,
+                              const uint16_t *res, float alpha, int M, int K, int S, int batch);
+/* Gradients of y = res + alpha * (w x + bias) from dy [batch][M][S]; dx, dw and dbias may each be NULL (not all three), x is needed
+ * for dw only, w for dx only:
+ *   dx = alpha * (w^T dy) * act'(x_pre): with act = MI355_ACT_NONE the gradient of x, else, where x = act(x_pre), that of x_pre
+ *        [batch][K][S] (the activation of the layer below);
+ *   dw[M][K] = (accumulate ? dw : 0) + alpha * sum of dy x^T, dbias[M] = (accumulate ? dbias : 0) + alpha * sum of dy, both fp32.
+ * The gradient of res is dy.  Where the layer has an activation of its own, dy is first taken through it: mi355_act_bwd_bf16_dev,
+ * dpre = alpha * dy * act'(pre) for n values (dpre may be dy), or by the call of the layer above. */
+int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, const uint16_t *dy, const uint16_t *x, const uint16_t *w,
+                              float alpha, int act, const uint16_t *x_pre, int accumulate, int M, int K, int S, int batch);
+int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *pre, float alpha, int act, size_t n);
+
 /* Causal attention over whole prompts.  Not among the reference's CPU ops (its attention is a part of the MIL kernels,
  * training/training_dynamic/mil_dynamic.h:131-168 on); it takes q and k as mi355_qknorm_rope_fwd_dev / mi355_rope_dev leave them.
  *   p[s][t] = exp(scale q_s.k_t - lse_s) for first_s <= t <= s, o_s = sum_t p[s][t] v_t, lse_s = log sum_t exp(scale q_s.k_t)
