@@ -42,24 +42,34 @@ constexpr float GELU_C = 0.797884583473205566406f;      // sqrt(2 / pi)
 
 // GELU in its tanh form, through tanh(y) = 2 sigmoid(2y) - 1.  Far below zero the exponential is infinite and the sigmoid zero, as it should.
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
-__device__ __forceinline__ float act_value(int act, float x) {
-    if (act == ACT_RELU) return x < 0.f ? 0.f : x;      // (a NaN stays one)
-    if (act == ACT_SILU) return x * sigmoid(x);
-    if (act == ACT_GELU) return x * sigmoid(2.f * GELU_C * (x + 0.044715f * x * x * x));
+template <int ACT>
+__device__ __forceinline__ float act_value(float x) {
+    if (ACT == ACT_RELU) return x < 0.f ? 0.f : x;      // (a NaN stays one)
+    if (ACT == ACT_SILU) return x * sigmoid(x);
+    if (ACT == ACT_GELU) return x * sigmoid(2.f * GELU_C * (x + 0.044715f * x * x * x));
     return x;
 }
-__device__ __forceinline__ float act_slope(int act, float x) {
-    if (act == ACT_RELU) return x > 0.f ? 1.f : (x == x ? 0.f : x);
-    if (act == ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ float act_slope(float x) {
+    if (ACT == ACT_RELU) return x > 0.f ? 1.f : (x == x ? 0.f : x);
+    if (ACT == ACT_SILU) {
         const float g = sigmoid(x);
         return g * (1.f + x * (1.f - g));
     }
-    if (act == ACT_GELU) {
+    if (ACT == ACT_GELU) {
         x = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 16.f), -16.f);       // the slope's limits, long reached; x^2 stays finite
         const float g = sigmoid(2.f * GELU_C * (x + 0.044715f * x * x * x));
         return g + x * (2.f * g * (1.f - g)) * GELU_C * (1.f + 0.134145f * x * x);
     }
     return 1.f;
+}
+// One branch for many values: with one for each, the epilogue of a 256 x 256 tile took four times as long.
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F f) {
+    if (act == ACT_NONE) f(std::integral_constant<int, ACT_NONE>());
+    else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>());
+    else if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>());
+    else f(std::integral_constant<int, ACT_GELU>());
 }
 
 // Eight values of row `m` of C from column n on (fewer at the end of a row) to where they belong.
@@ -97,19 +107,25 @@ __device__ __forceinline__ void finish(const Epilogue &e, float (&v)[8], int m, 
             if (e.pre_out) stb<8>(e.pre_out + at, v);
             float r[8];
             if (e.res) ldb<8, true>(r, e.res + at);
+            by_act(e.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[j] = e.alpha * act_value(e.act, v[j]);
-                if (e.res) v[j] += r[j];
+                for (int j = 0; j < 8; j++) v[j] = e.alpha * act_value<decltype(act)::value>(v[j]);
+            });
+            if (e.res) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] += r[j];
             }
         } else {
             float r[8];
             if (e.act != ACT_NONE) ldb<8, true>(r, e.pre + at);
+            by_act(e.act, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[j] *= e.alpha;
-                if (e.act != ACT_NONE) v[j] *= act_slope(e.act, r[j]);
-            }
+                for (int j = 0; j < 8; j++) {
+                    v[j] *= e.alpha;
+                    if (ACT != ACT_NONE) v[j] *= act_slope<ACT>(r[j]);
+                }
+            });
         }
         stb<8>(e.out + at, v);
         return;
@@ -124,72 +140,117 @@ __device__ __forceinline__ void finish(const Epilogue &e, float (&v)[8], int m, 
         if (KIND == FORWARD) {
             if (e.bias) x += bias;
             if (e.pre_out) e.pre_out[at] = (bf16_t)f_to_bf(x);
-            x = e.alpha * act_value(e.act, x);
+            by_act(e.act, [&](auto act) { x = e.alpha * act_value<decltype(act)::value>(x); });
             if (e.res) x += bf_to_f(e.res[at]);
         } else {
             x *= e.alpha;
-            if (e.act != ACT_NONE) x *= act_slope(e.act, bf_to_f(e.pre[at]));
+            if (e.act != ACT_NONE) by_act(e.act, [&](auto act) { x *= act_slope<decltype(act)::value>(bf_to_f(e.pre[at])); });
         }
         e.out[at] = (bf16_t)f_to_bf(x);
     }
 }
 
-// Rows [row0, row0 + ROWS) and columns [col0, col0 + 64) of a tensor on their way to LDS; zero outside.
-template <int ROWS, int THREADS>
-struct Stage {
-    static constexpr int N = ROWS * 8 / THREADS;
-    v4u w[N];
-    __device__ __forceinline__ void load(const Mat &a, int row0, int col0) {
-        const int chunk = threadIdx.x & 7, col = col0 + chunk * 8;
-        const int b = col / a.S, s = col - b * a.S;
-        const bf16_t *p = a.p + ((size_t)b * a.rows + row0 + (threadIdx.x >> 3)) * a.S + s;
-        const bool vec = s + 8 <= a.S && col < a.cols;
-        const int left = a.rows - row0 - (int)(threadIdx.x >> 3);
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            v4u v = {0u, 0u, 0u, 0u};
-            if (i * (THREADS / 8) < left) {
-                const bf16_t *q = p + (size_t)(i * (THREADS / 8)) * a.S;
-                if (vec) v = *reinterpret_cast<const v4u_any *>(q);
-                else if (col < a.cols) v = pieces(a, row0 + (int)(threadIdx.x >> 3) + i * (THREADS / 8), col);
-            }
-            w[i] = v;
-        }
-    }
-    static __device__ __forceinline__ v4u pieces(const Mat &a, int row, int col) {
-        unsigned e[8];
-        int b = col / a.S, s = col - b * a.S;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            e[j] = col + j < a.cols ? a.p[((size_t)b * a.rows + row) * a.S + s] : 0u;
-            if (++s == a.S) s = 0, b++;
-        }
-        return v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
-    }
-    __device__ __forceinline__ void store(char *panel) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int t = threadIdx.x + i * THREADS;
-            *reinterpret_cast<v4u *>(panel + panel_at(t >> 3, t & 7)) = w[i];
-        }
-    }
-};
+// Rows and columns of a tensor on their way to LDS.  Loads go straight into LDS, 16 bytes a lane, the lanes of an instruction one after the
+// other (eight rows of a panel), so what panel_at() would put elsewhere is fetched by another lane instead.  The tensors are aligned:
+// base and S in units of eight values (repacked() brings others to that).  A read outside of the buffer gives zero.
+constexpr unsigned OUTSIDE = 0xfffffff0u;
 
-// An operand's 64 steps of the sum for B indexes: by columns B / 64 panels of 64 rows (the sum) x 64 columns, else one of B rows.
+typedef int rsrc_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long bytes) {
+    const unsigned long long a = (unsigned long long)p;
+    return rsrc_t{(int)a, (int)(a >> 32) & 0xffff, (int)(unsigned)(bytes < 0xffffff00ull ? bytes : 0xffffff00ull), 0x00027000};
+}
+// lds[16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.  (With
+// the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0, which
+// no other instruction of these kernels needs, is set with it.
+__device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, const char *lds) {
+    const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds;
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(r), "s"(soffset), "s"(at) : "memory");
+}
+// All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
+template <int LEFT, int READS>
+__device__ __forceinline__ void loads_and_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" :: "n"(LEFT), "n"(READS) : "memory");
+}
+
+// An operand's 64 steps of the sum for B indexes.  COLUMNS: the sum goes over the rows: B / 64 panels of 64 rows x 64 columns; else over the
+// columns: one panel of B rows.
 template <int B, bool COLUMNS, int THREADS>
 struct Operand {
-    static constexpr int PANELS = COLUMNS ? B / 64 : 1, ROWS = COLUMNS ? 64 : B, BYTES = B * PANEL_ROW;
-    Stage<ROWS, THREADS> s[PANELS];
-    __device__ __forceinline__ void load(const Mat &a, int index0, int sum0) {
+    static constexpr int PANELS = COLUMNS ? B / 64 : 1, ROWS = COLUMNS ? 64 : B, BYTES = B * PANEL_ROW, WAVES = THREADS / 64;
+    static constexpr int PER = ROWS / (8 * WAVES), LOADS = PANELS * PER;        // instructions of a wave to a panel, to a stage
+    static_assert(PER * 8 * WAVES == ROWS && WAVES % 2 == 0, "whole instructions per wave, one swizzle for all of a lane's rows");
+    static constexpr int READS = COLUMNS ? 2 : 1;           // reads of LDS to a fragment
+    rsrc_t r;               // begins at the slab that the next load is in
+    unsigned long long bytes;
+    unsigned voff[PANELS];
+    unsigned soff, row_bytes, slab_bytes, wave_at;
+    int rows, cols, S, s0;
+    bool even;              // by columns, or every 64 steps lie in one slab: a lane's offset stays what it is
+
+    // index0: the tile's first index; sum0: where the sum starts
+    __device__ __forceinline__ void begin(const Mat &a, int index0, int sum0) {
+        const int t = threadIdx.x, row = t >> 3, chunk = (t & 7) ^ panel_swz(row);
+        rows = a.rows;
+        cols = a.cols;
+        S = a.S;
+        row_bytes = (unsigned)a.S * 2;
+        slab_bytes = (unsigned)a.rows * row_bytes;
+        wave_at = __builtin_amdgcn_readfirstlane(t >> 6) * 1024;
+        const int first = COLUMNS ? index0 : sum0;              // the first column of all that this reads
+        const int b0 = first / a.S;
+        s0 = first - b0 * a.S;
+        const size_t skip = ((size_t)b0 * a.rows + (COLUMNS ? sum0 : index0)) * a.S;
+        bytes = ((size_t)(a.cols / a.S) * a.rows * a.S - skip) * 2;
+        r = buffer_at(a.p + skip, bytes);
+        even = COLUMNS || a.S % 64 == 0 || a.cols == a.S;
+        soff = COLUMNS ? 0 : s0 * 2;
 #pragma unroll
-        for (int p = 0; p < PANELS; p++) {
-            if (COLUMNS) s[p].load(a, sum0, index0 + p * 64);
-            else s[p].load(a, index0, sum0);
+        for (int i = 0; i < PANELS; i++) {
+            if (COLUMNS) {
+                const int s = s0 + i * 64 + chunk * 8, db = s / a.S;
+                voff[i] = (((unsigned)db * rows + row) * a.S + (s - db * a.S)) * 2;
+            } else voff[i] = (unsigned)row * row_bytes + chunk * 16;
         }
     }
-    __device__ __forceinline__ void store(char *lds) const {
+    // the next 64 steps of the sum, `left` of which exist, to a stage of LDS; moves on
+    __device__ __forceinline__ void load(const char *lds, int left) {
+        lds += wave_at;
+        if (even && left >= 64) {
 #pragma unroll
-        for (int p = 0; p < PANELS; p++) s[p].store(lds + p * (ROWS * PANEL_ROW));
+            for (int i = 0; i < PANELS; i++)
+#pragma unroll
+                for (int j = 0; j < PER; j++)
+                    load_to_lds(r, voff[i], soff + j * 8 * WAVES * row_bytes, lds + i * (64 * PANEL_ROW) + j * WAVES * 1024);
+        } else {
+            const int row = threadIdx.x >> 3, chunk = (threadIdx.x & 7) ^ panel_swz(row);
+#pragma unroll
+            for (int i = 0; i < PANELS; i++)
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    unsigned v = voff[i];
+                    if (COLUMNS) v = row + j * 8 * WAVES < left ? v : OUTSIDE;
+                    else {
+                        for (int s = s0 + chunk * 8; s >= S; s -= S) v += slab_bytes - row_bytes;
+                        v = chunk * 8 < left ? v : OUTSIDE;
+                    }
+                    load_to_lds(r, v, soff + j * 8 * WAVES * row_bytes, lds + i * (64 * PANEL_ROW) + j * WAVES * 1024);
+                }
+        }
+        if constexpr (COLUMNS) soff += 64 * row_bytes;
+        else {
+            soff += 128;
+            s0 += 64;
+            if (s0 >= S) {
+                const int n = s0 / S;
+                s0 -= n * S;
+                soff = s0 * 2;
+                const unsigned long long skip = (unsigned long long)n * slab_bytes, at = ((unsigned long long)(unsigned)r[1] << 32 | (unsigned)r[0]) + skip;
+                bytes -= skip;
+                r = buffer_at((const void *)at, bytes);
+            }
+        }
     }
     // the fragment of indexes block*32 .. +31 at 16 steps of the sum
     static __device__ __forceinline__ M16::Frag frag(const char *lds, int block, int step) {
@@ -198,82 +259,266 @@ struct Operand {
     }
 };
 
-template <int KIND, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Mat b, Epilogue e, float *__restrict__ part, int M, int N, int steps,
-                                                                       int slice_steps, int tiles_m, int tiles_n) {
-    constexpr int WAVES_N = BN / WN, THREADS = BM / WM * WAVES_N * 64, FM = WM / 32, FN = WN / 32;
+// What a wave has of C, written where it belongs.  The product is formed with C's columns in the registers (four consecutive ones at a time)
+// and a row to the lane; 32 rows at a time then go through LDS that is the wave's own, so that memory sees whole rows of the tile.  The
+// residual, or what the activation below was applied to, comes in by the same way.
+template <int KIND, int FM, int FN>
+struct WaveOut {
+    static constexpr int WN = FN * 32;
+    static constexpr int BYTES = 32 * (WN * 4 + 16);        // for fp32 rows; the 16 bytes behind each row spread them over the banks
+    static __device__ __forceinline__ void settle() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+    static __device__ __forceinline__ void floats(char *lds, const v16f (&acc)[FN], float *out, size_t pitch, int m0, int n0, int M, int N, float alpha, bool accumulate) {
+        constexpr int PITCH = WN * 4 + 16, LANES = WN / 4;
+        const int lane = threadIdx.x & 63, h = lane >> 5, at = lane % LANES * 4;
+        settle();
+#pragma unroll
+        for (int k = 0; k < FN; k++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<v4f *>(lds + (lane & 31) * PITCH + (k * 32 + 8 * q + 4 * h) * 4) =
+                    v4f{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
+        settle();
+        const int n = n0 + at;
+#pragma unroll
+        for (int i = 0; i < 32; i += 64 / LANES) {
+            const int row = i + lane / LANES;
+            v4f v = *reinterpret_cast<const v4f *>(lds + row * PITCH + at * 4);
+            if (m0 + row >= M || n >= N) continue;
+            float *p = out + (size_t)(m0 + row) * pitch + n;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] *= alpha;
+            if (n + 4 <= N) {
+                if (accumulate) {
+                    const v4f old = ld4(p);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] += old[j];
+                }
+                st4(p, v);
+            } else
+                for (int j = 0; n + j < N; j++) p[j] = accumulate ? p[j] + v[j] : v[j];
+        }
+    }
+
+    // Eight columns of a row between memory and LDS.
+    struct Columns { int n, b, s, N, S; };
+    static __device__ __forceinline__ v4u read8(const bf16_t *src, int rows, int m, const Columns &c) {
+        if (c.s + 8 <= c.S) return *reinterpret_cast<const v4u_any *>(src + ((size_t)c.b * rows + m) * c.S + c.s);
+        unsigned e[8];
+        int b = c.b, s = c.s;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            e[j] = c.n + j < c.N ? src[((size_t)b * rows + m) * c.S + s] : 0u;
+            if (++s == c.S) s = 0, b++;
+        }
+        return v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+    }
+    static __device__ __forceinline__ void write8(bf16_t *dst, int rows, int m, const Columns &c, v4u v) {
+        if (c.s + 8 <= c.S) {
+            *reinterpret_cast<v4u_any *>(dst + ((size_t)c.b * rows + m) * c.S + c.s) = v;
+            return;
+        }
+        int b = c.b, s = c.s;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (c.n + j < c.N) dst[((size_t)b * rows + m) * c.S + s] = (bf16_t)(v[j >> 1] >> (j & 1) * 16);
+            if (++s == c.S) s = 0, b++;
+        }
+    }
+
+    static __device__ __forceinline__ void halves(char *lds, const v16f (&acc)[FN], const Epilogue &e, int m0, int M, const Columns &c) {
+        constexpr int PITCH = WN * 2 + 16, LANES = WN / 8;
+        const int lane = threadIdx.x & 63, h = lane >> 5, row0 = lane / LANES;
+        const bf16_t *in = KIND == FORWARD ? e.res : e.act != ACT_NONE ? e.pre : nullptr;
+        char *mine = lds + (lane & 31) * PITCH + h * 8, *rows = lds + row0 * PITCH + lane % LANES * 16;
+        if (in) {
+            v4u w[32 * LANES / 64];
+#pragma unroll
+            for (int i = 0; i < 32 * LANES / 64; i++) {
+                const int m = m0 + row0 + i * (64 / LANES);
+                w[i] = m < M && c.n < c.N ? read8(in, M, m, c) : v4u{0u, 0u, 0u, 0u};
+            }
+            settle();
+#pragma unroll
+            for (int i = 0; i < 32 * LANES / 64; i++) *reinterpret_cast<v4u *>(rows + i * (64 / LANES) * PITCH) = w[i];
+        }
+        settle();
+        const float bias = KIND == FORWARD && e.bias && m0 + (lane & 31) < M ? e.bias[m0 + (lane & 31)] : 0.f;
+        by_act(e.act, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            auto quads = [&](auto with) {           // with: whether LDS holds something of these columns
+                constexpr bool IN = decltype(with)::value;
+#pragma unroll
+                for (int k = 0; k < FN; k++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        typedef unsigned v2u __attribute__((ext_vector_type(2)));
+                        v2u *at = reinterpret_cast<v2u *>(mine + k * 64 + q * 16);
+                        v2u r = {0u, 0u};
+                        if (IN) r = *at;
+                        float v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float x = bf_to_f(j & 1 ? r[j >> 1] >> 16 : r[j >> 1] & 0xffffu);
+                            if (KIND == FORWARD) {
+                                v[j] = e.alpha * act_value<ACT>(acc[k][4 * q + j] + bias);
+                                if (IN) v[j] += x;
+                            } else {
+                                v[j] = e.alpha * acc[k][4 * q + j];
+                                if (IN) v[j] *= act_slope<ACT>(x);
+                            }
+                        }
+                        *at = v2u{f2_to_bf2(v[0], v[1]), f2_to_bf2(v[2], v[3])};
+                    }
+            };
+            if (KIND == DX) quads(std::integral_constant<bool, ACT != ACT_NONE>());
+            else if (in) quads(std::true_type());
+            else quads(std::false_type());
+        });
+        settle();
+#pragma unroll
+        for (int i = 0; i < 32 * LANES / 64; i++) {
+            const int m = m0 + row0 + i * (64 / LANES);
+            const v4u v = *reinterpret_cast<const v4u *>(rows + i * (64 / LANES) * PITCH);
+            if (m < M && c.n < c.N) write8(e.out, M, m, c, v);
+        }
+        if (KIND == FORWARD && e.pre_out) {
+            settle();
+#pragma unroll
+            for (int k = 0; k < FN; k++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+                    *reinterpret_cast<v2u *>(mine + k * 64 + q * 16) = v2u{f2_to_bf2(acc[k][4 * q] + bias, acc[k][4 * q + 1] + bias),
+                                                                           f2_to_bf2(acc[k][4 * q + 2] + bias, acc[k][4 * q + 3] + bias)};
+                }
+            settle();
+#pragma unroll
+            for (int i = 0; i < 32 * LANES / 64; i++) {
+                const int m = m0 + row0 + i * (64 / LANES);
+                const v4u v = *reinterpret_cast<const v4u *>(rows + i * (64 / LANES) * PITCH);
+                if (m < M && c.n < c.N) write8(e.pre_out, M, m, c, v);
+            }
+        }
+    }
+};
+
+template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Mat b, Epilogue e, float *__restrict__ part, int M, int N, int out_s,
+                                                                       int sum, int slice_steps, int tiles_m, int tiles_n) {
+    constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, THREADS = WAVES_M * WAVES_N * 64, FM = WM / 32, FN = WN / 32;
     typedef Operand<BM, KIND == DX, THREADS> A;
     typedef Operand<BN, KIND != DW, THREADS> B;
-    constexpr int PITCH = BN + 8;               // floats between the rows of the tile of C in LDS
-    constexpr int TILE = BM * PITCH * 4, PANELS = 2 * (A::BYTES + B::BYTES);
-    __shared__ __attribute__((aligned(16))) char lds[TILE > PANELS ? TILE : PANELS];
+    typedef WaveOut<KIND, FM, FN> Out;
+    constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS, OUT = WAVES_M * WAVES_N * Out::BYTES;
+    // With three stages or more the one after the present one has arrived too, so that its first fragments can be read ahead.
+    constexpr bool AHEAD = STAGES > 2;
+    constexpr int LEFT = LOADS * (AHEAD ? STAGES - 3 : 0), FULL = AHEAD ? STAGES - 1 : 2;
+    __shared__ __attribute__((aligned(1024))) char lds[OUT > STAGES * STAGE ? OUT : STAGES * STAGE];
     const int tile = xcd_remap(blockIdx.x, tiles_m * tiles_n);
     const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
-    const int i0 = blockIdx.y * slice_steps, i1 = min(steps, i0 + slice_steps);
+    const int sum0 = blockIdx.y * slice_steps * 64, sum1 = min(sum, sum0 + slice_steps * 64), steps = (sum1 - sum0 + 63) / 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave / WAVES_N * FM, wn = wave % WAVES_N * FN;
 
+    A la;
+    B lb;
+    la.begin(a, m0, sum0);
+    lb.begin(b, n0, sum0);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++)
+        if (i < steps) {
+            la.load(lds + i * STAGE, sum1 - sum0 - i * 64);
+            lb.load(lds + i * STAGE + A::BYTES, sum1 - sum0 - i * 64);
+        }
     v16f acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
         for (int j = 0; j < FN; j++) acc[i][j] = v16_zero();
-    A la;
-    B lb;
-    la.load(a, m0, i0 * 64);
-    lb.load(b, n0, i0 * 64);
-    la.store(lds);
-    lb.store(lds + A::BYTES);
-    __syncthreads();
-    for (int i = i0; i < i1; i++) {
-        const char *at = lds + ((i - i0) & 1) * (A::BYTES + B::BYTES);
-        if (i + 1 < i1) {
-            la.load(a, m0, (i + 1) * 64);
-            lb.load(b, n0, (i + 1) * 64);
+    // Fragments are read DEEP steps of 16 before they are multiplied: a read takes longer than one step's products.  They are a ring.
+    constexpr int DEEP = AHEAD ? 2 : 1, RING = DEEP == 2 ? 4 : 2;
+    M16::Frag fa[RING][FM], fb[RING][FN];
+    auto fetch = [&](int set, const char *p, int s) {
+#pragma unroll
+        for (int j = 0; j < FM; j++) fa[set][j] = A::frag(p, wm + j, s);
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[set][j] = B::frag(p + A::BYTES, wn + j, s);
+    };
+    if (AHEAD) {
+        if (steps >= STAGES - 1) loads_and_barrier<LOADS *(STAGES - 2), 0>();
+        else loads_and_barrier<0, 0>();
+        __builtin_amdgcn_s_waitcnt(0xc07f);     // lgkmcnt(0), for the compiler to know that no scalar load is under way in the loop
+        fetch(0, lds, 0);
+        fetch(1, lds, 1);
+    }
+    // reads of the stage to come that are under way at the barrier; all before them are done when no more than these are
+    constexpr int READS = AHEAD ? DEEP * (FM * A::READS + FN * B::READS) : 0, READS_LEFT = READS < 15 ? READS : 15;
+    int at = 0, next = STAGES - 1;              // the stages that are read and written
+    for (int i = 0; i < steps; i++) {
+        // everybody is done with the stage before `at`, which is filled again
+        if (steps - i >= FULL) loads_and_barrier<LEFT, READS_LEFT>();
+        else loads_and_barrier<0, READS_LEFT>();
+        if (i + STAGES - 1 < steps) {
+            la.load(lds + next * STAGE, sum1 - sum0 - (i + STAGES - 1) * 64);
+            lb.load(lds + next * STAGE + A::BYTES, sum1 - sum0 - (i + STAGES - 1) * 64);
         }
+        const char *p = lds + at * STAGE;
+        at = at + 1 == STAGES ? 0 : at + 1;
+        next = next + 1 == STAGES ? 0 : next + 1;
+        const char *p1 = lds + at * STAGE;
+        if (!AHEAD) fetch(0, p, 0);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            M16::Frag fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FM; j++) fa[j] = A::frag(at, wm + j, s);
-#pragma unroll
-            for (int j = 0; j < FN; j++) fb[j] = B::frag(at + A::BYTES, wn + j, s);
+            // (past the last stage: read, not used)
+            if (s + DEEP < 4) fetch((s + DEEP) & (RING - 1), p, s + DEEP);
+            else if (AHEAD) fetch((s + DEEP) & (RING - 1), p1, s + DEEP - 4);
+            __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler puts each read right before the product that needs it)
 #pragma unroll
             for (int j = 0; j < FM; j++)
 #pragma unroll
-                for (int k = 0; k < FN; k++) acc[j][k] = M16::mul(fa[j], fb[k], acc[j][k]);
+                for (int k = 0; k < FN; k++) acc[j][k] = M16::mul(fb[s & (RING - 1)][k], fa[s & (RING - 1)][j], acc[j][k]);
         }
-        if (i + 1 < i1) {
-            char *next = lds + ((i + 1 - i0) & 1) * (A::BYTES + B::BYTES);
-            la.store(next);
-            lb.store(next + A::BYTES);
-        }
-        __syncthreads();
     }
-    // The tile goes through LDS so that a thread ends with eight columns of one row.
-    float *c = reinterpret_cast<float *>(lds);
-#pragma unroll
-    for (int j = 0; j < FM; j++)
-#pragma unroll
-        for (int k = 0; k < FN; k++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                c[((wm + j) * 32 + acc_row(r) + 4 * (lane >> 5)) * PITCH + (wn + k) * 32 + (lane & 31)] = acc[j][k][r];
     __syncthreads();
-    for (int t = threadIdx.x; t < BM * BN / 8; t += THREADS) {
-        const int row = t / (BN / 8), col = t % (BN / 8) * 8, m = m0 + row, n = n0 + col;
-        if (m >= M || n >= N) continue;
-        float v[8];
-        const v4f lo = *reinterpret_cast<const v4f *>(c + row * PITCH + col), hi = *reinterpret_cast<const v4f *>(c + row * PITCH + col + 4);
+    char *mine = lds + wave * Out::BYTES;
+    const int n = n0 + wn * 32 + lane % (FN * 4) * 8, slab = KIND == DW ? 0 : n / out_s;
+    const typename Out::Columns cols = {n, slab, n - slab * out_s, N, out_s};
+#pragma unroll 1
+    for (int i = 0; i < FM; i++) {              // (one copy of the code for all blocks of 32 rows)
+        v16f cur[FN];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = lo[j], v[4 + j] = hi[j];
-        if (part) {
-            float *p = part + ((size_t)blockIdx.y * M + m) * N + n;
-            if (n + 8 <= N) st4(p, lo), st4(p + 4, hi);
-            else
-                for (int j = 0; n + j < N; j++) p[j] = v[j];
-        } else finish<KIND>(e, v, m, M, n, N, KIND == DW ? N : b.S);
+        for (int j = 0; j < FM; j++)
+            if (i == j) {
+#pragma unroll
+                for (int k = 0; k < FN; k++) cur[k] = acc[j][k];
+            }
+        const int m = m0 + (wm + i) * 32;
+        if (part || KIND == DW)
+            Out::floats(mine, cur, part ? part + (size_t)blockIdx.y * M * N : e.dw, N, m, n0 + wn * 32, M, N, part ? 1.f : e.alpha, !part && e.accumulate);
+        else Out::halves(mine, cur, e, m, M, cols);
     }
+}
+
+// A tensor whose rows begin at any value, as one of [rows][cols8] whose rows begin at multiples of eight: zeros from its last column on.
+__global__ __launch_bounds__(256) void repack_kernel(bf16_t *__restrict__ out, Mat a, int cols8) {
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int groups = cols8 / 8;
+    if (t >= (size_t)a.rows * groups) return;
+    const int row = (int)(t / groups), col = (int)(t % groups) * 8;
+    int b = col / a.S, s = col - b * a.S;
+    v4u v;
+    if (col + 8 <= a.cols && s + 8 <= a.S) v = *reinterpret_cast<const v4u_any *>(a.p + ((size_t)b * a.rows + row) * a.S + s);
+    else {
+        unsigned e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            e[j] = col + j < a.cols ? a.p[((size_t)b * a.rows + row) * a.S + s] : 0u;
+            if (++s == a.S) s = 0, b++;
+        }
+        v = v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+    }
+    *reinterpret_cast<v4u *>(out + (size_t)row * cols8 + col) = v;
 }
 
 // The slices of a product added up in their order, and its epilogue.
@@ -300,6 +545,55 @@ __global__ __launch_bounds__(256) void linear_join_kernel(Epilogue e, const floa
                 if (n + j < N) v[j] += p[j];
     }
     finish<KIND>(e, v, m, M, n, N, S);
+}
+
+// Few columns: y is bound by reading w once, in rows.  A wave takes rows of w, its lanes eight steps of the sum at a time; x, as fp32 in LDS
+// [column][step], serves the workgroup's rows.  NC columns at once.
+constexpr int GEMV_MAX = 8;
+template <int NC>
+__global__ __launch_bounds__(256) void gemv_kernel(const bf16_t *__restrict__ w, const bf16_t *__restrict__ x, Epilogue e, int M, int K, int N, int S,
+                                                   int kpad) {
+    extern __shared__ __attribute__((aligned(16))) float xs[];
+    for (int i = threadIdx.x; i < kpad * NC; i += 256) {
+        const int n = i / kpad, k = i - n * kpad, b = n / S;
+        xs[i] = n < N && k < K ? bf_to_f(x[((size_t)b * K + k) * S + (n - b * S)]) : 0.f;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 63, m = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= M) return;
+    float acc[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++) acc[n] = 0.f;
+    const bf16_t *row = w + (size_t)m * K;
+#pragma unroll 4
+    for (int k = lane * 8; k < kpad; k += 512) {
+        float v[8];
+        if (k + 8 <= K) ldb<8, true>(v, row + k);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = k + j < K ? bf_to_f(row[k + j]) : 0.f;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const v4f a = *reinterpret_cast<const v4f *>(xs + n * kpad + k), b = *reinterpret_cast<const v4f *>(xs + n * kpad + k + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[n] = __builtin_fmaf(v[4 + j], b[j], __builtin_fmaf(v[j], a[j], acc[n]));
+        }
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const float s = wave_sum_far_first(acc[n]);
+        mine = lane == n ? s : mine;
+    }
+    if (lane < N && lane < NC) {
+        const int b = lane / S;
+        const size_t at = ((size_t)b * M + m) * S + (lane - b * S);
+        if (e.bias) mine += e.bias[m];
+        if (e.pre_out) e.pre_out[at] = (bf16_t)f_to_bf(mine);
+        by_act(e.act, [&](auto act) { mine = e.alpha * act_value<decltype(act)::value>(mine); });
+        if (e.res) mine += bf_to_f(e.res[at]);
+        e.out[at] = (bf16_t)f_to_bf(mine);
+    }
 }
 
 // dbias[m] (+)= alpha * sum of row m of dy over the batch: a workgroup to a row, a fixed tree.
@@ -336,39 +630,65 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *__restrict__ dpre,
         float g[8], x[8];
         ldb<8, true>(g, dy + i);
         ldb<8, true>(x, pre + i);
+        by_act(act, [&](auto a) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) g[j] = alpha * g[j] * act_slope(act, x[j]);
+            for (int j = 0; j < 8; j++) g[j] = alpha * g[j] * act_slope<decltype(a)::value>(x[j]);
+        });
         stb<8>(dpre + i, g);
     } else
-        for (size_t j = i; j < n; j++) dpre[j] = (bf16_t)f_to_bf(alpha * bf_to_f(dy[j]) * act_slope(act, bf_to_f(pre[j])));
+        for (size_t j = i; j < n; j++)
+            by_act(act, [&](auto a) { dpre[j] = (bf16_t)f_to_bf(alpha * bf_to_f(dy[j]) * act_slope<decltype(a)::value>(bf_to_f(pre[j]))); });
 }
 
-// C of M x N from a sum of `sum` terms.
-template <int KIND>
-int product(const char *who, const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int sum) {
+// Whether linear_kernel can read a tensor as it is: chunks of eight values that begin at multiples of 16 bytes, and 32-bit offsets from the
+// slab where a workgroup begins (rows of at most 256 positions, or 64 of the sum).
+bool direct(const Mat &a) {
+    return aligned16(a.p) && a.S % 8 == 0 && ((double)(256 / a.S + 2) * a.rows + 256) * a.S * 2 < 4e9;
+}
+size_t repacked_bytes(const Mat &a) { return direct(a) ? 0 : ((size_t)a.rows * ((a.cols + 7) & ~7) * 2 + 255) & ~(size_t)255; }
+int repack(const char *who, Mat &a, char *&ws) {
+    if (direct(a)) return 0;
+    const int cols8 = (a.cols + 7) & ~7;
+    const size_t threads = (size_t)a.rows * (cols8 / 8);
+    repack_kernel<<<(unsigned)ceil_div(threads, 256), 256, 0, g_ctx.stream>>>((bf16_t *)ws, a, cols8);
+    LAUNCH_OK(who);
+    const size_t bytes = repacked_bytes(a);
+    a = Mat{(bf16_t *)ws, a.rows, cols8, cols8};
+    ws += bytes;
+    return 0;
+}
+
+struct Tiling { int tile, slices, per; };
+Tiling tiling(int M, int N, int sum) {
     const int steps = (int)ceil_div(sum, 64), cu = g_ctx.num_cu;
-    const bool big = ceil_div(M, 128) * ceil_div(N, 128) >= (size_t)cu;
-    const int tile = big ? 128 : 64;
-    const int tm = (int)ceil_div(M, tile), tn = (int)ceil_div(N, tile);
-    if ((size_t)tm * tn > 0xffffff) return mi355_fail("%s: %d x %d results are too many", who, M, N);
-    // slices of the sum until every compute unit has two workgroups, each with at least four panels of the sum
-    int slices = (int)(2 * (size_t)cu / ((size_t)tm * tn));
-    if (slices > steps / 4) slices = steps / 4;
+    auto tiles = [&](int t) { return ceil_div(M, t) * ceil_div(N, t); };
+    Tiling r;
+    r.tile = tiles(256) >= (size_t)2 * cu ? 256 : tiles(128) >= (size_t)cu ? 128 : 64;
+    // slices of the sum until every compute unit has work, each with at least four panels of the sum
+    size_t slices = (size_t)cu / tiles(r.tile);
+    if (slices > (size_t)steps / 4) slices = steps / 4;
     if (slices < 1) slices = 1;
-    const int per = (int)ceil_div(steps, slices);
-    slices = (int)ceil_div(steps, per);
-    float *part = nullptr;
-    if (slices > 1) {
-        part = (float *)mi355_ws((size_t)slices * M * N * sizeof(float));
-        if (!part) return -1;
-    }
-    const dim3 grid((unsigned)(tm * tn), (unsigned)slices);
-    if (big) linear_kernel<KIND, 128, 128, 64, 64><<<grid, 256, 0, g_ctx.stream>>>(a, b, e, part, M, N, steps, per, tm, tn);
-    else linear_kernel<KIND, 64, 64, 32, 32><<<grid, 256, 0, g_ctx.stream>>>(a, b, e, part, M, N, steps, per, tm, tn);
+    r.per = (int)ceil_div(steps, slices);
+    r.slices = (int)ceil_div(steps, r.per);
+    return r;
+}
+size_t part_bytes(const Tiling &t, int M, int N) { return t.slices > 1 ? (size_t)t.slices * M * N * sizeof(float) : 0; }
+
+// C of M x N from a sum of `sum` terms; a and b are direct().
+template <int KIND>
+int product(const char *who, const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s, int sum, char *ws) {
+    const Tiling t = tiling(M, N, sum);
+    const int tm = (int)ceil_div(M, t.tile), tn = (int)ceil_div(N, t.tile);
+    if ((size_t)tm * tn > 0xffffff) return mi355_fail("%s: %d x %d results are too many", who, M, N);
+    float *part = t.slices > 1 ? (float *)ws : nullptr;
+    const dim3 grid((unsigned)(tm * tn), (unsigned)t.slices);
+    if (t.tile == 256) linear_kernel<KIND, 256, 256, 128, 64, 2><<<grid, 512, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
+    else if (t.tile == 128) linear_kernel<KIND, 128, 128, 64, 32, 4><<<grid, 512, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
+    else linear_kernel<KIND, 64, 64, 32, 32, 4><<<grid, 256, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
     LAUNCH_OK(who);
     if (part) {
         const size_t threads = (size_t)M * ceil_div(N, 8);
-        linear_join_kernel<KIND><<<(unsigned)ceil_div(threads, 256), 256, 0, g_ctx.stream>>>(e, part, M, N, KIND == DW ? N : b.S, slices);
+        linear_join_kernel<KIND><<<(unsigned)ceil_div(threads, 256), 256, 0, g_ctx.stream>>>(e, part, M, N, out_s, t.slices);
         LAUNCH_OK(who);
     }
     return 0;
@@ -379,8 +699,8 @@ bool sizes_ok(const char *who, int M, int K, int S, int batch, int act) {
         mi355_fail("%s: bad shape M=%d K=%d S=%d batch=%d", who, M, K, S, batch);
         return false;
     }
-    if ((double)S * batch > 1 << 30 || M > 1 << 30 || K > 1 << 30) {
-        mi355_fail("%s: M, K and batch * S are at most 2^30", who);
+    if ((double)S * batch > 1 << 22 || M > 1 << 22 || K > 1 << 22) {        // (256 rows of that many values: 32-bit offsets)
+        mi355_fail("%s: M, K and batch * S are at most 2^22", who);
         return false;
     }
     if (act < ACT_NONE || act > ACT_GELU) {
@@ -399,8 +719,23 @@ MI355_API int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16
     if (!sizes_ok("linear_fwd_bf16", M, K, S, batch, act)) return -1;
     Epilogue e = {};
     e.act = act; e.alpha = alpha; e.bias = bias; e.res = res; e.pre_out = pre; e.out = y;
-    const Mat a = {w, M, K, K}, b = {x, K, S, batch * S};
-    return product<FORWARD>("linear_fwd_bf16", a, b, e, M, batch * S, K);
+    const int N = batch * S, kpad = (K + 7) & ~7;
+    const size_t xs = (size_t)(N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * kpad * sizeof(float);
+    if (N <= GEMV_MAX && xs <= 64 * 1024) {
+        const unsigned grid = (unsigned)ceil_div(M, 4);
+        if (N <= 1) gemv_kernel<1><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
+        else if (N <= 2) gemv_kernel<2><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
+        else if (N <= 4) gemv_kernel<4><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
+        else gemv_kernel<8><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
+        LAUNCH_OK("linear_fwd_bf16");
+        return 0;
+    }
+    Mat a = {w, M, K, K}, b = {x, K, S, N};
+    const size_t packed = repacked_bytes(a) + repacked_bytes(b), need = packed + part_bytes(tiling(M, N, K), M, N);
+    char *ws = nullptr;
+    if (need && !(ws = (char *)mi355_ws(need))) return -1;
+    if (repack("linear_fwd_bf16", a, ws) || repack("linear_fwd_bf16", b, ws)) return -1;
+    return product<FORWARD>("linear_fwd_bf16", a, b, e, M, N, S, K, ws);
 }
 
 MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, const uint16_t *dy, const uint16_t *x, const uint16_t *w,
@@ -409,17 +744,21 @@ MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, c
     if (!dy || (dx && !w) || (dw && !x) || (!dx && !dw && !dbias)) return mi355_fail("linear_bwd_bf16: NULL pointer");
     if (!sizes_ok("linear_bwd_bf16", M, K, S, batch, act)) return -1;
     if (dx && act != ACT_NONE && !x_pre) return mi355_fail("linear_bwd_bf16: act=%d needs x_pre", act);
-    const Mat g = {dy, M, S, batch * S};
     Epilogue e = {};
     e.act = act; e.alpha = alpha; e.pre = x_pre; e.out = dx; e.dw = dw; e.accumulate = accumulate;
-    if (dx) {
-        const Mat a = {w, M, K, K};
-        if (product<DX>("linear_bwd_bf16", a, g, e, K, batch * S, M)) return -1;
-    }
-    if (dw) {
-        const Mat b = {x, K, S, batch * S};
-        if (product<DW>("linear_bwd_bf16", g, b, e, M, K, batch * S)) return -1;
-    }
+    const int N = batch * S;
+    Mat g = {dy, M, S, N}, wm = {w, M, K, K}, xm = {x, K, S, N};
+    // dx and dw use what is behind the repacked tensors one after the other
+    const size_t packed = (dx || dw ? repacked_bytes(g) : 0) + (dx ? repacked_bytes(wm) : 0) + (dw ? repacked_bytes(xm) : 0);
+    const size_t p1 = dx ? part_bytes(tiling(K, N, M), K, N) : 0, p2 = dw ? part_bytes(tiling(M, K, N), M, K) : 0;
+    const size_t need = packed + (p1 > p2 ? p1 : p2);
+    char *ws = nullptr;
+    if (need && !(ws = (char *)mi355_ws(need))) return -1;
+    if ((dx || dw) && repack("linear_bwd_bf16", g, ws)) return -1;
+    if (dx && repack("linear_bwd_bf16", wm, ws)) return -1;
+    if (dw && repack("linear_bwd_bf16", xm, ws)) return -1;
+    if (dx && product<DX>("linear_bwd_bf16", wm, g, e, K, N, S, M, ws)) return -1;
+    if (dw && product<DW>("linear_bwd_bf16", g, xm, e, M, K, K, g.cols, ws)) return -1;
     if (dbias) {
         row_sum_kernel<<<(unsigned)M, 256, 0, g_ctx.stream>>>(dbias, dy, M, S, batch, alpha, accumulate);
         LAUNCH_OK("linear_bwd_bf16");
