@@ -18,9 +18,9 @@
 
 // dk and dv from lse and delta (attn_dkv.hip): the second launch of the backward entry points, which have checked the arguments.
 int mi355_attn_dkv(const char *who, float *dk, float *dv, const float *d_o, const float *q, const float *k, const float *v, const float *lse,
-                   const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale);
+                   const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale);
 int mi355_attn_dkv(const char *who, bf16_t *dk, bf16_t *dv, const bf16_t *d_o, const bf16_t *q, const bf16_t *k, const bf16_t *v,
-                   const float *lse, const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale);
+                   const float *lse, const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale);
 
 namespace {
 
@@ -71,6 +71,56 @@ __device__ void add_odd(v16f (&acc)[HDB], const char *panel, int sub, const v16f
     }
 }
 
+// A panel of ROWS rows on its way from memory to LDS by way of registers, from any alignment: the chunks of one thread.  src: row 0, column 0 of a tensor with `pitch` values
+// between rows; columns [lo, hi) and rows below `rows` are read, the others become zero.
+template <typename T, int ROWS, int THREADS>
+struct PanelLoad {
+    static constexpr int N = ROWS * 8 / THREADS;
+    static_assert(N * THREADS == ROWS * 8, "whole chunks per thread");
+    v4u w[N];
+    __device__ __forceinline__ void load(const T *src, size_t pitch, int rows, int col0, int lo, int hi) {
+        typedef Mma<T> M;
+        const bool whole = rows >= ROWS && col0 >= lo && col0 + M::COLS <= hi;       // the same for every thread
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int t = threadIdx.x + i * THREADS;
+                const T *p = src + (size_t)(t >> 3) * pitch + col0 + (t & 7) * M::EPC;
+                w[i] = *reinterpret_cast<const typename M::Any16 *>(p);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int t = threadIdx.x + i * THREADS, row = t >> 3, col = col0 + (t & 7) * M::EPC;
+                v4u v = {0u, 0u, 0u, 0u};
+                if (row < rows) {
+                    const T *p = src + (size_t)row * pitch + col;
+                    if (col >= lo && col + M::EPC <= hi) v = *reinterpret_cast<const typename M::Any16 *>(p);
+                    else if (col < hi && col + M::EPC > lo) {
+                        unsigned e[M::EPC];
+#pragma unroll
+                        for (int j = 0; j < M::EPC; j++) e[j] = col + j >= lo && col + j < hi ? bits(p[j]) : 0u;
+                        if constexpr (M::EPC == 4) v = v4u{e[0], e[1], e[2], e[3]};
+                        else v = v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+                    }
+                }
+                w[i] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *panel) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int t = threadIdx.x + i * THREADS;
+            *reinterpret_cast<v4u *>(panel + panel_at(t >> 3, t & 7)) = w[i];
+        }
+    }
+
+private:
+    static __device__ __forceinline__ unsigned bits(bf16_t v) { return v; }
+    static __device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
+};
+
 template <int HDB>
 __device__ __forceinline__ bool has_nan(const v16f (&acc)[HDB]) {
     float s = 0.f;      // (infinities of both signs count too: that costs time, nothing else)
@@ -81,38 +131,112 @@ __device__ __forceinline__ bool has_nan(const v16f (&acc)[HDB]) {
     return s != s;
 }
 
-// acc[channel][position] * f to rows of a tensor; `pos` is the lane's own column of it
+// acc[channel][position] * f to the columns pos0 .. pos0 + 31 of `dst` whose lanes are active.  fp32: as they lie, a row of 32 columns to
+// half a wave.  bfloat16: through LDS that is the wave's own, [position][channel], which the transposing read gives back as eight
+// positions of a channel to a lane (rows of 64 bytes; two bytes a lane and a store for each register without it).
 template <typename T, int HDB>
-__device__ __forceinline__ void store_columns(T *dst, size_t pitch, int hd, const v16f (&acc)[HDB], float f) {
-    const int h = (threadIdx.x & 63) >> 5;
+__device__ __forceinline__ void store_columns(T *dst, size_t pitch, int hd, const v16f (&acc)[HDB], float f, int pos0, bool active, char *lds) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+        if (!active) return;
+        T *p = dst + pos0 + (lane & 31);
 #pragma unroll
-    for (int d = 0; d < HDB; d++)
+        for (int d = 0; d < HDB; d++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int row = d * 32 + acc_row(r) + 4 * h;
-            if (row < hd) dst[(size_t)row * pitch] = Mma<T>::narrow(acc[d][r] * f);
+            for (int r = 0; r < 16; r++) {
+                const int row = d * 32 + acc_row(r) + 4 * h;
+                if (row < hd) p[(size_t)row * pitch] = acc[d][r] * f;
+            }
+    } else {
+        constexpr int ROW = HDB * 64 + 16;          // (the 16 bytes spread the rows over the banks)
+        typedef unsigned v2u __attribute__((ext_vector_type(2)));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int d = 0; d < HDB; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<v2u *>(lds + (lane & 31) * ROW + (d * 32 + acc_row(r) + 4 * h) * 2) =
+                    v2u{f2_to_bf2(acc[d][r] * f, acc[d][r + 1] * f), f2_to_bf2(acc[d][r + 2] * f, acc[d][r + 3] * f)};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const unsigned mask = (unsigned)__ballot(active) >> (lane >> 4) * 8 & 0xff;       // the lane's eight positions
+        const int i = lane & 15, q = (lane >> 4) * 8;
+        const char *at = lds + (q + (i >> 2)) * ROW + (i & 3) * 8;
+#pragma unroll
+        for (int c = 0; c < HDB * 2; c++) {
+            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + c * 32));
+            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + c * 32 + 4 * ROW));
+            const v8s v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            const int row = c * 16 + i;
+            T *p = dst + (size_t)row * pitch + pos0 + q;
+            if (row >= hd) continue;
+            if (mask == 0xff) *reinterpret_cast<v4u_any *>(p) = __builtin_bit_cast(v4u, v);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (mask >> j & 1) p[j] = (T)v[j];
         }
+    }
 }
 
-// The 32 columns of this wave, of 32 * WAVES from col0 on, as fragments of a product over the channels.  Needs as many panels of LDS as
-// the columns fill; ends with a barrier.
+// The 32 positions of this wave, of 32 * WAVES from col0 on, as fragments of a product over the channels.  bfloat16: through LDS, as many
+// panels of it as the positions fill; begins when all waves are done with that place, ends with a barrier.  fp32: a fragment is a value of
+// each lane, rows of 32 positions, straight from memory.
 template <typename T, int HDB, int WAVES, int STEPS>
 __device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], char *lds, const T *src, size_t pitch, int hd, int col0, int S) {
     typedef Mma<T> M;
-    constexpr int PANELS = (32 * WAVES + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if constexpr (sizeof(T) == 4) {
+        const int col = col0 + wave * 32 + (lane & 31), h = lane >> 5;
+        const T *p = src + (size_t)h * pitch + col;
 #pragma unroll
-    for (int p = 0; p < PANELS; p++) {
-        PanelLoad<T, HDB * 32, WAVES * 64> ld;
-        ld.load(src, pitch, hd, col0 + p * M::COLS, 0, S);
-        ld.store(lds + p * BYTES);
+        for (int s = 0; s < STEPS; s++) f[s] = col < S && 2 * s + h < hd ? p[(size_t)(2 * s) * pitch] : 0.f;
+    } else {
+        constexpr int PANELS = (32 * WAVES + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
+#pragma unroll
+        for (int p = 0; p < PANELS; p++) {
+            PanelLoad<T, HDB * 32, WAVES * 64> ld;
+            ld.load(src, pitch, hd, col0 + p * M::COLS, 0, S);
+            ld.store(lds + p * BYTES);
+        }
+        __syncthreads();
+        const char *panel = lds + (wave * 32 / M::COLS) * BYTES;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) f[s] = M::columns(panel, wave * 32 % M::COLS / 32, s);
+        __syncthreads();
     }
-    __syncthreads();
-    const char *panel = lds + (wave * 32 / M::COLS) * BYTES;
-#pragma unroll
-    for (int s = 0; s < STEPS; s++) f[s] = M::columns(panel, wave * 32 % M::COLS / 32, s);
-    __syncthreads();
 }
+
+// The panels of a head on their way into LDS, one after the other: columns col0 .. col0 + COLS, whole chunks outside of [from, to) and rows
+// from hd on zero.  `pitch` values between rows, a multiple of a chunk, as is the address of the first.
+template <typename T, int ROWS, int WAVES>
+struct PanelStream {
+    static constexpr int LOADS = ROWS / (8 * WAVES);
+    static_assert(LOADS * 8 * WAVES == ROWS && WAVES % 2 == 0, "whole instructions per wave, one swizzle for all of a lane's rows");
+    rsrc_t r;
+    unsigned voff, row_bytes;
+    int hd;
+    __device__ __forceinline__ void begin(const T *head, int pitch, int channels) {
+        const int row = threadIdx.x >> 3, chunk = (threadIdx.x & 7) ^ panel_swz(row);
+        hd = channels;
+        row_bytes = (unsigned)pitch * sizeof(T);
+        r = buffer_at(head, (unsigned long long)channels * row_bytes);
+        voff = row * row_bytes + chunk * 16;
+    }
+    __device__ __forceinline__ void load(const char *panel, int col0, int from, int to) {
+        panel += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+        const unsigned soff = (unsigned)col0 * sizeof(T);
+        if (col0 >= from && col0 + Mma<T>::COLS <= to && hd == ROWS) {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) load_to_lds(r, voff, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
+        } else {
+            const int row = threadIdx.x >> 3, col = col0 + ((threadIdx.x & 7) ^ panel_swz(row)) * Mma<T>::EPC;
+            const bool in = col < to && col + Mma<T>::EPC > from;
+#pragma unroll
+            for (int j = 0; j < LOADS; j++)
+                load_to_lds(r, in && row + j * 8 * WAVES < hd ? voff : OUTSIDE, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
+        }
+    }
+};
 
 // Which position block of which head a workgroup has: blocks in the given order, heads of one KV group on one XCD where the heads deal
 // out evenly (their L2 then holds the group's keys and values once).
@@ -148,12 +272,54 @@ bool shape_ok(const char *who, int heads, int kv_heads, int hd, int S, int batch
         mi355_fail("%s: scale must be positive and finite", who);
         return false;
     }
-    // what a launch can number (2^32 threads, two waves to 64 positions), and 32-bit positions
-    if (S > 1 << 30 || (double)heads * batch * ceil_div(S, 64) > (double)((1 << 25) - 1)) {
-        mi355_fail("%s: heads * batch * ceil(S / 64) = %.0f (at most 2^25 - 1), S = %d (at most 2^30)", who, (double)heads * batch * ceil_div(S, 64), S);
+    // what a launch can number (2^32 threads, two waves to 64 positions), and 32-bit offsets into a head
+    if (S > 1 << 22 || (double)heads * batch * ceil_div(S, 64) > (double)((1 << 25) - 1)) {
+        mi355_fail("%s: heads * batch * ceil(S / 64) = %.0f (at most 2^25 - 1), S = %d (at most 2^22)", who, (double)heads * batch * ceil_div(S, 64), S);
         return false;
     }
     return true;
+}
+
+// Whether rows of S values can be loaded in whole chunks of 16 bytes as they lie.
+template <typename T>
+bool streams_directly(const T *p, int S) { return aligned16(p) && S % (16 / sizeof(T)) == 0; }
+
+// Rows of S values into rows of whole chunks, zeros behind: up to two tensors of as many rows.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(T *__restrict__ out0, T *__restrict__ out1, const T *__restrict__ in0, const T *__restrict__ in1,
+                                                        size_t rows, int S, int pitch) {
+    constexpr int EPC = Mma<T>::EPC;
+    const T *in = blockIdx.y ? in1 : in0;
+    T *out = blockIdx.y ? out1 : out0;
+    const int chunks = pitch / EPC;
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x, row = t / chunks;
+    const int col = (int)(t - row * chunks) * EPC;
+    if (row >= rows) return;
+    const T *p = in + row * S + col;
+    if (col + EPC <= S) {
+        *reinterpret_cast<v4u *>(out + row * pitch + col) = *reinterpret_cast<const typename Mma<T>::Any16 *>(p);
+    } else
+#pragma unroll
+        for (int j = 0; j < EPC; j++) out[row * pitch + col + j] = col + j < S ? p[j] : (T)0;
+}
+template <typename T>
+size_t packed_bytes(size_t rows, int S) {
+    constexpr int EPC = Mma<T>::EPC;
+    return (rows * ((S + EPC - 1) / EPC * EPC) * sizeof(T) + 255) & ~(size_t)255;
+}
+// Two tensors to `ws`, packed_bytes() for each.
+template <typename T>
+int pack_rows(const char *who, const T **a, const T **b, size_t rows, int S, int *pitch, void *ws) {
+    constexpr int EPC = Mma<T>::EPC;
+    *pitch = (S + EPC - 1) / EPC * EPC;
+    const size_t threads = rows * (*pitch / EPC);
+    if (ceil_div(threads, 256) > 0xffffff) return mi355_fail("%s: %zu rows of %d positions, which are no whole 16 bytes, are too many", who, rows, S);
+    T *d0 = (T *)ws, *d1 = (T *)((char *)ws + packed_bytes<T>(rows, S));
+    pack_rows_kernel<T><<<dim3((unsigned)ceil_div(threads, 256), 2), 256, 0, g_ctx.stream>>>(d0, d1, *a, *b, rows, S, *pitch);
+    LAUNCH_OK(who);
+    *a = d0;
+    *b = d1;
+    return 0;
 }
 
 // Waves (32 positions each) to a workgroup: four share the panels that they read, unless that leaves compute units without work.

@@ -5,14 +5,14 @@ namespace {
 
 // ---- backward: dq and delta -----------------------------------------------------------------------------------------------------
 
+// k and v have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                                                             const int *__restrict__ bounds, int S, int heads, int kv_heads, int hd,
-                                                             float scale, const T *__restrict__ o, const T *__restrict__ d_o,
-                                                             const float *__restrict__ lse, T *__restrict__ dq, float *__restrict__ delta,
-                                                             int batch, int blocks) {
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 2))) void attn_dq_kernel(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
+    int kv_heads, int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq,
+    float *__restrict__ delta, int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP, THREADS = WAVES * 64;
+    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
     __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
     __shared__ int firsts[WAVES];
     const Place at = place(blocks, heads, batch, true);
@@ -36,47 +36,44 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(const T *__restrict
     if (from >= S) return;
     const int to = min(q0 + QT, S);
     const int kvh = at.h / (heads / kv_heads);
-    const T *kb = k + ((size_t)at.b * kv_heads + kvh) * hd * S, *vb = v + ((size_t)at.b * kv_heads + kvh) * hd * S;
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S, row = ((size_t)at.b * heads + at.h) * S;
+    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
 
+    // delta from the fragments: two lanes share a query, each has half of the channels
     typename M::Frag qf[STEPS], gf[STEPS];
-    own_columns<T, HDB, WAVES, STEPS>(qf, lds, q + slab, S, hd, q0, S);
     own_columns<T, HDB, WAVES, STEPS>(gf, lds, d_o + slab, S, hd, q0, S);
-    // delta: two lanes share a query, each takes every other channel
-    float dlt = 0.f, lse2 = 0.f;
-    if (active) {
-        for (int d = h; d < hd; d += 2)
-            dlt += M::widen(o[slab + (size_t)d * S + mine]) * M::widen(d_o[slab + (size_t)d * S + mine]);
-        lse2 = lse[row + mine] * LOG2E;
-    }
+    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, o + slab, S, hd, q0, S);
+    float dlt = 0.f;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) dlt = M::dot(qf[i], gf[i], dlt);
     dlt += lane_xor<32>(dlt);
+    const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
     if (active && h == 0) delta[row + mine] = dlt;
+
+    PanelStream<T, HDB * 32, WAVES> ks, vs;
+    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
+    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
+    ks.load(lds, t0 * M::COLS, from, to);
+    vs.load(lds + BYTES, t0 * M::COLS, from, to);
+    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, q + slab, S, hd, q0, S);
     const float scale2 = scale * LOG2E;
 
     v16f acc[HDB];
-    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
-    auto walk = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    auto walk = [&](bool careful) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        PanelLoad<T, HDB * 32, THREADS> lk, lv;
-        lk.load(kb, S, hd, t0 * M::COLS, from, to);
-        lv.load(vb, S, hd, t0 * M::COLS, from, to);
-        __syncthreads();
-        lk.store(lds);
-        lv.store(lds + BYTES);
-        __syncthreads();
         for (int t = t0; t <= t1; t++) {
-            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES;
+            // what this tile needs is there; everybody is done with the tile before it
+            loads_and_barrier<0, 0>();
+            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES, *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
             if (t < t1) {
-                lk.load(kb, S, hd, (t + 1) * M::COLS, from, to);
-                lv.load(vb, S, hd, (t + 1) * M::COLS, from, to);
+                ks.load(next, (t + 1) * M::COLS, from, to);
+                vs.load(next + BYTES, (t + 1) * M::COLS, from, to);
             }
             const int c0 = t * M::COLS;
             if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
                 const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-                unsigned long long odd = 0;
-                if constexpr (CAREFUL) odd = masked ? odd_columns<T, HDB * 32>(kp) : 0;
+                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(kp) : 0;
 #pragma unroll
                 for (int u = 0; u < M::SUBS; u++) {
                     v16f s = v16_zero(), g = v16_zero();
@@ -97,25 +94,26 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(const T *__restrict
                         }
                     }
                     const typename M::Packed p = M::pack(s);
+                    if (odd) {
 #pragma unroll
-                    for (int d = 0; d < HDB; d++) {
-                        if (CAREFUL && odd) acc[d] = M::template rows<true>(kp, d, u, p, acc[d]);
-                        else acc[d] = M::template rows<false>(kp, d, u, p, acc[d]);
+                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<true>(kp, d, u, p, acc[d]);
+                        add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<false>(kp, d, u, p, acc[d]);
                     }
-                    if (CAREFUL && odd) add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
                 }
             }
-            if (t < t1) {
-                char *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
-                lk.store(next);
-                lv.store(next + BYTES);
-            }
-            __syncthreads();
         }
+        __syncthreads();
     };
-    walk(std::false_type());
-    if (__syncthreads_or(active && has_nan<HDB>(acc))) walk(std::true_type());
-    if (active) store_columns<T, HDB>(dq + slab + mine, S, hd, acc, scale);
+    walk(false);
+    if (__syncthreads_or(active && has_nan<HDB>(acc))) {       // (see the forward kernel)
+        ks.load(lds, t0 * M::COLS, from, to);
+        vs.load(lds + BYTES, t0 * M::COLS, from, to);
+        walk(true);
+    }
+    store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + wave * (HDB * 64 + 16) * 32);
 }
 
 template <typename T>
@@ -125,18 +123,30 @@ int attn_bwd(const char *who, T *dq, T *dk, T *dv, const T *d_o, const T *q, con
     if (!dq || !dk || !dv || !d_o || !q || !k || !v || !o || !lse) return mi355_fail("%s: NULL pointer", who);
     if (!shape_ok(who, heads, kv_heads, hd, S, batch, scale)) return -1;
     const size_t n = (size_t)heads * batch;
-    float *delta = (float *)mi355_ws(n * S * sizeof(float));
-    if (!delta) return -1;
+    // Workspace: delta; the streamed tensors (k and v here, q and d_o in the launch for dk and dv) where their rows are no whole chunks, at
+    // the same place one after the other.
+    const size_t delta_bytes = (n * S * sizeof(float) + 255) & ~(size_t)255;
+    const bool pack_kv = !streams_directly(k, S) || !streams_directly(v, S), pack_q = !streams_directly(q, S) || !streams_directly(d_o, S);
+    const size_t packed = 2 * (packed_bytes<T>((size_t)batch * (pack_q ? heads : kv_heads) * hd, S));
+    char *ws = (char *)mi355_ws(delta_bytes + (pack_q || pack_kv ? packed : 0));
+    if (!ws) return -1;
+    float *delta = (float *)ws;
+    int pitch = S;
+    const T *ks = k, *vs = v;
+    if (pack_kv && pack_rows(who, &ks, &vs, (size_t)batch * kv_heads * hd, S, &pitch, ws + delta_bytes)) return -1;
     int rc = dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, heads, kv_heads, hd, scale, o, d_o,
-                                                                                       lse, dq, delta, batch, blocks);
+        attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, ks, vs, bounds, S, pitch, heads, kv_heads, hd,
+                                                                                       scale, o, d_o, lse, dq, delta, batch, blocks);
         LAUNCH_OK(who);
         return 0;
     });
     if (rc) return rc;
-    return mi355_attn_dkv(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, batch, scale);
+    pitch = S;
+    const T *qs = q, *gs = d_o;
+    if (pack_q && pack_rows(who, &qs, &gs, n * hd, S, &pitch, ws + delta_bytes)) return -1;
+    return mi355_attn_dkv(who, dk, dv, gs, qs, k, v, lse, delta, bounds, heads, kv_heads, hd, S, pitch, batch, scale);
 }
 
 }  // namespace

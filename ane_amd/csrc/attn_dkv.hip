@@ -5,14 +5,15 @@ namespace {
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------------
 
+// q and d_o have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                                                              const int *__restrict__ bounds, int S, int heads, int kv_heads, int hd,
-                                                              float scale, const T *__restrict__ d_o, const float *__restrict__ lse,
+                                                              const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+                                                              int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse,
                                                               const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
                                                               int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int KT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP, THREADS = WAVES * 64;
+    constexpr int KT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
     __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
     __shared__ __attribute__((aligned(16))) float rows[2][2][M::COLS];      // [buffer][lse * log2(e), delta][query]
     __shared__ int lasts[WAVES];
@@ -41,50 +42,45 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
 
     typename M::Frag kf[STEPS], vf[STEPS];
     own_columns<T, HDB, WAVES, STEPS>(kf, lds, k + slab, S, hd, k0, S);
-    own_columns<T, HDB, WAVES, STEPS>(vf, lds, v + slab, S, hd, k0, S);
+    own_columns<T, HDB, WAVES, STEPS>(vf, lds + 2 * BYTES, v + slab, S, hd, k0, S);
     const float scale2 = scale * LOG2E;
 
     v16f ak[HDB], av[HDB];
     const int t0 = k0 / M::COLS, tiles = (to - 1) / M::COLS - t0 + 1, steps = tiles * group;
-    auto walk = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    auto walk = [&](bool careful) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
-        PanelLoad<T, HDB * 32, THREADS> lq, lg;
+        PanelStream<T, HDB * 32, WAVES> qs, gs;
         float lr = 0.f;
         // tile i of the walk: a group's heads one after the other, each over its queries
-        auto load = [&](int g, int t) {
+        auto load = [&](int g, int t, int buf) {
             const size_t head = head0 + g;
-            lq.load(q + head * hd * S, S, hd, t * M::COLS, k0, to);
-            lg.load(d_o + head * hd * S, S, hd, t * M::COLS, k0, to);
             const int at_q = t * M::COLS + (int)(threadIdx.x & (M::COLS - 1));
             if (threadIdx.x < 2 * M::COLS)
                 lr = at_q < S ? (threadIdx.x < M::COLS ? lse[head * S + at_q] * LOG2E : delta[head * S + at_q]) : 0.f;
-        };
-        auto store = [&](int buf) {
             char *p = lds + buf * 2 * BYTES;
-            lq.store(p);
-            lg.store(p + BYTES);
+            qs.begin(q + head * hd * pitch, pitch, hd);
+            gs.begin(d_o + head * hd * pitch, pitch, hd);
+            qs.load(p, t * M::COLS, k0, to);
+            gs.load(p + BYTES, t * M::COLS, k0, to);
+        };
+        auto store_rows = [&](int buf) {
             if (threadIdx.x < 2 * M::COLS) rows[buf][threadIdx.x / M::COLS][threadIdx.x & (M::COLS - 1)] = lr;
         };
-        load(0, t0);
-        __syncthreads();
-        store(0);
-        __syncthreads();
+        load(0, t0, 0);
+        store_rows(0);
         int g_at = 0, t = t0;
         for (int i = 0; i < steps; i++) {
+            // what this tile needs is there; everybody is done with the tile before it
+            loads_and_barrier<0, 0>();
             const char *qp = lds + (i & 1) * 2 * BYTES, *gp = qp + BYTES;
             const int c0 = t * M::COLS;
             int g_next = g_at, t_next = t + 1;
             if (t_next == t0 + tiles) t_next = t0, g_next++;
-            if (i + 1 < steps) load(g_next, t_next);
+            if (i + 1 < steps) load(g_next, t_next, (i + 1) & 1);
             if (c0 + M::COLS > wk && c0 < wto) {
                 const bool masked = c0 < wk + 31 || c0 + M::COLS > wfull;
-                unsigned long long odd_q = 0, odd_g = 0;
-                if constexpr (CAREFUL) {
-                    odd_q = masked ? odd_columns<T, HDB * 32>(qp) : 0;
-                    odd_g = masked ? odd_columns<T, HDB * 32>(gp) : 0;
-                }
+                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
 #pragma unroll
                 for (int u = 0; u < M::SUBS; u++) {
                     v16f s = v16_zero(), g = v16_zero();
@@ -113,44 +109,44 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
                         }
                     }
                     const typename M::Packed ps = M::pack(s), pg = M::pack(g);
+                    if (odd) {
 #pragma unroll
-                    for (int d = 0; d < HDB; d++) {
-                        if (CAREFUL && odd_g) av[d] = M::template rows<true>(gp, d, u, ps, av[d]);
-                        else av[d] = M::template rows<false>(gp, d, u, ps, av[d]);
-                    }
-#pragma unroll
-                    for (int d = 0; d < HDB; d++) {
-                        if (CAREFUL && odd_q) ak[d] = M::template rows<true>(qp, d, u, pg, ak[d]);
-                        else ak[d] = M::template rows<false>(qp, d, u, pg, ak[d]);
-                    }
-                    if constexpr (CAREFUL) {
+                        for (int d = 0; d < HDB; d++) {
+                            av[d] = M::template rows<true>(gp, d, u, ps, av[d]);
+                            ak[d] = M::template rows<true>(qp, d, u, pg, ak[d]);
+                        }
                         auto ok = [&](int c) { return c0 + c >= mine && c0 + c < end; };
-                        if (odd_g) add_odd<T, HDB>(av, gp, u, s, odd_g, ok);
-                        if (odd_q) add_odd<T, HDB>(ak, qp, u, g, odd_q, ok);
+                        add_odd<T, HDB>(av, gp, u, s, odd, ok);
+                        add_odd<T, HDB>(ak, qp, u, g, odd, ok);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < HDB; d++) av[d] = M::template rows<false>(gp, d, u, ps, av[d]);
+#pragma unroll
+                        for (int d = 0; d < HDB; d++) ak[d] = M::template rows<false>(qp, d, u, pg, ak[d]);
                     }
                 }
             }
-            if (i + 1 < steps) store((i + 1) & 1);
+            if (i + 1 < steps) store_rows((i + 1) & 1);
             t = t_next;
             g_at = g_next;
-            __syncthreads();
         }
+        __syncthreads();
     };
-    walk(std::false_type());
-    if (__syncthreads_or(active && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) walk(std::true_type());
-    if (!active) return;
-    store_columns<T, HDB>(dk + slab + mine, S, hd, ak, scale);
-    store_columns<T, HDB>(dv + slab + mine, S, hd, av, 1.f);
+    walk(false);
+    if (__syncthreads_or(active && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) walk(true);        // (see the forward kernel)
+    char *mine_lds = lds + wave * (HDB * 64 + 16) * 32;
+    store_columns<T, HDB>(dk + slab, S, hd, ak, scale, wk, active, mine_lds);
+    store_columns<T, HDB>(dv + slab, S, hd, av, 1.f, wk, active, mine_lds);
 }
 
 template <typename T>
 int launch_dkv(const char *who, T *dk, T *dv, const T *d_o, const T *q, const T *k, const T *v, const float *lse, const float *delta,
-               const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale) {
+               const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale) {
     const size_t nk = (size_t)kv_heads * batch;
     return dispatch(hd, waves_for(nk, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_dkv_kernel<T, HDB, W><<<(unsigned)(blocks * nk), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, heads, kv_heads, hd, scale, d_o,
+        attn_dkv_kernel<T, HDB, W><<<(unsigned)(blocks * nk), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o,
                                                                                          lse, delta, dk, dv, batch, blocks);
         LAUNCH_OK(who);
         return 0;
@@ -161,10 +157,10 @@ int launch_dkv(const char *who, T *dk, T *dv, const T *d_o, const T *q, const T 
 }  // namespace
 
 int mi355_attn_dkv(const char *who, float *dk, float *dv, const float *d_o, const float *q, const float *k, const float *v, const float *lse,
-                   const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale) {
-    return launch_dkv<float>(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, batch, scale);
+                   const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale) {
+    return launch_dkv<float>(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, pitch, batch, scale);
 }
 int mi355_attn_dkv(const char *who, bf16_t *dk, bf16_t *dv, const bf16_t *d_o, const bf16_t *q, const bf16_t *k, const bf16_t *v,
-                   const float *lse, const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale) {
-    return launch_dkv<bf16_t>(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, batch, scale);
+                   const float *lse, const float *delta, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale) {
+    return launch_dkv<bf16_t>(who, dk, dv, d_o, q, k, v, lse, delta, bounds, heads, kv_heads, hd, S, pitch, batch, scale);
 }

@@ -5,12 +5,13 @@ namespace {
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 
+// k and v have `pitch` values between rows (PanelStream), q and o S.
 template <typename T, int HDB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                                                              const int *__restrict__ bounds, int S, int heads, int kv_heads, int hd,
-                                                              float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 2))) void attn_fwd_kernel(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
+    int kv_heads, int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP, THREADS = WAVES * 64;
+    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
     __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
     __shared__ int firsts[WAVES];
     const Place at = place(blocks, heads, batch, true);
@@ -34,39 +35,36 @@ __global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(const T *__restric
     if (from >= S) return;
     const int to = min(q0 + QT, S);
     const int kvh = at.h / (heads / kv_heads);
-    const T *kb = k + ((size_t)at.b * kv_heads + kvh) * hd * S, *vb = v + ((size_t)at.b * kv_heads + kvh) * hd * S;
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S;
+    PanelStream<T, HDB * 32, WAVES> ks, vs;
+    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
+    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
+    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
+    ks.load(lds, t0 * M::COLS, from, to);
+    vs.load(lds + BYTES, t0 * M::COLS, from, to);
 
     typename M::Frag qf[STEPS];
-    own_columns<T, HDB, WAVES, STEPS>(qf, lds, q + slab, S, hd, q0, S);
+    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, q + slab, S, hd, q0, S);
 
     v16f acc[HDB];
     float m, l;
-    const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
-    auto walk = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    auto walk = [&](bool careful) {
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
         for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        PanelLoad<T, HDB * 32, THREADS> lk, lv;
-        lk.load(kb, S, hd, t0 * M::COLS, from, to);
-        lv.load(vb, S, hd, t0 * M::COLS, from, to);
-        __syncthreads();                    // nobody reads the panels of an earlier walk any more
-        lk.store(lds);
-        lv.store(lds + BYTES);
-        __syncthreads();
         for (int t = t0; t <= t1; t++) {
-            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES;
+            // what this tile needs is there; everybody is done with the tile before it
+            loads_and_barrier<0, 0>();
+            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES, *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
             if (t < t1) {
-                lk.load(kb, S, hd, (t + 1) * M::COLS, from, to);
-                lv.load(vb, S, hd, (t + 1) * M::COLS, from, to);
+                ks.load(next, (t + 1) * M::COLS, from, to);
+                vs.load(next + BYTES, (t + 1) * M::COLS, from, to);
             }
             const int c0 = t * M::COLS;
             if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
                 const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-                unsigned long long odd = 0;
-                if constexpr (CAREFUL) odd = masked ? odd_columns<T, HDB * 32>(vp) : 0;
+                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(vp) : 0;
                 v16f s[M::SUBS];
                 float mx = -INFINITY;
 #pragma unroll
@@ -107,31 +105,30 @@ __global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(const T *__restric
                         l += s[u][r];
                     }
                     const typename M::Packed p = M::pack(s[u]);
+                    if (odd) {
 #pragma unroll
-                    for (int d = 0; d < HDB; d++) {
-                        if (CAREFUL && odd) acc[d] = M::template rows<true>(vp, d, u, p, acc[d]);
-                        else acc[d] = M::template rows<false>(vp, d, u, p, acc[d]);
-                    }
-                    if (CAREFUL && odd)
+                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<true>(vp, d, u, p, acc[d]);
                         add_odd<T, HDB>(acc, vp, u, s[u], odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<false>(vp, d, u, p, acc[d]);
+                    }
                 }
             }
-            if (t < t1) {
-                char *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
-                lk.store(next);
-                lv.store(next + BYTES);
-            }
-            __syncthreads();
         }
+        __syncthreads();
         l += lane_xor<32>(l);
     };
-    walk(std::false_type());
+    walk(false);
     // An infinity or a NaN among the values of keys that the mask hides makes 0 * inf of their weights: such rows are computed again,
     // with those values taken out of the product and added for the pairs that count.
-    if (__syncthreads_or(active && has_nan<HDB>(acc))) walk(std::true_type());
-    if (!active) return;
-    store_columns<T, HDB>(o + slab + mine, S, hd, acc, 1.f / l);
-    if (lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (__syncthreads_or(active && has_nan<HDB>(acc))) {
+        ks.load(lds, t0 * M::COLS, from, to);
+        vs.load(lds + BYTES, t0 * M::COLS, from, to);
+        walk(true);
+    }
+    store_columns<T, HDB>(o + slab, S, hd, acc, 1.f / l, wq, active, lds + wave * (HDB * 64 + 16) * 32);
+    if (active && lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---- the plan of packed rows ----------------------------------------------------------------------------------------------------
@@ -159,11 +156,17 @@ int attn_fwd(const char *who, T *o, float *lse, const T *q, const T *k, const T 
     if (!o || !q || !k || !v) return mi355_fail("%s: NULL pointer", who);
     if (!shape_ok(who, heads, kv_heads, hd, S, batch, scale)) return -1;
     const size_t n = (size_t)heads * batch;
+    int pitch = S;
+    if (!streams_directly(k, S) || !streams_directly(v, S)) {
+        const size_t rows = (size_t)batch * kv_heads * hd;
+        void *ws = mi355_ws(2 * packed_bytes<T>(rows, S));
+        if (!ws || pack_rows(who, &k, &v, rows, S, &pitch, ws)) return -1;
+    }
     return dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, heads, kv_heads, hd, scale * LOG2E,
-                                                                                        o, lse, batch, blocks);
+        attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd,
+                                                                                        scale * LOG2E, o, lse, batch, blocks);
         LAUNCH_OK(who);
         return 0;
     });

@@ -150,30 +150,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, float (&v)[8], int m, 
     }
 }
 
-// Rows and columns of a tensor on their way to LDS.  Loads go straight into LDS, 16 bytes a lane, the lanes of an instruction one after the
-// other (eight rows of a panel), so what panel_at() would put elsewhere is fetched by another lane instead.  The tensors are aligned:
-// base and S in units of eight values (repacked() brings others to that).  A read outside of the buffer gives zero.
-constexpr unsigned OUTSIDE = 0xfffffff0u;
-
-typedef int rsrc_t __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long bytes) {
-    const unsigned long long a = (unsigned long long)p;
-    return rsrc_t{(int)a, (int)(a >> 32) & 0xffff, (int)(unsigned)(bytes < 0xffffff00ull ? bytes : 0xffffff00ull), 0x00027000};
-}
-// lds[16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.  (With
-// the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0, which
-// no other instruction of these kernels needs, is set with it.
-__device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, const char *lds) {
-    const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds;
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(r), "s"(soffset), "s"(at) : "memory");
-}
-// All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
-template <int LEFT, int READS>
-__device__ __forceinline__ void loads_and_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" :: "n"(LEFT), "n"(READS) : "memory");
-}
-
+// Tensors go straight into LDS (load_to_lds).  They are aligned: base and S in units of eight values; repack() brings others to that.
 // An operand's 64 steps of the sum for B indexes.  COLUMNS: the sum goes over the rows: B / 64 panels of 64 rows x 64 columns; else over the
 // columns: one panel of B rows.
 template <int B, bool COLUMNS, int THREADS>

@@ -96,8 +96,12 @@ template <> struct Mma<bf16_t> {
     static __device__ __forceinline__ float value(const char *panel, int row, int col) {
         return bf_to_f(*reinterpret_cast<const bf16_t *>(panel + panel_at(row, col >> 3) + ((col & 7) << 1)));
     }
-    static __device__ __forceinline__ float widen(bf16_t v) { return bf_to_f(v); }
-    static __device__ __forceinline__ bf16_t narrow(float v) { return (bf16_t)f_to_bf(v); }
+    // c + the sum of a lane's products
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float c) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) c = __builtin_fmaf((float)a[j], (float)b[j], c);
+        return c;
+    }
 };
 
 template <> struct Mma<float> {
@@ -127,56 +131,30 @@ template <> struct Mma<float> {
     static __device__ __forceinline__ float value(const char *panel, int row, int col) {
         return *reinterpret_cast<const float *>(panel + panel_at(row, col >> 2) + ((col & 3) << 2));
     }
-    static __device__ __forceinline__ float widen(float v) { return v; }
-    static __device__ __forceinline__ float narrow(float v) { return v; }
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float c) { return __builtin_fmaf(a, b, c); }
 };
 
-// A panel of ROWS rows on its way from memory to LDS: the chunks of one thread.  src: row 0, column 0 of a tensor with `pitch` values
-// between rows; columns [lo, hi) and rows below `rows` are read, the others become zero.
-template <typename T, int ROWS, int THREADS>
-struct PanelLoad {
-    static constexpr int N = ROWS * 8 / THREADS;
-    static_assert(N * THREADS == ROWS * 8, "whole chunks per thread");
-    v4u w[N];
-    __device__ __forceinline__ void load(const T *src, size_t pitch, int rows, int col0, int lo, int hi) {
-        typedef Mma<T> M;
-        const bool whole = rows >= ROWS && col0 >= lo && col0 + M::COLS <= hi;       // the same for every thread
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int t = threadIdx.x + i * THREADS;
-                const T *p = src + (size_t)(t >> 3) * pitch + col0 + (t & 7) * M::EPC;
-                w[i] = *reinterpret_cast<const typename M::Any16 *>(p);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int t = threadIdx.x + i * THREADS, row = t >> 3, col = col0 + (t & 7) * M::EPC;
-                v4u v = {0u, 0u, 0u, 0u};
-                if (row < rows) {
-                    const T *p = src + (size_t)row * pitch + col;
-                    if (col >= lo && col + M::EPC <= hi) v = *reinterpret_cast<const typename M::Any16 *>(p);
-                    else if (col < hi && col + M::EPC > lo) {
-                        unsigned e[M::EPC];
-#pragma unroll
-                        for (int j = 0; j < M::EPC; j++) e[j] = col + j >= lo && col + j < hi ? bits(p[j]) : 0u;
-                        if constexpr (M::EPC == 4) v = v4u{e[0], e[1], e[2], e[3]};
-                        else v = v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
-                    }
-                }
-                w[i] = v;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(char *panel) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int t = threadIdx.x + i * THREADS;
-            *reinterpret_cast<v4u *>(panel + panel_at(t >> 3, t & 7)) = w[i];
-        }
-    }
+// ---- from memory straight into LDS ----
+// 16 bytes a lane, the lanes of an instruction one after the other (eight rows of a panel), so what panel_at() would put elsewhere is
+// fetched by another lane instead: lane l reads chunk (l & 7) ^ panel_swz(row) of row l / 8.  Addresses are multiples of 16 bytes.  A read
+// outside of the buffer gives zero.
+constexpr unsigned OUTSIDE = 0xfffffff0u;
 
-private:
-    static __device__ __forceinline__ unsigned bits(bf16_t v) { return v; }
-    static __device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
-};
+typedef int rsrc_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long bytes) {
+    const unsigned long long a = (unsigned long long)p;
+    return rsrc_t{(int)a, (int)(a >> 32) & 0xffff, (int)(unsigned)(bytes < 0xffffff00ull ? bytes : 0xffffff00ull), 0x00027000};
+}
+// lds[16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.  (With
+// the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0, which
+// no other instruction of these kernels needs, is set with it.
+__device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, const char *lds) {
+    const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds;
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(r), "s"(soffset), "s"(at) : "memory");
+}
+// All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
+template <int LEFT, int READS>
+__device__ __forceinline__ void loads_and_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" :: "n"(LEFT), "n"(READS) : "memory");
+}
