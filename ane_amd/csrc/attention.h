@@ -178,65 +178,97 @@ __device__ __forceinline__ void store_columns(T *dst, size_t pitch, int hd, cons
     }
 }
 
-// The 32 positions of this wave, of 32 * WAVES from col0 on, as fragments of a product over the channels.  bfloat16: through LDS, as many
-// panels of it as the positions fill; begins when all waves are done with that place, ends with a barrier.  fp32: a fragment is a value of
-// each lane, rows of 32 positions, straight from memory.
-template <typename T, int HDB, int WAVES, int STEPS>
-__device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], char *lds, const T *src, size_t pitch, int hd, int col0, int S) {
+// The 32 positions of this wave (number `pos` of POS side by side, from col0 on), as fragments of a product over the channels.  bfloat16:
+// through LDS, as many panels of it as the positions fill; begins when all waves are done with that place, ends with a barrier.  fp32: a
+// fragment is a value of each lane, rows of 32 positions, straight from memory.
+template <typename T, int HDB, int POS, int THREADS, int STEPS>
+__device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], char *lds, const T *src, size_t pitch, int hd, int col0, int S, int pos) {
     typedef Mma<T> M;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 4) {
-        const int col = col0 + wave * 32 + (lane & 31), h = lane >> 5;
+        const int col = col0 + pos * 32 + (lane & 31), h = lane >> 5;
         const T *p = src + (size_t)h * pitch + col;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) f[s] = col < S && 2 * s + h < hd ? p[(size_t)(2 * s) * pitch] : 0.f;
     } else {
-        constexpr int PANELS = (32 * WAVES + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
+        constexpr int PANELS = (32 * POS + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
 #pragma unroll
         for (int p = 0; p < PANELS; p++) {
-            PanelLoad<T, HDB * 32, WAVES * 64> ld;
+            PanelLoad<T, HDB * 32, THREADS> ld;
             ld.load(src, pitch, hd, col0 + p * M::COLS, 0, S);
             ld.store(lds + p * BYTES);
         }
         __syncthreads();
-        const char *panel = lds + (wave * 32 / M::COLS) * BYTES;
+        const char *panel = lds + (pos * 32 / M::COLS) * BYTES;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) f[s] = M::columns(panel, wave * 32 % M::COLS / 32, s);
+        for (int s = 0; s < STEPS; s++) f[s] = M::columns(panel, pos * 32 % M::COLS / 32, s);
         __syncthreads();
     }
 }
 
 // The panels of a head on their way into LDS, one after the other: columns col0 .. col0 + COLS, whole chunks outside of [from, to) and rows
-// from hd on zero.  `pitch` values between rows, a multiple of a chunk, as is the address of the first.
+// from hd on zero.  `pitch` values between rows, a multiple of a chunk, as is the address of the first.  Loaded by WAVES waves, of which
+// this is number `wave`.
 template <typename T, int ROWS, int WAVES>
 struct PanelStream {
     static constexpr int LOADS = ROWS / (8 * WAVES);
-    static_assert(LOADS * 8 * WAVES == ROWS && WAVES % 2 == 0, "whole instructions per wave, one swizzle for all of a lane's rows");
+    static_assert(LOADS * 8 * WAVES == ROWS, "whole instructions per wave");
     rsrc_t r;
-    unsigned voff, row_bytes;
-    int hd;
-    __device__ __forceinline__ void begin(const T *head, int pitch, int channels) {
-        const int row = threadIdx.x >> 3, chunk = (threadIdx.x & 7) ^ panel_swz(row);
+    unsigned voff, odd_voff, row_bytes;         // odd_voff: for one wave, whose rows of odd eights have another swizzle
+    int hd, row, wave;
+    __device__ __forceinline__ int chunk_of(int r) { return (threadIdx.x & 7) ^ panel_swz(r); }
+    __device__ __forceinline__ void begin(const T *head, int pitch, int channels, int wave_) {
+        wave = wave_;
+        row = wave * 8 + ((threadIdx.x & 63) >> 3);
         hd = channels;
         row_bytes = (unsigned)pitch * sizeof(T);
         r = buffer_at(head, (unsigned long long)channels * row_bytes);
-        voff = row * row_bytes + chunk * 16;
+        voff = row * row_bytes + chunk_of(row) * 16;
+        odd_voff = row * row_bytes + chunk_of(row + 8) * 16;
     }
     __device__ __forceinline__ void load(const char *panel, int col0, int from, int to) {
-        panel += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+        panel += wave * 1024;
         const unsigned soff = (unsigned)col0 * sizeof(T);
-        if (col0 >= from && col0 + Mma<T>::COLS <= to && hd == ROWS) {
+        const bool whole = col0 >= from && col0 + Mma<T>::COLS <= to && hd == ROWS;
 #pragma unroll
-            for (int j = 0; j < LOADS; j++) load_to_lds(r, voff, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
-        } else {
-            const int row = threadIdx.x >> 3, col = col0 + ((threadIdx.x & 7) ^ panel_swz(row)) * Mma<T>::EPC;
-            const bool in = col < to && col + Mma<T>::EPC > from;
-#pragma unroll
-            for (int j = 0; j < LOADS; j++)
-                load_to_lds(r, in && row + j * 8 * WAVES < hd ? voff : OUTSIDE, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
+        for (int j = 0; j < LOADS; j++) {
+            unsigned v = WAVES == 1 && (j & 1) ? odd_voff : voff;
+            if (!whole) {
+                const int at = row + j * 8 * WAVES, col = col0 + chunk_of(at) * Mma<T>::EPC;
+                v = at < hd && col < to && col + Mma<T>::EPC > from ? v : OUTSIDE;
+            }
+            load_to_lds(r, v, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
         }
     }
 };
+
+// The accumulators of a position's teams added up in the order of the teams; the first team ends with the sum.  Begins and ends with
+// everybody done with LDS.
+template <int HDB, int POS, int TEAMS>
+__device__ __forceinline__ void add_teams(v16f (&acc)[HDB], char *lds, int pos, int team) {
+    const int lane = threadIdx.x & 63;
+    auto at = [&](int t, int d, int r) { return reinterpret_cast<v4f *>(lds) + ((((t - 1) * POS + pos) * HDB + d) * 4 + r) * 64 + lane; };
+    if (team > 0) {
+#pragma unroll
+        for (int d = 0; d < HDB; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) *at(team, d, r) = v4f{acc[d][4 * r], acc[d][4 * r + 1], acc[d][4 * r + 2], acc[d][4 * r + 3]};
+    }
+    __syncthreads();
+    if (team == 0) {
+#pragma unroll
+        for (int t = 1; t < TEAMS; t++)
+#pragma unroll
+            for (int d = 0; d < HDB; d++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const v4f v = *at(t, d, r);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[d][4 * r + e] += v[e];
+                }
+    }
+    __syncthreads();
+}
 
 // Which position block of which head a workgroup has: blocks in the given order, heads of one KV group on one XCD where the heads deal
 // out evenly (their L2 then holds the group's keys and values once).
@@ -322,16 +354,22 @@ int pack_rows(const char *who, const T **a, const T **b, size_t rows, int S, int
     return 0;
 }
 
-// Waves (32 positions each) to a workgroup: four share the panels that they read, unless that leaves compute units without work.
+// How many waves of a workgroup stand side by side (32 positions each, sharing the panels that they read), and in how many teams, which
+// share the walk: team i takes every TEAMS-th tile of it, with panels of its own.  Four side by side where that gives every compute unit two
+// workgroups, else two by two, and where even that leaves compute units without work one position block to four teams.
 int waves_for(size_t heads_batch, int S) {
-    return ceil_div(S, 128) * heads_batch >= (size_t)g_ctx.num_cu ? 4 : 2;
+    if (ceil_div(S, 128) * heads_batch >= 2 * (size_t)g_ctx.num_cu) return 4;
+    return ceil_div(S, 64) * heads_batch >= (size_t)g_ctx.num_cu ? 2 : 1;
 }
+// Panels for two tiles of each team, or for one where two would not fit.
+constexpr int stages_for(int hdb, int teams) { return 2 * 2 * teams * hdb * 32 * PANEL_ROW <= 128 * 1024 ? 2 : 1; }
 
 template <typename F>
 int dispatch(int hd, int waves, F go) {
     auto by_waves = [&](auto hdb) {
         if (waves == 4) return go(hdb, std::integral_constant<int, 4>());
-        return go(hdb, std::integral_constant<int, 2>());
+        if (waves == 2) return go(hdb, std::integral_constant<int, 2>());
+        return go(hdb, std::integral_constant<int, 1>());
     };
     if (hd <= 64) return by_waves(std::integral_constant<int, 2>());
     if (hd <= 96) return by_waves(std::integral_constant<int, 3>());

@@ -6,18 +6,18 @@ namespace {
 // ---- backward: dq and delta -----------------------------------------------------------------------------------------------------
 
 // k and v have `pitch` values between rows (PanelStream), the others S.
-template <typename T, int HDB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 2))) void attn_dq_kernel(
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && POS == 4 ? 2 : 1))) void attn_dq_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
     int kv_heads, int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq,
     float *__restrict__ delta, int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
-    __shared__ int firsts[WAVES];
+    constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), QT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
+    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
+    __shared__ int firsts[POS];
     const Place at = place(blocks, heads, batch, true);
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
-    const int q0 = at.block * QT, wq = q0 + wave * 32, mine = wq + (lane & 31);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
+    const int q0 = at.block * QT, wq = q0 + pos * 32, mine = wq + (lane & 31);
     int start = S;
     if (mine < S) start = bounds ? max(bounds[(size_t)at.b * 2 * S + mine], 0) : 0;
     const bool active = mine < S && start <= mine;
@@ -27,11 +27,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
         wfull = uniform(wave_max_int(active ? start : 0));
     } else if (wq >= S) wfrom = S;
     int from = wfrom;
-    if constexpr (WAVES > 1) {
-        if (lane == 0) firsts[wave] = wfrom;
+    if constexpr (POS > 1) {
+        if (lane == 0 && team == 0) firsts[pos] = wfrom;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) from = min(from, uniform(firsts[w]));
+        for (int w = 0; w < POS; w++) from = min(from, uniform(firsts[w]));
     }
     if (from >= S) return;
     const int to = min(q0 + QT, S);
@@ -40,38 +40,47 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
     const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
 
     // delta from the fragments: two lanes share a query, each has half of the channels
+    char *second = STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds;
     typename M::Frag qf[STEPS], gf[STEPS];
-    own_columns<T, HDB, WAVES, STEPS>(gf, lds, d_o + slab, S, hd, q0, S);
-    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, o + slab, S, hd, q0, S);
+    own_columns<T, HDB, POS, 256, STEPS>(gf, lds, d_o + slab, S, hd, q0, S, pos);
+    own_columns<T, HDB, POS, 256, STEPS>(qf, second, o + slab, S, hd, q0, S, pos);
     float dlt = 0.f;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) dlt = M::dot(qf[i], gf[i], dlt);
     dlt += lane_xor<32>(dlt);
     const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
-    if (active && h == 0) delta[row + mine] = dlt;
+    if (active && h == 0 && team == 0) delta[row + mine] = dlt;
 
-    PanelStream<T, HDB * 32, WAVES> ks, vs;
-    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
-    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
-    ks.load(lds, t0 * M::COLS, from, to);
-    vs.load(lds + BYTES, t0 * M::COLS, from, to);
-    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, q + slab, S, hd, q0, S);
+    PanelStream<T, HDB * 32, POS> ks, vs;
+    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
+    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
+    // the team's tiles are t0 + team, + TEAMS, ...; its panels lie side by side, those of one stage behind those of the other
+    char *panels = lds + team * 2 * BYTES;
+    auto load = [&](int i) {
+        const int t = t0 + i * TEAMS + team;
+        if (t > t1) return;
+        ks.load(panels + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
+        vs.load(panels + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
+    };
+    constexpr bool EARLY = sizeof(T) == 4 || STAGES == 2;       // (own positions need the place of the second stage)
+    if (EARLY) load(0);
+    own_columns<T, HDB, POS, 256, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), q + slab, S, hd, q0, S, pos);
+    if (!EARLY) load(0);
     const float scale2 = scale * LOG2E;
 
     v16f acc[HDB];
     auto walk = [&](bool careful) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        for (int t = t0; t <= t1; t++) {
+        const int count = (t1 - t0) / TEAMS + 1;
+        for (int i = 0; i < count; i++) {
             // what this tile needs is there; everybody is done with the tile before it
             loads_and_barrier<0, 0>();
-            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES, *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
-            if (t < t1) {
-                ks.load(next, (t + 1) * M::COLS, from, to);
-                vs.load(next + BYTES, (t + 1) * M::COLS, from, to);
-            }
+            const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
+            if (STAGES == 2) load(i + 1);
+            const int t = t0 + i * TEAMS + team;
             const int c0 = t * M::COLS;
-            if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+            if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
                 const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
                 const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(kp) : 0;
 #pragma unroll
@@ -104,16 +113,21 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
                     }
                 }
             }
+            if (STAGES == 1) {
+                __syncthreads();
+                load(i + 1);
+            }
         }
         __syncthreads();
+        if constexpr (TEAMS > 1) add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
     };
     walk(false);
-    if (__syncthreads_or(active && has_nan<HDB>(acc))) {       // (see the forward kernel)
-        ks.load(lds, t0 * M::COLS, from, to);
-        vs.load(lds + BYTES, t0 * M::COLS, from, to);
+    if (__syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) {       // (see the forward kernel)
+        load(0);
         walk(true);
     }
-    store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + wave * (HDB * 64 + 16) * 32);
+    if (team > 0) return;
+    store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + pos * (HDB * 64 + 16) * 32);
 }
 
 template <typename T>
@@ -137,7 +151,7 @@ int attn_bwd(const char *who, T *dq, T *dk, T *dv, const T *d_o, const T *q, con
     int rc = dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, ks, vs, bounds, S, pitch, heads, kv_heads, hd,
+        attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), 256, 0, g_ctx.stream>>>(q, ks, vs, bounds, S, pitch, heads, kv_heads, hd,
                                                                                        scale, o, d_o, lse, dq, delta, batch, blocks);
         LAUNCH_OK(who);
         return 0;

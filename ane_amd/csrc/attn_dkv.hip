@@ -6,20 +6,20 @@ namespace {
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------------
 
 // q and d_o have `pitch` values between rows (PanelStream), the others S.
-template <typename T, int HDB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                               const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
                                                               int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse,
                                                               const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
                                                               int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int KT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
-    __shared__ __attribute__((aligned(16))) float rows[2][2][M::COLS];      // [buffer][lse * log2(e), delta][query]
-    __shared__ int lasts[WAVES];
+    constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), KT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
+    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
+    __shared__ __attribute__((aligned(16))) float rows[STAGES][TEAMS][2][M::COLS];      // [stage][team][lse * log2(e), delta][query]
+    __shared__ int lasts[POS];
     const Place at = place(blocks, kv_heads, batch, false);
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
-    const int k0 = at.block * KT, wk = k0 + wave * 32, mine = wk + (lane & 31);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
+    const int k0 = at.block * KT, wk = k0 + pos * 32, mine = wk + (lane & 31);
     int end = 0;
     if (mine < S) end = bounds ? min(bounds[((size_t)at.b * 2 + 1) * S + mine], S) : S;
     const bool active = mine < S && end > mine;
@@ -29,11 +29,11 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
         wfull = uniform(wave_min_int(active ? end : S));
     } else if (wk >= S) wto = 0;
     int to = wto;
-    if constexpr (WAVES > 1) {
-        if (lane == 0) lasts[wave] = wto;
+    if constexpr (POS > 1) {
+        if (lane == 0 && team == 0) lasts[pos] = wto;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) to = max(to, uniform(lasts[w]));
+        for (int w = 0; w < POS; w++) to = max(to, uniform(lasts[w]));
     }
     if (to <= k0) return;
     const int group = heads / kv_heads;
@@ -41,43 +41,50 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
     const size_t head0 = (size_t)at.b * heads + (size_t)at.h * group;
 
     typename M::Frag kf[STEPS], vf[STEPS];
-    own_columns<T, HDB, WAVES, STEPS>(kf, lds, k + slab, S, hd, k0, S);
-    own_columns<T, HDB, WAVES, STEPS>(vf, lds + 2 * BYTES, v + slab, S, hd, k0, S);
+    own_columns<T, HDB, POS, 256, STEPS>(kf, lds, k + slab, S, hd, k0, S, pos);
+    own_columns<T, HDB, POS, 256, STEPS>(vf, STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds, v + slab, S, hd, k0, S, pos);
     const float scale2 = scale * LOG2E;
 
     v16f ak[HDB], av[HDB];
     const int t0 = k0 / M::COLS, tiles = (to - 1) / M::COLS - t0 + 1, steps = tiles * group;
+    const int count = (steps + TEAMS - 1) / TEAMS;
+    char *panels = lds + team * 2 * BYTES;
     auto walk = [&](bool careful) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
-        PanelStream<T, HDB * 32, WAVES> qs, gs;
-        float lr = 0.f;
-        // tile i of the walk: a group's heads one after the other, each over its queries
-        auto load = [&](int g, int t, int buf) {
-            const size_t head = head0 + g;
-            const int at_q = t * M::COLS + (int)(threadIdx.x & (M::COLS - 1));
-            if (threadIdx.x < 2 * M::COLS)
-                lr = at_q < S ? (threadIdx.x < M::COLS ? lse[head * S + at_q] * LOG2E : delta[head * S + at_q]) : 0.f;
-            char *p = lds + buf * 2 * BYTES;
-            qs.begin(q + head * hd * pitch, pitch, hd);
-            gs.begin(d_o + head * hd * pitch, pitch, hd);
+        PanelStream<T, HDB * 32, POS> qs, gs;
+        float lr[2] = {0.f, 0.f};
+        // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
+        // lse and delta a thread loads goes to LDS when the tile before is done.
+        int head = team / tiles, tile = team % tiles;           // of the load to come
+        auto load = [&](int stage) {
+            if (head >= group) return;
+            const size_t hh = head0 + head;
+            const int t = t0 + tile, at_q = t * M::COLS + lane;
+            if (pos == 0) {
+                lr[0] = lane < M::COLS && at_q < S ? lse[hh * S + at_q] * LOG2E : 0.f;
+                lr[1] = lane < M::COLS && at_q < S ? delta[hh * S + at_q] : 0.f;
+            }
+            char *p = panels + stage * (TEAMS * 2 * BYTES);
+            qs.begin(q + hh * hd * pitch, pitch, hd, pos);
+            gs.begin(d_o + hh * hd * pitch, pitch, hd, pos);
             qs.load(p, t * M::COLS, k0, to);
             gs.load(p + BYTES, t * M::COLS, k0, to);
         };
-        auto store_rows = [&](int buf) {
-            if (threadIdx.x < 2 * M::COLS) rows[buf][threadIdx.x / M::COLS][threadIdx.x & (M::COLS - 1)] = lr;
+        auto store_rows = [&](int stage) {
+            if (pos == 0 && lane < M::COLS) rows[stage][team][0][lane] = lr[0], rows[stage][team][1][lane] = lr[1];
         };
-        load(0, t0, 0);
+        load(0);
         store_rows(0);
-        int g_at = 0, t = t0;
-        for (int i = 0; i < steps; i++) {
+        for (int i = 0; i < count; i++) {
             // what this tile needs is there; everybody is done with the tile before it
             loads_and_barrier<0, 0>();
-            const char *qp = lds + (i & 1) * 2 * BYTES, *gp = qp + BYTES;
-            const int c0 = t * M::COLS;
-            int g_next = g_at, t_next = t + 1;
-            if (t_next == t0 + tiles) t_next = t0, g_next++;
-            if (i + 1 < steps) load(g_next, t_next, (i + 1) & 1);
+            const char *qp = panels + i % STAGES * (TEAMS * 2 * BYTES), *gp = qp + BYTES;
+            const float *ls_row = rows[i % STAGES][team][0], *dl_row = rows[i % STAGES][team][1];
+            const int c0 = head < group ? (t0 + tile) * M::COLS : to;
+            tile += TEAMS;
+            while (tile >= tiles && head < group) tile -= tiles, head++;
+            if (STAGES == 2) load((i + 1) % STAGES);
             if (c0 + M::COLS > wk && c0 < wto) {
                 const bool masked = c0 < wk + 31 || c0 + M::COLS > wfull;
                 const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
@@ -90,8 +97,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
                     for (int j = 0; j < STEPS; j++) g = M::mul(M::columns(gp, u, j), vf[j], g);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const v4f ls = *reinterpret_cast<const v4f *>(&rows[i & 1][0][u * 32 + 8 * j + 4 * h]);
-                        const v4f dl = *reinterpret_cast<const v4f *>(&rows[i & 1][1][u * 32 + 8 * j + 4 * h]);
+                        const v4f ls = *reinterpret_cast<const v4f *>(ls_row + u * 32 + 8 * j + 4 * h);
+                        const v4f dl = *reinterpret_cast<const v4f *>(dl_row + u * 32 + 8 * j + 4 * h);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int r = 4 * j + e;
@@ -126,15 +133,22 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(const T *__restric
                     }
                 }
             }
-            if (i + 1 < steps) store_rows((i + 1) & 1);
-            t = t_next;
-            g_at = g_next;
+            if (STAGES == 1) {
+                __syncthreads();
+                load(0);
+            }
+            store_rows((i + 1) % STAGES);
         }
         __syncthreads();
+        if constexpr (TEAMS > 1) {
+            add_teams<HDB, POS, TEAMS>(ak, lds, pos, team);
+            add_teams<HDB, POS, TEAMS>(av, lds, pos, team);
+        }
     };
     walk(false);
-    if (__syncthreads_or(active && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) walk(true);        // (see the forward kernel)
-    char *mine_lds = lds + wave * (HDB * 64 + 16) * 32;
+    if (__syncthreads_or(active && team == 0 && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) walk(true);       // (see the forward kernel)
+    if (team > 0) return;
+    char *mine_lds = lds + pos * (HDB * 64 + 16) * 32;
     store_columns<T, HDB>(dk + slab, S, hd, ak, scale, wk, active, mine_lds);
     store_columns<T, HDB>(dv + slab, S, hd, av, 1.f, wk, active, mine_lds);
 }
@@ -146,7 +160,7 @@ int launch_dkv(const char *who, T *dk, T *dv, const T *d_o, const T *q, const T 
     return dispatch(hd, waves_for(nk, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_dkv_kernel<T, HDB, W><<<(unsigned)(blocks * nk), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o,
+        attn_dkv_kernel<T, HDB, W><<<(unsigned)(blocks * nk), 256, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o,
                                                                                          lse, delta, dk, dv, batch, blocks);
         LAUNCH_OK(who);
         return 0;

@@ -6,17 +6,17 @@ namespace {
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 
 // k and v have `pitch` values between rows (PanelStream), q and o S.
-template <typename T, int HDB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 2))) void attn_fwd_kernel(
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && POS == 4 ? 2 : 1))) void attn_fwd_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
     int kv_heads, int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
     typedef Mma<T> M;
-    constexpr int QT = 32 * WAVES, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
-    __shared__ int firsts[WAVES];
+    constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), QT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
+    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
+    __shared__ int firsts[POS];
     const Place at = place(blocks, heads, batch, true);
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
-    const int q0 = at.block * QT, wq = q0 + wave * 32, mine = wq + (lane & 31);
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
+    const int q0 = at.block * QT, wq = q0 + pos * 32, mine = wq + (lane & 31);
     int start = S;
     if (mine < S) start = bounds ? max(bounds[(size_t)at.b * 2 * S + mine], 0) : 0;
     const bool active = mine < S && start <= mine;
@@ -26,25 +26,34 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
         wfull = uniform(wave_max_int(active ? start : 0));
     } else if (wq >= S) wfrom = S;
     int from = wfrom;
-    if constexpr (WAVES > 1) {
-        if (lane == 0) firsts[wave] = wfrom;
+    if constexpr (POS > 1) {
+        if (lane == 0 && team == 0) firsts[pos] = wfrom;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) from = min(from, uniform(firsts[w]));
+        for (int w = 0; w < POS; w++) from = min(from, uniform(firsts[w]));
     }
     if (from >= S) return;
     const int to = min(q0 + QT, S);
     const int kvh = at.h / (heads / kv_heads);
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S;
-    PanelStream<T, HDB * 32, WAVES> ks, vs;
-    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
-    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd);
+    PanelStream<T, HDB * 32, POS> ks, vs;
+    ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
+    vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
     const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
-    ks.load(lds, t0 * M::COLS, from, to);
-    vs.load(lds + BYTES, t0 * M::COLS, from, to);
+    // the team's tiles are t0 + team, + TEAMS, ...; its panels lie side by side, those of one stage behind those of the other
+    char *panels = lds + team * 2 * BYTES;
+    auto load = [&](int i) {
+        const int t = t0 + i * TEAMS + team;
+        if (t > t1) return;
+        ks.load(panels + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
+        vs.load(panels + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
+    };
+    constexpr bool EARLY = sizeof(T) == 4 || STAGES == 2;       // (own positions need the place of the second stage)
+    if (EARLY) load(0);
 
     typename M::Frag qf[STEPS];
-    own_columns<T, HDB, WAVES, STEPS>(qf, lds + 2 * BYTES, q + slab, S, hd, q0, S);
+    own_columns<T, HDB, POS, 256, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), q + slab, S, hd, q0, S, pos);
+    if (!EARLY) load(0);
 
     v16f acc[HDB];
     float m, l;
@@ -53,16 +62,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
         l = 0.f;
 #pragma unroll
         for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        for (int t = t0; t <= t1; t++) {
+        const int count = (t1 - t0) / TEAMS + 1;
+        for (int i = 0; i < count; i++) {
             // what this tile needs is there; everybody is done with the tile before it
             loads_and_barrier<0, 0>();
-            const char *kp = lds + ((t - t0) & 1) * 2 * BYTES, *vp = kp + BYTES, *next = lds + ((t + 1 - t0) & 1) * 2 * BYTES;
-            if (t < t1) {
-                ks.load(next, (t + 1) * M::COLS, from, to);
-                vs.load(next + BYTES, (t + 1) * M::COLS, from, to);
-            }
+            const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
+            if (STAGES == 2) load(i + 1);
+            const int t = t0 + i * TEAMS + team;
             const int c0 = t * M::COLS;
-            if (c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+            if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
                 const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
                 const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(vp) : 0;
                 v16f s[M::SUBS];
@@ -115,19 +123,44 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
                     }
                 }
             }
+            if (STAGES == 1) {
+                __syncthreads();
+                load(i + 1);
+            }
         }
         __syncthreads();
         l += lane_xor<32>(l);
+        if constexpr (TEAMS > 1) {          // brought to the largest of the teams' maxima, then added up
+            float *ms = reinterpret_cast<float *>(lds);
+            ms[(wave * 64 + lane) * 2] = m;
+            ms[(wave * 64 + lane) * 2 + 1] = l;
+            __syncthreads();
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < TEAMS; w++) top = fmaxf(top, ms[((w * POS + pos) * 64 + lane) * 2]);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < TEAMS; w++) sum += ms[((w * POS + pos) * 64 + lane) * 2 + 1] * __builtin_amdgcn_exp2f(ms[((w * POS + pos) * 64 + lane) * 2] - base);
+            const float f = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l = sum;
+#pragma unroll
+            for (int d = 0; d < HDB; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[d][r] *= f;
+            __syncthreads();
+            add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
+        }
     };
     walk(false);
     // An infinity or a NaN among the values of keys that the mask hides makes 0 * inf of their weights: such rows are computed again,
     // with those values taken out of the product and added for the pairs that count.
-    if (__syncthreads_or(active && has_nan<HDB>(acc))) {
-        ks.load(lds, t0 * M::COLS, from, to);
-        vs.load(lds + BYTES, t0 * M::COLS, from, to);
+    if (__syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) {
+        load(0);
         walk(true);
     }
-    store_columns<T, HDB>(o + slab, S, hd, acc, 1.f / l, wq, active, lds + wave * (HDB * 64 + 16) * 32);
+    if (team > 0) return;
+    store_columns<T, HDB>(o + slab, S, hd, acc, 1.f / l, wq, active, lds + pos * (HDB * 64 + 16) * 32);
     if (active && lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
@@ -165,7 +198,7 @@ int attn_fwd(const char *who, T *o, float *lse, const T *q, const T *k, const T 
     return dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
-        attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), W * 64, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd,
+        attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), 256, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd,
                                                                                         scale * LOG2E, o, lse, batch, blocks);
         LAUNCH_OK(who);
         return 0;

@@ -150,8 +150,10 @@ __device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long by
 // the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0, which
 // no other instruction of these kernels needs, is set with it.
 __device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, const char *lds) {
-    const unsigned at = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)lds;
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(r), "s"(soffset), "s"(at) : "memory");
+    auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };        // (nothing, where the compiler sees it by itself)
+    const int at = uni((int)(unsigned long long)(__attribute__((address_space(3))) const char *)lds), so = uni((int)soffset);
+    const rsrc_t u = {uni(r[0]), uni(r[1]), uni(r[2]), uni(r[3])};
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(u), "s"(so), "s"(at) : "memory");
 }
 // All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
 template <int LEFT, int READS>
