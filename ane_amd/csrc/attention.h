@@ -226,18 +226,20 @@ struct PanelStream {
         voff = row * row_bytes + chunk_of(row) * 16;
         odd_voff = row * row_bytes + chunk_of(row + 8) * 16;
     }
-    __device__ __forceinline__ void load(const char *panel, int col0, int from, int to) {
+    __device__ __forceinline__ void load(unsigned panel, int col0, int from, int to) {
         panel += wave * 1024;
         const unsigned soff = (unsigned)col0 * sizeof(T);
-        const bool whole = col0 >= from && col0 + Mma<T>::COLS <= to && hd == ROWS;
+        if (col0 >= from && col0 + Mma<T>::COLS <= to && hd == ROWS) {
 #pragma unroll
-        for (int j = 0; j < LOADS; j++) {
-            unsigned v = WAVES == 1 && (j & 1) ? odd_voff : voff;
-            if (!whole) {
+            for (int j = 0; j < LOADS; j++)
+                load_to_lds(r, WAVES == 1 && (j & 1) ? odd_voff : voff, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < LOADS; j++) {
                 const int at = row + j * 8 * WAVES, col = col0 + chunk_of(at) * Mma<T>::EPC;
-                v = at < hd && col < to && col + Mma<T>::EPC > from ? v : OUTSIDE;
+                const unsigned v = WAVES == 1 && (j & 1) ? odd_voff : voff;
+                load_to_lds(r, at < hd && col < to && col + Mma<T>::EPC > from ? v : OUTSIDE, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
             }
-            load_to_lds(r, v, soff + j * 8 * WAVES * row_bytes, panel + j * WAVES * 1024);
         }
     }
 };

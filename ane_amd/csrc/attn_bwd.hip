@@ -55,12 +55,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
     vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
     // the team's tiles are t0 + team, + TEAMS, ...; its panels lie side by side, those of one stage behind those of the other
-    char *panels = lds + team * 2 * BYTES;
-    auto load = [&](int i) {
+    const char *panels = lds + team * 2 * BYTES;
+    const unsigned place = lds_place(lds) + team * 2 * BYTES;
+    auto load = [&](int i) __attribute__((always_inline)) {
         const int t = t0 + i * TEAMS + team;
         if (t > t1) return;
-        ks.load(panels + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
-        vs.load(panels + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
+        ks.load(place + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
+        vs.load(place + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
     };
     constexpr bool EARLY = sizeof(T) == 4 || STAGES == 2;       // (own positions need the place of the second stage)
     if (EARLY) load(0);
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const float scale2 = scale * LOG2E;
 
     v16f acc[HDB];
-    auto walk = [&](bool careful) {
+    auto walk = [&](bool careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
         const int count = (t1 - t0) / TEAMS + 1;

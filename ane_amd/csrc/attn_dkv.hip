@@ -48,8 +48,9 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, 
     v16f ak[HDB], av[HDB];
     const int t0 = k0 / M::COLS, tiles = (to - 1) / M::COLS - t0 + 1, steps = tiles * group;
     const int count = (steps + TEAMS - 1) / TEAMS;
-    char *panels = lds + team * 2 * BYTES;
-    auto walk = [&](bool careful) {
+    const char *panels = lds + team * 2 * BYTES;
+    const unsigned place = lds_place(lds) + team * 2 * BYTES;
+    auto walk = [&](bool careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
         PanelStream<T, HDB * 32, POS> qs, gs;
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, 
         // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
         // lse and delta a thread loads goes to LDS when the tile before is done.
         int head = team / tiles, tile = team % tiles;           // of the load to come
-        auto load = [&](int stage) {
+        auto load = [&](int stage) __attribute__((always_inline)) {
             if (head >= group) return;
             const size_t hh = head0 + head;
             const int t = t0 + tile, at_q = t * M::COLS + lane;
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, 
                 lr[0] = lane < M::COLS && at_q < S ? lse[hh * S + at_q] * LOG2E : 0.f;
                 lr[1] = lane < M::COLS && at_q < S ? delta[hh * S + at_q] : 0.f;
             }
-            char *p = panels + stage * (TEAMS * 2 * BYTES);
+            const unsigned p = place + stage * (TEAMS * 2 * BYTES);
             qs.begin(q + hh * hd * pitch, pitch, hd, pos);
             gs.begin(d_o + hh * hd * pitch, pitch, hd, pos);
             qs.load(p, t * M::COLS, k0, to);

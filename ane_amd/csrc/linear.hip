@@ -192,7 +192,7 @@ struct Operand {
         }
     }
     // the next 64 steps of the sum, `left` of which exist, to a stage of LDS; moves on
-    __device__ __forceinline__ void load(const char *lds, int left) {
+    __device__ __forceinline__ void load(unsigned lds, int left) {
         lds += wave_at;
         if (even && left >= 64) {
 #pragma unroll
@@ -398,6 +398,7 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Ma
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave / WAVES_N * FM, wn = wave % WAVES_N * FN;
 
+    const unsigned place = lds_place(lds);
     A la;
     B lb;
     la.begin(a, m0, sum0);
@@ -405,8 +406,8 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Ma
 #pragma unroll
     for (int i = 0; i < STAGES - 1; i++)
         if (i < steps) {
-            la.load(lds + i * STAGE, sum1 - sum0 - i * 64);
-            lb.load(lds + i * STAGE + A::BYTES, sum1 - sum0 - i * 64);
+            la.load(place + i * STAGE, sum1 - sum0 - i * 64);
+            lb.load(place + i * STAGE + A::BYTES, sum1 - sum0 - i * 64);
         }
     v16f acc[FM][FN];
 #pragma unroll
@@ -437,8 +438,8 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Ma
         if (steps - i >= FULL) loads_and_barrier<LEFT, READS_LEFT>();
         else loads_and_barrier<0, READS_LEFT>();
         if (i + STAGES - 1 < steps) {
-            la.load(lds + next * STAGE, sum1 - sum0 - (i + STAGES - 1) * 64);
-            lb.load(lds + next * STAGE + A::BYTES, sum1 - sum0 - (i + STAGES - 1) * 64);
+            la.load(place + next * STAGE, sum1 - sum0 - (i + STAGES - 1) * 64);
+            lb.load(place + next * STAGE + A::BYTES, sum1 - sum0 - (i + STAGES - 1) * 64);
         }
         const char *p = lds + at * STAGE;
         at = at + 1 == STAGES ? 0 : at + 1;

@@ -146,14 +146,19 @@ __device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long by
     const unsigned long long a = (unsigned long long)p;
     return rsrc_t{(int)a, (int)(a >> 32) & 0xffff, (int)(unsigned)(bytes < 0xffffff00ull ? bytes : 0xffffff00ull), 0x00027000};
 }
-// lds[16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.  (With
-// the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0, which
-// no other instruction of these kernels needs, is set with it.
-__device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, const char *lds) {
+// Place in LDS, as loads to it are told: taken once from the array, then counted on as a number (each conversion of a pointer would compare
+// it with null).
+__device__ __forceinline__ unsigned lds_place(const char *array) {
+    return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const char *)array;
+}
+// LDS[place + 16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.
+// (With the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register; m0,
+// which no other instruction of these kernels needs, is set with it.
+__device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, unsigned place) {
     auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };        // (nothing, where the compiler sees it by itself)
-    const int at = uni((int)(unsigned long long)(__attribute__((address_space(3))) const char *)lds), so = uni((int)soffset);
     const rsrc_t u = {uni(r[0]), uni(r[1]), uni(r[2]), uni(r[3])};
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voffset), "s"(u), "s"(so), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :: "v"(voffset), "s"(u), "s"(uni((int)soffset)), "s"(uni((int)place)) : "memory");
 }
 // All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
 template <int LEFT, int READS>
