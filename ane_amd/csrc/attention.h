@@ -26,6 +26,14 @@ namespace {
 
 constexpr float LOG2E = 1.44269502162933349609375f, LN2 = 0.693147182464599609375f;
 
+typedef __attribute__((address_space(3))) char lds_char;
+
+// Panels for two tiles of each team, or for one where two would not fit; their bytes; and how many waves to a SIMD they leave room for.
+constexpr int stages_for(int hdb, int teams) { return 2 * 2 * teams * hdb * 32 * PANEL_ROW <= 128 * 1024 ? 2 : 1; }
+constexpr int panel_bytes(int hdb, int pos) { return 4 / pos * stages_for(hdb, 4 / pos) * 2 * hdb * 32 * PANEL_ROW; }
+template <typename T>
+constexpr int waves_per_simd(int hdb, int pos) { return panel_bytes(hdb, pos) <= 72 * 1024 && (sizeof(T) == 2 || hdb == 2) ? 2 : 1; }
+
 __device__ __forceinline__ int wave_min_int(int v) {
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) v = min(v, __shfl_xor(v, m, 64));
@@ -186,10 +194,15 @@ __device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], c
     typedef Mma<T> M;
     const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 4) {
-        const int col = col0 + pos * 32 + (lane & 31), h = lane >> 5;
-        const T *p = src + (size_t)h * pitch + col;
+        // as offsets into the head's rows: no load is behind a condition, or has an address of its own (positions behind the row's end: the
+        // last one again, whose results nobody keeps)
+        const int h = lane >> 5;
+        const unsigned row_bytes = (unsigned)pitch * 4, voff = h * row_bytes + min(col0 + pos * 32 + (lane & 31), S - 1) * 4;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(src), 0, (int)(hd * row_bytes), 0x00027000);
+        const bool whole = hd >= 2 * STEPS;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) f[s] = col < S && 2 * s + h < hd ? p[(size_t)(2 * s) * pitch] : 0.f;
+        for (int s = 0; s < STEPS; s++)
+            f[s] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)(whole || 2 * s + h < hd ? voff : OUTSIDE), (int)(2 * s * row_bytes), 0));
     } else {
         constexpr int PANELS = (32 * POS + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
 #pragma unroll
@@ -363,9 +376,6 @@ int waves_for(size_t heads_batch, int S) {
     if (ceil_div(S, 128) * heads_batch >= 2 * (size_t)g_ctx.num_cu) return 4;
     return ceil_div(S, 64) * heads_batch >= (size_t)g_ctx.num_cu ? 2 : 1;
 }
-// Panels for two tiles of each team, or for one where two would not fit.
-constexpr int stages_for(int hdb, int teams) { return 2 * 2 * teams * hdb * 32 * PANEL_ROW <= 128 * 1024 ? 2 : 1; }
-
 template <typename F>
 int dispatch(int hd, int waves, F go) {
     auto by_waves = [&](auto hdb) {

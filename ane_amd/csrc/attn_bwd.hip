@@ -5,16 +5,16 @@ namespace {
 
 // ---- backward: dq and delta -----------------------------------------------------------------------------------------------------
 
-// k and v have `pitch` values between rows (PanelStream), the others S.
-template <typename T, int HDB, int POS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && POS == 4 ? 2 : 1))) void attn_dq_kernel(
-    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
-    int kv_heads, int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq,
-    float *__restrict__ delta, int batch, int blocks) {
+// One position block; CAREFUL as in the forward pass.  k and v have `pitch` values between rows (PanelStream), the others S.
+template <typename T, int HDB, int POS, bool CAREFUL>
+__device__ __forceinline__ bool dq_block(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq, float *__restrict__ delta,
+    int batch, int blocks, lds_char *lds_) {
     typedef Mma<T> M;
     constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), QT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
-    __shared__ int firsts[POS];
+    char *lds = (char *)lds_;
+    int *firsts = reinterpret_cast<int *>(lds + TEAMS * STAGES * 2 * BYTES);
     const Place at = place(blocks, heads, batch, true);
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
     const int q0 = at.block * QT, wq = q0 + pos * 32, mine = wq + (lane & 31);
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
         for (int w = 0; w < POS; w++) from = min(from, uniform(firsts[w]));
     }
-    if (from >= S) return;
+    if (from >= S) return true;
     const int to = min(q0 + QT, S);
     const int kvh = at.h / (heads / kv_heads);
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S, row = ((size_t)at.b * heads + at.h) * S;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     own_columns<T, HDB, POS, 256, STEPS>(gf, lds, d_o + slab, S, hd, q0, S, pos);
     own_columns<T, HDB, POS, 256, STEPS>(qf, second, o + slab, S, hd, q0, S, pos);
     float dlt = 0.f;
-#pragma unroll
+    #pragma unroll
     for (int i = 0; i < STEPS; i++) dlt = M::dot(qf[i], gf[i], dlt);
     dlt += lane_xor<32>(dlt);
     const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
@@ -70,65 +70,70 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const float scale2 = scale * LOG2E;
 
     v16f acc[HDB];
-    auto walk = [&](bool careful) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        const int count = (t1 - t0) / TEAMS + 1;
-        for (int i = 0; i < count; i++) {
-            // what this tile needs is there; everybody is done with the tile before it
-            loads_and_barrier<0, 0>();
-            const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
-            if (STAGES == 2) load(i + 1);
-            const int t = t0 + i * TEAMS + team;
-            const int c0 = t * M::COLS;
-            if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
-                const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(kp) : 0;
+    for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
+    const int count = (t1 - t0) / TEAMS + 1;
+    for (int i = 0; i < count; i++) {
+        // what this tile needs is there; everybody is done with the tile before it
+        loads_and_barrier<0, 0>();
+        const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
+        if (STAGES == 2) load(i + 1);
+        const int t = t0 + i * TEAMS + team;
+        const int c0 = t * M::COLS;
+        if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+            const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
+            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(kp) : 0;
 #pragma unroll
-                for (int u = 0; u < M::SUBS; u++) {
-                    v16f s = v16_zero(), g = v16_zero();
+            for (int u = 0; u < M::SUBS; u++) {
+                v16f s = over_channels<T, STEPS>(kp, u, qf, v16_zero()), g = over_channels<T, STEPS>(vp, u, gf, v16_zero());
 #pragma unroll
-                    for (int i = 0; i < STEPS; i++) s = M::mul(M::columns(kp, u, i), qf[i], s);
-#pragma unroll
-                    for (int i = 0; i < STEPS; i++) g = M::mul(M::columns(vp, u, i), gf[i], g);
+                for (int r = 0; r < 16; r++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -lse2));
+                    s[r] = p * (g[r] - dlt);
+                }
+                if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -lse2));
-                        s[r] = p * (g[r] - dlt);
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int key = c0 + u * 32 + acc_row(r) + 4 * h;
-                            s[r] = key <= mine && key >= start ? s[r] : 0.f;
-                        }
-                    }
-                    const typename M::Packed p = M::pack(s);
-                    if (odd) {
-#pragma unroll
-                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<true>(kp, d, u, p, acc[d]);
-                        add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<false>(kp, d, u, p, acc[d]);
+                        const int key = c0 + u * 32 + acc_row(r) + 4 * h;
+                        s[r] = key <= mine && key >= start ? s[r] : 0.f;
                     }
                 }
-            }
-            if (STAGES == 1) {
-                __syncthreads();
-                load(i + 1);
+                const typename M::Packed p = M::pack(s);
+                if (odd) {
+                    over_positions<T, HDB, true>(acc, kp, u, p);
+                    add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                } else {
+                    over_positions<T, HDB, false>(acc, kp, u, p);
+                }
             }
         }
-        __syncthreads();
-        if constexpr (TEAMS > 1) add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
-    };
-    walk(false);
-    if (__syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) {       // (see the forward kernel)
-        load(0);
-        walk(true);
+        if (STAGES == 1) {
+            __syncthreads();
+            load(i + 1);
+        }
     }
-    if (team > 0) return;
-    store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + pos * (HDB * 64 + 16) * 32);
+    __syncthreads();
+    if constexpr (TEAMS > 1) add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
+    if (!CAREFUL && __syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) return false;
+    if (team == 0) store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + pos * (HDB * 64 + 16) * 32);
+    return true;
+}
+template <typename T, int HDB, int POS>
+__device__ __attribute__((noinline)) void dq_block_again(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq, float *__restrict__ delta,
+    int batch, int blocks, lds_char *lds) {
+    dq_block<T, HDB, POS, true>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, o, d_o, lse, dq, delta, batch, blocks, lds);
+}
+
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_per_simd<T>(HDB, POS)))) void attn_dq_kernel(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ o, const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq, float *__restrict__ delta,
+    int batch, int blocks) {
+    __shared__ __attribute__((aligned(16))) char lds[panel_bytes(HDB, POS) + 16];
+    if (!dq_block<T, HDB, POS, false>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, o, d_o, lse, dq, delta, batch, blocks, (lds_char *)lds))
+        dq_block_again<T, HDB, POS>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, o, d_o, lse, dq, delta, batch, blocks, (lds_char *)lds);
 }
 
 template <typename T>

@@ -5,18 +5,18 @@ namespace {
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------------
 
-// q and d_o have `pitch` values between rows (PanelStream), the others S.
-template <typename T, int HDB, int POS>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-                                                              const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
-                                                              int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse,
-                                                              const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
-                                                              int batch, int blocks) {
+// One position block; CAREFUL as in the forward pass.  q and d_o have `pitch` values between rows (PanelStream), the others S.
+template <typename T, int HDB, int POS, bool CAREFUL>
+__device__ __forceinline__ bool dkv_block(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse, const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
+    int batch, int blocks, lds_char *lds_) {
     typedef Mma<T> M;
     constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), KT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
-    __shared__ __attribute__((aligned(16))) float rows[STAGES][TEAMS][2][M::COLS];      // [stage][team][lse * log2(e), delta][query]
-    __shared__ int lasts[POS];
+    char *lds = (char *)lds_;
+    typedef float Rows[TEAMS][2][M::COLS];          // [team][lse * log2(e), delta][query], of a stage
+    Rows *rows = reinterpret_cast<Rows *>(lds + TEAMS * STAGES * 2 * BYTES);
+    int *lasts = reinterpret_cast<int *>(rows + STAGES);
     const Place at = place(blocks, kv_heads, batch, false);
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
     const int k0 = at.block * KT, wk = k0 + pos * 32, mine = wk + (lane & 31);
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, 
 #pragma unroll
         for (int w = 0; w < POS; w++) to = max(to, uniform(lasts[w]));
     }
-    if (to <= k0) return;
+    if (to <= k0) return true;
     const int group = heads / kv_heads;
     const size_t slab = ((size_t)at.b * kv_heads + at.h) * hd * S;
     const size_t head0 = (size_t)at.b * heads + (size_t)at.h * group;
@@ -50,108 +50,115 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const T *__restrict__ q, 
     const int count = (steps + TEAMS - 1) / TEAMS;
     const char *panels = lds + team * 2 * BYTES;
     const unsigned place = lds_place(lds) + team * 2 * BYTES;
-    auto walk = [&](bool careful) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
-        PanelStream<T, HDB * 32, POS> qs, gs;
-        float lr[2] = {0.f, 0.f};
-        // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
-        // lse and delta a thread loads goes to LDS when the tile before is done.
-        int head = team / tiles, tile = team % tiles;           // of the load to come
-        auto load = [&](int stage) __attribute__((always_inline)) {
-            if (head >= group) return;
-            const size_t hh = head0 + head;
-            const int t = t0 + tile, at_q = t * M::COLS + lane;
-            if (pos == 0) {
-                lr[0] = lane < M::COLS && at_q < S ? lse[hh * S + at_q] * LOG2E : 0.f;
-                lr[1] = lane < M::COLS && at_q < S ? delta[hh * S + at_q] : 0.f;
-            }
-            const unsigned p = place + stage * (TEAMS * 2 * BYTES);
-            qs.begin(q + hh * hd * pitch, pitch, hd, pos);
-            gs.begin(d_o + hh * hd * pitch, pitch, hd, pos);
-            qs.load(p, t * M::COLS, k0, to);
-            gs.load(p + BYTES, t * M::COLS, k0, to);
-        };
-        auto store_rows = [&](int stage) {
-            if (pos == 0 && lane < M::COLS) rows[stage][team][0][lane] = lr[0], rows[stage][team][1][lane] = lr[1];
-        };
-        load(0);
-        store_rows(0);
-        for (int i = 0; i < count; i++) {
-            // what this tile needs is there; everybody is done with the tile before it
-            loads_and_barrier<0, 0>();
-            const char *qp = panels + i % STAGES * (TEAMS * 2 * BYTES), *gp = qp + BYTES;
-            const float *ls_row = rows[i % STAGES][team][0], *dl_row = rows[i % STAGES][team][1];
-            const int c0 = head < group ? (t0 + tile) * M::COLS : to;
-            tile += TEAMS;
-            while (tile >= tiles && head < group) tile -= tiles, head++;
-            if (STAGES == 2) load((i + 1) % STAGES);
-            if (c0 + M::COLS > wk && c0 < wto) {
-                const bool masked = c0 < wk + 31 || c0 + M::COLS > wfull;
-                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
+    for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
+    PanelStream<T, HDB * 32, POS> qs, gs;
+    float lr[2] = {0.f, 0.f};
+    // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
+    // lse and delta a thread loads goes to LDS when the tile before is done.
+    int head = team / tiles, tile = team % tiles;           // of the load to come
+    auto load = [&](int stage) __attribute__((always_inline)) {
+        if (head >= group) return;
+        const size_t hh = head0 + head;
+        const int t = t0 + tile, at_q = t * M::COLS + lane;
+        if (pos == 0) {
+            lr[0] = lane < M::COLS && at_q < S ? lse[hh * S + at_q] * LOG2E : 0.f;
+            lr[1] = lane < M::COLS && at_q < S ? delta[hh * S + at_q] : 0.f;
+        }
+        const unsigned p = place + stage * (TEAMS * 2 * BYTES);
+        qs.begin(q + hh * hd * pitch, pitch, hd, pos);
+        gs.begin(d_o + hh * hd * pitch, pitch, hd, pos);
+        qs.load(p, t * M::COLS, k0, to);
+        gs.load(p + BYTES, t * M::COLS, k0, to);
+    };
+    auto store_rows = [&](int stage) {
+        if (pos == 0 && lane < M::COLS) rows[stage][team][0][lane] = lr[0], rows[stage][team][1][lane] = lr[1];
+    };
+    load(0);
+    store_rows(0);
+    for (int i = 0; i < count; i++) {
+        // what this tile needs is there; everybody is done with the tile before it
+        loads_and_barrier<0, 0>();
+        const char *qp = panels + i % STAGES * (TEAMS * 2 * BYTES), *gp = qp + BYTES;
+        const float *ls_row = rows[i % STAGES][team][0], *dl_row = rows[i % STAGES][team][1];
+        const int c0 = head < group ? (t0 + tile) * M::COLS : to;
+        tile += TEAMS;
+        while (tile >= tiles && head < group) tile -= tiles, head++;
+        if (STAGES == 2) load((i + 1) % STAGES);
+        if (c0 + M::COLS > wk && c0 < wto) {
+            const bool masked = c0 < wk + 31 || c0 + M::COLS > wfull;
+            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
 #pragma unroll
-                for (int u = 0; u < M::SUBS; u++) {
-                    v16f s = v16_zero(), g = v16_zero();
+            for (int u = 0; u < M::SUBS; u++) {
+                v16f s = over_channels<T, STEPS>(qp, u, kf, v16_zero()), g = over_channels<T, STEPS>(gp, u, vf, v16_zero());
 #pragma unroll
-                    for (int j = 0; j < STEPS; j++) s = M::mul(M::columns(qp, u, j), kf[j], s);
+                for (int j = 0; j < 4; j++) {
+                    const v4f ls = *reinterpret_cast<const v4f *>(ls_row + u * 32 + 8 * j + 4 * h);
+                    const v4f dl = *reinterpret_cast<const v4f *>(dl_row + u * 32 + 8 * j + 4 * h);
 #pragma unroll
-                    for (int j = 0; j < STEPS; j++) g = M::mul(M::columns(gp, u, j), vf[j], g);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const v4f ls = *reinterpret_cast<const v4f *>(ls_row + u * 32 + 8 * j + 4 * h);
-                        const v4f dl = *reinterpret_cast<const v4f *>(dl_row + u * 32 + 8 * j + 4 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int r = 4 * j + e;
-                            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -ls[e]));
-                            g[r] = s[r] * (g[r] - dl[e]);
-                        }
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int qq = c0 + u * 32 + acc_row(r) + 4 * h;
-                            const bool ok = qq >= mine && qq < end;
-                            s[r] = ok ? s[r] : 0.f;
-                            g[r] = ok ? g[r] : 0.f;
-                        }
-                    }
-                    const typename M::Packed ps = M::pack(s), pg = M::pack(g);
-                    if (odd) {
-#pragma unroll
-                        for (int d = 0; d < HDB; d++) {
-                            av[d] = M::template rows<true>(gp, d, u, ps, av[d]);
-                            ak[d] = M::template rows<true>(qp, d, u, pg, ak[d]);
-                        }
-                        auto ok = [&](int c) { return c0 + c >= mine && c0 + c < end; };
-                        add_odd<T, HDB>(av, gp, u, s, odd, ok);
-                        add_odd<T, HDB>(ak, qp, u, g, odd, ok);
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < HDB; d++) av[d] = M::template rows<false>(gp, d, u, ps, av[d]);
-#pragma unroll
-                        for (int d = 0; d < HDB; d++) ak[d] = M::template rows<false>(qp, d, u, pg, ak[d]);
+                    for (int e = 0; e < 4; e++) {
+                        const int r = 4 * j + e;
+                        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -ls[e]));
+                        g[r] = s[r] * (g[r] - dl[e]);
                     }
                 }
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int qq = c0 + u * 32 + acc_row(r) + 4 * h;
+                        const bool ok = qq >= mine && qq < end;
+                        s[r] = ok ? s[r] : 0.f;
+                        g[r] = ok ? g[r] : 0.f;
+                    }
+                }
+                const typename M::Packed ps = M::pack(s), pg = M::pack(g);
+                if (odd) {
+                    over_positions<T, HDB, true>(av, gp, u, ps);
+                    over_positions<T, HDB, true>(ak, qp, u, pg);
+                    auto ok = [&](int c) { return c0 + c >= mine && c0 + c < end; };
+                    add_odd<T, HDB>(av, gp, u, s, odd, ok);
+                    add_odd<T, HDB>(ak, qp, u, g, odd, ok);
+                } else {
+                    over_positions<T, HDB, false>(av, gp, u, ps);
+                    over_positions<T, HDB, false>(ak, qp, u, pg);
+                }
             }
-            if (STAGES == 1) {
-                __syncthreads();
-                load(0);
-            }
-            store_rows((i + 1) % STAGES);
         }
-        __syncthreads();
-        if constexpr (TEAMS > 1) {
-            add_teams<HDB, POS, TEAMS>(ak, lds, pos, team);
-            add_teams<HDB, POS, TEAMS>(av, lds, pos, team);
+        if (STAGES == 1) {
+            __syncthreads();
+            load(0);
         }
-    };
-    walk(false);
-    if (__syncthreads_or(active && team == 0 && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) walk(true);       // (see the forward kernel)
-    if (team > 0) return;
+        store_rows((i + 1) % STAGES);
+    }
+    __syncthreads();
+    if constexpr (TEAMS > 1) {
+        add_teams<HDB, POS, TEAMS>(ak, lds, pos, team);
+        add_teams<HDB, POS, TEAMS>(av, lds, pos, team);
+    }
+    if (!CAREFUL && __syncthreads_or(active && team == 0 && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) return false;
+    if (team > 0) return true;
     char *mine_lds = lds + pos * (HDB * 64 + 16) * 32;
     store_columns<T, HDB>(dk + slab, S, hd, ak, scale, wk, active, mine_lds);
     store_columns<T, HDB>(dv + slab, S, hd, av, 1.f, wk, active, mine_lds);
+    return true;
+}
+template <typename T, int HDB, int POS>
+__device__ __attribute__((noinline)) void dkv_block_again(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse, const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
+    int batch, int blocks, lds_char *lds) {
+    dkv_block<T, HDB, POS, true>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o, lse, delta, dk, dv, batch, blocks, lds);
+}
+
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) void attn_dkv_kernel(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse, const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
+    int batch, int blocks) {
+    constexpr int TEAMS = 4 / POS, ROWS = stages_for(HDB, TEAMS) * TEAMS * 2 * Mma<T>::COLS * 4;
+    __shared__ __attribute__((aligned(16))) char lds[panel_bytes(HDB, POS) + ROWS + 16];
+    if (!dkv_block<T, HDB, POS, false>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o, lse, delta, dk, dv, batch, blocks, (lds_char *)lds))
+        dkv_block_again<T, HDB, POS>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o, lse, delta, dk, dv, batch, blocks, (lds_char *)lds);
 }
 
 template <typename T>

@@ -5,15 +5,15 @@ namespace {
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 
-// k and v have `pitch` values between rows (PanelStream), q and o S.
-template <typename T, int HDB, int POS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && POS == 4 ? 2 : 1))) void attn_fwd_kernel(
-    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads,
-    int kv_heads, int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
+// One position block.  CAREFUL: see below; else false where that is needed.  k and v have `pitch` values between rows (PanelStream), q and o S.
+template <typename T, int HDB, int POS, bool CAREFUL>
+__device__ __forceinline__ bool fwd_block(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks, lds_char *lds_) {
     typedef Mma<T> M;
     constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), QT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
-    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * BYTES];
-    __shared__ int firsts[POS];
+    char *lds = (char *)lds_;
+    int *firsts = reinterpret_cast<int *>(lds + TEAMS * STAGES * 2 * BYTES);
     const Place at = place(blocks, heads, batch, true);
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6), pos = wave % POS, team = wave / POS;
     const int q0 = at.block * QT, wq = q0 + pos * 32, mine = wq + (lane & 31);
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 #pragma unroll
         for (int w = 0; w < POS; w++) from = min(from, uniform(firsts[w]));
     }
-    if (from >= S) return;
+    if (from >= S) return true;
     const int to = min(q0 + QT, S);
     const int kvh = at.h / (heads / kv_heads);
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S;
@@ -58,111 +58,119 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
     v16f acc[HDB];
     float m, l;
-    auto walk = [&](bool careful) __attribute__((always_inline)) {
-        m = -INFINITY;
-        l = 0.f;
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-        for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
-        const int count = (t1 - t0) / TEAMS + 1;
-        for (int i = 0; i < count; i++) {
-            // what this tile needs is there; everybody is done with the tile before it
-            loads_and_barrier<0, 0>();
-            const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
-            if (STAGES == 2) load(i + 1);
-            const int t = t0 + i * TEAMS + team;
-            const int c0 = t * M::COLS;
-            if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
-                const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-                const unsigned long long odd = careful && masked ? odd_columns<T, HDB * 32>(vp) : 0;
-                v16f s[M::SUBS];
-                float mx = -INFINITY;
+    for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
+    const int count = (t1 - t0) / TEAMS + 1;
+    for (int i = 0; i < count; i++) {
+        // what this tile needs is there; everybody is done with the tile before it
+        loads_and_barrier<0, 0>();
+        const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
+        if (STAGES == 2) load(i + 1);
+        const int t = t0 + i * TEAMS + team;
+        const int c0 = t * M::COLS;
+        if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
+            const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
+            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(vp) : 0;
+            v16f s[M::SUBS];
+            float mx = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < M::SUBS; u++) {
-                    s[u] = v16_zero();
-#pragma unroll
-                    for (int i = 0; i < STEPS; i++) s[u] = M::mul(M::columns(kp, u, i), qf[i], s[u]);
-                }
-                if (masked) {
-#pragma unroll
-                    for (int u = 0; u < M::SUBS; u++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int key = c0 + u * 32 + acc_row(r) + 4 * h;
-                            s[u][r] = key <= mine && key >= start ? s[u][r] : -INFINITY;
-                        }
-                }
+            for (int u = 0; u < M::SUBS; u++) {
+                s[u] = over_channels<T, STEPS>(kp, u, qf, v16_zero());
+            }
+            if (masked) {
 #pragma unroll
                 for (int u = 0; u < M::SUBS; u++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
-                mx = fmaxf(mx, lane_xor<32>(mx)) * scale2;
-                if (__any(mx > m)) {        // the running maximum moves: what is there is brought to the new one
-                    const float to_m = fmaxf(m, mx), f = to_m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to_m);
-                    l *= f;
-#pragma unroll
-                    for (int d = 0; d < HDB; d++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) acc[d][r] *= f;
-                    m = to_m;
-                }
-                const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                for (int u = 0; u < M::SUBS; u++) {
-#pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, -base));
-                        l += s[u][r];
+                        const int key = c0 + u * 32 + acc_row(r) + 4 * h;
+                        s[u][r] = key <= mine && key >= start ? s[u][r] : -INFINITY;
                     }
-                    const typename M::Packed p = M::pack(s[u]);
-                    if (odd) {
+            }
 #pragma unroll
-                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<true>(vp, d, u, p, acc[d]);
-                        add_odd<T, HDB>(acc, vp, u, s[u], odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
-                    } else {
+            for (int u = 0; u < M::SUBS; u++)
 #pragma unroll
-                        for (int d = 0; d < HDB; d++) acc[d] = M::template rows<false>(vp, d, u, p, acc[d]);
-                    }
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
+            mx = fmaxf(mx, lane_xor<32>(mx)) * scale2;
+            if (__any(mx > m)) {        // the running maximum moves: what is there is brought to the new one
+                const float to_m = fmaxf(m, mx), f = to_m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to_m);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < HDB; d++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[d][r] *= f;
+                m = to_m;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < M::SUBS; u++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, -base));
+                    l += s[u][r];
+                }
+                const typename M::Packed p = M::pack(s[u]);
+                if (odd) {
+                    over_positions<T, HDB, true>(acc, vp, u, p);
+                    add_odd<T, HDB>(acc, vp, u, s[u], odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
+                } else {
+                    over_positions<T, HDB, false>(acc, vp, u, p);
                 }
             }
-            if (STAGES == 1) {
-                __syncthreads();
-                load(i + 1);
-            }
         }
-        __syncthreads();
-        l += lane_xor<32>(l);
-        if constexpr (TEAMS > 1) {          // brought to the largest of the teams' maxima, then added up
-            float *ms = reinterpret_cast<float *>(lds);
-            ms[(wave * 64 + lane) * 2] = m;
-            ms[(wave * 64 + lane) * 2 + 1] = l;
+        if (STAGES == 1) {
             __syncthreads();
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < TEAMS; w++) top = fmaxf(top, ms[((w * POS + pos) * 64 + lane) * 2]);
-            const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int w = 0; w < TEAMS; w++) sum += ms[((w * POS + pos) * 64 + lane) * 2 + 1] * __builtin_amdgcn_exp2f(ms[((w * POS + pos) * 64 + lane) * 2] - base);
-            const float f = __builtin_amdgcn_exp2f(m - base);
-            m = top;
-            l = sum;
-#pragma unroll
-            for (int d = 0; d < HDB; d++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) acc[d][r] *= f;
-            __syncthreads();
-            add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
+            load(i + 1);
         }
-    };
-    walk(false);
-    // An infinity or a NaN among the values of keys that the mask hides makes 0 * inf of their weights: such rows are computed again,
-    // with those values taken out of the product and added for the pairs that count.
-    if (__syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) {
-        load(0);
-        walk(true);
     }
-    if (team > 0) return;
+    __syncthreads();
+    l += lane_xor<32>(l);
+    if constexpr (TEAMS > 1) {          // brought to the largest of the teams' maxima, then added up
+        float *ms = reinterpret_cast<float *>(lds);
+        ms[(wave * 64 + lane) * 2] = m;
+        ms[(wave * 64 + lane) * 2 + 1] = l;
+        __syncthreads();
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < TEAMS; w++) top = fmaxf(top, ms[((w * POS + pos) * 64 + lane) * 2]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < TEAMS; w++) sum += ms[((w * POS + pos) * 64 + lane) * 2 + 1] * __builtin_amdgcn_exp2f(ms[((w * POS + pos) * 64 + lane) * 2] - base);
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l = sum;
+#pragma unroll
+        for (int d = 0; d < HDB; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[d][r] *= f;
+        __syncthreads();
+        add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
+    }
+    if (!CAREFUL && __syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) return false;
+    if (team > 0) return true;
     store_columns<T, HDB>(o + slab, S, hd, acc, 1.f / l, wq, active, lds + pos * (HDB * 64 + 16) * 32);
     if (active && lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    return true;
+}
+
+// An infinity or a NaN among the values of positions that the mask hides makes 0 * inf of their weights.  A block that ends with a NaN is
+// computed again, with those values taken out of the products and added for the pairs that count.  It is a function of its own, for its
+// registers not to be the kernel's.
+template <typename T, int HDB, int POS>
+__device__ __attribute__((noinline)) void fwd_block_again(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks, lds_char *lds) {
+    fwd_block<T, HDB, POS, true>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale2, o, lse, batch, blocks, lds);
+}
+
+template <typename T, int HDB, int POS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_per_simd<T>(HDB, POS)))) void attn_fwd_kernel(
+    const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
+    int hd, float scale2, T *__restrict__ o, float *__restrict__ lse, int batch, int blocks) {
+    __shared__ __attribute__((aligned(16))) char lds[panel_bytes(HDB, POS) + 16];
+    if (!fwd_block<T, HDB, POS, false>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale2, o, lse, batch, blocks, (lds_char *)lds))
+        fwd_block_again<T, HDB, POS>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale2, o, lse, batch, blocks, (lds_char *)lds);
 }
 
 // ---- the plan of packed rows ----------------------------------------------------------------------------------------------------

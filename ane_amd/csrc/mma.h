@@ -74,17 +74,26 @@ template <> struct Mma<bf16_t> {
         }
         return out;
     }
-    // acc[row block][column] += sum over the panel's 32 columns `sub` of panel[row][.] * p[.][column]; FINITE: infinities and NaNs
-    // of the panel count as zero.
-    template <bool FINITE>
-    static __device__ __forceinline__ v16f rows(const char *panel, int block, int sub, const Packed &p, v16f acc) {
+    // The values of the panel's 32 columns `sub` at rows block*32 + lane%32, in the order of a product's registers.
+    struct Row { v8s v[2]; };
+    static __device__ __forceinline__ Row row(const char *panel, int block, int sub) {
         const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
         const char *at = panel + block * (32 * PANEL_ROW) + (h << 3);
+        Row out;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const v4s lo = *reinterpret_cast<const v4s *>(at + panel_at(row, sub * 4 + 2 * j));
             const v4s hi = *reinterpret_cast<const v4s *>(at + panel_at(row, sub * 4 + 2 * j + 1));
-            v8s v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            out.v[j] = v8s{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+        return out;
+    }
+    // acc[row][column] += sum over them of row[.] * p[.][column]; FINITE: infinities and NaNs of the panel count as zero.
+    template <bool FINITE>
+    static __device__ __forceinline__ v16f mul_row(const Row &r, const Packed &p, v16f acc) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            v8s v = r.v[j];
             if constexpr (FINITE) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
@@ -116,16 +125,21 @@ template <> struct Mma<float> {
     static __device__ __forceinline__ v16f mul(Frag a, Frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
     typedef v16f Packed;
     static __device__ __forceinline__ Packed pack(const v16f &p) { return p; }
-    template <bool FINITE>
-    static __device__ __forceinline__ v16f rows(const char *panel, int block, int, const Packed &p, v16f acc) {
+    struct Row { v4f v[4]; };
+    static __device__ __forceinline__ Row row(const char *panel, int block, int) {
         const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
         const char *at = panel + block * (32 * PANEL_ROW);
+        Row out;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const v4f v = *reinterpret_cast<const v4f *>(at + panel_at(row, 2 * j + h));
+        for (int j = 0; j < 4; j++) out.v[j] = *reinterpret_cast<const v4f *>(at + panel_at(row, 2 * j + h));
+        return out;
+    }
+    template <bool FINITE>
+    static __device__ __forceinline__ v16f mul_row(const Row &r, const Packed &p, v16f acc) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc = mul(FINITE && !is_finite(v[e]) ? 0.f : v[e], p[4 * j + e], acc);
-        }
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc = mul(FINITE && !is_finite(r.v[j][e]) ? 0.f : r.v[j][e], p[4 * j + e], acc);
         return acc;
     }
     static __device__ __forceinline__ float value(const char *panel, int row, int col) {
@@ -133,6 +147,42 @@ template <> struct Mma<float> {
     }
     static __device__ __forceinline__ float dot(Frag a, Frag b, float c) { return __builtin_fmaf(a, b, c); }
 };
+
+// acc + sum over the channels of panel[channel][sub*32 + .] * own[channel][.]: what a group of products takes is read while the group before
+// it is multiplied.  (Left alone, the compiler reads right before each product, or so far ahead that registers spill.)
+template <typename T, int STEPS>
+__device__ __forceinline__ v16f over_channels(const char *panel, int sub, const typename Mma<T>::Frag (&own)[STEPS], v16f acc) {
+    constexpr int GROUP = sizeof(T) == 2 ? 2 : 16, GROUPS = STEPS / GROUP;
+    static_assert(GROUPS * GROUP == STEPS, "whole groups");
+    typename Mma<T>::Frag f[2][GROUP];
+#pragma unroll
+    for (int i = 0; i < GROUP; i++) f[0][i] = Mma<T>::columns(panel, sub, i);
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        if (g + 1 < GROUPS) {
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) f[(g + 1) & 1][i] = Mma<T>::columns(panel, sub, (g + 1) * GROUP + i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < GROUP; i++) acc = Mma<T>::mul(f[g & 1][i], own[g * GROUP + i], acc);
+    }
+    return acc;
+}
+// acc[channel][.] += sum over the panel's 32 columns `sub` of panel[channel][.] * p[.][.], for all channels
+template <typename T, int HDB, bool FINITE>
+__device__ __forceinline__ void over_positions(v16f (&acc)[HDB], const char *panel, int sub, const typename Mma<T>::Packed &p) {
+    typename Mma<T>::Row r[2];
+    r[0] = Mma<T>::row(panel, 0, sub);
+#pragma unroll
+    for (int d = 0; d < HDB; d++) {
+        if (d + 1 < HDB) {
+            r[(d + 1) & 1] = Mma<T>::row(panel, d + 1, sub);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        acc[d] = Mma<T>::template mul_row<FINITE>(r[d & 1], p, acc[d]);
+    }
+}
 
 // ---- from memory straight into LDS ----
 // 16 bytes a lane, the lanes of an instruction one after the other (eight rows of a panel), so what panel_at() would put elsewhere is
