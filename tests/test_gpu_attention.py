@@ -168,3 +168,177 @@ def test_forward_and_gradients(br, i, storage):
     o, lse = forward(br, c)
     check(c, dict(o=o, lse=lse), reference(c))
     check(c, backward(br, c, o, lse), reference(c, o, lse))
+
+
+def test_plan(br):
+    cu = np.array([[0, 0, 3, 3, 10, 12], [2, 5, 5, 5, 9, 9], [0, 0, 0, 0, 0, 0]], np.int32)
+    c = Case("f32", 1, 1, 4, 12, 3, cu)
+    start, end = c.plan()
+    assert np.array_equal(plan_dev(br, c).numpy(), np.stack([start, end], 1))
+
+
+def test_plan_of_bad_offsets_stays_inside(br):
+    """Offsets that descend or leave the row give some plan, and one that the kernels can be run with."""
+    for cu in ([-5, 3, 900], [50, 10, 0], [7, 7, 2 ** 31 - 1], [-2 ** 31, -1, 5]):
+        c = Case("bf16", 2, 1, 64, 100, 1, [cu])
+        plan = plan_dev(br, c)
+        p = plan.numpy()
+        assert p.min() >= 0 and p.max() <= 100
+        o, lse = forward(br, c, bounds=plan)
+        backward(br, c, o, lse)
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hd,S,cu", [(64, 300, [[0, 70, 71, 200, 260]]), (128, 140, [[3, 40, 140]]), (96, 1030, [[0, 0, 1000]])])
+def test_what_the_mask_hides_is_not_seen(br, storage, bad, hd, S, cu):
+    """Infinities and NaNs in another sequence, behind the last one and in later positions leave a result as it is, to the bit."""
+    c = Case(storage, 4, 2, hd, S, 1, cu, seed=3)
+    lo, hi = cu[0][1], cu[0][2]         # the sequence that is looked at
+    late = hi - 5                       # its positions from here on are spoilt too
+    o, lse = forward(br, c)
+    seen = np.arange(lo, late)
+    spoilt = np.array([s for s in range(S) if s < lo or s >= late])
+    names = ("q", "k", "v", "do")
+    clean = {n: getattr(c, n).copy() for n in names}
+    for n in names:
+        a = clean[n].copy()
+        a[:, :, spoilt] = c.stored(np.full(1, bad))[0]
+        setattr(c, n, a)
+    o2, lse2 = forward(br, c)
+    assert np.array_equal(o2[:, :, seen], o[:, :, seen]) and np.array_equal(lse2[:, :, seen], lse[:, :, seen])
+    # gradients: dq of a position sees earlier ones only; dk and dv see later ones, so there the others alone are spoilt
+    for n in names:
+        setattr(c, n, clean[n])
+    g = backward(br, c, o, lse)
+    for n in names:
+        a = clean[n].copy()
+        a[:, :, spoilt] = c.stored(np.full(1, bad))[0]
+        setattr(c, n, a)
+    o_s, lse_s = o.copy(), lse.copy()
+    o_s[:, :, spoilt], lse_s[:, :, spoilt] = c.stored(np.full(1, bad))[0], bad
+    g2 = backward(br, c, o_s, lse_s)
+    assert np.array_equal(g2["dq"][:, :, seen], g["dq"][:, :, seen])
+    others = np.array([s for s in range(S) if s < lo or s >= hi])
+    for n in names:
+        a = clean[n].copy()
+        a[:, :, others] = c.stored(np.full(1, bad))[0]
+        setattr(c, n, a)
+    o_s, lse_s = o.copy(), lse.copy()
+    o_s[:, :, others], lse_s[:, :, others] = c.stored(np.full(1, bad))[0], bad
+    g3 = backward(br, c, o_s, lse_s)
+    for n in ("dq", "dk", "dv"):
+        assert np.array_equal(g3[n][:, :, lo:hi], g[n][:, :, lo:hi]), n
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_a_value_that_counts_is_seen(br, storage):
+    """A NaN among a sequence's own values reaches every position from there on, and none before; nor one head another's."""
+    c = Case(storage, 2, 2, 64, 100, 1, seed=4)
+    o, _ = forward(br, c)
+    c.v[0, 5, 60] = c.stored(np.full(1, np.nan))[0]
+    o2, _ = forward(br, c)
+    v2 = o2 if storage == "f32" else from_bf16(o2)
+    assert np.all(np.isnan(v2[0, 5, 60:])) and np.array_equal(o2[0, 5, :60], o[0, 5, :60])
+    rest = [r for r in range(128) if r != 5]
+    assert np.array_equal(o2[0, rest], o[0, rest])
+
+
+def test_scores_of_any_size(br):
+    """Scores whose exponentials overflow, and rows of equal ones."""
+    c = Case("f32", 1, 1, 64, 80, 1, seed=5, spread=12.0)       # scores in the hundreds
+    c.q[:, :, 10] = 0.0                                         # equal scores: the mean of the values
+    o, lse = forward(br, c)
+    assert np.all(np.isfinite(o)) and np.all(np.isfinite(lse))
+    assert np.allclose(o[0, :, 10], c.v[0, :, :11].mean(1), atol=1e-4 * 12)
+    want = reference(c)
+    check(c, dict(o=o, lse=lse), want)
+
+
+def test_gradients_match_differences(br):
+    """dq, dk, dv along random directions against differences of the loss <do, o> in 64 bits."""
+    c = Case("f32", 2, 1, 16, 40, 1, [[0, 25, 40]], seed=6)
+    o, lse = forward(br, c)
+    g = backward(br, c, o, lse)
+    rng = np.random.default_rng(7)
+
+    def loss(dq, dk, dv):
+        q, k, v = c.q.astype(np.float64) + dq, c.k.astype(np.float64) + dk, c.v.astype(np.float64) + dv
+        total, ok = 0.0, c.allowed(0)
+        for h in range(2):
+            rq = slice(16 * h, 16 * h + 16)
+            z = np.where(ok, c.scale * (q[0, rq].T @ k[0]), -np.inf)
+            e = np.exp(z - z.max(1, keepdims=True))
+            total += np.sum((e / e.sum(1, keepdims=True) @ v[0].T).T * c.do[0, rq])
+        return total
+
+    for n, shape in (("dq", c.q.shape), ("dk", c.k.shape), ("dv", c.v.shape)):
+        d = rng.standard_normal(shape)
+        arg = {m: d * (m == n) if m == n else 0.0 for m in ("dq", "dk", "dv")}
+        h = 1e-5
+        num = (loss(**{m: h * a for m, a in arg.items()}) - loss(**{m: -h * a for m, a in arg.items()})) / (2 * h)
+        # fp32 sums of the gradient against differences that are good to about h^2
+        assert abs(np.sum(g[n].astype(np.float64) * d) - num) < 2e-5 * np.sum(np.abs(g[n] * d)) + 1e-6, n
+
+
+def test_rows_that_begin_anywhere(br):
+    """Tensors at any element and rows of any length give what aligned ones do."""
+    for storage, shift in (("bf16", 1), ("bf16", 3), ("f32", 1)):
+        c = Case(storage, 2, 1, 64, 136, 1, seed=8)
+        o, lse = forward(br, c)
+        D, size = br.DevArray.from_numpy, c.q.dtype.itemsize
+        off = [D(np.concatenate([np.zeros(shift, a.dtype), a.ravel()])) for a in (c.q, c.k, c.v, np.zeros_like(c.q))]
+        fn = br.lib.mi355_attn_fwd_dev if storage == "f32" else br.lib.mi355_attn_fwd_bf16_dev
+        br.check(fn(off[3].ptr + shift * size, None, off[0].ptr + shift * size, off[1].ptr + shift * size, off[2].ptr + shift * size, None, 2, 1, 64, 136, 1, c.scale))
+        assert np.array_equal(off[3].numpy()[shift:].reshape(o.shape), o)
+
+
+def test_refusals(br):
+    D = br.DevArray((4096,))
+    p, lib = D.ptr, br.lib
+    ok = [p, p, p, p, p, None, 2, 1, 8, 4, 1, 1.0]
+    for i, v in ((0, None), (2, None), (3, None), (4, None), (6, 0), (7, 0), (7, 3), (8, 0), (8, 129), (9, 0), (9, -1), (9, 2 ** 23), (10, 0), (11, 0.0),
+                 (11, -1.0), (11, float("nan")), (11, float("inf")), (10, 2 ** 30)):
+        for fn in (lib.mi355_attn_fwd_dev, lib.mi355_attn_fwd_bf16_dev):
+            a = list(ok)
+            a[i] = v
+            assert fn(*a) == -1, (i, v)
+            assert br.last_error()
+    bwd = [p] * 9 + [None, 2, 1, 8, 4, 1, 1.0]
+    for i, v in [(j, None) for j in range(9)] + [(10, 0), (11, 3), (12, 200), (13, 0), (14, 0), (15, 0.0)]:
+        for fn in (lib.mi355_attn_bwd_dev, lib.mi355_attn_bwd_bf16_dev):
+            a = list(bwd)
+            a[i] = v
+            assert fn(*a) == -1, (i, v)
+    for a in ((None, p, 1, 4, 1), (p, None, 1, 4, 1), (p, p, 0, 4, 1), (p, p, 1, 0, 1), (p, p, 1, 4, 0), (p, p, 1, 4, 70000)):
+        assert lib.mi355_attn_plan_dev(*a) == -1
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_replayed_graph(br, storage):
+    """Forward and backward recorded into a graph, with other work between the replays."""
+    c = Case(storage, 4, 2, 64, 200, 2, [[0, 90, 200]] * 2, seed=9)
+    o, lse = forward(br, c)
+    g = backward(br, c, o, lse)
+    D = br.DevArray.from_numpy
+    q, k, v, do = (D(a) for a in (c.q, c.k, c.v, c.do))
+    bounds = plan_dev(br, c)
+    od, ld = D(np.zeros_like(o)), br.DevArray(lse.shape)
+    outs = [D(np.zeros_like(a)) for a in (c.q, c.k, c.v)]
+    end = "_dev" if storage == "f32" else "_bf16_dev"
+    shape = (c.heads, c.kv, c.hd, c.S, c.batch, c.scale)
+    br.check(br.lib.mi355_graph_begin())
+    br.check(getattr(br.lib, "mi355_attn_fwd" + end)(od.ptr, ld.ptr, q.ptr, k.ptr, v.ptr, bounds.ptr, *shape))
+    br.check(getattr(br.lib, "mi355_attn_bwd" + end)(*[a.ptr for a in outs], do.ptr, q.ptr, k.ptr, v.ptr, od.ptr, ld.ptr, bounds.ptr, *shape))
+    graph = br.lib.mi355_graph_end()
+    assert graph
+    for _ in range(3):
+        for a in outs + [od]:
+            a.zero()
+        br.check(br.lib.mi355_graph_launch(graph))
+        assert np.array_equal(od.numpy(), o) and np.array_equal(ld.numpy(), lse)
+        for a, n in zip(outs, ("dq", "dk", "dv")):
+            assert np.array_equal(a.numpy(), g[n])
+        other = Case(storage, 4, 2, 64, 200, 2, [[0, 90, 200]] * 2, seed=10)
+        forward(br, other)
+    br.lib.mi355_graph_free(graph)

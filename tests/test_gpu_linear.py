@@ -121,3 +121,173 @@ def test_gradients(br, i):
 @pytest.mark.parametrize("parts", [("dx",), ("dw",), ("dbias",), ("dx", "dbias")])
 def test_gradients_one_at_a_time(br, parts):
     check_backward(br, 70, 66, 50, 2, SILU, 1, 3, parts)
+
+
+@pytest.mark.parametrize("a", [NONE, RELU, SILU, GELU])
+def test_activation_gradient(br, a):
+    rng = np.random.default_rng(a)
+    n = 100003
+    pre, dy = to_bf16(4 * rng.standard_normal(n)), to_bf16(rng.standard_normal(n))
+    pre[:8] = to_bf16([0.0, -0.0, 88.0, -88.0, 3e38, -3e38, 1e-30, -1e-30])
+    D = br.DevArray.from_numpy
+    out, g, p = br.DevArray(n, np.uint16), D(dy), D(pre)
+    br.check(br.lib.mi355_act_bwd_bf16_dev(out.ptr, g.ptr, p.ptr, 0.5, a, n))
+    P, G = from_bf16(pre).astype(np.float64), from_bf16(dy).astype(np.float64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        s = np.where(np.abs(P) > 40, (P > 0) if a else 1.0, slope(a, np.clip(P, -40, 40)))
+    want = 0.5 * G * s
+    off = 0.5 * np.abs(G) * 2.0 ** -19 * (1 + np.minimum(np.abs(P), 40)) * (a != NONE)
+    close(out.numpy(), want, off + 2.0 ** -8 * (np.abs(want) + off) + TINY)
+    br.check(br.lib.mi355_act_bwd_bf16_dev(g.ptr, g.ptr, p.ptr, 0.5, a, n))       # in place
+    assert np.array_equal(g.numpy(), out.numpy())
+
+
+def test_residual_in_place(br):
+    rng = np.random.default_rng(1)
+    x, w, res = to_bf16(rng.standard_normal((3, 96, 75))), to_bf16(rng.standard_normal((130, 96)) / 10), to_bf16(rng.standard_normal((3, 130, 75)))
+    want, _ = run_forward(br, x, w, None, NONE, res, 0.25)
+    D = br.DevArray.from_numpy
+    y, xd, wd = D(res), D(x), D(w)
+    br.check(br.lib.mi355_linear_fwd_bf16_dev(y.ptr, None, xd.ptr, wd.ptr, None, NONE, y.ptr, 0.25, 130, 96, 75, 3))
+    assert np.array_equal(y.numpy(), want)
+
+
+@pytest.mark.parametrize("M,K,S,B", [(64, 128, 64, 2), (40, 72, 8, 1), (16, 256, 1, 1)])
+def test_tensors_at_any_element(br, M, K, S, B):
+    rng = np.random.default_rng(2)
+    x, w = to_bf16(rng.standard_normal((B, K, S))), to_bf16(rng.standard_normal((M, K)))
+    want, _ = run_forward(br, x, w, None, NONE, None, 1.0)
+    D = br.DevArray.from_numpy
+    for sx, sw, sy in ((1, 0, 0), (0, 3, 0), (0, 0, 5), (1, 1, 1)):
+        xd, wd = D(np.concatenate([np.zeros(sx, np.uint16), x.ravel()])), D(np.concatenate([np.zeros(sw, np.uint16), w.ravel()]))
+        yd = D(np.full(sy + B * M * S + 8, 7, np.uint16))
+        br.check(br.lib.mi355_linear_fwd_bf16_dev(yd.ptr + 2 * sy, None, xd.ptr + 2 * sx, wd.ptr + 2 * sw, None, NONE, None, 1.0, M, K, S, B))
+        got = yd.numpy()
+        assert np.array_equal(got[sy:sy + B * M * S].reshape(want.shape), want)
+        assert np.all(got[:sy] == 7) and np.all(got[sy + B * M * S:] == 7)
+
+
+def test_what_is_outside_is_not_seen(br):
+    """Infinities right behind every tensor: sums end where they should, whatever the sizes leave of the last steps."""
+    for M, K, S, B in ((70, 72, 40, 3), (33, 65, 19, 2), (130, 130, 256, 1), (9, 520, 8, 1)):
+        rng = np.random.default_rng(M)
+        x, w, dy = to_bf16(rng.standard_normal((B, K, S))), to_bf16(rng.standard_normal((M, K))), to_bf16(rng.standard_normal((B, M, S)))
+        D, inf = br.DevArray.from_numpy, np.full(4096, 0x7F80, np.uint16)
+        xd, wd, gd = (D(np.concatenate([t.ravel(), inf])) for t in (x, w, dy))
+        y, dx, dw, db = br.DevArray((B, M, S), np.uint16), br.DevArray((B, K, S), np.uint16), br.DevArray((M, K)), br.DevArray(M)
+        br.check(br.lib.mi355_linear_fwd_bf16_dev(y.ptr, None, xd.ptr, wd.ptr, None, NONE, None, 1.0, M, K, S, B))
+        br.check(br.lib.mi355_linear_bwd_bf16_dev(dx.ptr, dw.ptr, db.ptr, gd.ptr, xd.ptr, wd.ptr, 1.0, NONE, None, 0, M, K, S, B))
+        for t in (from_bf16(y.numpy()), from_bf16(dx.numpy()), dw.numpy(), db.numpy()):
+            assert np.all(np.isfinite(t)), (M, K, S, B)
+
+
+def test_a_nan_stays_in_its_column(br):
+    rng = np.random.default_rng(3)
+    x, w = to_bf16(rng.standard_normal((2, 64, 50))), to_bf16(rng.standard_normal((70, 64)))
+    want, _ = run_forward(br, x, w, None, GELU, None, 1.0)
+    x[1, 7, 20] = to_bf16([np.nan])[0]
+    got, _ = run_forward(br, x, w, None, GELU, None, 1.0)
+    bad = np.isnan(from_bf16(got))
+    assert bad[1, :, 20].all() and bad.sum() == 70
+    got[1, :, 20] = want[1, :, 20]
+    assert np.array_equal(got, want)
+
+
+def test_refusals(br):
+    d = br.DevArray((4096,))
+    p, lib = d.ptr, br.lib
+    fwd = [p, None, p, p, None, 0, None, 1.0, 4, 4, 4, 1]
+    for i, v in ((0, None), (2, None), (3, None), (5, -1), (5, 4), (8, 0), (9, 0), (10, 0), (11, 0), (8, -3), (8, 2 ** 23), (10, 2 ** 23), (11, 2 ** 22)):
+        a = list(fwd)
+        a[i] = v
+        assert lib.mi355_linear_fwd_bf16_dev(*a) == -1, (i, v)
+        assert br.last_error()
+    bwd = [p, p, p, p, p, p, 1.0, 0, None, 0, 4, 4, 4, 1]
+    for change in ({3: None}, {4: None}, {5: None}, {0: None, 1: None, 2: None}, {7: 2}, {7: 9}, {10: 0}, {11: 0}, {12: 0}, {13: 0}, {13: 2 ** 22}):
+        a = list(bwd)
+        for i, v in change.items():
+            a[i] = v
+        assert lib.mi355_linear_bwd_bf16_dev(*a) == -1, change
+    for a in ((None, p, p, 1.0, 0, 4), (p, None, p, 1.0, 0, 4), (p, p, None, 1.0, 0, 4), (p, p, p, 1.0, 7, 4)):
+        assert lib.mi355_act_bwd_bf16_dev(*a) == -1
+    assert lib.mi355_act_bwd_bf16_dev(p, p, p, 1.0, 0, 0) == 0
+
+
+@pytest.mark.parametrize("M,K,S,B", [(128, 192, 64, 2), (96, 100, 33, 3)])
+def test_replayed_graph(br, M, K, S, B):
+    """Recorded and replayed, other calls that use the same workspace in between."""
+    rng = np.random.default_rng(4)
+    x, w, dy = to_bf16(rng.standard_normal((B, K, S))), to_bf16(rng.standard_normal((M, K))), to_bf16(rng.standard_normal((B, M, S)))
+    D = br.DevArray.from_numpy
+    xd, wd, gd = D(x), D(w), D(dy)
+    y, dx, dw, db = br.DevArray((B, M, S), np.uint16), br.DevArray((B, K, S), np.uint16), br.DevArray((M, K)), br.DevArray(M)
+
+    def calls():
+        br.check(br.lib.mi355_linear_fwd_bf16_dev(y.ptr, None, xd.ptr, wd.ptr, None, SILU, None, 1.0, M, K, S, B))
+        br.check(br.lib.mi355_linear_bwd_bf16_dev(dx.ptr, dw.ptr, db.ptr, gd.ptr, xd.ptr, wd.ptr, 1.0, NONE, None, 0, M, K, S, B))
+
+    calls()
+    want = [t.numpy() for t in (y, dx, dw, db)]
+    br.check(br.lib.mi355_graph_begin())
+    calls()
+    graph = br.lib.mi355_graph_end()
+    assert graph
+    for _ in range(3):
+        for t in (y, dx, dw, db):
+            t.zero()
+        br.check(br.lib.mi355_graph_launch(graph))
+        for t, r in zip((y, dx, dw, db), want):
+            assert np.array_equal(t.numpy(), r)
+        run_forward(br, to_bf16(rng.standard_normal((1, 96, 31))), to_bf16(rng.standard_normal((64, 96))), None, NONE, None, 1.0)
+    br.lib.mi355_graph_free(graph)
+
+
+def test_attention_block_in_one_run(br):
+    """A layer's attention as a step runs it, bfloat16 storage: norm, q/k/v products, rotation, attention, output product with the scaled
+    residual; back through all of it.  Every stage against the formulas in 64 bits on the stage's own stored inputs."""
+    import test_gpu_attention as A
+    C, heads, kv, hd, S, B = 96, 4, 2, 32, 75, 2
+    rng = np.random.default_rng(5)
+    D, lib, n = br.DevArray.from_numpy, br.lib, S
+    new = lambda c: br.DevArray((B, c, S), np.uint16)       # noqa: E731
+    x, dy = to_bf16(rng.standard_normal((B, C, S))), to_bf16(rng.standard_normal((B, C, S)))
+    wn = np.ones(C, np.float32)
+    w = {k: to_bf16(rng.standard_normal(s) / np.sqrt(s[1])) for k, s in dict(q=(heads * hd, C), k=(kv * hd, C), v=(kv * hd, C), o=(C, heads * hd)).items()}
+    wd = {k: D(v) for k, v in w.items()}
+    xd, wnd, xn, y = D(x), D(wn), new(C), new(C)
+    q, k, v, qr, kr, o = new(heads * hd), new(kv * hd), new(kv * hd), new(heads * hd), new(kv * hd), new(heads * hd)
+    lse = br.DevArray((B, heads, S))
+    cos, sin = br.rope_tables_dev(S, hd, 1e4)
+    alpha, scale = 0.25, float(np.float32(hd ** -0.5))
+    br.check(lib.mi355_rmsnorm_fwd_bf16_dev(xn.ptr, xd.ptr, wnd.ptr, C, S, B, 1e-5))
+    for t, out in (("q", q), ("k", k), ("v", v)):
+        br.check(lib.mi355_linear_fwd_bf16_dev(out.ptr, None, xn.ptr, wd[t].ptr, None, NONE, None, 1.0, w[t].shape[0], C, S, B))
+    br.check(lib.mi355_rope_bf16_dev(qr.ptr, kr.ptr, q.ptr, k.ptr, heads, kv, hd, S, B, cos, sin, 1))
+    br.check(lib.mi355_attn_fwd_bf16_dev(o.ptr, lse.ptr, qr.ptr, kr.ptr, v.ptr, None, heads, kv, hd, S, B, scale))
+    br.check(lib.mi355_linear_fwd_bf16_dev(y.ptr, None, o.ptr, wd["o"].ptr, None, NONE, xd.ptr, alpha, C, heads * hd, S, B))
+    f = lambda t: from_bf16(t.numpy()).astype(np.float64)   # noqa: E731
+    W = {t: from_bf16(a).astype(np.float64) for t, a in w.items()}
+    for t, out in (("q", q), ("k", k), ("v", v)):
+        z, off = W[t] @ f(xn), E32 * (C + 4) * (np.abs(W[t]) @ np.abs(f(xn)))
+        close(out.numpy(), z, off + 2.0 ** -8 * (np.abs(z) + off))
+    c = A.Case("bf16", heads, kv, hd, S, B)
+    c.q, c.k, c.v, c.scale = qr.numpy(), kr.numpy(), v.numpy(), scale
+    A.check(c, dict(o=o.numpy(), lse=lse.numpy()), A.reference(c))
+    z, off = from_bf16(x) + alpha * (W["o"] @ f(o)), alpha * E32 * (heads * hd + 8) * (np.abs(W["o"]) @ np.abs(f(o)))
+    close(y.numpy(), z, off + 2.0 ** -8 * (np.abs(z) + off) + E32 * 4)
+    # back: dy -> d_o, dw_o; attention; rotation; dw_q, dw_k, dw_v
+    dyd, d_o, dqr, dkr, dv, dq, dk = D(dy), new(heads * hd), new(heads * hd), new(kv * hd), new(kv * hd), new(heads * hd), new(kv * hd)
+    dwo = br.DevArray(w["o"].shape)
+    br.check(lib.mi355_linear_bwd_bf16_dev(d_o.ptr, dwo.ptr, None, dyd.ptr, o.ptr, wd["o"].ptr, alpha, NONE, None, 0, C, heads * hd, S, B))
+    br.check(lib.mi355_attn_bwd_bf16_dev(dqr.ptr, dkr.ptr, dv.ptr, d_o.ptr, qr.ptr, kr.ptr, v.ptr, o.ptr, lse.ptr, None, heads, kv, hd, S, B, scale))
+    br.check(lib.mi355_rope_bf16_dev(dq.ptr, dk.ptr, dqr.ptr, dkr.ptr, heads, kv, hd, S, B, cos, sin, -1))
+    c.do = d_o.numpy()
+    A.check(c, dict(dq=dqr.numpy(), dk=dkr.numpy(), dv=dv.numpy()), A.reference(c, o.numpy(), lse.numpy()))
+    G, O = from_bf16(dy).astype(np.float64), f(o)
+    want = alpha * np.einsum("bms,bks->mk", G, O)
+    close(dwo.numpy(), want, E32 * (B * n + 6) * np.einsum("bms,bks->mk", np.abs(G), np.abs(O)))
+    for t, g in (("q", dq), ("k", dk), ("v", dv)):
+        dw = br.DevArray(w[t].shape)
+        br.check(lib.mi355_linear_bwd_bf16_dev(None, dw.ptr, None, g.ptr, xn.ptr, None, 1.0, NONE, None, 0, w[t].shape[0], C, S, B))
+        want = np.einsum("bms,bks->mk", f(g), f(xn))
+        close(dw.numpy(), want, E32 * (B * n + 6) * np.einsum("bms,bks->mk", np.abs(f(g)), np.abs(f(xn))) + TINY)
