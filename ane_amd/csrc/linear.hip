@@ -41,7 +41,7 @@ struct Epilogue {
 constexpr float GELU_C = 0.797884583473205566406f;      // sqrt(2 / pi)
 
 // GELU in its tanh form, through tanh(y) = 2 sigmoid(2y) - 1.  Far below zero the exponential is infinite and the sigmoid zero, as it should.
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }      // (1 / inf is 0 there too)
 template <int ACT>
 __device__ __forceinline__ float act_value(float x) {
     if (ACT == ACT_RELU) return x < 0.f ? 0.f : x;      // (a NaN stays one)
@@ -256,13 +256,12 @@ struct WaveOut {
                 *reinterpret_cast<v4f *>(lds + (lane & 31) * PITCH + (k * 32 + 8 * q + 4 * h) * 4) =
                     v4f{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
         settle();
-        const int n = n0 + at;
+        const int n = n0 + at, left = n < N ? M - m0 - lane / LANES : 0;
+        float *p = out + (size_t)(m0 + lane / LANES) * pitch + n;
 #pragma unroll
-        for (int i = 0; i < 32; i += 64 / LANES) {
-            const int row = i + lane / LANES;
-            v4f v = *reinterpret_cast<const v4f *>(lds + row * PITCH + at * 4);
-            if (m0 + row >= M || n >= N) continue;
-            float *p = out + (size_t)(m0 + row) * pitch + n;
+        for (int i = 0; i < 32; i += 64 / LANES, p += 64 / LANES * pitch) {
+            v4f v = *reinterpret_cast<const v4f *>(lds + (i + lane / LANES) * PITCH + at * 4);
+            if (i >= left) continue;
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] *= alpha;
             if (n + 4 <= N) {
@@ -277,29 +276,41 @@ struct WaveOut {
         }
     }
 
-    // Eight columns of a row between memory and LDS.
+    // Eight columns of rows m, m + STEP, ... between memory and LDS: a lane's own place in each of them.  Where a sequence ends within the
+    // eight, or the columns do, one by one.
     struct Columns { int n, b, s, N, S; };
-    static __device__ __forceinline__ v4u read8(const bf16_t *src, int rows, int m, const Columns &c) {
-        if (c.s + 8 <= c.S) return *reinterpret_cast<const v4u_any *>(src + ((size_t)c.b * rows + m) * c.S + c.s);
+    template <typename F>
+    static __device__ __forceinline__ void each_row(const Columns &c, int rows, int m, int M, F f) {
+        constexpr int STEP = 64 / (WN / 8);
+        size_t at = ((size_t)c.b * rows + m) * c.S + c.s;
+        const int left = c.n < c.N ? M - m : 0;
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; i++, at += (unsigned)(STEP * c.S))
+            f(i, at, i * STEP < left);
+    }
+    static __device__ __forceinline__ v4u read8(const bf16_t *src, size_t at, int rows, const Columns &c) {
+        if (c.s + 8 <= c.S) return *reinterpret_cast<const v4u_any *>(src + at);
         unsigned e[8];
-        int b = c.b, s = c.s;
+        int s = c.s;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            e[j] = c.n + j < c.N ? src[((size_t)b * rows + m) * c.S + s] : 0u;
-            if (++s == c.S) s = 0, b++;
+            e[j] = c.n + j < c.N ? src[at] : 0u;
+            at++;
+            if (++s == c.S) s = 0, at += (size_t)(rows - 1) * c.S;
         }
         return v4u{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
     }
-    static __device__ __forceinline__ void write8(bf16_t *dst, int rows, int m, const Columns &c, v4u v) {
+    static __device__ __forceinline__ void write8(bf16_t *dst, size_t at, int rows, const Columns &c, v4u v) {
         if (c.s + 8 <= c.S) {
-            *reinterpret_cast<v4u_any *>(dst + ((size_t)c.b * rows + m) * c.S + c.s) = v;
+            *reinterpret_cast<v4u_any *>(dst + at) = v;
             return;
         }
-        int b = c.b, s = c.s;
+        int s = c.s;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if (c.n + j < c.N) dst[((size_t)b * rows + m) * c.S + s] = (bf16_t)(v[j >> 1] >> (j & 1) * 16);
-            if (++s == c.S) s = 0, b++;
+            if (c.n + j < c.N) dst[at] = (bf16_t)(v[j >> 1] >> (j & 1) * 16);
+            at++;
+            if (++s == c.S) s = 0, at += (size_t)(rows - 1) * c.S;
         }
     }
 
@@ -310,11 +321,7 @@ struct WaveOut {
         char *mine = lds + (lane & 31) * PITCH + h * 8, *rows = lds + row0 * PITCH + lane % LANES * 16;
         if (in) {
             v4u w[32 * LANES / 64];
-#pragma unroll
-            for (int i = 0; i < 32 * LANES / 64; i++) {
-                const int m = m0 + row0 + i * (64 / LANES);
-                w[i] = m < M && c.n < c.N ? read8(in, M, m, c) : v4u{0u, 0u, 0u, 0u};
-            }
+            each_row(c, M, m0 + row0, M, [&](int i, size_t at, bool there) { w[i] = there ? read8(in, at, M, c) : v4u{0u, 0u, 0u, 0u}; });
             settle();
 #pragma unroll
             for (int i = 0; i < 32 * LANES / 64; i++) *reinterpret_cast<v4u *>(rows + i * (64 / LANES) * PITCH) = w[i];
@@ -353,12 +360,10 @@ struct WaveOut {
             else quads(std::false_type());
         });
         settle();
-#pragma unroll
-        for (int i = 0; i < 32 * LANES / 64; i++) {
-            const int m = m0 + row0 + i * (64 / LANES);
+        each_row(c, M, m0 + row0, M, [&](int i, size_t at, bool there) {
             const v4u v = *reinterpret_cast<const v4u *>(rows + i * (64 / LANES) * PITCH);
-            if (m < M && c.n < c.N) write8(e.out, M, m, c, v);
-        }
+            if (there) write8(e.out, at, M, c, v);
+        });
         if (KIND == FORWARD && e.pre_out) {
             settle();
 #pragma unroll
@@ -370,12 +375,10 @@ struct WaveOut {
                                                                            f2_to_bf2(acc[k][4 * q + 2] + bias, acc[k][4 * q + 3] + bias)};
                 }
             settle();
-#pragma unroll
-            for (int i = 0; i < 32 * LANES / 64; i++) {
-                const int m = m0 + row0 + i * (64 / LANES);
+            each_row(c, M, m0 + row0, M, [&](int i, size_t at, bool there) {
                 const v4u v = *reinterpret_cast<const v4u *>(rows + i * (64 / LANES) * PITCH);
-                if (m < M && c.n < c.N) write8(e.pre_out, M, m, c, v);
-            }
+                if (there) write8(e.pre_out, at, M, c, v);
+            });
         }
     }
 };
@@ -641,7 +644,7 @@ Tiling tiling(int M, int N, int sum) {
     const int steps = (int)ceil_div(sum, 64), cu = g_ctx.num_cu;
     auto tiles = [&](int t) { return ceil_div(M, t) * ceil_div(N, t); };
     Tiling r;
-    r.tile = tiles(256) >= (size_t)2 * cu ? 256 : tiles(128) >= (size_t)cu ? 128 : 64;
+    r.tile = tiles(256) >= (size_t)2 * cu ? 256 : 2 * tiles(128) >= (size_t)cu ? 128 : 64;
     // slices of the sum until every compute unit has work, each with at least four panels of the sum
     size_t slices = (size_t)cu / tiles(r.tile);
     if (slices > (size_t)steps / 4) slices = steps / 4;
