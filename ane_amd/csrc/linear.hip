@@ -383,21 +383,36 @@ struct WaveOut {
     }
 };
 
+// One product of a launch: C[M][N] in tiles, each over a slice of the sum.
+struct Work {
+    Mat a, b;
+    Epilogue e;
+    float *part;                // slices of C, where there are more than one
+    int M, N, out_s, sum, slice_steps, tiles_m, tiles_n, units;
+};
+
 template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Mat b, Epilogue e, float *__restrict__ part, int M, int N, int out_s,
-                                                                       int sum, int slice_steps, int tiles_m, int tiles_n) {
+constexpr int lds_bytes() {
+    constexpr int waves = BM / WM * (BN / WN), out = waves * WaveOut<KIND, WM / 32, WN / 32>::BYTES, stages = STAGES * (BM + BN) * PANEL_ROW;
+    return out > stages ? out : stages;
+}
+
+template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
+__device__ __forceinline__ void product_unit(const Work &w, int unit, char *lds) {
+    const Mat &a = w.a, &b = w.b;
+    const Epilogue &e = w.e;
+    float *const part = w.part;
+    const int M = w.M, N = w.N, out_s = w.out_s, tiles = w.tiles_m * w.tiles_n, slice = unit / tiles, tile = unit - slice * tiles;
     constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN, THREADS = WAVES_M * WAVES_N * 64, FM = WM / 32, FN = WN / 32;
     typedef Operand<BM, KIND == DX, THREADS> A;
     typedef Operand<BN, KIND != DW, THREADS> B;
     typedef WaveOut<KIND, FM, FN> Out;
-    constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS, OUT = WAVES_M * WAVES_N * Out::BYTES;
+    constexpr int STAGE = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS;
     // With three stages or more the one after the present one has arrived too, so that its first fragments can be read ahead.
     constexpr bool AHEAD = STAGES > 2;
     constexpr int LEFT = LOADS * (AHEAD ? STAGES - 3 : 0), FULL = AHEAD ? STAGES - 1 : 2;
-    __shared__ __attribute__((aligned(1024))) char lds[OUT > STAGES * STAGE ? OUT : STAGES * STAGE];
-    const int tile = xcd_remap(blockIdx.x, tiles_m * tiles_n);
-    const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
-    const int sum0 = blockIdx.y * slice_steps * 64, sum1 = min(sum, sum0 + slice_steps * 64), steps = (sum1 - sum0 + 63) / 64;
+    const int m0 = tile % w.tiles_m * BM, n0 = tile / w.tiles_m * BN;
+    const int sum0 = slice * w.slice_steps * 64, sum1 = min(w.sum, sum0 + w.slice_steps * 64), steps = (sum1 - sum0 + 63) / 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave / WAVES_N * FM, wn = wave % WAVES_N * FN;
 
@@ -476,8 +491,27 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Mat a, Ma
             }
         const int m = m0 + (wm + i) * 32;
         if (part || KIND == DW)
-            Out::floats(mine, cur, part ? part + (size_t)blockIdx.y * M * N : e.dw, N, m, n0 + wn * 32, M, N, part ? 1.f : e.alpha, !part && e.accumulate);
+            Out::floats(mine, cur, part ? part + (size_t)slice * M * N : e.dw, N, m, n0 + wn * 32, M, N, part ? 1.f : e.alpha, !part && e.accumulate);
         else Out::halves(mine, cur, e, m, M, cols);
+    }
+}
+
+// The units of one or two products, a workgroup to each, neighbours on one XCD (xcd_remap).  (As many workgroups as run
+// at once, each with several units: 278 -> 297 us for 32000 x 4096 results.  A unit's first loads then come behind the stores of the one
+// before, and so does the wait for them.)
+template <int KIND0, int KIND1, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Work w0, Work w1, int one_first) {
+    constexpr int B0 = lds_bytes<KIND0, BM, BN, WM, WN, STAGES>(), B1 = lds_bytes<KIND1, BM, BN, WM, WN, STAGES>();
+    __shared__ __attribute__((aligned(1024))) char lds[B0 > B1 ? B0 : B1];
+    int u = xcd_remap(blockIdx.x, gridDim.x);
+    if constexpr (KIND0 == KIND1) product_unit<KIND0, BM, BN, WM, WN, STAGES>(w0, u, lds);
+    else {
+        // the longer product's units come first
+        const int n0 = one_first ? w1.units : w0.units;
+        const bool second = u >= n0;
+        if (second) u -= n0;
+        if (second == (one_first != 0)) product_unit<KIND0, BM, BN, WM, WN, STAGES>(w0, u, lds);
+        else product_unit<KIND1, BM, BN, WM, WN, STAGES>(w1, u, lds);
     }
 }
 
@@ -502,30 +536,71 @@ __global__ __launch_bounds__(256) void repack_kernel(bf16_t *__restrict__ out, M
     *reinterpret_cast<v4u *>(out + (size_t)row * cols8 + col) = v;
 }
 
-// The slices of a product added up in their order, and its epilogue.
+// The slices of a product added up in their order, and its epilogue: eight columns of a row to a thread.
 template <int KIND>
-__global__ __launch_bounds__(256) void linear_join_kernel(Epilogue e, const float *__restrict__ part, int M, int N, int S, int slices) {
-    const int groups = (N + 7) / 8;
-    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= (size_t)M * groups) return;
+__device__ __forceinline__ void join(const Work &w, size_t t) {
+    const int groups = (w.N + 7) / 8, N = w.N, slices = w.units / (w.tiles_m * w.tiles_n);
     const int m = (int)(t / groups), n = (int)(t % groups) * 8;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = 0.f;
-    const float *p = part + (size_t)m * N + n;
+    const float *p = w.part + (size_t)m * N + n;
     if (n + 8 <= N) {
-        for (int i = 0; i < slices; i++, p += (size_t)M * N) {
+#pragma unroll 4
+        for (int i = 0; i < slices; i++, p += (size_t)w.M * N) {
             const v4f a = ld4(p), b = ld4(p + 4);
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] += a[j], v[4 + j] += b[j];
         }
     } else {
-        for (int i = 0; i < slices; i++, p += (size_t)M * N)
+        for (int i = 0; i < slices; i++, p += (size_t)w.M * N)
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (n + j < N) v[j] += p[j];
     }
-    finish<KIND>(e, v, m, M, n, N, S);
+    finish<KIND>(w.e, v, m, w.M, n, N, w.out_s);
+}
+// dbias[m] (+)= alpha * sum of row m of dy over the batch: a wave to a row, a fixed tree.
+struct RowSums {
+    float *out;
+    const bf16_t *dy;
+    int M, S, batch, accumulate;
+    float alpha;
+};
+__device__ __forceinline__ void row_sum(const RowSums &r, int m) {
+    const int lane = threadIdx.x & 63;
+    const int chunks = (r.S + 7) / 8, total = r.batch * chunks;
+    float s = 0.f;
+#pragma unroll 4
+    for (int c = lane; c < total; c += 64) {
+        const int b = c / chunks, i = (c - b * chunks) * 8;
+        const bf16_t *p = r.dy + ((size_t)b * r.M + m) * r.S + i;
+        if (i + 8 <= r.S) {
+            float v[8];
+            ldb<8, false>(v, p);
+#pragma unroll
+            for (int j = 0; j < 8; j++) s += v[j];
+        } else
+            for (int j = 0; i + j < r.S; j++) s += bf_to_f(p[j]);
+    }
+    s = wave_sum_far_first(s) * r.alpha;
+    if (lane == 0) r.out[m] = r.accumulate ? r.out[m] + s : s;
+}
+
+// What comes after the products: workgroups for the first one's slices, for the second one's, for the row sums.
+template <int KIND0, int KIND1>
+__global__ __launch_bounds__(256) void linear_join_kernel(Work w0, Work w1, RowSums r, int groups0, int groups1) {
+    const int g = blockIdx.x;
+    if (KIND1 != KIND0 && g >= groups0 + groups1) {
+        const int m = (g - groups0 - groups1) * 4 + (threadIdx.x >> 6);
+        if (m < r.M) row_sum(r, m);
+    } else if (KIND1 != KIND0 && g >= groups0) {
+        const size_t t = (size_t)(g - groups0) * 256 + threadIdx.x;
+        if (t < (size_t)w1.M * ((w1.N + 7) / 8)) join<KIND1>(w1, t);
+    } else {
+        const size_t t = (size_t)g * 256 + threadIdx.x;
+        if (t < (size_t)w0.M * ((w0.N + 7) / 8)) join<KIND0>(w0, t);
+    }
 }
 
 // Few columns: y is bound by reading w once, in rows.  A wave takes rows of w, its lanes eight steps of the sum at a time; x, as fp32 in LDS
@@ -577,33 +652,6 @@ __global__ __launch_bounds__(256) void gemv_kernel(const bf16_t *__restrict__ w,
     }
 }
 
-// dbias[m] (+)= alpha * sum of row m of dy over the batch: a workgroup to a row, a fixed tree.
-__global__ __launch_bounds__(256) void row_sum_kernel(float *__restrict__ out, const bf16_t *__restrict__ dy, int M, int S, int batch, float alpha,
-                                                      int accumulate) {
-    __shared__ float sums[4];
-    const int m = blockIdx.x;
-    float s = 0.f;
-    for (int b = 0; b < batch; b++) {
-        const bf16_t *row = dy + ((size_t)b * M + m) * S;
-        for (int i = threadIdx.x * 8; i < S; i += 2048) {
-            if (i + 8 <= S) {
-                float v[8];
-                ldb<8, false>(v, row + i);
-#pragma unroll
-                for (int j = 0; j < 8; j++) s += v[j];
-            } else
-                for (int j = i; j < S; j++) s += bf_to_f(row[j]);
-        }
-    }
-    s = wave_sum_far_first(s);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s = alpha * (sums[0] + sums[1] + sums[2] + sums[3]);
-        out[m] = accumulate ? out[m] + s : s;
-    }
-}
-
 __global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *__restrict__ dpre, const bf16_t *__restrict__ dy, const bf16_t *__restrict__ pre,
                                                       float alpha, int act, size_t n) {
     const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
@@ -639,37 +687,58 @@ int repack(const char *who, Mat &a, char *&ws) {
     return 0;
 }
 
-struct Tiling { int tile, slices, per; };
-Tiling tiling(int M, int N, int sum) {
-    const int steps = (int)ceil_div(sum, 64), cu = g_ctx.num_cu;
+// Tiles of C by the size of C alone, so that both products of a backward call can share a launch: 256 x 256 (eight waves, the fewest reads of
+// LDS to a product) from two rounds of the compute units on, 128 x 128 from half a round on, else 64 x 64.
+int tile_for(int M, int N) {
+    const size_t cu = g_ctx.num_cu;
     auto tiles = [&](int t) { return ceil_div(M, t) * ceil_div(N, t); };
-    Tiling r;
-    r.tile = tiles(256) >= (size_t)2 * cu ? 256 : 2 * tiles(128) >= (size_t)cu ? 128 : 64;
-    // slices of the sum until every compute unit has work, each with at least four panels of the sum
-    size_t slices = (size_t)cu / tiles(r.tile);
-    if (slices > (size_t)steps / 4) slices = steps / 4;
-    if (slices < 1) slices = 1;
-    r.per = (int)ceil_div(steps, slices);
-    r.slices = (int)ceil_div(steps, r.per);
-    return r;
+    return tiles(256) >= 2 * cu ? 256 : 2 * tiles(128) >= cu ? 128 : 64;
 }
-size_t part_bytes(const Tiling &t, int M, int N) { return t.slices > 1 ? (size_t)t.slices * M * N * sizeof(float) : 0; }
+// C of M x N from a sum of `sum` terms; `share`: how many compute units' worth of work it should make.
+Work work(const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s, int sum, int tile, size_t share) {
+    Work w = {};
+    w.a = a; w.b = b; w.e = e; w.M = M; w.N = N; w.out_s = out_s; w.sum = sum;
+    w.tiles_m = (int)ceil_div(M, tile);
+    w.tiles_n = (int)ceil_div(N, tile);
+    const size_t tiles = (size_t)w.tiles_m * w.tiles_n, steps = ceil_div(sum, 64);
+    // slices of the sum until every compute unit has work, each with at least four panels of the sum
+    size_t slices = share / tiles;
+    if (slices > steps / 4) slices = steps / 4;
+    if (slices < 1) slices = 1;
+    w.slice_steps = (int)ceil_div(steps, slices);
+    slices = ceil_div(steps, w.slice_steps);
+    w.units = tiles * slices <= 0xffffff ? (int)(tiles * slices) : -1;
+    return w;
+}
+int slices_of(const Work &w) { return w.M ? w.units / (w.tiles_m * w.tiles_n) : 0; }
+size_t part_bytes(const Work &w) { return slices_of(w) > 1 ? ((size_t)slices_of(w) * w.M * w.N * sizeof(float) + 255) & ~(size_t)255 : 0; }
 
-// C of M x N from a sum of `sum` terms; a and b are direct().
-template <int KIND>
-int product(const char *who, const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s, int sum, char *ws) {
-    const Tiling t = tiling(M, N, sum);
-    const int tm = (int)ceil_div(M, t.tile), tn = (int)ceil_div(N, t.tile);
-    if ((size_t)tm * tn > 0xffffff) return mi355_fail("%s: %d x %d results are too many", who, M, N);
-    float *part = t.slices > 1 ? (float *)ws : nullptr;
-    const dim3 grid((unsigned)(tm * tn), (unsigned)t.slices);
-    if (t.tile == 256) linear_kernel<KIND, 256, 256, 128, 64, 2><<<grid, 512, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
-    else if (t.tile == 128) linear_kernel<KIND, 128, 128, 64, 32, 4><<<grid, 512, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
-    else linear_kernel<KIND, 64, 64, 32, 32, 4><<<grid, 256, 0, g_ctx.stream>>>(a, b, e, part, M, N, out_s, sum, t.per, tm, tn);
-    LAUNCH_OK(who);
-    if (part) {
-        const size_t threads = (size_t)M * ceil_div(N, 8);
-        linear_join_kernel<KIND><<<(unsigned)ceil_div(threads, 256), 256, 0, g_ctx.stream>>>(e, part, M, N, out_s, t.slices);
+// The products' tensors are direct(); ws: room for the slices of both.
+template <int KIND0, int KIND1>
+int run(const char *who, Work w0, Work w1, const RowSums &r, int tile, char *ws) {
+    if (w0.units < 0 || w1.units < 0) return mi355_fail("%s: too many results", who);
+    for (Work *w : {&w0, &w1})
+        if (part_bytes(*w)) {
+            w->part = (float *)ws;
+            ws += part_bytes(*w);
+        }
+    const unsigned grid = (unsigned)(w0.units + w1.units);
+    if (grid > 0x7fffff) return mi355_fail("%s: too many results", who);
+    const int one_first = w1.units && w1.slice_steps > w0.slice_steps;
+    if (grid) {
+        if (tile == 256) linear_kernel<KIND0, KIND1, 256, 256, 128, 64, 2><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
+        // 128 x 128: with two stages two workgroups share a compute unit, with four one of them reads further ahead.  512 units 20.5 us
+        // with two, 28.6 with four; 256 units of twice the sum 26.1 and 22.7.
+        else if (tile == 128 && grid > (unsigned)g_ctx.num_cu) linear_kernel<KIND0, KIND1, 128, 128, 64, 32, 2><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
+        else if (tile == 128) linear_kernel<KIND0, KIND1, 128, 128, 64, 32, 4><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
+        else linear_kernel<KIND0, KIND1, 64, 64, 32, 32, 4><<<grid, 256, 0, g_ctx.stream>>>(w0, w1, one_first);
+        LAUNCH_OK(who);
+    }
+    // (few results to a sum that is cut into slices: their groups are far from what an int holds)
+    const int g0 = w0.part ? (int)ceil_div((size_t)w0.M * ceil_div(w0.N, 8), 256) : 0, g1 = w1.part ? (int)ceil_div((size_t)w1.M * ceil_div(w1.N, 8), 256) : 0;
+    const int g2 = (r.M + 3) / 4;
+    if (g0 + g1 + g2) {
+        linear_join_kernel<KIND0, KIND1><<<(unsigned)(g0 + g1 + g2), 256, 0, g_ctx.stream>>>(w0, w1, r, g0, g1);
         LAUNCH_OK(who);
     }
     return 0;
@@ -712,11 +781,12 @@ MI355_API int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16
         return 0;
     }
     Mat a = {w, M, K, K}, b = {x, K, S, N};
-    const size_t packed = repacked_bytes(a) + repacked_bytes(b), need = packed + part_bytes(tiling(M, N, K), M, N);
+    const int tile = tile_for(M, N);
+    const size_t packed = repacked_bytes(a) + repacked_bytes(b), need = packed + part_bytes(work(a, b, e, M, N, S, K, tile, g_ctx.num_cu));
     char *ws = nullptr;
     if (need && !(ws = (char *)mi355_ws(need))) return -1;
     if (repack("linear_fwd_bf16", a, ws) || repack("linear_fwd_bf16", b, ws)) return -1;
-    return product<FORWARD>("linear_fwd_bf16", a, b, e, M, N, S, K, ws);
+    return run<FORWARD, FORWARD>("linear_fwd_bf16", work(a, b, e, M, N, S, K, tile, g_ctx.num_cu), Work{}, RowSums{}, tile, ws);
 }
 
 MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, const uint16_t *dy, const uint16_t *x, const uint16_t *w,
@@ -729,22 +799,28 @@ MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, c
     e.act = act; e.alpha = alpha; e.pre = x_pre; e.out = dx; e.dw = dw; e.accumulate = accumulate;
     const int N = batch * S;
     Mat g = {dy, M, S, N}, wm = {w, M, K, K}, xm = {x, K, S, N};
-    // dx and dw use what is behind the repacked tensors one after the other
     const size_t packed = (dx || dw ? repacked_bytes(g) : 0) + (dx ? repacked_bytes(wm) : 0) + (dw ? repacked_bytes(xm) : 0);
-    const size_t p1 = dx ? part_bytes(tiling(K, N, M), K, N) : 0, p2 = dw ? part_bytes(tiling(M, K, N), M, K) : 0;
-    const size_t need = packed + (p1 > p2 ? p1 : p2);
+    // Both products in one launch, in the smaller of the tiles that suit them; the sum over N columns is as long when they are repacked.
+    const int t0 = dx ? tile_for(K, N) : 256, t1 = dw ? tile_for(M, K) : 256, tile = t0 < t1 ? t0 : t1;
+    auto works = [&](Work &w0, Work &w1) {
+        const size_t cu = g_ctx.num_cu;
+        w0 = dx ? work(wm, g, e, K, N, S, M, tile, cu) : Work{};
+        w1 = dw ? work(g, xm, e, M, K, K, g.cols, tile, cu) : Work{};
+    };
+    Work w0, w1;
+    works(w0, w1);
+    const size_t need = packed + part_bytes(w0) + part_bytes(w1);
     char *ws = nullptr;
     if (need && !(ws = (char *)mi355_ws(need))) return -1;
     if ((dx || dw) && repack("linear_bwd_bf16", g, ws)) return -1;
     if (dx && repack("linear_bwd_bf16", wm, ws)) return -1;
     if (dw && repack("linear_bwd_bf16", xm, ws)) return -1;
-    if (dx && product<DX>("linear_bwd_bf16", wm, g, e, K, N, S, M, ws)) return -1;
-    if (dw && product<DW>("linear_bwd_bf16", g, xm, e, M, K, K, g.cols, ws)) return -1;
+    works(w0, w1);
+    RowSums r = {};
     if (dbias) {
-        row_sum_kernel<<<(unsigned)M, 256, 0, g_ctx.stream>>>(dbias, dy, M, S, batch, alpha, accumulate);
-        LAUNCH_OK("linear_bwd_bf16");
+        r.out = dbias; r.dy = dy; r.M = M; r.S = S; r.batch = batch; r.accumulate = accumulate; r.alpha = alpha;
     }
-    return 0;
+    return run<DX, DW>("linear_bwd_bf16", w0, w1, r, tile, ws);
 }
 
 MI355_API int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *pre, float alpha, int act, size_t n) {
