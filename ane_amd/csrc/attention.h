@@ -374,7 +374,7 @@ int pack_rows(const char *who, const T **a, const T **b, size_t rows, int S, int
 // workgroups, else two by two, and where even that leaves compute units without work one position block to four teams.
 int waves_for(size_t heads_batch, int S) {
     if (ceil_div(S, 128) * heads_batch >= 2 * (size_t)g_ctx.num_cu) return 4;
-    return ceil_div(S, 64) * heads_batch >= (size_t)g_ctx.num_cu ? 2 : 1;
+    return ceil_div(S, 64) * heads_batch >= 2 * (size_t)g_ctx.num_cu ? 2 : 1;
 }
 template <typename F>
 int dispatch(int hd, int waves, F go) {

@@ -39,18 +39,6 @@ __device__ __forceinline__ bool dq_block(
     const size_t slab = ((size_t)at.b * heads + at.h) * hd * S, row = ((size_t)at.b * heads + at.h) * S;
     const int t0 = from / M::COLS, t1 = (to - 1) / M::COLS;
 
-    // delta from the fragments: two lanes share a query, each has half of the channels
-    char *second = STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds;
-    typename M::Frag qf[STEPS], gf[STEPS];
-    own_columns<T, HDB, POS, 256, STEPS>(gf, lds, d_o + slab, S, hd, q0, S, pos);
-    own_columns<T, HDB, POS, 256, STEPS>(qf, second, o + slab, S, hd, q0, S, pos);
-    float dlt = 0.f;
-    #pragma unroll
-    for (int i = 0; i < STEPS; i++) dlt = M::dot(qf[i], gf[i], dlt);
-    dlt += lane_xor<32>(dlt);
-    const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
-    if (active && h == 0 && team == 0) delta[row + mine] = dlt;
-
     PanelStream<T, HDB * 32, POS> ks, vs;
     ks.begin(k + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
     vs.begin(v + ((size_t)at.b * kv_heads + kvh) * hd * pitch, pitch, hd, pos);
@@ -63,10 +51,22 @@ __device__ __forceinline__ bool dq_block(
         ks.load(place + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
         vs.load(place + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
     };
-    constexpr bool EARLY = sizeof(T) == 4 || STAGES == 2;       // (own positions need the place of the second stage)
-    if (EARLY) load(0);
+    // Own positions of fp32 come without LDS, all at once and behind the first panels; those of bfloat16 by way of the panels' places.
+    constexpr bool DIRECT = sizeof(T) == 4, EARLY = STAGES == 2;
+    if (DIRECT) load(0);
+    typename M::Frag qf[STEPS], gf[STEPS], of[STEPS];
+    own_columns<T, HDB, POS, 256, STEPS>(gf, lds, d_o + slab, S, hd, q0, S, pos);
+    own_columns<T, HDB, POS, 256, STEPS>(of, STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds, o + slab, S, hd, q0, S, pos);
+    if (!DIRECT && EARLY) load(0);
     own_columns<T, HDB, POS, 256, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), q + slab, S, hd, q0, S, pos);
-    if (!EARLY) load(0);
+    if (!DIRECT && !EARLY) load(0);
+    // delta from the fragments: two lanes share a query, each has half of the channels
+    float dlt = 0.f;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) dlt = M::dot(of[i], gf[i], dlt);
+    dlt += lane_xor<32>(dlt);
+    const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
+    if (active && h == 0 && team == 0) delta[row + mine] = dlt;
     const float scale2 = scale * LOG2E;
 
     v16f acc[HDB];
