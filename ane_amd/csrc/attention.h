@@ -34,6 +34,14 @@ constexpr int panel_bytes(int hdb, int pos) { return 4 / pos * stages_for(hdb, 4
 template <typename T>
 constexpr int waves_per_simd(int hdb, int pos) { return panel_bytes(hdb, pos) <= 72 * 1024 && (sizeof(T) == 2 || hdb == 2) ? 2 : 1; }
 
+// Keeps accumulators where a kernel of one wave to a SIMD has its products write them.  Without it each tile copied them out of those
+// registers and back: dkv of bf16, 128 channels: 731 vector instructions a tile for 471 with it.
+template <int HDB>
+__device__ __forceinline__ void in_agprs(v16f (&acc)[HDB]) {
+#pragma unroll
+    for (int d = 0; d < HDB; d++) asm("" : "+a"(acc[d]));
+}
+
 __device__ __forceinline__ int wave_min_int(int v) {
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) v = min(v, __shfl_xor(v, m, 64));
@@ -146,14 +154,16 @@ template <typename T, int HDB>
 __device__ __forceinline__ void store_columns(T *dst, size_t pitch, int hd, const v16f (&acc)[HDB], float f, int pos0, bool active, char *lds) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (sizeof(T) == 4) {
-        if (!active) return;
-        T *p = dst + pos0 + (lane & 31);
+        // offsets into the head's rows: 64-bit addresses and a condition for each row took ten times as long
+        const unsigned row_bytes = (unsigned)pitch * 4, voff = active ? 4 * h * row_bytes + (pos0 + (lane & 31)) * 4 : OUTSIDE;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(dst, 0, (int)(hd * row_bytes), 0x00027000);
+        const bool whole = hd >= HDB * 32;
 #pragma unroll
         for (int d = 0; d < HDB; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int row = d * 32 + acc_row(r) + 4 * h;
-                if (row < hd) p[(size_t)row * pitch] = acc[d][r] * f;
+            for (int i = 0; i < 16; i++) {
+                const int row = d * 32 + acc_row(i);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(acc[d][i] * f), r, (int)(whole || row + 4 * h < hd ? voff : OUTSIDE), (int)(row * row_bytes), 0);
             }
     } else {
         constexpr int ROW = HDB * 64 + 16;          // (the 16 bytes spread the rows over the banks)
@@ -257,32 +267,62 @@ struct PanelStream {
     }
 };
 
-// The accumulators of a position's teams added up in the order of the teams; the first team ends with the sum.  Begins and ends with
-// everybody done with LDS.
-template <int HDB, int POS, int TEAMS>
-__device__ __forceinline__ void add_teams(v16f (&acc)[HDB], char *lds, int pos, int team) {
-    const int lane = threadIdx.x & 63;
-    auto at = [&](int t, int d, int r) { return reinterpret_cast<v4f *>(lds) + ((((t - 1) * POS + pos) * HDB + d) * 4 + r) * 64 + lane; };
-    if (team > 0) {
+// A position block's results, N of them: the accumulators of a position's teams added up in the order of the teams, and stored times f.
+// A team does that for its share of the channels.  False if a sum is NaN, and nothing is stored then; `anyway` stores it.  Begins with
+// everybody done with LDS, of which it takes N * HDB * 16 KB.
+template <typename T, int HDB, int POS, int N>
+__device__ __forceinline__ bool store_sums(T *const (&dst)[N], size_t pitch, int hd, const v16f (*const (&acc)[N])[HDB], const float (&f)[N], int pos0,
+                                           bool active, char *lds, int pos, int team, bool anyway) {
+    constexpr int TEAMS = 4 / POS, MINE = (HDB + TEAMS - 1) / TEAMS;       // blocks of 32 channels to a team
+    char *own = lds + (threadIdx.x >> 6) * ((MINE * 64 + 16) * 32);
+    bool odd = false;
+    if constexpr (TEAMS == 1) {
 #pragma unroll
-        for (int d = 0; d < HDB; d++)
+        for (int n = 0; n < N; n++) odd |= has_nan(*acc[n]);
+        if (!anyway && __syncthreads_or(active && odd)) return false;
 #pragma unroll
-            for (int r = 0; r < 4; r++) *at(team, d, r) = v4f{acc[d][4 * r], acc[d][4 * r + 1], acc[d][4 * r + 2], acc[d][4 * r + 3]};
-    }
-    __syncthreads();
-    if (team == 0) {
+        for (int n = 0; n < N; n++) store_columns<T, HDB>(dst[n], pitch, hd, *acc[n], f[n], pos0, active, own);
+    } else {
+        const int lane = threadIdx.x & 63, first = team * MINE * 32;
+        auto at = [&](int n, int t, int d, int r) { return reinterpret_cast<v4f *>(lds) + ((((n * TEAMS + t) * POS + pos) * HDB + d) * 4 + r) * 64 + lane; };
 #pragma unroll
-        for (int t = 1; t < TEAMS; t++)
+        for (int n = 0; n < N; n++)
 #pragma unroll
             for (int d = 0; d < HDB; d++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const v4f v = *at(t, d, r);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[d][4 * r + e] += v[e];
+                    const v16f &v = (*acc[n])[d];
+                    *at(n, team, d, r) = v4f{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
                 }
+        __syncthreads();
+        v16f sum[N][MINE];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+#pragma unroll
+            for (int j = 0; j < MINE; j++) {
+                sum[n][j] = v16_zero();
+                if (team * MINE + j < HDB)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        v4f v = *at(n, 0, team * MINE + j, r);
+#pragma unroll
+                        for (int t = 1; t < TEAMS; t++) {
+                            const v4f o = *at(n, t, team * MINE + j, r);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[e] += o[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum[n][j][4 * r + e] = v[e];
+                    }
+            }
+            odd |= has_nan(sum[n]);
+        }
+        if (__syncthreads_or(active && odd) && !anyway) return false;
+        if (first < hd)
+#pragma unroll
+            for (int n = 0; n < N; n++) store_columns<T, MINE>(dst[n] + (size_t)first * pitch, pitch, hd - first, sum[n], f[n], pos0, active, own);
     }
-    __syncthreads();
+    return true;
 }
 
 // Which position block of which head a workgroup has: blocks in the given order, heads of one KV group on one XCD where the heads deal

@@ -72,10 +72,12 @@ __device__ __forceinline__ bool dq_block(
     v16f acc[HDB];
 #pragma unroll
     for (int d = 0; d < HDB; d++) acc[d] = v16_zero();
+    if constexpr (waves_per_simd<T>(HDB, POS) == 1) in_agprs(acc);
     const int count = (t1 - t0) / TEAMS + 1;
     for (int i = 0; i < count; i++) {
         // what this tile needs is there; everybody is done with the tile before it
         loads_and_barrier<0, 0>();
+        if constexpr (waves_per_simd<T>(HDB, POS) == 1) in_agprs(acc);
         const char *kp = panels + i % STAGES * (TEAMS * 2 * BYTES), *vp = kp + BYTES;
         if (STAGES == 2) load(i + 1);
         const int t = t0 + i * TEAMS + team;
@@ -113,9 +115,7 @@ __device__ __forceinline__ bool dq_block(
         }
     }
     __syncthreads();
-    if constexpr (TEAMS > 1) add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
-    if (!CAREFUL && __syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) return false;
-    if (team == 0) store_columns<T, HDB>(dq + slab, S, hd, acc, scale, wq, active, lds + pos * (HDB * 64 + 16) * 32);
+    if (!store_sums<T, HDB, POS, 1>({dq + slab}, S, hd, {&acc}, {scale}, wq, active, lds, pos, team, CAREFUL)) return false;
     return true;
 }
 template <typename T, int HDB, int POS>

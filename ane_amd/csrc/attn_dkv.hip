@@ -52,6 +52,7 @@ __device__ __forceinline__ bool dkv_block(
     const unsigned place = lds_place(lds) + team * 2 * BYTES;
 #pragma unroll
     for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
+    in_agprs(ak), in_agprs(av);
     PanelStream<T, HDB * 32, POS> qs, gs;
     float lr[2] = {0.f, 0.f};
     // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
@@ -79,6 +80,7 @@ __device__ __forceinline__ bool dkv_block(
     for (int i = 0; i < count; i++) {
         // what this tile needs is there; everybody is done with the tile before it
         loads_and_barrier<0, 0>();
+        in_agprs(ak), in_agprs(av);
         const char *qp = panels + i % STAGES * (TEAMS * 2 * BYTES), *gp = qp + BYTES;
         const float *ls_row = rows[i % STAGES][team][0], *dl_row = rows[i % STAGES][team][1];
         const int c0 = head < group ? (t0 + tile) * M::COLS : to;
@@ -131,15 +133,7 @@ __device__ __forceinline__ bool dkv_block(
         store_rows((i + 1) % STAGES);
     }
     __syncthreads();
-    if constexpr (TEAMS > 1) {
-        add_teams<HDB, POS, TEAMS>(ak, lds, pos, team);
-        add_teams<HDB, POS, TEAMS>(av, lds, pos, team);
-    }
-    if (!CAREFUL && __syncthreads_or(active && team == 0 && (has_nan<HDB>(ak) || has_nan<HDB>(av)))) return false;
-    if (team > 0) return true;
-    char *mine_lds = lds + pos * (HDB * 64 + 16) * 32;
-    store_columns<T, HDB>(dk + slab, S, hd, ak, scale, wk, active, mine_lds);
-    store_columns<T, HDB>(dv + slab, S, hd, av, 1.f, wk, active, mine_lds);
+    if (!store_sums<T, HDB, POS, 2>({dk + slab, dv + slab}, S, hd, {&ak, &av}, {scale, 1.f}, wk, active, lds, pos, team, CAREFUL)) return false;
     return true;
 }
 template <typename T, int HDB, int POS>

@@ -145,12 +145,9 @@ __device__ __forceinline__ bool fwd_block(
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[d][r] *= f;
         __syncthreads();
-        add_teams<HDB, POS, TEAMS>(acc, lds, pos, team);
     }
-    if (!CAREFUL && __syncthreads_or(active && team == 0 && has_nan<HDB>(acc))) return false;
-    if (team > 0) return true;
-    store_columns<T, HDB>(o + slab, S, hd, acc, 1.f / l, wq, active, lds + pos * (HDB * 64 + 16) * 32);
-    if (active && lse && h == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (!store_sums<T, HDB, POS, 1>({o + slab}, S, hd, {&acc}, {1.f / l}, wq, active, lds, pos, team, CAREFUL)) return false;
+    if (active && lse && h == 0 && team == 0) lse[((size_t)at.b * heads + at.h) * S + mine] = (m + __builtin_amdgcn_logf(l)) * LN2;
     return true;
 }
 
