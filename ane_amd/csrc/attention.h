@@ -196,11 +196,14 @@ __device__ __forceinline__ void store_columns(T *dst, size_t pitch, int hd, cons
     }
 }
 
-// The 32 positions of this wave (number `pos` of POS side by side, from col0 on), as fragments of a product over the channels.  bfloat16:
-// through LDS, as many panels of it as the positions fill; begins when all waves are done with that place, ends with a barrier.  fp32: a
-// fragment is a value of each lane, rows of 32 positions, straight from memory.
-template <typename T, int HDB, int POS, int THREADS, int STEPS>
-__device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], char *lds, const T *src, size_t pitch, int hd, int col0, int S, int pos) {
+// The 32 positions of this wave (number `pos` of POS side by side, from col0 on) in N tensors, as fragments of a product over the channels.
+// All their loads are under way together.  bfloat16: through LDS, as many panels of a tensor as the positions fill; begins when all waves
+// are done with that place, ends with a barrier.  fp32: a fragment is a value of each lane, rows of 32 positions, straight from memory.
+template <typename T, int POS>
+constexpr int own_panels() { return (32 * POS + Mma<T>::COLS - 1) / Mma<T>::COLS; }
+template <typename T, int HDB, int POS, int N, int STEPS>
+__device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[N][STEPS], char *lds, const T *const (&src)[N], size_t pitch, int hd, int col0, int S,
+                                            int pos) {
     typedef Mma<T> M;
     const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 4) {
@@ -208,23 +211,31 @@ __device__ __forceinline__ void own_columns(typename Mma<T>::Frag (&f)[STEPS], c
         // last one again, whose results nobody keeps)
         const int h = lane >> 5;
         const unsigned row_bytes = (unsigned)pitch * 4, voff = h * row_bytes + min(col0 + pos * 32 + (lane & 31), S - 1) * 4;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(src), 0, (int)(hd * row_bytes), 0x00027000);
         const bool whole = hd >= 2 * STEPS;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++)
-            f[s] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)(whole || 2 * s + h < hd ? voff : OUTSIDE), (int)(2 * s * row_bytes), 0));
-    } else {
-        constexpr int PANELS = (32 * POS + M::COLS - 1) / M::COLS, BYTES = HDB * 32 * PANEL_ROW;
+        for (int n = 0; n < N; n++) {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(src[n]), 0, (int)(hd * row_bytes), 0x00027000);
 #pragma unroll
-        for (int p = 0; p < PANELS; p++) {
-            PanelLoad<T, HDB * 32, THREADS> ld;
-            ld.load(src, pitch, hd, col0 + p * M::COLS, 0, S);
-            ld.store(lds + p * BYTES);
+            for (int s = 0; s < STEPS; s++)
+                f[n][s] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)(whole || 2 * s + h < hd ? voff : OUTSIDE), (int)(2 * s * row_bytes), 0));
         }
+    } else {
+        constexpr int PANELS = own_panels<T, POS>(), BYTES = HDB * 32 * PANEL_ROW;
+        PanelLoad<T, HDB * 32, 256> ld[N][PANELS];
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int p = 0; p < PANELS; p++) ld[n][p].load(src[n], pitch, hd, col0 + p * M::COLS, 0, S);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int p = 0; p < PANELS; p++) ld[n][p].store(lds + (n * PANELS + p) * BYTES);
         __syncthreads();
         const char *panel = lds + (pos * 32 / M::COLS) * BYTES;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) f[s] = M::columns(panel, pos * 32 % M::COLS / 32, s);
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) f[n][s] = M::columns(panel + n * PANELS * BYTES, pos * 32 % M::COLS / 32, s);
         __syncthreads();
     }
 }
@@ -300,20 +311,19 @@ __device__ __forceinline__ bool store_sums(T *const (&dst)[N], size_t pitch, int
         for (int n = 0; n < N; n++) {
 #pragma unroll
             for (int j = 0; j < MINE; j++) {
-                sum[n][j] = v16_zero();
-                if (team * MINE + j < HDB)
+                const int d = min(team * MINE + j, HDB - 1);        // (a block behind the last: nobody stores it)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        v4f v = *at(n, 0, team * MINE + j, r);
+                for (int r = 0; r < 4; r++) {
+                    v4f v = *at(n, 0, d, r);
 #pragma unroll
-                        for (int t = 1; t < TEAMS; t++) {
-                            const v4f o = *at(n, t, team * MINE + j, r);
+                    for (int t = 1; t < TEAMS; t++) {
+                        const v4f o = *at(n, t, d, r);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) v[e] += o[e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) sum[n][j][4 * r + e] = v[e];
+                        for (int e = 0; e < 4; e++) v[e] += o[e];
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[n][j][4 * r + e] = v[e];
+                }
             }
             odd |= has_nan(sum[n]);
         }
@@ -411,10 +421,21 @@ int pack_rows(const char *who, const T **a, const T **b, size_t rows, int S, int
 
 // How many waves of a workgroup stand side by side (32 positions each, sharing the panels that they read), and in how many teams, which
 // share the walk: team i takes every TEAMS-th tile of it, with panels of its own.  Four side by side where that gives every compute unit two
-// workgroups, else two by two, and where even that leaves compute units without work one position block to four teams.
-int waves_for(size_t heads_batch, int S) {
+// workgroups; else two by two, where that gives it `two_from` half workgroups; else one position block to four teams.  Measured on 256
+// compute units with four / two / one side by side, us:
+//   four blocks of 512, 1024 of two: forward, bfloat16, 128 channels, 4096 positions of 16 heads 108 / 146 / 213
+//   192, 384: forward, 64 channels, 256 positions of 96 heads: bfloat16 9.5 / 7.6 / 16.9, fp32 24.5 / 18.7 / 25.5; all gradients: bfloat16
+//             27.4 / 24.7 / 34.1, fp32 71.0 / 63.9 / 70.0
+//   128, 256: 128 channels, 512 positions of 32 heads, bfloat16: forward 17.0 / 13.4 / 17.5, all gradients (only dq changed) 41.9 / 36.6 /
+//             42.2; but dk and dv, 64 channels, 1024 positions of 16 heads for 48: 113 / 71.8 / 59.8, and fp32, 2048 positions of 8 heads:
+//             forward 156 / 81.5 / 56.5, with dk and dv 352 / 219 / 163
+//   32, 64:   forward, bfloat16, 96 channels, 1024 positions of 4 heads 24.2 / 17.8 / 13.2
+constexpr int TWO_FROM = 3;                                                     // half workgroups to a compute unit
+template <typename T>
+constexpr int TWO_FROM_QUERIES = sizeof(T) == 2 ? 2 : TWO_FROM;                 // (the forward pass and dq)
+int waves_for(size_t heads_batch, int S, int two_from) {
     if (ceil_div(S, 128) * heads_batch >= 2 * (size_t)g_ctx.num_cu) return 4;
-    return ceil_div(S, 64) * heads_batch >= 2 * (size_t)g_ctx.num_cu ? 2 : 1;
+    return 2 * ceil_div(S, 64) * heads_batch >= two_from * (size_t)g_ctx.num_cu ? 2 : 1;
 }
 template <typename F>
 int dispatch(int hd, int waves, F go) {

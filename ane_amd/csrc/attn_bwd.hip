@@ -51,19 +51,29 @@ __device__ __forceinline__ bool dq_block(
         ks.load(place + i % STAGES * (TEAMS * 2 * BYTES), t * M::COLS, from, to);
         vs.load(place + i % STAGES * (TEAMS * 2 * BYTES) + BYTES, t * M::COLS, from, to);
     };
-    // Own positions of fp32 come without LDS, all at once and behind the first panels; those of bfloat16 by way of the panels' places.
-    constexpr bool DIRECT = sizeof(T) == 4, EARLY = STAGES == 2;
-    if (DIRECT) load(0);
-    typename M::Frag qf[STEPS], gf[STEPS], of[STEPS];
-    own_columns<T, HDB, POS, 256, STEPS>(gf, lds, d_o + slab, S, hd, q0, S, pos);
-    own_columns<T, HDB, POS, 256, STEPS>(of, STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds, o + slab, S, hd, q0, S, pos);
-    if (!DIRECT && EARLY) load(0);
-    own_columns<T, HDB, POS, 256, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), q + slab, S, hd, q0, S, pos);
-    if (!DIRECT && !EARLY) load(0);
+    // Own positions: those of fp32 come without LDS and behind the first panels; those of bfloat16 by way of the panels' places, all three
+    // by the second stage's where that is large enough, else two before the first panels and q by the second stage's.
+    constexpr int OWN = own_panels<T, POS>();
+    constexpr bool DIRECT = sizeof(T) == 4, ALL = STAGES == 2 && 3 * OWN <= TEAMS * 2;
+    char *second = lds + (STAGES == 2 ? TEAMS * 2 * BYTES : 0);
+    typename M::Frag own[3][STEPS];         // of d_o, o and q
+    if constexpr (DIRECT || ALL) {
+        load(0);
+        own_columns<T, HDB, POS, 3, STEPS>(own, second, {d_o + slab, o + slab, q + slab}, S, hd, q0, S, pos);
+    } else {
+        static_assert(2 * OWN <= STAGES * TEAMS * 2 && OWN <= TEAMS * 2, "they fit the panels' places");
+        typename M::Frag two[2][STEPS], one[1][STEPS];
+        own_columns<T, HDB, POS, 2, STEPS>(two, lds, {d_o + slab, o + slab}, S, hd, q0, S, pos);
+        if (STAGES == 2) load(0);
+        own_columns<T, HDB, POS, 1, STEPS>(one, second, {q + slab}, S, hd, q0, S, pos);
+        if (STAGES == 1) load(0);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) own[0][s] = two[0][s], own[1][s] = two[1][s], own[2][s] = one[0][s];
+    }
     // delta from the fragments: two lanes share a query, each has half of the channels
     float dlt = 0.f;
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) dlt = M::dot(of[i], gf[i], dlt);
+    for (int i = 0; i < STEPS; i++) dlt = M::dot(own[1][i], own[0][i], dlt);
     dlt += lane_xor<32>(dlt);
     const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
     if (active && h == 0 && team == 0) delta[row + mine] = dlt;
@@ -87,7 +97,7 @@ __device__ __forceinline__ bool dq_block(
             const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(kp) : 0;
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
-                v16f s = over_channels<T, STEPS>(kp, u, qf, v16_zero()), g = over_channels<T, STEPS>(vp, u, gf, v16_zero());
+                v16f s = over_channels<T, STEPS>(kp, u, own[2], v16_zero()), g = over_channels<T, STEPS>(vp, u, own[0], v16_zero());
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale2, -lse2));
@@ -154,7 +164,7 @@ int attn_bwd(const char *who, T *dq, T *dk, T *dv, const T *d_o, const T *q, con
     int pitch = S;
     const T *ks = k, *vs = v;
     if (pack_kv && pack_rows(who, &ks, &vs, (size_t)batch * kv_heads * hd, S, &pitch, ws + delta_bytes)) return -1;
-    int rc = dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
+    int rc = dispatch(hd, waves_for(n, S, TWO_FROM_QUERIES<T>), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
         attn_dq_kernel<T, HDB, W><<<(unsigned)(blocks * n), 256, 0, g_ctx.stream>>>(q, ks, vs, bounds, S, pitch, heads, kv_heads, hd,

@@ -5,6 +5,14 @@ namespace {
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------------
 
+// bfloat16 and up to 64 channels: what a wave keeps fits 256 registers, so two workgroups share a compute unit if their LDS lets them, which
+// four teams' panels for two tiles do not.  One tile at a time and two workgroups: 1024 positions of 96 heads 95 us (all gradients) where
+// one workgroup with two tiles took 111; packed rows of 997 positions, 12 heads for 48, 64.3 and 68.
+template <typename T>
+constexpr bool two_workgroups(int hdb) { return sizeof(T) == 2 && hdb == 2; }
+template <typename T>
+constexpr int dkv_stages(int hdb, int teams) { return two_workgroups<T>(hdb) && teams == 4 ? 1 : stages_for(hdb, teams); }
+
 // One position block; CAREFUL as in the forward pass.  q and d_o have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int POS, bool CAREFUL>
 __device__ __forceinline__ bool dkv_block(
@@ -12,7 +20,7 @@ __device__ __forceinline__ bool dkv_block(
     int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse, const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
     int batch, int blocks, lds_char *lds_) {
     typedef Mma<T> M;
-    constexpr int TEAMS = 4 / POS, STAGES = stages_for(HDB, TEAMS), KT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
+    constexpr int TEAMS = 4 / POS, STAGES = dkv_stages<T>(HDB, TEAMS), KT = 32 * POS, BYTES = HDB * 32 * PANEL_ROW, STEPS = HDB * 32 / M::STEP;
     char *lds = (char *)lds_;
     typedef float Rows[TEAMS][2][M::COLS];          // [team][lse * log2(e), delta][query], of a stage
     Rows *rows = reinterpret_cast<Rows *>(lds + TEAMS * STAGES * 2 * BYTES);
@@ -40,9 +48,9 @@ __device__ __forceinline__ bool dkv_block(
     const size_t slab = ((size_t)at.b * kv_heads + at.h) * hd * S;
     const size_t head0 = (size_t)at.b * heads + (size_t)at.h * group;
 
-    typename M::Frag kf[STEPS], vf[STEPS];
-    own_columns<T, HDB, POS, 256, STEPS>(kf, lds, k + slab, S, hd, k0, S, pos);
-    own_columns<T, HDB, POS, 256, STEPS>(vf, STAGES * TEAMS > 1 ? lds + 2 * BYTES : lds, v + slab, S, hd, k0, S, pos);
+    typename M::Frag own[2][STEPS];         // of k and v
+    static_assert(sizeof(T) == 4 || 2 * own_panels<T, POS>() <= STAGES * TEAMS * 2, "they fit the panels' places");
+    own_columns<T, HDB, POS, 2, STEPS>(own, lds, {k + slab, v + slab}, S, hd, k0, S, pos);
     const float scale2 = scale * LOG2E;
 
     v16f ak[HDB], av[HDB];
@@ -52,7 +60,7 @@ __device__ __forceinline__ bool dkv_block(
     const unsigned place = lds_place(lds) + team * 2 * BYTES;
 #pragma unroll
     for (int d = 0; d < HDB; d++) ak[d] = v16_zero(), av[d] = v16_zero();
-    in_agprs(ak), in_agprs(av);
+    if constexpr (!two_workgroups<T>(HDB)) in_agprs(ak), in_agprs(av);
     PanelStream<T, HDB * 32, POS> qs, gs;
     float lr[2] = {0.f, 0.f};
     // The walk goes over a group's heads one after the other, each over its queries; the team takes every TEAMS-th of all tiles.  What of
@@ -80,7 +88,7 @@ __device__ __forceinline__ bool dkv_block(
     for (int i = 0; i < count; i++) {
         // what this tile needs is there; everybody is done with the tile before it
         loads_and_barrier<0, 0>();
-        in_agprs(ak), in_agprs(av);
+        if constexpr (!two_workgroups<T>(HDB)) in_agprs(ak), in_agprs(av);
         const char *qp = panels + i % STAGES * (TEAMS * 2 * BYTES), *gp = qp + BYTES;
         const float *ls_row = rows[i % STAGES][team][0], *dl_row = rows[i % STAGES][team][1];
         const int c0 = head < group ? (t0 + tile) * M::COLS : to;
@@ -92,7 +100,7 @@ __device__ __forceinline__ bool dkv_block(
             const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
-                v16f s = over_channels<T, STEPS>(qp, u, kf, v16_zero()), g = over_channels<T, STEPS>(gp, u, vf, v16_zero());
+                v16f s = over_channels<T, STEPS>(qp, u, own[0], v16_zero()), g = over_channels<T, STEPS>(gp, u, own[1], v16_zero());
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const v4f ls = *reinterpret_cast<const v4f *>(ls_row + u * 32 + 8 * j + 4 * h);
@@ -145,12 +153,12 @@ __device__ __attribute__((noinline)) void dkv_block_again(
 }
 
 template <typename T, int HDB, int POS>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(two_workgroups<T>(HDB) ? 2 : 1))) void attn_dkv_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const int *__restrict__ bounds, int S, int pitch, int heads, int kv_heads,
     int hd, float scale, const T *__restrict__ d_o, const float *__restrict__ lse, const float *__restrict__ delta, T *__restrict__ dk, T *__restrict__ dv,
     int batch, int blocks) {
-    constexpr int TEAMS = 4 / POS, ROWS = stages_for(HDB, TEAMS) * TEAMS * 2 * Mma<T>::COLS * 4;
-    __shared__ __attribute__((aligned(16))) char lds[panel_bytes(HDB, POS) + ROWS + 16];
+    constexpr int TEAMS = 4 / POS, STAGES = dkv_stages<T>(HDB, TEAMS), ROWS = STAGES * TEAMS * 2 * Mma<T>::COLS * 4;
+    __shared__ __attribute__((aligned(16))) char lds[TEAMS * STAGES * 2 * HDB * 32 * PANEL_ROW + ROWS + 16];
     if (!dkv_block<T, HDB, POS, false>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o, lse, delta, dk, dv, batch, blocks, (lds_char *)lds))
         dkv_block_again<T, HDB, POS>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o, lse, delta, dk, dv, batch, blocks, (lds_char *)lds);
 }
@@ -159,7 +167,7 @@ template <typename T>
 int launch_dkv(const char *who, T *dk, T *dv, const T *d_o, const T *q, const T *k, const T *v, const float *lse, const float *delta,
                const int32_t *bounds, int heads, int kv_heads, int hd, int S, int pitch, int batch, float scale) {
     const size_t nk = (size_t)kv_heads * batch;
-    return dispatch(hd, waves_for(nk, S), [&](auto hdb, auto waves) {
+    return dispatch(hd, waves_for(nk, S, TWO_FROM), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
         attn_dkv_kernel<T, HDB, W><<<(unsigned)(blocks * nk), 256, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd, scale, d_o,

@@ -52,8 +52,8 @@ __device__ __forceinline__ bool fwd_block(
     constexpr bool EARLY = sizeof(T) == 4 || STAGES == 2;       // (own positions need the place of the second stage)
     if (EARLY) load(0);
 
-    typename M::Frag qf[STEPS];
-    own_columns<T, HDB, POS, 256, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), q + slab, S, hd, q0, S, pos);
+    typename M::Frag qf[1][STEPS];
+    own_columns<T, HDB, POS, 1, STEPS>(qf, lds + (EARLY ? TEAMS * 2 * BYTES : 0), {q + slab}, S, hd, q0, S, pos);
     if (!EARLY) load(0);
 
     v16f acc[HDB];
@@ -77,7 +77,7 @@ __device__ __forceinline__ bool fwd_block(
             float mx = -INFINITY;
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
-                s[u] = over_channels<T, STEPS>(kp, u, qf, v16_zero());
+                s[u] = over_channels<T, STEPS>(kp, u, qf[0], v16_zero());
             }
             if (masked) {
 #pragma unroll
@@ -201,7 +201,7 @@ int attn_fwd(const char *who, T *o, float *lse, const T *q, const T *k, const T 
         void *ws = mi355_ws(2 * packed_bytes<T>(rows, S));
         if (!ws || pack_rows(who, &k, &v, rows, S, &pitch, ws)) return -1;
     }
-    return dispatch(hd, waves_for(n, S), [&](auto hdb, auto waves) {
+    return dispatch(hd, waves_for(n, S, TWO_FROM_QUERIES<T>), [&](auto hdb, auto waves) {
         constexpr int HDB = decltype(hdb)::value, W = decltype(waves)::value;
         const int blocks = (int)ceil_div(S, 32 * W);
         attn_fwd_kernel<T, HDB, W><<<(unsigned)(blocks * n), 256, 0, g_ctx.stream>>>(q, k, v, bounds, S, pitch, heads, kv_heads, hd,
