@@ -11,6 +11,10 @@
 // dv have the same position in the lane, and scores go into the second product as they lie (mma.h).  The forward pass and dq have a
 // query to the lane and walk over the keys, dk and dv a key to the lane and walk over the queries: seven products in place of five, and
 // no gradient is added up by atomics.
+//
+// In bfloat16 p and ds are rounded to eight bits of mantissa before they are multiplied again (the matrix cores take no other operand beside
+// bfloat16 values at that rate): 2^-9 of each term on average, as much as the rounding of the results themselves.  Scores, statistics, sums,
+// delta and all accumulators are fp32.
 #pragma once
 #include "mma.h"
 
@@ -28,7 +32,8 @@ constexpr float LOG2E = 1.44269502162933349609375f, LN2 = 0.69314718246459960937
 
 typedef __attribute__((address_space(3))) char lds_char;
 
-// Panels for two tiles of each team, or for one where two would not fit; their bytes; and how many waves to a SIMD they leave room for.
+// Panels for two tiles of each team, or for one where two would not fit the 160 KB of a compute unit beside what else there is; their bytes;
+// and how many waves to a SIMD they leave room for.
 constexpr int stages_for(int hdb, int teams) { return 2 * 2 * teams * hdb * 32 * PANEL_ROW <= 128 * 1024 ? 2 : 1; }
 constexpr int panel_bytes(int hdb, int pos) { return 4 / pos * stages_for(hdb, 4 / pos) * 2 * hdb * 32 * PANEL_ROW; }
 template <typename T>

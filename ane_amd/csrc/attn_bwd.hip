@@ -78,6 +78,9 @@ __device__ __forceinline__ bool dq_block(
     const float lse2 = active ? lse[row + mine] * LOG2E : 0.f;
     if (active && h == 0 && team == 0) delta[row + mine] = dlt;
     const float scale2 = scale * LOG2E;
+    // A query with a single key has p = 1 whatever its score: do.v and delta are the same sum in two orders, and what is left of their
+    // difference by rounding is taken out.  (A product, for NaNs to stay.)
+    const float only = start == mine ? 0.f : 1.f;
 
     v16f acc[HDB];
 #pragma unroll
@@ -107,7 +110,7 @@ __device__ __forceinline__ bool dq_block(
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const int key = c0 + u * 32 + acc_row(r) + 4 * h;
-                        s[r] = key <= mine && key >= start ? s[r] : 0.f;
+                        s[r] = key <= mine && key >= start ? s[r] * only : 0.f;
                     }
                 }
                 const typename M::Packed p = M::pack(s);

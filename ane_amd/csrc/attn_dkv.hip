@@ -52,6 +52,8 @@ __device__ __forceinline__ bool dkv_block(
     static_assert(sizeof(T) == 4 || 2 * own_panels<T, POS>() <= STAGES * TEAMS * 2, "they fit the panels' places");
     own_columns<T, HDB, POS, 2, STEPS>(own, lds, {k + slab, v + slab}, S, hd, k0, S, pos);
     const float scale2 = scale * LOG2E;
+    // the query at this lane's position, if this key is its only one (attn_bwd.hip)
+    const int first = mine < S && (bounds ? max(bounds[(size_t)at.b * 2 * S + mine], 0) == mine : mine == 0) ? mine : -1;
 
     v16f ak[HDB], av[HDB];
     const int t0 = k0 / M::COLS, tiles = (to - 1) / M::COLS - t0 + 1, steps = tiles * group;
@@ -118,7 +120,7 @@ __device__ __forceinline__ bool dkv_block(
                         const int qq = c0 + u * 32 + acc_row(r) + 4 * h;
                         const bool ok = qq >= mine && qq < end;
                         s[r] = ok ? s[r] : 0.f;
-                        g[r] = ok ? g[r] : 0.f;
+                        g[r] = ok ? qq == first ? g[r] * 0.f : g[r] : 0.f;
                     }
                 }
                 const typename M::Packed ps = M::pack(s), pg = M::pack(g);

@@ -342,3 +342,27 @@ def test_replayed_graph(br, storage):
         other = Case(storage, 4, 2, 64, 200, 2, [[0, 90, 200]] * 2, seed=10)
         forward(br, other)
     br.lib.mi355_graph_free(graph)
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(4, 2, 64, 1, 5, None), (2, 2, 128, 70, 1, list(range(71))), (3, 1, 96, 40, 2, [[0, 1, 2, 2, 40], [7, 8, 39, 40, 40]]),
+                                   (128, 128, 72, 3, 8, [[0, 1, 2, 3]] * 8)])
+def test_a_single_key(br, storage, shape):
+    """A query with one key has a weight of 1 whatever its score: exactly no gradient for it, nor for a key that no other query has; dv is do
+    times exp of what the score's and lse's rounding leave (a few units of 2^-24 of a score below 2^6, so 2^-14), rounded."""
+    heads, kv, hd, S, batch, cu = shape
+    c = Case(storage, heads, kv, hd, S, batch, cu, seed=11)
+    o, lse = forward(br, c)
+    g = backward(br, c, o, lse)
+    start, end = c.plan()
+    for b in range(batch):
+        s = np.arange(S)
+        first, alone = start[b] == s, (start[b] == s) & (end[b] == s + 1)
+        assert alone.any()
+        assert not np.any(c.f64(g["dq"])[b][:, first]) and not np.any(c.f64(g["dk"])[b][:, alone])
+        # o = (p v) * (1 / p): three roundings of fp32 (each 2^-24 of the value), and 2^-22 in all is lost again when v itself has eight bits
+        v = c.f64(np.repeat(c.v[b].reshape(kv, hd, S), heads // kv, 0).reshape(heads * hd, S)[:, first])
+        assert np.all(np.abs(c.f64(o)[b][:, first] - v) <= (4 * E32 * np.abs(v) if storage == "f32" else 0.0))
+        do = c.f64(c.do)[b].reshape(kv, heads // kv, hd, S)
+        off = np.abs(c.f64(g["dv"])[b].reshape(kv, hd, S) - do.sum(1))[..., alone]
+        assert np.all(off <= ((2.0 ** -14 + 2 * STEP[storage]) * np.abs(do).sum(1))[..., alone])
