@@ -13,6 +13,10 @@ constexpr bool two_workgroups(int hdb) { return sizeof(T) == 2 && hdb == 2; }
 template <typename T>
 constexpr int dkv_stages(int hdb, int teams) { return two_workgroups<T>(hdb) && teams == 4 ? 1 : stages_for(hdb, teams); }
 
+// Four products of 2 * hd operations for each allowed pair, and two accumulators: one wave to a SIMD beyond 64 channels of bfloat16.
+// bfloat16, 4096 positions of 16 heads over 8, 128 channels: 190 us, 720 TFLOP/s; what a tile does comes one after the other in that
+// wave.  fp32, 256 positions of 128 heads over 64: 68 us, 64 TFLOP/s of 150 in two rounds of workgroups, each 37 us: 23 the walk, 11 own
+// positions, first loads, the teams' sums and stores.
 // One position block; CAREFUL as in the forward pass.  q and d_o have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int POS, bool CAREFUL>
 __device__ __forceinline__ bool dkv_block(

@@ -11,6 +11,7 @@
 // tiles for the compute units) are added in a fixed order by a second launch, which then has the epilogue.
 #include "mma.h"
 
+#include <initializer_list>
 #include <math.h>
 
 namespace {
@@ -496,6 +497,10 @@ __device__ __forceinline__ void product_unit(const Work &w, int unit, char *lds)
     }
 }
 
+// What bounds it: 256 x 256 tiles, 32000 x 4096 results of 768 terms 275 us, 730 TFLOP/s (a library product of that size 205): a tile takes
+// 26 us of which 18 are the sum's products at 1.5 times what the matrix cores alone need, 7.3 the way of its 128 KB of results to memory,
+// and its successor starts 3.5 later, with nobody else on the compute unit.  128 x 128 tiles: 1024 x 4096 results of 2048 terms with the
+// residual 23 to 25 us, 690 TFLOP/s (the library's product alone 24.5).  Both gradients of that layer 66 us, 520 TFLOP/s, of which 57 for the products.
 // The units of one or two products, a workgroup to each, neighbours on one XCD (xcd_remap).  (As many workgroups as run
 // at once, each with several units: 278 -> 297 us for 32000 x 4096 results.  A unit's first loads then come behind the stores of the one
 // before, and so does the wait for them.)
@@ -515,6 +520,7 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Work w0, 
     }
 }
 
+// (8 rows of 197 positions x 768 channels: 4 to 5 us, of 21 for the whole call; read from there as often as tiles need it.)
 // A tensor whose rows begin at any value, as one of [rows][cols8] whose rows begin at multiples of eight: zeros from its last column on.
 __global__ __launch_bounds__(256) void repack_kernel(bf16_t *__restrict__ out, Mat a, int cols8) {
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -604,51 +610,55 @@ __global__ __launch_bounds__(256) void linear_join_kernel(Work w0, Work w1, RowS
 }
 
 // Few columns: y is bound by reading w once, in rows.  A wave takes rows of w, its lanes eight steps of the sum at a time; x, as fp32 in LDS
-// [column][step], serves the workgroup's rows.  NC columns at once.
-constexpr int GEMV_MAX = 8;
+// [column][step], serves all rows of the workgroup.  NC columns at once.
+constexpr int GEMV_MAX = 4;
 template <int NC>
 __global__ __launch_bounds__(256) void gemv_kernel(const bf16_t *__restrict__ w, const bf16_t *__restrict__ x, Epilogue e, int M, int K, int N, int S,
                                                    int kpad) {
     extern __shared__ __attribute__((aligned(16))) float xs[];
-    for (int i = threadIdx.x; i < kpad * NC; i += 256) {
-        const int n = i / kpad, k = i - n * kpad, b = n / S;
-        xs[i] = n < N && k < K ? bf_to_f(x[((size_t)b * K + k) * S + (n - b * S)]) : 0.f;
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, m = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (m >= M) return;
-    float acc[NC];
+    size_t column[NC];
 #pragma unroll
-    for (int n = 0; n < NC; n++) acc[n] = 0.f;
-    const bf16_t *row = w + (size_t)m * K;
+    for (int n = 0; n < NC; n++) column[n] = n < N ? (size_t)(n / S) * K * S + n % S : 0;
 #pragma unroll 4
-    for (int k = lane * 8; k < kpad; k += 512) {
-        float v[8];
-        if (k + 8 <= K) ldb<8, true>(v, row + k);
-        else
+    for (int k = threadIdx.x; k < kpad; k += 256)
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = k + j < K ? bf_to_f(row[k + j]) : 0.f;
+        for (int n = 0; n < NC; n++) xs[n * kpad + k] = n < N && k < K ? bf_to_f(x[column[n] + (size_t)k * S]) : 0.f;
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    for (int m = blockIdx.x * 4 + (threadIdx.x >> 6); m < M; m += gridDim.x * 4) {
+        float acc[NC];
+#pragma unroll
+        for (int n = 0; n < NC; n++) acc[n] = 0.f;
+        const bf16_t *row = w + (size_t)m * K;
+#pragma unroll 4
+        for (int k = lane * 8; k < kpad; k += 512) {
+            float v[8];
+            if (k + 8 <= K) ldb<8, true>(v, row + k);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = k + j < K ? bf_to_f(row[k + j]) : 0.f;
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const v4f a = *reinterpret_cast<const v4f *>(xs + n * kpad + k), b = *reinterpret_cast<const v4f *>(xs + n * kpad + k + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[n] = __builtin_fmaf(v[4 + j], b[j], __builtin_fmaf(v[j], a[j], acc[n]));
+            }
+        }
+        float mine = 0.f;
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            const v4f a = *reinterpret_cast<const v4f *>(xs + n * kpad + k), b = *reinterpret_cast<const v4f *>(xs + n * kpad + k + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[n] = __builtin_fmaf(v[4 + j], b[j], __builtin_fmaf(v[j], a[j], acc[n]));
+            const float s = wave_sum_far_first(acc[n]);
+            mine = lane == n ? s : mine;
         }
-    }
-    float mine = 0.f;
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        const float s = wave_sum_far_first(acc[n]);
-        mine = lane == n ? s : mine;
-    }
-    if (lane < N && lane < NC) {
-        const int b = lane / S;
-        const size_t at = ((size_t)b * M + m) * S + (lane - b * S);
-        if (e.bias) mine += e.bias[m];
-        if (e.pre_out) e.pre_out[at] = (bf16_t)f_to_bf(mine);
-        by_act(e.act, [&](auto act) { mine = e.alpha * act_value<decltype(act)::value>(mine); });
-        if (e.res) mine += bf_to_f(e.res[at]);
-        e.out[at] = (bf16_t)f_to_bf(mine);
+        if (lane < N && lane < NC) {
+            const int b = lane / S;
+            const size_t at = ((size_t)b * M + m) * S + (lane - b * S);
+            if (e.bias) mine += e.bias[m];
+            if (e.pre_out) e.pre_out[at] = (bf16_t)f_to_bf(mine);
+            by_act(e.act, [&](auto act) { mine = e.alpha * act_value<decltype(act)::value>(mine); });
+            if (e.res) mine += bf_to_f(e.res[at]);
+            e.out[at] = (bf16_t)f_to_bf(mine);
+        }
     }
 }
 
@@ -687,12 +697,22 @@ int repack(const char *who, Mat &a, char *&ws) {
     return 0;
 }
 
-// Tiles of C by the size of C alone, so that both products of a backward call can share a launch: 256 x 256 (eight waves, the fewest reads of
-// LDS to a product) from two rounds of the compute units on, 128 x 128 from half a round on, else 64 x 64.
-int tile_for(int M, int N) {
+// Tiles of C: 256 x 256 (eight waves, the fewest reads of LDS to a product), 128 x 128 or 64 x 64, the largest of which there are enough.
+// In `need`, how many quarters of a round of the compute units that is, for 256 and for 128; a backward call counts both products' tiles.
+// Measured, us, with 64 / 128 / 256:
+//   forward, sums of 1024: 8192 x 4096 results 153 / 95 / 83, 4096 x 5120 99 / 57 / 71, 4096 x 4096 85 / 46 / 44, 1024 x 2048 10.7 / 13 / 32;
+//            sums of 2048: 768 x 4096 26 / 21 / 39; sums of 4096 and 8192: 1024 x 2048 34 / 32 / 44 and 59 / 49 / 55
+//   both gradients: weights of 1024 x 4096, 4096 columns 258 / 155 / 96, 768 x 2048, 2048 columns 44 / 26 / 58, 768 x 768, 4096 columns
+//            54 / 22 / 54, 1024 columns 10.4 / 13 / 31
+struct Shape { int m, n; };
+int tile_for(std::initializer_list<Shape> products, const int (&need)[2]) {
     const size_t cu = g_ctx.num_cu;
-    auto tiles = [&](int t) { return ceil_div(M, t) * ceil_div(N, t); };
-    return tiles(256) >= 2 * cu ? 256 : 2 * tiles(128) >= cu ? 128 : 64;
+    auto enough = [&](int t, int quarters) {
+        size_t tiles = 0;
+        for (const Shape &p : products) tiles += ceil_div(p.m, t) * ceil_div(p.n, t);
+        return 4 * tiles >= quarters * cu;
+    };
+    return enough(256, need[0]) ? 256 : enough(128, need[1]) ? 128 : 64;
 }
 // C of M x N from a sum of `sum` terms; `share`: how many compute units' worth of work it should make.
 Work work(const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s, int sum, int tile, size_t share) {
@@ -701,10 +721,12 @@ Work work(const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s
     w.tiles_m = (int)ceil_div(M, tile);
     w.tiles_n = (int)ceil_div(N, tile);
     const size_t tiles = (size_t)w.tiles_m * w.tiles_n, steps = ceil_div(sum, 64);
-    // slices of the sum until every compute unit has work, each with at least four panels of the sum
+    // Slices of the sum until every compute unit has work, each with at least four panels of the sum, and only where a workgroup's walk gets
+    // 16 panels shorter: joining them is a launch and two ways through memory.  Forward, 1024 x 2048 results, sums of 4096 in two slices 32 us and
+    // in one 38, of 1024 21 and 13; both gradients of 768 x 768 over 256 columns, in three slices 9.5 us, in one 7.1.
     size_t slices = share / tiles;
     if (slices > steps / 4) slices = steps / 4;
-    if (slices < 1) slices = 1;
+    if (slices < 1 || steps - ceil_div(steps, slices) < 16) slices = 1;
     w.slice_steps = (int)ceil_div(steps, slices);
     slices = ceil_div(steps, w.slice_steps);
     w.units = tiles * slices <= 0xffffff ? (int)(tiles * slices) : -1;
@@ -770,18 +792,20 @@ MI355_API int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16
     Epilogue e = {};
     e.act = act; e.alpha = alpha; e.bias = bias; e.res = res; e.pre_out = pre; e.out = y;
     const int N = batch * S, kpad = (K + 7) & ~7;
-    const size_t xs = (size_t)(N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8) * kpad * sizeof(float);
-    if (N <= GEMV_MAX && xs <= 64 * 1024) {
-        const unsigned grid = (unsigned)ceil_div(M, 4);
+    const size_t xs = (size_t)(N <= 1 ? 1 : N <= 2 ? 2 : 4) * kpad * sizeof(float);
+    // Few columns: 2048 x 1024 weights and 1, 2, 4 columns 4.6, 4.6 and 6.7 us with gemv_kernel, 9.9 to 10.1 with tiles; 4096 x 4096 and 1, 2 columns
+    // 10.3 and 16.2, 13.7 and 14.5; 2048 x 4096 and 4 columns 18.7 and 14.6: it multiplies without the matrix cores.
+    if (N <= GEMV_MAX && (double)M * K * N <= 1 << 24 && xs <= 64 * 1024) {
+        // at most four workgroups to a compute unit: each fetches x for itself
+        const unsigned grid = (unsigned)(ceil_div(M, 4) < 4 * (size_t)g_ctx.num_cu ? ceil_div(M, 4) : 4 * (size_t)g_ctx.num_cu);
         if (N <= 1) gemv_kernel<1><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
         else if (N <= 2) gemv_kernel<2><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
-        else if (N <= 4) gemv_kernel<4><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
-        else gemv_kernel<8><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
+        else gemv_kernel<4><<<grid, 256, xs, g_ctx.stream>>>(w, x, e, M, K, N, S, kpad);
         LAUNCH_OK("linear_fwd_bf16");
         return 0;
     }
     Mat a = {w, M, K, K}, b = {x, K, S, N};
-    const int tile = tile_for(M, N);
+    const int tile = tile_for({{M, N}}, {8, K >= 2048 ? 2 : 3});
     const size_t packed = repacked_bytes(a) + repacked_bytes(b), need = packed + part_bytes(work(a, b, e, M, N, S, K, tile, g_ctx.num_cu));
     char *ws = nullptr;
     if (need && !(ws = (char *)mi355_ws(need))) return -1;
@@ -800,8 +824,8 @@ MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, c
     const int N = batch * S;
     Mat g = {dy, M, S, N}, wm = {w, M, K, K}, xm = {x, K, S, N};
     const size_t packed = (dx || dw ? repacked_bytes(g) : 0) + (dx ? repacked_bytes(wm) : 0) + (dw ? repacked_bytes(xm) : 0);
-    // Both products in one launch, in the smaller of the tiles that suit them; the sum over N columns is as long when they are repacked.
-    const int t0 = dx ? tile_for(K, N) : 256, t1 = dw ? tile_for(M, K) : 256, tile = t0 < t1 ? t0 : t1;
+    // both products in one launch and one size of tile; the sum over N columns is as long when they are repacked
+    const int tile = tile_for({{dx ? K : 0, dx ? N : 0}, {dw ? M : 0, dw ? K : 0}}, {5, 3});
     auto works = [&](Work &w0, Work &w1) {
         const size_t cu = g_ctx.num_cu;
         w0 = dx ? work(wm, g, e, K, N, S, M, tile, cu) : Work{};

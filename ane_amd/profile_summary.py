@@ -51,7 +51,8 @@ def short(name):
 
 
 def skipped(name):
-    return name.startswith("__amd") or name.startswith("fill_") or name.startswith("at::native")
+    # (Cijk_, elementwise_kernel: the library's products and torch's kernels in the making of inputs)
+    return name.startswith(("__amd", "fill_", "at::native", "Cijk_", "elementwise_kernel"))
 
 
 def find_csv(directory, suffix):
