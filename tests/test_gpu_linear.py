@@ -291,3 +291,15 @@ def test_attention_block_in_one_run(br):
         br.check(lib.mi355_linear_bwd_bf16_dev(None, dw.ptr, None, g.ptr, xn.ptr, None, 1.0, NONE, None, 0, w[t].shape[0], C, S, B))
         want = np.einsum("bms,bks->mk", f(g), f(xn))
         close(dw.numpy(), want, E32 * (B * n + 6) * np.einsum("bms,bks->mk", np.abs(f(g)), np.abs(f(xn))) + TINY)
+
+
+@pytest.mark.parametrize("M,K,S,B", [(5003, 72, 1, 1), (5003, 70, 3, 1), (4200, 8, 1, 4),           # more rows than a round of the grid
+                                     (2100, 2050, 4, 1), (4104, 1024, 1, 4), (300, 96, 5, 1)])      # the same columns in tiles
+def test_few_columns(br, M, K, S, B):
+    check_forward(br, M, K, S, B, SILU, True, True, seed=M)
+
+
+@pytest.mark.parametrize("M,K,S,B", [(24, 8190, 2565, 1), (16, 8192, 1280, 2),         # one product's many tiles decide for both
+                                     (20, 1600, 1901, 1), (1600, 24, 66, 2), (33, 40, 5000, 1)])
+def test_gradients_of_unequal_products(br, M, K, S, B):
+    check_backward(br, M, K, S, B, NONE, 1, seed=K)
