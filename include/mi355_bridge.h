@@ -151,7 +151,8 @@ int mi355_qknorm_rope_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, float *dwq, float
  *            receives z [batch][M][S].  act is applied to the sum itself, not to its rounding.  y may be res.
  *   act: MI355_ACT_NONE, MI355_ACT_RELU, MI355_ACT_SILU, MI355_ACT_GELU (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))))
  * Sums are fp32; y, pre and dx are rounded once.  Deterministic (slices of a long sum are added in a fixed order, through the
- * workspace).  Outputs must not overlap inputs otherwise. */
+ * workspace, which also holds copies of tensors whose rows do not begin at multiples of 16 bytes).  Outputs must not overlap inputs
+ * otherwise.  M, K and batch * S at most 2^22. */
 enum { MI355_ACT_NONE = 0, MI355_ACT_RELU = 1, MI355_ACT_SILU = 2, MI355_ACT_GELU = 3 };
 int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16_t *x, const uint16_t *w, const float *bias, int act,
                               const uint16_t *res, float alpha, int M, int K, int S, int batch);
@@ -184,7 +185,8 @@ int mi355_attn_fwd_bf16_dev(uint16_t *o, float *lse, const uint16_t *q, const ui
                             const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch, float scale);
 /* Its gradients: dq, dk and dv are assigned (dk and dv summed over the query heads that share them).  o and lse: what the forward call
  * gave.  delta_s = do_s.o_s, ds[s][t] = p[s][t] (do_s.v_t - delta_s); dv_t = sum_s p[s][t] do_s, dq_s = scale sum_t ds[s][t] k_t,
- * dk_t = scale sum_s ds[s][t] q_s.  The workspace holds delta (4 * batch * heads * S bytes). */
+ * dk_t = scale sum_s ds[s][t] q_s; exactly nothing from a query with a single key.  The workspace holds delta (4 * batch * heads * S bytes)
+ * and, where rows are no multiple of 16 bytes or do not begin at one, copies of k and v (the forward pass too), then of q and d_o. */
 int mi355_attn_bwd_dev(float *dq, float *dk, float *dv, const float *d_o, const float *q, const float *k, const float *v,
                        const float *o, const float *lse, const int32_t *bounds, int heads, int kv_heads, int hd, int S, int batch,
                        float scale);
