@@ -216,8 +216,15 @@ struct Operand {
                     load_to_lds(r, v, soff + j * 8 * WAVES * row_bytes, lds + i * (64 * PANEL_ROW) + j * WAVES * 1024);
                 }
         }
-        if constexpr (COLUMNS) soff += 64 * row_bytes;
-        else {
+        if constexpr (COLUMNS) {
+            soff += 64 * row_bytes;
+            if (soff >= 1u << 31) {             // rows of up to 2^23 bytes: what 32 bits hold ends after 512 of them
+                const unsigned long long at = ((unsigned long long)(unsigned)r[1] << 32 | (unsigned)r[0]) + soff;
+                bytes = bytes > soff ? bytes - soff : 0;
+                r = buffer_at((const void *)at, bytes);
+                soff = 0;
+            }
+        } else {
             soff += 128;
             s0 += 64;
             if (s0 >= S) {
@@ -679,10 +686,10 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *__restrict__ dpre,
             by_act(act, [&](auto a) { dpre[j] = (bf16_t)f_to_bf(alpha * bf_to_f(dy[j]) * act_slope<decltype(a)::value>(bf_to_f(pre[j]))); });
 }
 
-// Whether linear_kernel can read a tensor as it is: chunks of eight values that begin at multiples of 16 bytes, and 32-bit offsets from the
-// slab where a workgroup begins (rows of at most 256 positions, or 64 of the sum).
+// Whether linear_kernel can read a tensor as it is: chunks of eight values that begin at multiples of 16 bytes, and one slab, or 32-bit offsets
+// over those that 256 columns (or 64 of the sum) reach from where they begin.
 bool direct(const Mat &a) {
-    return aligned16(a.p) && a.S % 8 == 0 && ((double)(256 / a.S + 2) * a.rows + 256) * a.S * 2 < 4e9;
+    return aligned16(a.p) && a.S % 8 == 0 && (a.cols == a.S || ((double)(256 / a.S + 2) * a.rows + 256) * a.S * 2 < 4e9);
 }
 size_t repacked_bytes(const Mat &a) { return direct(a) ? 0 : ((size_t)a.rows * ((a.cols + 7) & ~7) * 2 + 255) & ~(size_t)255; }
 int repack(const char *who, Mat &a, char *&ws) {

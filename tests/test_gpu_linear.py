@@ -303,3 +303,31 @@ def test_few_columns(br, M, K, S, B):
                                      (20, 1600, 1901, 1), (1600, 24, 66, 2), (33, 40, 5000, 1)])
 def test_gradients_of_unequal_products(br, M, K, S, B):
     check_backward(br, M, K, S, B, NONE, 1, seed=K)
+
+
+def test_offsets_beyond_32_bits(br):
+    """A tensor of 1100 rows of 2^21 values (4.6 GB) as x, as dy of dx and as dy of dw: what its few rows that are not zero hold arrives,
+    those behind 2^32 bytes included."""
+    N, R, C, rows = 1 << 21, 1100, 8, (3, 511, 1030, 1097)
+    rng = np.random.default_rng(8)
+    big = br.DevArray((R, N), np.uint16).zero()
+    held = to_bf16(rng.standard_normal((len(rows), N)))
+    for r, a in zip(rows, held):
+        br.lib.mi355_buf_write(big.handle, r * N * 2, a.ctypes.data, a.nbytes)
+    w = to_bf16(rng.standard_normal((C, R)))
+    D, out = br.DevArray.from_numpy, br.DevArray((C, N), np.uint16)
+    X, W = from_bf16(held).astype(np.float64), from_bf16(w).astype(np.float64)[:, rows]
+    off = E32 * (len(rows) + 4) * (np.abs(W) @ np.abs(X))           # (sums of zeros but for four terms)
+    wd, wtd = D(w), D(np.ascontiguousarray(w.T))
+    br.check(br.lib.mi355_linear_fwd_bf16_dev(out.ptr, None, big.ptr, wd.ptr, None, NONE, None, 1.0, C, R, N, 1))
+    close(out.numpy(), W @ X, off + 2.0 ** -8 * (np.abs(W @ X) + off) + TINY)
+    out.zero()
+    br.check(br.lib.mi355_linear_bwd_bf16_dev(out.ptr, None, None, big.ptr, None, wtd.ptr, 1.0, NONE, None, 0, R, C, N, 1))
+    got = out.numpy()
+    close(got, W @ X, off + 2.0 ** -8 * (np.abs(W @ X) + off) + TINY)
+    dw, db, Y = br.DevArray((R, C)), br.DevArray(R), from_bf16(got).astype(np.float64)
+    br.check(br.lib.mi355_linear_bwd_bf16_dev(None, dw.ptr, db.ptr, big.ptr, out.ptr, None, 1.0, NONE, None, 0, R, C, N, 1))
+    want, bound = np.zeros((R, C)), np.zeros((R, C))
+    want[rows, :], bound[rows, :] = X @ Y.T, E32 * (N + 6) * (np.abs(X) @ np.abs(Y).T)
+    close(dw.numpy(), want, bound)
+    assert not np.any(np.delete(dw.numpy(), rows, 0)) and not np.any(np.delete(db.numpy(), rows))
