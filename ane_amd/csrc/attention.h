@@ -374,9 +374,9 @@ bool shape_ok(const char *who, int heads, int kv_heads, int hd, int S, int batch
         mi355_fail("%s: scale must be positive and finite", who);
         return false;
     }
-    // what a launch can number (2^32 threads, two waves to 64 positions), and 32-bit offsets into a head
-    if (S > 1 << 22 || (double)heads * batch * ceil_div(S, 64) > (double)((1 << 25) - 1)) {
-        mi355_fail("%s: heads * batch * ceil(S / 64) = %.0f (at most 2^25 - 1), S = %d (at most 2^22)", who, (double)heads * batch * ceil_div(S, 64), S);
+    // what a launch can number (2^32 threads, 256 to 64 positions at most), and 32-bit offsets into a head
+    if (S > 1 << 22 || (double)heads * batch * ceil_div(S, 64) > (double)((1 << 24) - 1)) {
+        mi355_fail("%s: heads * batch * ceil(S / 64) = %.0f (at most 2^24 - 1), S = %d (at most 2^22)", who, (double)heads * batch * ceil_div(S, 64), S);
         return false;
     }
     return true;

@@ -696,6 +696,7 @@ int repack(const char *who, Mat &a, char *&ws) {
     if (direct(a)) return 0;
     const int cols8 = (a.cols + 7) & ~7;
     const size_t threads = (size_t)a.rows * (cols8 / 8);
+    if (ceil_div(threads, 256) > 0xffffff) return mi355_fail("%s: %d rows of %d columns, which do not begin at whole 16 bytes, are too many", who, a.rows, a.cols);
     repack_kernel<<<(unsigned)ceil_div(threads, 256), 256, 0, g_ctx.stream>>>((bf16_t *)ws, a, cols8);
     LAUNCH_OK(who);
     const size_t bytes = repacked_bytes(a);
@@ -858,7 +859,7 @@ MI355_API int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const u
     if (!mi355_ready("act_bwd_bf16")) return -1;
     if (!dpre || !dy || !pre) return mi355_fail("act_bwd_bf16: NULL pointer");
     if (act < ACT_NONE || act > ACT_GELU) return mi355_fail("act_bwd_bf16: act=%d (0 none, 1 ReLU, 2 SiLU, 3 GELU)", act);
-    if (ceil_div(n, 2048) > 0x7fffffff) return mi355_fail("act_bwd_bf16: n=%zu is too large", n);
+    if (ceil_div(n, 2048) > 0xffffff) return mi355_fail("act_bwd_bf16: n=%zu is too large", n);
     if (!n) return 0;
     act_bwd_kernel<<<(unsigned)ceil_div(n, 2048), 256, 0, g_ctx.stream>>>(dpre, dy, pre, alpha, act, n);
     LAUNCH_OK("act_bwd_bf16");

@@ -171,7 +171,8 @@ int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *p
  * training/training_dynamic/mil_dynamic.h:131-168 on); it takes q and k as mi355_qknorm_rope_fwd_dev / mi355_rope_dev leave them.
  *   p[s][t] = exp(scale q_s.k_t - lse_s) for first_s <= t <= s, o_s = sum_t p[s][t] v_t, lse_s = log sum_t exp(scale q_s.k_t)
  * q, o: [batch][heads*hd][S]; k, v: [batch][kv_heads*hd][S], heads a multiple of kv_heads (query heads h*heads/kv_heads .. share KV
- * head h); lse: [batch][heads][S] fp32, may be NULL when no gradient follows.  hd <= 128, scale > 0.
+ * head h); lse: [batch][heads][S] fp32, may be NULL when no gradient follows.  hd <= 128, scale > 0, S <= 2^22 and
+ * heads * batch * ceil(S / 64) < 2^24.
  * bounds: NULL when every row is one sequence of S positions, else the plan of rows into which sequences of different lengths are
  * packed, from mi355_attn_plan_dev, kept for all layers and both directions: bounds[b][0][s] is the first position of the sequence that
  * s belongs to (S if it is in none), bounds[b][1][s] one past its last (0).  Columns of no sequence are neither read for another

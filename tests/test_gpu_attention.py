@@ -366,3 +366,13 @@ def test_a_single_key(br, storage, shape):
         do = c.f64(c.do)[b].reshape(kv, heads // kv, hd, S)
         off = np.abs(c.f64(g["dv"])[b].reshape(kv, hd, S) - do.sum(1))[..., alone]
         assert np.all(off <= ((2.0 ** -14 + 2 * STEP[storage]) * np.abs(do).sum(1))[..., alone])
+
+
+def test_more_than_a_launch_numbers_is_refused(br):
+    p = br.DevArray((4096,)).ptr
+    for fn in (br.lib.mi355_attn_fwd_dev, br.lib.mi355_attn_fwd_bf16_dev):
+        for heads, S, batch in ((1, 1, 1 << 24), (1 << 12, 64, 1 << 12), (64, 1 << 22, 4)):
+            assert fn(p, p, p, p, p, None, heads, 1, 1, S, batch, 1.0) == -1 and br.last_error()
+    for fn in (br.lib.mi355_attn_bwd_dev, br.lib.mi355_attn_bwd_bf16_dev):
+        assert fn(*[p] * 9, None, 1, 1, 1, 1, 1 << 24, 1.0) == -1 and br.last_error()
+    assert br.lib.mi355_act_bwd_bf16_dev(p, p, p, 1.0, 0, 1 << 35) == -1 and br.last_error()
