@@ -12,9 +12,11 @@
 // query to the lane and walk over the keys, dk and dv a key to the lane and walk over the queries: seven products in place of five, and
 // no gradient is added up by atomics.
 //
-// In bfloat16 p and ds are rounded to eight bits of mantissa before they are multiplied again (the matrix cores take no other operand beside
-// bfloat16 values at that rate): 2^-9 of each term on average, as much as the rounding of the results themselves.  Scores, statistics, sums,
-// delta and all accumulators are fp32.
+// In bfloat16 p and ds go into the second product as pairs of bfloat16 values that are off by 2^-15 of them (mma.h): the matrix cores take
+// no other operand beside bfloat16 values, and one value each, off by 2^-8, is as much again as the rounding of the results.  The second
+// half costs a product more for each of those: 4096 positions of 16 heads, 128 channels, forward 107 -> 133 us, all gradients 311 -> 391;
+// 256 positions of 256 heads, forward 17.5 -> 19.7.  Scores, statistics, sums, delta and all accumulators are fp32; delta is of o as it is
+// stored, so it has the rounding of that in it.
 #pragma once
 #include "mma.h"
 

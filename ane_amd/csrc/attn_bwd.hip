@@ -100,7 +100,7 @@ __device__ __forceinline__ bool dq_block(
         const int c0 = t * M::COLS;
         if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
             const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(kp) : 0;
+            const unsigned long long odd = CAREFUL && (masked || sizeof(T) == 2) ? odd_columns<T, HDB * 32>(kp) : 0;
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
                 v16f s = over_channels<T, STEPS>(kp, u, own[2], v16_zero()), g = over_channels<T, STEPS>(vp, u, own[0], v16_zero());
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool dq_block(
                         s[r] = key <= mine && key >= start ? s[r] * only : 0.f;
                     }
                 }
-                const typename M::Packed p = M::pack(s);
+                const typename M::Packed p = M::template pack<CAREFUL>(s);
                 if (odd) {
                     over_positions<T, HDB, true>(acc, kp, u, p);
                     add_odd<T, HDB>(acc, kp, u, s, odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });

@@ -103,7 +103,7 @@ __device__ __forceinline__ bool dkv_block(
         if (STAGES == 2) load((i + 1) % STAGES);
         if (c0 + M::COLS > wk && c0 < wto) {
             const bool masked = c0 < wk + 31 || c0 + M::COLS > wfull;
-            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
+            const unsigned long long odd = CAREFUL && (masked || sizeof(T) == 2) ? odd_columns<T, HDB * 32>(qp) | odd_columns<T, HDB * 32>(gp) : 0;
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
                 v16f s = over_channels<T, STEPS>(qp, u, own[0], v16_zero()), g = over_channels<T, STEPS>(gp, u, own[1], v16_zero());
@@ -127,7 +127,7 @@ __device__ __forceinline__ bool dkv_block(
                         g[r] = ok ? qq == first ? g[r] * 0.f : g[r] : 0.f;
                     }
                 }
-                const typename M::Packed ps = M::pack(s), pg = M::pack(g);
+                const typename M::Packed ps = M::template pack<CAREFUL>(s), pg = M::template pack<CAREFUL>(g);
                 if (odd) {
                     over_positions<T, HDB, true>(av, gp, u, ps);
                     over_positions<T, HDB, true>(ak, qp, u, pg);

@@ -77,7 +77,7 @@ __device__ __forceinline__ bool fwd_block(
         const int c0 = t * M::COLS;
         if (t <= t1 && c0 <= wq + 31 && c0 + M::COLS > wfrom) {
             const bool masked = c0 + M::COLS - 1 > wq || c0 < wfull;
-            const unsigned long long odd = CAREFUL && masked ? odd_columns<T, HDB * 32>(vp) : 0;
+            const unsigned long long odd = CAREFUL && (masked || sizeof(T) == 2) ? odd_columns<T, HDB * 32>(vp) : 0;
             v16f s[M::SUBS];
             float mx = -INFINITY;
 #pragma unroll
@@ -115,7 +115,7 @@ __device__ __forceinline__ bool fwd_block(
                     s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, -base));
                     l += s[u][r];
                 }
-                const typename M::Packed p = M::pack(s[u]);
+                const typename M::Packed p = M::template pack<CAREFUL>(s[u]);
                 if (odd) {
                     over_positions<T, HDB, true>(acc, vp, u, p);
                     add_odd<T, HDB>(acc, vp, u, s[u], odd, [&](int c) { return c0 + c <= mine && c0 + c >= start; });
@@ -156,8 +156,9 @@ __device__ __forceinline__ bool fwd_block(
     return true;
 }
 
-// An infinity or a NaN among the values of positions that the mask hides makes 0 * inf of their weights.  A block that ends with a NaN is
-// computed again, with those values taken out of the products and added for the pairs that count.  It is a function of its own, for its
+// An infinity or a NaN among the values of positions that the mask hides makes 0 * inf of their weights, and so does an infinity that counts
+// of the second half of a bfloat16 weight.  A block that ends with a NaN is computed again, with those values taken out of the products
+// (fp32: where something is masked) and added for the pairs that count.  It is a function of its own, for its
 // registers not to be the kernel's.
 template <typename T, int HDB, int POS>
 __device__ __attribute__((noinline)) void fwd_block_again(

@@ -62,15 +62,30 @@ template <> struct Mma<bf16_t> {
         return *reinterpret_cast<const Frag *>(panel + block * (32 * PANEL_ROW) + panel_at(lane & 31, step * 2 + (lane >> 5)));
     }
 
-    // A product's registers as the second operand of a product over its rows.
-    struct Packed { Frag f[2]; };
+    // A product's registers as the second operand of a product over its rows: each value's upper half, and what that leaves of it rounded
+    // to bfloat16, so that the pair is off by 2^-15 of the value at most.  (One bfloat16 value, 2^-8, shows in results of that type: error
+    // of a batch's attention against 64 bits 0.0019 where the rounding of the results alone is 0.0016, of its gradients 0.0026 for 0.0017.)
+    // An infinity leaves NaN; WILD: nothing.
+    struct Packed { Frag hi[2], lo[2]; };
+    template <bool WILD>
     static __device__ __forceinline__ Packed pack(const v16f &p) {
         Packed out;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const v4u w = {f2_to_bf2(p[8 * j], p[8 * j + 1]), f2_to_bf2(p[8 * j + 2], p[8 * j + 3]), f2_to_bf2(p[8 * j + 4], p[8 * j + 5]),
-                           f2_to_bf2(p[8 * j + 6], p[8 * j + 7])};
-            out.f[j] = __builtin_bit_cast(Frag, w);
+            v4u hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const unsigned a = __float_as_uint(p[8 * j + 2 * i]), b = __float_as_uint(p[8 * j + 2 * i + 1]);
+                hi[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                float ra = p[8 * j + 2 * i] - __uint_as_float(a & 0xffff0000u), rb = p[8 * j + 2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+                if (WILD) {
+                    ra = is_finite(p[8 * j + 2 * i]) ? ra : 0.f;
+                    rb = is_finite(p[8 * j + 2 * i + 1]) ? rb : 0.f;
+                }
+                lo[i] = f2_to_bf2(ra, rb);
+            }
+            out.hi[j] = __builtin_bit_cast(Frag, hi);
+            out.lo[j] = __builtin_bit_cast(Frag, lo);
         }
         return out;
     }
@@ -98,7 +113,8 @@ template <> struct Mma<bf16_t> {
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = (v[e] & 0x7f80) == 0x7f80 ? (short)0 : v[e];
             }
-            acc = mul(__builtin_bit_cast(Frag, v), p.f[j], acc);
+            acc = mul(__builtin_bit_cast(Frag, v), p.lo[j], acc);
+            acc = mul(__builtin_bit_cast(Frag, v), p.hi[j], acc);
         }
         return acc;
     }
@@ -124,6 +140,7 @@ template <> struct Mma<float> {
     }
     static __device__ __forceinline__ v16f mul(Frag a, Frag b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
     typedef v16f Packed;
+    template <bool WILD>
     static __device__ __forceinline__ Packed pack(const v16f &p) { return p; }
     struct Row { v4f v[4]; };
     static __device__ __forceinline__ Row row(const char *panel, int block, int) {

@@ -1,0 +1,76 @@
+"""Attention on bfloat16 storage is as exact as its results' type: weights and score gradients are multiplied again as pairs of bfloat16
+values, so what is left beside the rounding of a result is 2^-15 of the magnitudes that enter it, and the error of fp32 sums.
+
+The bound of an element: the fp32 chain's (test_gpu_attention.reference on the same values held as fp32), 2^-15 of the sum of magnitudes
+of its last product, and half a step of bfloat16 at the result, which is 2^-8 of the power of two at or below it."""
+import numpy as np
+import pytest
+
+import test_gpu_attention as A
+
+pytestmark = pytest.mark.gpu
+
+PAIR = 2.0 ** -15
+
+
+def as_fp32(c):
+    """The same case with its values held as fp32."""
+    w = A.Case("f32", c.heads, c.kv, c.hd, c.S, c.batch, c.cu)
+    w.q, w.k, w.v, w.do, w.scale = *(A.from_bf16(a) for a in (c.q, c.k, c.v, c.do)), c.scale
+    return w
+
+
+def magnitudes(w, o=None, lse=None):
+    """Sums of magnitudes of the last products: of o, or, given o and lse, of dq, dk and dv."""
+    G, hd, S = w.heads // w.kv, w.hd, w.S
+    out = {n: np.zeros((w.batch, (w.kv if n in ("dk", "dv") else w.heads) * hd, S)) for n in (("o",) if o is None else ("dq", "dk", "dv"))}
+    for b in range(w.batch):
+        ok = w.allowed(b)
+        used = ok.any(1)
+        for h in range(w.heads):
+            rq, rk = slice(h * hd, (h + 1) * hd), slice(h // G * hd, (h // G + 1) * hd)
+            Q, K, V, dO = (a.astype(np.float64) for a in (w.q[b, rq], w.k[b, rk], w.v[b, rk], w.do[b, rq]))
+            z = np.where(ok, w.scale * (Q.T @ K), -np.inf)
+            if o is None:
+                e = np.exp(z - np.where(used, np.max(z, axis=1, initial=-1e300), 0.0)[:, None])
+                p = e / np.where(used, e.sum(1), 1.0)[:, None]
+                out["o"][b, rq] = np.abs(V) @ p.T
+                continue
+            p = np.where(ok, np.exp(np.where(ok, z, 0.0) - np.where(used, lse[b, h], 0.0)[:, None]), 0.0)
+            dO, O = np.where(used, dO, 0.0), np.where(used, o[b, rq].astype(np.float64), 0.0)
+            ds = np.abs(p * (dO.T @ V - (dO * O).sum(0)[:, None]))
+            out["dq"][b, rq] = w.scale * (np.abs(K) @ ds.T)
+            out["dk"][b, rk] += w.scale * (np.abs(Q) @ ds)
+            out["dv"][b, rk] += np.abs(dO) @ p
+    return out
+
+
+def check(c, got, want, mags):
+    _, end = c.plan()
+    for name, mag in mags.items():
+        val, bound = want[name]
+        bound = bound + 1.01 * PAIR * mag
+        top = np.abs(val) + bound
+        half = np.exp2(np.floor(np.log2(np.maximum(top, 2.0 ** -126))) - 8)
+        used = np.broadcast_to((end > 0)[:, None, :], val.shape)
+        over = np.where(used, np.abs(A.from_bf16(got[name]).astype(np.float64) - val) / (bound + half), 0.0)
+        assert np.all(over <= 1.0), (name, float(over.max()), float((over > 1.0).mean()))
+
+
+CASES = [
+    # heads, kv, hd, S, batch, offsets: one, two and four position blocks side by side
+    (4, 2, 64, 200, 2, [[0, 2, 5, 40, 200]] * 2), (2, 1, 128, 130, 1, None), (3, 1, 96, 300, 1, [[0, 3, 300]]),
+    (12, 12, 64, 256, 8, None), (24, 8, 128, 197, 4, None), (24, 24, 72, 140, 6, [[0, 60, 62, 139]] * 6),
+    (64, 32, 64, 300, 3, [[0, 4, 50, 300]] * 3), (64, 64, 128, 270, 3, None), (48, 24, 96, 150, 6, None),
+]
+
+
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_as_exact_as_the_type(br, i):
+    c = A.Case("bf16", *CASES[i], seed=20 + i)
+    w = as_fp32(c)
+    o, lse = A.forward(br, c)
+    check(c, dict(o=o), A.reference(w), magnitudes(w))
+    g = A.backward(br, c, o, lse)
+    O = A.from_bf16(o)
+    check(c, g, A.reference(w, O, lse), magnitudes(w, O, lse))
