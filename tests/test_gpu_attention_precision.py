@@ -74,3 +74,28 @@ def test_as_exact_as_the_type(br, i):
     g = A.backward(br, c, o, lse)
     O = A.from_bf16(o)
     check(c, g, A.reference(w, O, lse), magnitudes(w, O, lse))
+
+
+@pytest.mark.parametrize("hd,S,heads", [(64, 200, 2), (128, 197, 24), (96, 300, 64)])
+def test_own_infinities_are_what_they_were(br, hd, S, heads):
+    """An infinity among a sequence's own values: o is infinite with its sign in that channel from there on, as the formula gives; where
+    two of both signs meet it is NaN.  dv of an infinite do likewise, for the keys that its query sees."""
+    c = A.Case("bf16", heads, heads, hd, S, 1, seed=3)
+    o, lse = A.forward(br, c)
+    for channel, at, value in ((5, 10, np.inf), (6, 70, -np.inf), (7, 5, np.inf), (7, 80, -np.inf)):
+        c.v[0, channel, at] = c.stored(np.full(1, value))[0]
+    got = A.from_bf16(A.forward(br, c)[0])[0, :hd]
+    assert np.all(got[5, 10:] == np.inf) and np.all(got[6, 70:] == -np.inf)
+    assert np.all(got[7, 5:80] == np.inf) and np.all(np.isnan(got[7, 80:]))
+    clean = A.from_bf16(o)[0, :hd]
+    rest = [r for r in range(hd) if r not in (5, 6, 7)]
+    assert np.array_equal(got[rest], clean[rest]) and np.array_equal(got[5, :10], clean[5, :10])
+
+    c = A.Case("bf16", heads, heads, hd, S, 1, seed=3)
+    base = A.backward(br, c, o, lse)
+    c.do[0, 9, 100] = c.stored(np.full(1, np.inf))[0]
+    dv = A.from_bf16(A.backward(br, c, o, lse)["dv"])[0, :hd]
+    assert np.all(dv[9, :101] == np.inf)
+    want = A.from_bf16(base["dv"])[0, :hd]
+    rest = [r for r in range(hd) if r != 9]
+    assert np.array_equal(dv[rest], want[rest]) and np.array_equal(dv[9, 101:], want[9, 101:])
