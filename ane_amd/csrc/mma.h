@@ -220,16 +220,18 @@ __device__ __forceinline__ unsigned lds_place(const char *array) {
 }
 // LDS[place + 16 * lane] = 16 bytes of the buffer at voffset + soffset.  Counts in vmcnt, and nothing but that counter tells when it is there.
 // (With the builtin for it the compiler waits for all loads under way before every transposing read of LDS.)  It has no result register.
+// m0, which it sets, is reserved: the compiler keeps nothing there, refuses to have it named as clobbered, and sets it right before an instruction
+// of its own that needs it; these kernels have none.
 // The compiler does not look into the asm, so its wait states are here: five between a vector instruction that writes a scalar register
 // (readfirstlane, where the compiler does not see by itself that a value is the same in all lanes) and a load that reads it, one between m0 and
-// a load into LDS.  (tests/test_wait_states.py looks the library's code over.  They are in every load, where the values are known to be
+// a load into LDS.  (tests/test_wait_states.py looks the library's code over for both.  They are in every load, where the values are known to be
 // the same too: that costs up to
 // 1 %: gradients of 4096 positions 398 -> 401 us, 32000 x 4096 results of 768 terms 282 -> 285, the others of ten cases no difference.)
 __device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, unsigned place) {
     auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };        // (nothing, where the compiler sees it by itself)
     const rsrc_t u = {uni(r[0]), uni(r[1]), uni(r[2]), uni(r[3])};
     asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-                 :: "v"(voffset), "s"(u), "s"(uni((int)soffset)), "s"(uni((int)place)) : "memory", "m0");
+                 :: "v"(voffset), "s"(u), "s"(uni((int)soffset)), "s"(uni((int)place)) : "memory");
 }
 // All but the newest LEFT of the wave's loads are there and all but its newest READS reads of LDS done, and so are the other waves'.
 template <int LEFT, int READS>

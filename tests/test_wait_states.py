@@ -1,6 +1,6 @@
 """Wait states in front of the loads that write LDS directly (load_to_lds in mma.h).  They are written in inline asm, which the compiler
 does not look into: a scalar register that a vector instruction has written may be read by a memory instruction five wait states later
-at the earliest, and m0 by a load into LDS one after it was written.  The built library's own code is looked over, along every way that
+at the earliest, and m0 by a load into LDS one after it was written; nothing else in a function with such loads may read m0.  The built library's own code is looked over, along every way that
 leads to such a load, whatever the compiler knew of its operands."""
 import os
 import re
@@ -83,6 +83,22 @@ def faults(code):
     return found, loads
 
 
+def other_uses_of_m0(code):
+    """(address, instruction) of what names m0 in a function with loads into LDS, but for the s_mov_b32 of such a load."""
+    found, function, loads = [], [], False
+    for c in code + [None]:
+        if c is None:
+            if loads:
+                found += function
+            function, loads = [], False
+            continue
+        loads |= c[1].startswith("buffer_load") and bool(re.search(r"\blds\b", c[2]))
+        if re.search(r"\bm0\b", c[2]) and not (c[1] == "s_mov_b32" and split(c[2])[0] == "m0") \
+                or c[1].startswith(("s_sendmsg", "v_movrel", "s_set_gpr_idx", "v_interp", "ds_gws")):
+            function.append((hex(c[0]), c[1], c[2]))
+    return found
+
+
 def listing(*lines):
     return "0000000000001000 <f>:\n" + "".join("\t%s // %012X: 00000000\n" % (t, 0x1000 + 4 * i) for i, t in enumerate(lines))
 
@@ -104,6 +120,9 @@ def test_the_looking_over_itself():
             (("s_nop 4", load, "v_readfirstlane_b32 s9, v0", "s_cbranch_vccnz 65533"), True)):      # back to the load
         found, loads = faults(parse(listing(*lines)))
         assert loads == 1 and bool(found) == bad, (lines, found)
+    for line, bad in (("s_mov_b32 m0, s3", False), ("s_mov_b32 s3, m0", True), ("v_readlane_b32 s1, v0, m0", True), ("s_set_gpr_idx_on s0, gpr_idx(SRC0)", True)):
+        assert bool(other_uses_of_m0(parse(listing(line, load)))) == bad, line
+        assert not other_uses_of_m0(parse(listing(line)))
 
 
 def test_loads_into_lds_wait_for_their_scalars(tmp_path):
@@ -112,15 +131,18 @@ def test_loads_into_lds_wait_for_their_scalars(tmp_path):
     import ane_amd.bridge as br
     shutil.copy(br.LIB_PATH, tmp_path / "lib.so")
     subprocess.run([OBJDUMP, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
-    found, loads = [], 0
+    found, loads, m0 = [], 0, []
     for name in sorted(os.listdir(tmp_path)):
         if not name.endswith("gfx950"):
             continue
         text = subprocess.run([OBJDUMP, "-d", name], cwd=tmp_path, check=True, capture_output=True, text=True).stdout
         if " lds" not in text:
             continue
-        f, n = faults(parse(text))
+        code = parse(text)
+        f, n = faults(code)
+        m0 += other_uses_of_m0(code)
         found += [(name,) + x for x in f]
         loads += n
     assert loads > 1000
     assert not found, (len(found), found[:5])
+    assert not m0, (len(m0), m0[:5])
