@@ -152,89 +152,41 @@ __device__ __forceinline__ void finish(const Epilogue &e, float (&v)[8], int m, 
 }
 
 // Tensors go straight into LDS (load_to_lds).  They are aligned: base and S in units of eight values; repack() brings others to that.
-// An operand's 64 steps of the sum for B indexes.  COLUMNS: the sum goes over the rows: B / 64 panels of 64 rows x 64 columns; else over the
-// columns: one panel of B rows.
+// An operand's 64 steps of the sum for B indexes (PanelWalk has the offsets).
 template <int B, bool COLUMNS, int THREADS>
 struct Operand {
-    static constexpr int PANELS = COLUMNS ? B / 64 : 1, ROWS = COLUMNS ? 64 : B, BYTES = B * PANEL_ROW, WAVES = THREADS / 64;
-    static constexpr int PER = ROWS / (8 * WAVES), LOADS = PANELS * PER;        // instructions of a wave to a panel, to a stage
-    static_assert(PER * 8 * WAVES == ROWS && WAVES % 2 == 0, "whole instructions per wave, one swizzle for all of a lane's rows");
+    typedef PanelWalk<B, COLUMNS, THREADS> Walk;
+    static constexpr int BYTES = B * PANEL_ROW, LOADS = Walk::PANELS * Walk::PER;       // of a stage; a wave's instructions to it
     static constexpr int READS = COLUMNS ? 2 : 1;           // reads of LDS to a fragment
-    rsrc_t r;               // begins at the slab that the next load is in
-    unsigned long long bytes;
-    unsigned voff[PANELS];
-    unsigned soff, row_bytes, slab_bytes, wave_at;
-    int rows, cols, S, s0;
-    bool even;              // by columns, or every 64 steps lie in one slab: a lane's offset stays what it is
+    rsrc_t r;
+    Walk walk;
+    unsigned wave_at;
 
     // index0: the tile's first index; sum0: where the sum starts
     __device__ __forceinline__ void begin(const Mat &a, int index0, int sum0) {
-        const int t = threadIdx.x, row = t >> 3, chunk = (t & 7) ^ panel_swz(row);
-        rows = a.rows;
-        cols = a.cols;
-        S = a.S;
-        row_bytes = (unsigned)a.S * 2;
-        slab_bytes = (unsigned)a.rows * row_bytes;
-        wave_at = __builtin_amdgcn_readfirstlane(t >> 6) * 1024;
-        const int first = COLUMNS ? index0 : sum0;              // the first column of all that this reads
-        const int b0 = first / a.S;
-        s0 = first - b0 * a.S;
-        const size_t skip = ((size_t)b0 * a.rows + (COLUMNS ? sum0 : index0)) * a.S;
-        bytes = ((size_t)(a.cols / a.S) * a.rows * a.S - skip) * 2;
-        r = buffer_at(a.p + skip, bytes);
-        even = COLUMNS || a.S % 64 == 0 || a.cols == a.S;
-        soff = COLUMNS ? 0 : s0 * 2;
-#pragma unroll
-        for (int i = 0; i < PANELS; i++) {
-            if (COLUMNS) {
-                const int s = s0 + i * 64 + chunk * 8, db = s / a.S;
-                voff[i] = (((unsigned)db * rows + row) * a.S + (s - db * a.S)) * 2;
-            } else voff[i] = (unsigned)row * row_bytes + chunk * 16;
-        }
+        wave_at = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+        const unsigned long long skip = walk.begin(a.rows, a.S, a.cols, index0, sum0, threadIdx.x);
+        r = buffer_at((const char *)a.p + skip, walk.bytes);
     }
     // the next 64 steps of the sum, `left` of which exist, to a stage of LDS; moves on
     __device__ __forceinline__ void load(unsigned lds, int left) {
         lds += wave_at;
-        if (even && left >= 64) {
+        if (walk.plain(left)) {
 #pragma unroll
-            for (int i = 0; i < PANELS; i++)
+            for (int i = 0; i < Walk::PANELS; i++)
 #pragma unroll
-                for (int j = 0; j < PER; j++)
-                    load_to_lds(r, voff[i], soff + j * 8 * WAVES * row_bytes, lds + i * (64 * PANEL_ROW) + j * WAVES * 1024);
+                for (int j = 0; j < Walk::PER; j++)
+                    load_to_lds(r, walk.voff[i], walk.soffset(j), lds + i * (64 * PANEL_ROW) + j * Walk::WAVES * 1024);
         } else {
-            const int row = threadIdx.x >> 3, chunk = (threadIdx.x & 7) ^ panel_swz(row);
 #pragma unroll
-            for (int i = 0; i < PANELS; i++)
+            for (int i = 0; i < Walk::PANELS; i++)
 #pragma unroll
-                for (int j = 0; j < PER; j++) {
-                    unsigned v = voff[i];
-                    if (COLUMNS) v = row + j * 8 * WAVES < left ? v : OUTSIDE;
-                    else {
-                        for (int s = s0 + chunk * 8; s >= S; s -= S) v += slab_bytes - row_bytes;
-                        v = chunk * 8 < left ? v : OUTSIDE;
-                    }
-                    load_to_lds(r, v, soff + j * 8 * WAVES * row_bytes, lds + i * (64 * PANEL_ROW) + j * WAVES * 1024);
-                }
+                for (int j = 0; j < Walk::PER; j++)
+                    load_to_lds(r, walk.voffset(i, j, left, threadIdx.x), walk.soffset(j), lds + i * (64 * PANEL_ROW) + j * Walk::WAVES * 1024);
         }
-        if constexpr (COLUMNS) {
-            soff += 64 * row_bytes;
-            if (soff >= 1u << 31) {             // rows of up to 2^23 bytes: what 32 bits hold ends after 512 of them
-                const unsigned long long at = ((unsigned long long)(unsigned)r[1] << 32 | (unsigned)r[0]) + soff;
-                bytes = bytes > soff ? bytes - soff : 0;
-                r = buffer_at((const void *)at, bytes);
-                soff = 0;
-            }
-        } else {
-            soff += 128;
-            s0 += 64;
-            if (s0 >= S) {
-                const int n = s0 / S;
-                s0 -= n * S;
-                soff = s0 * 2;
-                const unsigned long long skip = (unsigned long long)n * slab_bytes, at = ((unsigned long long)(unsigned)r[1] << 32 | (unsigned)r[0]) + skip;
-                bytes -= skip;
-                r = buffer_at((const void *)at, bytes);
-            }
+        if (const unsigned long long move = walk.advance()) {
+            const unsigned long long at = ((unsigned long long)(unsigned)r[1] << 32 | (unsigned)r[0]) + move;
+            r = buffer_at((const void *)at, walk.bytes);
         }
     }
     // the fragment of indexes block*32 .. +31 at 16 steps of the sum

@@ -14,6 +14,7 @@
 // touches each at most twice with 512 bytes, a row read of 8 bytes per lane all of them with 16 rows, one of 16 bytes no bank twice
 // with 8 rows.
 #pragma once
+#include "panel_walk.h"
 #include "tile.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -24,7 +25,6 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 constexpr int PANEL_ROW = 128;      // bytes
 
-__device__ __forceinline__ int panel_swz(int row) { return (row >> 1 & 1) << 2 | (row >> 2 & 1) | (row >> 3 & 1) << 1; }
 __device__ __forceinline__ int panel_at(int row, int chunk) { return row * PANEL_ROW + ((chunk ^ panel_swz(row)) << 4); }
 
 // row of register r of a 32 x 32 product, less the 4 that lanes 32..63 add
@@ -205,8 +205,6 @@ __device__ __forceinline__ void over_positions(v16f (&acc)[HDB], const char *pan
 // 16 bytes a lane, the lanes of an instruction one after the other (eight rows of a panel), so what panel_at() would put elsewhere is
 // fetched by another lane instead: lane l reads chunk (l & 7) ^ panel_swz(row) of row l / 8.  Addresses are multiples of 16 bytes.  A read
 // outside of the buffer gives zero.
-constexpr unsigned OUTSIDE = 0xfffffff0u;
-
 typedef int rsrc_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ rsrc_t buffer_at(const void *p, unsigned long long bytes) {
