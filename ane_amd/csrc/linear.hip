@@ -621,8 +621,8 @@ __global__ __launch_bounds__(256) void gemv_kernel(const bf16_t *__restrict__ w,
     }
 }
 
-__global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *__restrict__ dpre, const bf16_t *__restrict__ dy, const bf16_t *__restrict__ pre,
-                                                      float alpha, int act, size_t n) {
+// dpre may be dy: a thread loads what it writes before it does.
+__global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *dpre, const bf16_t *dy, const bf16_t *__restrict__ pre, float alpha, int act, size_t n) {
     const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (i + 8 <= n) {
         float g[8], x[8];
