@@ -10,6 +10,8 @@ namespace {
 // of LDS that feed both take turns in a wave, and two waves to a SIMD overlap part of it.  At 256 positions of 256 heads (50 MB) 16 us or
 // 3.2 TB/s: start, first loads and stores of one round of workgroups.  One sequence of 256 positions, 12 heads of 64 channels, fp32: 10.2 us.
 // A panel has 64 keys (32 in fp32) and is fetched while the one before is used; four waves of 32 queries share it.
+constexpr float FAR = 16777216.f;           // 2^24
+
 // One position block.  CAREFUL: see below; else false where that is needed.  k and v have `pitch` values between rows (PanelStream), q and o S.
 template <typename T, int HDB, int POS, bool CAREFUL>
 __device__ __forceinline__ bool fwd_block(
@@ -108,11 +110,22 @@ __device__ __forceinline__ bool fwd_block(
                 m = to_m;
             }
             const float base = m == -INFINITY ? 0.f : m;
+            // m is rounded and the fused product is not: their difference, up to 2^-24 m, is in every weight of a row and in its sum alike,
+            // until it is beyond what an exponential holds.  From FAR on products are rounded as m is, and the largest is exactly 0 off.
+            float by = scale2;
+            if (__any(fabsf(base) > FAR)) {
+                const bool far = fabsf(base) > FAR;
+#pragma unroll
+                for (int u = 0; u < M::SUBS; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[u][r] = far ? s[u][r] * scale2 : s[u][r];
+                by = far ? 1.f : scale2;
+            }
 #pragma unroll
             for (int u = 0; u < M::SUBS; u++) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, -base));
+                    s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], by, -base));
                     l += s[u][r];
                 }
                 const typename M::Packed p = M::template pack<CAREFUL>(s[u]);

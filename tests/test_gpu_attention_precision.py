@@ -99,3 +99,35 @@ def test_own_infinities_are_what_they_were(br, hd, S, heads):
     want = A.from_bf16(base["dv"])[0, :hd]
     rest = [r for r in range(hd) if r != 9]
     assert np.array_equal(dv[rest], want[rest]) and np.array_equal(dv[9, 101:], want[9, 101:])
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e4, 3e6, 1e12])
+@pytest.mark.parametrize("shape", [(2, 1, 64, 150, 1, None), (24, 8, 96, 200, 4, [[0, 50, 200]] * 4), (64, 64, 128, 270, 3, None)])
+def test_scores_beyond_what_an_exponential_holds(br, storage, size, shape):
+    """Scores of 1e8 to 1e25: all of a row's weight goes to its largest score, one key or several equal ones.  A row is held to that where
+    its second largest score is behind by 100 and by more than both sums' errors (E32 * (hd + 6) of the sums of
+    magnitudes, twice for each); lse has a rounding each of two constants, of scale times one of them, of two products and of a sum."""
+    c = A.Case(storage, *shape, seed=31)
+    f = lambda a: (a if storage == "f32" else A.from_bf16(a))       # noqa: E731
+    c.q, c.k = c.stored(f(c.q) * np.float32(size)), c.stored(f(c.k) * np.float32(size))
+    o, lse = A.forward(br, c)
+    start, end = c.plan()
+    held = 0
+    for b in range(c.batch):
+        ok, used = c.allowed(b), end[b] > 0
+        for h in range(0, c.heads, 5):
+            rq, rk = slice(h * c.hd, (h + 1) * c.hd), slice(h // (c.heads // c.kv) * c.hd, (h // (c.heads // c.kv) + 1) * c.hd)
+            Q, K, V = c.f64(c.q)[b, rq], c.f64(c.k)[b, rk], c.f64(c.v)[b, rk]
+            z = np.where(ok, c.scale * (Q.T @ K), -np.inf)
+            err = A.E32 * (c.hd + 6) * c.scale * (np.abs(Q).T @ np.abs(K))
+            order = np.sort(z, axis=1)
+            gap = order[:, -1] - np.where(np.isfinite(order[:, -2]), order[:, -2], -1e30)
+            clear = used & (gap > 100 + 4 * np.where(ok, err, 0).max(1))
+            got = c.f64(o)[b, rq]
+            assert np.all(np.isfinite(got[:, used])) and np.all(np.isfinite(lse[b, h, used]))
+            best = V[:, z.argmax(1)]
+            assert np.all(np.abs(got - best)[:, clear] <= 8 * A.E32 * np.abs(best)[:, clear])
+            assert np.all(np.abs(lse[b, h] - order[:, -1])[clear] <= (err.max(1) + 7 * A.E32 * np.abs(order[:, -1]))[clear])
+            held += clear.sum()
+    assert held > 100
