@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include "../../include/mi355_bridge.h"
+#include "xcd.h"
 
 #define MI355_API extern "C" __attribute__((visibility("default")))
 
@@ -98,15 +99,6 @@ static inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 // -------------------------------------------------------------------------------------------
 // Device helpers
 // -------------------------------------------------------------------------------------------
-
-// MI355X has 8 XCDs, each with a private L2; consecutive workgroup ids are dealt round-robin
-// to the XCDs.  This maps the hardware id to a logical id so that consecutive LOGICAL ids
-// (neighbouring tiles that share cache lines) run on the same XCD.
-__device__ __forceinline__ int xcd_remap(int bid, int n) {
-    const int q = n >> 3, r = n & 7;
-    const int xcd = bid & 7, idx = bid >> 3;
-    return xcd * q + (xcd < r ? xcd : r) + idx;
-}
 
 __device__ __forceinline__ v4f ld4(const float *p) { return *reinterpret_cast<const v4f_any *>(p); }
 __device__ __forceinline__ void st4(float *p, v4f v) { *reinterpret_cast<v4f_any *>(p) = v; }
