@@ -372,8 +372,8 @@ bool shape_ok(const char *who, int heads, int kv_heads, int hd, int S, int batch
         mi355_fail("%s: head size %d (at most 128)", who, hd);
         return false;
     }
-    if (!(scale > 0.f) || !isfinite(scale)) {
-        mi355_fail("%s: scale must be positive and finite", who);
+    if (!(scale > 0.f) || !isfinite(scale * LOG2E)) {          // (exponents are of base 2)
+        mi355_fail("%s: scale must be positive, and finite times log2(e)", who);
         return false;
     }
     // what a launch can number (2^32 threads, 256 to 64 positions at most), and 32-bit offsets into a head

@@ -171,7 +171,7 @@ int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *p
  * training/training_dynamic/mil_dynamic.h:131-168 on); it takes q and k as mi355_qknorm_rope_fwd_dev / mi355_rope_dev leave them.
  *   p[s][t] = exp(scale q_s.k_t - lse_s) for first_s <= t <= s, o_s = sum_t p[s][t] v_t, lse_s = log sum_t exp(scale q_s.k_t)
  * q, o: [batch][heads*hd][S]; k, v: [batch][kv_heads*hd][S], heads a multiple of kv_heads (query heads h*heads/kv_heads .. share KV
- * head h); lse: [batch][heads][S] fp32, may be NULL when no gradient follows.  hd <= 128, scale > 0, S <= 2^22 and
+ * head h); lse: [batch][heads][S] fp32, may be NULL when no gradient follows.  hd <= 128, 0 < scale <= 2.3e38, S <= 2^22 and
  * heads * batch * ceil(S / 64) < 2^24.
  * bounds: NULL when every row is one sequence of S positions, else the plan of rows into which sequences of different lengths are
  * packed, from mi355_attn_plan_dev, kept for all layers and both directions: bounds[b][0][s] is the first position of the sequence that
@@ -180,7 +180,7 @@ int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *p
  * position's on what later ones hold, infinities and NaNs included (a row whose own values hold one is what the formula gives).
  * Sums and the softmax are fp32; with bfloat16 storage p and the score gradients are multiplied again to 2^-15 of themselves, so a result
  * is as exact as its type lets it be.  A backward call's delta is of o as stored, and its p is as exact as lse is, which is off by up to
- * 2^-22 of itself.
+ * 2^-21 of itself beside what its scores' sums are.
  * Outputs must not overlap inputs.  Deterministic: no atomics. */
 int mi355_attn_fwd_dev(float *o, float *lse, const float *q, const float *k, const float *v, const int32_t *bounds, int heads,
                        int kv_heads, int hd, int S, int batch, float scale);
@@ -198,7 +198,7 @@ int mi355_attn_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, uint16_t *dv, const uint
                             int hd, int S, int batch, float scale);
 /* The plan of packed rows: cu[batch][n_seqs + 1], ascending offsets (device memory): sequence i of row b is cu[b][i] .. cu[b][i+1]-1,
  * of any length, zero included; positions before cu[b][0] and from cu[b][n_seqs] on are in no sequence (a batch padded to S is
- * {0, length}, n_seqs = 1).  bounds: [batch][2][S]. */
+ * {0, length}, n_seqs = 1).  bounds: [batch][2][S].  batch at most 65535, S and n_seqs at most 2^30. */
 int mi355_attn_plan_dev(int32_t *bounds, const int32_t *cu, int n_seqs, int S, int batch);
 
 /* Graphs: record a launch-bound sequence of device-resident ops once, replay it as one submission.  No

@@ -131,3 +131,21 @@ def test_scores_beyond_what_an_exponential_holds(br, storage, size, shape):
             assert np.all(np.abs(lse[b, h] - order[:, -1])[clear] <= (err.max(1) + 7 * A.E32 * np.abs(order[:, -1]))[clear])
             held += clear.sum()
     assert held > 100
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_the_largest_scale(br, storage):
+    """A scale whose product with log2(e) is beyond fp32 is refused; the largest below it gives what the formula does (scores of equal
+    keys: the mean of the values, as good as its sum of 40 terms and a product)."""
+    c = A.Case(storage, 1, 1, 8, 40, 1, seed=33)
+    p, fn = br.DevArray((4096,)).ptr, br.lib.mi355_attn_fwd_dev if storage == "f32" else br.lib.mi355_attn_fwd_bf16_dev
+    bwd = br.lib.mi355_attn_bwd_dev if storage == "f32" else br.lib.mi355_attn_bwd_bf16_dev
+    for scale in (2.5e38, 3.4e38):
+        assert fn(p, p, p, p, p, None, 1, 1, 8, 40, 1, scale) == -1 and "scale" in br.last_error()
+        assert bwd(*[p] * 9, None, 1, 1, 8, 40, 1, scale) == -1
+    c.scale, c.q = 2.3e38, np.zeros_like(c.q)
+    o, _ = A.forward(br, c)
+    v = c.f64(c.v)[0]
+    n = np.arange(1, 41)
+    want, off = v.cumsum(1) / n, 48 * A.E32 * np.abs(v).cumsum(1) / n
+    assert np.all(np.abs(c.f64(o)[0] - want) <= off + A.STEP[storage] * (np.abs(want) + off))
