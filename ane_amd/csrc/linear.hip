@@ -658,10 +658,12 @@ int repack(const char *who, Mat &a, char *&ws) {
 // Tiles of C: 256 x 256 (eight waves, the fewest reads of LDS to a product), 128 x 128 or 64 x 64, the largest of which there are enough.
 // In `need`, how many quarters of a round of the compute units that is, for 256 and for 128; a backward call counts both products' tiles.
 // Measured, us, with 64 / 128 / 256:
-//   forward, sums of 1024: 8192 x 4096 results 153 / 95 / 83, 4096 x 5120 99 / 57 / 71, 4096 x 4096 85 / 46 / 44, 1024 x 2048 10.7 / 13 / 32;
-//            sums of 2048: 768 x 4096 26 / 21 / 39; sums of 4096 and 8192: 1024 x 2048 34 / 32 / 44 and 59 / 49 / 55
-//   both gradients: weights of 1024 x 4096, 4096 columns 258 / 155 / 96, 768 x 2048, 2048 columns 44 / 26 / 58, 768 x 768, 4096 columns
-//            54 / 22 / 54, 1024 columns 10.4 / 13 / 31
+//   forward, sums of 1024: 8192 x 4096 results 165 / 101 / 92, 4096 x 5120 101 / 59 / 75, 4096 x 4096 82 / 45 / 43, 1024 x 2048 10.9 / 14 / 36;
+//            sums of 2048: 768 x 4096 28 / 23.5 / 41; sums of 4096 and 8192: 1024 x 2048 31 / 31 / 43 and 57 / 49 / 55
+//   both gradients: weights of 768 x 2048, 2048 columns 29 / 26 / 44, 768 x 768, 4096 columns 28 / 24 / 41, 1024 columns 9.8 / 14 / 36;
+//            with 128 / 256, tiles of 256: 1024 x 4096, 4096 columns (320) 91 / 104, 2048 x 2048, 8192 columns (320) 142 / 153, 300 x 4200,
+//            4531 columns (340) 76 / 108, 2048 x 4096, 4096 columns (384) 157 / 158, 4096 x 4096, 2048 columns (384) 160 / 156,
+//            32000 x 768, 4096 columns (423) 486 / 447, 4096 x 4096, 4096 columns (512) 306 / 254
 struct Shape { int m, n; };
 int tile_for(std::initializer_list<Shape> products, const int (&need)[2]) {
     const size_t cu = g_ctx.num_cu;
@@ -680,8 +682,8 @@ Work work(const Mat &a, const Mat &b, const Epilogue &e, int M, int N, int out_s
     w.tiles_n = (int)ceil_div(N, tile);
     const size_t tiles = (size_t)w.tiles_m * w.tiles_n, steps = ceil_div(sum, 64);
     // Slices of the sum until every compute unit has work, each with at least four panels of the sum, and only where a workgroup's walk gets
-    // 16 panels shorter: joining them is a launch and two ways through memory.  Forward, 1024 x 2048 results, sums of 4096 in two slices 32 us and
-    // in one 38, of 1024 21 and 13; both gradients of 768 x 768 over 256 columns, in three slices 9.5 us, in one 7.1.
+    // 16 panels shorter: joining them is a launch and two ways through memory.  Forward, 1024 x 2048 results, sums of 4096 in two slices 34.6 us and
+    // in one 39.8, of 1024 12.0 and 11.3; both gradients of 768 x 768 over 256 columns, in three slices 9.6 us, in one 7.4 to 8.1.
     size_t slices = share / tiles;
     if (slices > steps / 4) slices = steps / 4;
     if (slices < 1 || steps - ceil_div(steps, slices) < 16) slices = 1;
@@ -707,8 +709,8 @@ int run(const char *who, Work w0, Work w1, const RowSums &r, int tile, char *ws)
     const int one_first = w1.units && w1.slice_steps > w0.slice_steps;
     if (grid) {
         if (tile == 256) linear_kernel<KIND0, KIND1, 256, 256, 128, 64, 2><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
-        // 128 x 128: with two stages two workgroups share a compute unit, with four one of them reads further ahead.  512 units 20.5 us
-        // with two, 28.6 with four; 256 units of twice the sum 26.1 and 22.7.
+        // 128 x 128: with two stages two workgroups share a compute unit, with four one of them reads further ahead.  512 units 25.8 us
+        // with two, 31.6 with four; 256 units of twice the sum 28.1 and 26.0.
         else if (tile == 128 && grid > (unsigned)g_ctx.num_cu) linear_kernel<KIND0, KIND1, 128, 128, 64, 32, 2><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
         else if (tile == 128) linear_kernel<KIND0, KIND1, 128, 128, 64, 32, 4><<<grid, 512, 0, g_ctx.stream>>>(w0, w1, one_first);
         else linear_kernel<KIND0, KIND1, 64, 64, 32, 32, 4><<<grid, 256, 0, g_ctx.stream>>>(w0, w1, one_first);
@@ -751,8 +753,9 @@ MI355_API int mi355_linear_fwd_bf16_dev(uint16_t *y, uint16_t *pre, const uint16
     e.act = act; e.alpha = alpha; e.bias = bias; e.res = res; e.pre_out = pre; e.out = y;
     const int N = batch * S, kpad = (K + 7) & ~7;
     const size_t xs = (size_t)(N <= 1 ? 1 : N <= 2 ? 2 : 4) * kpad * sizeof(float);
-    // Few columns: 2048 x 1024 weights and 1, 2, 4 columns 4.6, 4.6 and 6.7 us with gemv_kernel, 9.9 to 10.1 with tiles; 4096 x 4096 and 1, 2 columns
-    // 10.3 and 16.2, 13.7 and 14.5; 2048 x 4096 and 4 columns 18.7 and 14.6: it multiplies without the matrix cores.
+    // Few columns: 2048 x 1024 weights and 1, 2, 4 columns 4.6, 4.9 and 7.2 us with gemv_kernel, 10.4 to 10.7 with tiles; 4096 x 4096 and 2 columns
+    // 16.2 and 14.8; 2048 x 4096 and 4 columns 20 and 15: it multiplies without the matrix cores.  One column alone has no such clear limit:
+    // 4096 x 4096 10.4 and 14.4, 32000 x 768 15.5 and 14.3, 8192 x 4096 16.4 and 18.4, 32000 x 2048 27.5 and 24.5, 151936 x 1024 66 and 116.
     if (N <= GEMV_MAX && (double)M * K * N <= 1 << 24 && xs <= 64 * 1024) {
         // at most four workgroups to a compute unit: each fetches x for itself
         const unsigned grid = (unsigned)(ceil_div(M, 4) < 4 * (size_t)g_ctx.num_cu ? ceil_div(M, 4) : 4 * (size_t)g_ctx.num_cu);
@@ -783,7 +786,7 @@ MI355_API int mi355_linear_bwd_bf16_dev(uint16_t *dx, float *dw, float *dbias, c
     Mat g = {dy, M, S, N}, wm = {w, M, K, K}, xm = {x, K, S, N};
     const size_t packed = (dx || dw ? repacked_bytes(g) : 0) + (dx ? repacked_bytes(wm) : 0) + (dw ? repacked_bytes(xm) : 0);
     // both products in one launch and one size of tile; the sum over N columns is as long when they are repacked
-    const int tile = tile_for({{dx ? K : 0, dx ? N : 0}, {dw ? M : 0, dw ? K : 0}}, {5, 3});
+    const int tile = tile_for({{dx ? K : 0, dx ? N : 0}, {dw ? M : 0, dw ? K : 0}}, {6, 3});
     auto works = [&](Work &w0, Work &w1) {
         const size_t cu = g_ctx.num_cu;
         w0 = dx ? work(wm, g, e, K, N, S, M, tile, cu) : Work{};

@@ -67,8 +67,8 @@ def test_forward_in_every_tile(br, i):
 BACKWARD = [  # M, K, S, batch, activation, accumulate, parts; the tile
     (200, 1500, 197, 11, SILU, 0, "dx dw db", 128), (200, 1500, 197, 11, GELU, 0, "dx", 128), (1500, 2100, 200, 3, NONE, 0, "dw", 128),
     (100, 8200, 40, 5, SILU, 0, "dx dw db", 128),           # several sequences of 40 columns, as many units as compute units or fewer
-    (90, 8200, 56, 4, GELU, 1, "dx dw db", 128), (300, 4200, 197, 23, GELU, 0, "dx dw db", 256), (304, 4208, 200, 23, RELU, 0, "dx dw db", 256),
-    (4200, 4300, 40, 7, NONE, 0, "dw db", 128), (4600, 4500, 24, 3, NONE, 1, "dw", 256), (66, 70, 50, 3, SILU, 0, "dx dw db", 64),
+    (90, 8200, 56, 4, GELU, 1, "dx dw db", 128), (300, 4300, 197, 27, GELU, 0, "dx dw db", 256), (304, 4312, 200, 27, RELU, 0, "dx dw db", 256),
+    (4200, 4300, 40, 7, NONE, 0, "dw db", 128), (5000, 5100, 24, 3, NONE, 1, "dw", 256), (66, 70, 50, 3, SILU, 0, "dx dw db", 64),
 ]
 
 
@@ -76,7 +76,7 @@ BACKWARD = [  # M, K, S, batch, activation, accumulate, parts; the tile
 def test_gradients_in_every_tile(br, i):
     M, K, S, B, a, accumulate, parts, tile = BACKWARD[i]
     if br.device_info()[2] == 256:
-        t, n = tile_of([(K, B * S)] * ("dx" in parts) + [(M, K)] * ("dw" in parts), (5, 3), 256)
+        t, n = tile_of([(K, B * S)] * ("dx" in parts) + [(M, K)] * ("dw" in parts), (6, 3), 256)
         assert t == tile, (t, n)
     rng = np.random.default_rng(100 + i)
     normal = lambda *s: to_bf16(rng.standard_normal(s, np.float32))         # noqa: E731
