@@ -42,7 +42,7 @@ template <typename T>
 constexpr int waves_per_simd(int hdb, int pos) { return panel_bytes(hdb, pos) <= 72 * 1024 && (sizeof(T) == 2 || hdb == 2) ? 2 : 1; }
 
 // Keeps accumulators where a kernel of one wave to a SIMD has its products write them.  Without it each tile copied them out of those
-// registers and back: dkv of bf16, 128 channels: 731 vector instructions a tile for 471 with it.
+// registers and back: dkv of bf16, 128 channels: 993 vector instructions a tile for 736 with it.
 template <int HDB>
 __device__ __forceinline__ void in_agprs(v16f (&acc)[HDB]) {
 #pragma unroll
@@ -430,13 +430,13 @@ int pack_rows(const char *who, const T **a, const T **b, size_t rows, int S, int
 // share the walk: team i takes every TEAMS-th tile of it, with panels of its own.  Four side by side where that gives every compute unit two
 // workgroups; else two by two, where that gives it `two_from` half workgroups; else one position block to four teams.  Measured on 256
 // compute units with four / two / one side by side, us:
-//   four blocks of 512, 1024 of two: forward, bfloat16, 128 channels, 4096 positions of 16 heads 108 / 146 / 213
-//   192, 384: forward, 64 channels, 256 positions of 96 heads: bfloat16 9.5 / 7.6 / 16.9, fp32 24.5 / 18.7 / 25.5; all gradients: bfloat16
-//             27.4 / 24.7 / 34.1, fp32 71.0 / 63.9 / 70.0
-//   128, 256: 128 channels, 512 positions of 32 heads, bfloat16: forward 17.0 / 13.4 / 17.5, all gradients (only dq changed) 41.9 / 36.6 /
-//             42.2; but dk and dv, 64 channels, 1024 positions of 16 heads for 48: 113 / 71.8 / 59.8, and fp32, 2048 positions of 8 heads:
-//             forward 156 / 81.5 / 56.5, with dk and dv 352 / 219 / 163
-//   32, 64:   forward, bfloat16, 96 channels, 1024 positions of 4 heads 24.2 / 17.8 / 13.2
+//   four blocks of 512, 1024 of two: forward, bfloat16, 128 channels, 4096 positions of 16 heads 141 / 181 / 242
+//   192, 384: forward, 64 channels, 256 positions of 96 heads: bfloat16 10.2 / 7.9 / 17.5, fp32 25.2 / 19.0 / 26.2; all gradients: bfloat16
+//             32 / 21.6 / 37, fp32 76 / 57 / 72
+//   128, 256: 128 channels, 512 positions of 32 heads, bfloat16: forward 20.0 / 15.4 / 19.3, all gradients (only dq changed) 57 / 51 /
+//             56; but all gradients (only dk and dv changed), 64 channels, 1024 positions of 16 heads for 48: 140 / 89 / 74, and fp32, 2048
+//             positions of 8 heads: forward 158 / 83 / 58, all gradients (both changed) 491 / 258 / 164
+//   32, 64:   forward, bfloat16, 96 channels, 1024 positions of 4 heads 29.0 / 20.6 / 14.7
 constexpr int TWO_FROM = 3;                                                     // half workgroups to a compute unit
 template <typename T>
 constexpr int TWO_FROM_QUERIES = sizeof(T) == 2 ? 2 : TWO_FROM;                 // (the forward pass and dq)

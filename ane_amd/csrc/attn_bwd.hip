@@ -5,9 +5,10 @@ namespace {
 
 // ---- backward: dq and delta -----------------------------------------------------------------------------------------------------
 
-// Three products of 2 * hd operations for each allowed pair.  bfloat16, 4096 positions of 16 heads, 128 channels: 135 us, 760 TFLOP/s, bound
-// like the forward pass by a tile's products, exponentials and reads of LDS in turn.  fp32, 256 positions of 128 heads, 128 channels: 53 us
-// (61 TFLOP/s of 150: two rounds of workgroups, each 128 KB of LDS, whose start and end nothing overlaps).
+// Three products of 2 * hd operations for each allowed pair, four where score gradients are pairs.  bfloat16, 4096 positions of 16 heads, 128
+// channels: 173 us in a kernel trace (167 to 184), 600 TFLOP/s of the three, bound like the forward pass by a tile's products, exponentials
+// and reads of LDS in turn.  fp32, 256 positions of 128 heads, 128 channels: 53 us (61 TFLOP/s of 150: two rounds of workgroups, each 128 KB
+// of LDS, whose start and end nothing overlaps).
 // One position block; CAREFUL as in the forward pass.  k and v have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int POS, bool CAREFUL>
 __device__ __forceinline__ bool dq_block(

@@ -6,17 +6,18 @@ namespace {
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------------
 
 // bfloat16 and up to 64 channels: what a wave keeps fits 256 registers, so two workgroups share a compute unit if their LDS lets them, which
-// four teams' panels for two tiles do not.  One tile at a time and two workgroups: 1024 positions of 96 heads 95 us (all gradients) where
-// one workgroup with two tiles took 111; packed rows of 997 positions, 12 heads for 48, 64.3 and 68.
+// four teams' panels for two tiles do not.  One tile at a time and two workgroups: 1024 positions of 96 heads 115 us (all gradients) where
+// one workgroup with two tiles took 133; 16 heads for 48, 69.5 and 76.5; packed rows of 997 positions, 16 for 48, 71 and 75.
 template <typename T>
 constexpr bool two_workgroups(int hdb) { return sizeof(T) == 2 && hdb == 2; }
 template <typename T>
 constexpr int dkv_stages(int hdb, int teams) { return two_workgroups<T>(hdb) && teams == 4 ? 1 : stages_for(hdb, teams); }
 
-// Four products of 2 * hd operations for each allowed pair, and two accumulators: one wave to a SIMD beyond 64 channels of bfloat16.
-// bfloat16, 4096 positions of 16 heads over 8, 128 channels: 190 us, 720 TFLOP/s; what a tile does comes one after the other in that
-// wave.  fp32, 256 positions of 128 heads over 64: 68 us, 64 TFLOP/s of 150 in two rounds of workgroups, each 37 us: 23 the walk, 11 own
-// positions, first loads, the teams' sums and stores.
+// Four products of 2 * hd operations for each allowed pair, six where weights and score gradients are pairs, and two accumulators: one wave to
+// a SIMD beyond 64 channels of bfloat16.  bfloat16, 4096 positions of 16 heads over 8, 128 channels: 277 us in a kernel trace (262 to 298; both
+// kernels are slower there than in the 386 us that an untraced call takes), 500 TFLOP/s of the four; what a tile does comes one after the other
+// in that wave.  fp32, 256 positions of 128 heads over 64: 68 us, 64 TFLOP/s of 150 in two rounds of workgroups, each 37 us: 23 the walk, 11
+// own positions, first loads, the teams' sums and stores.
 // One position block; CAREFUL as in the forward pass.  q and d_o have `pitch` values between rows (PanelStream), the others S.
 template <typename T, int HDB, int POS, bool CAREFUL>
 __device__ __forceinline__ bool dkv_block(

@@ -5,10 +5,11 @@ namespace {
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 
-// Two products of 2 * hd operations for each allowed pair.  What bounds it: at 4096 positions of 16 heads, 128 channels, bfloat16, 106 us or
-// 650 TFLOP/s, the walk of the last block over its 64 tiles, 1.6 us each: products (34 cycles for 32 x 32 x 16), exponentials and the reads
-// of LDS that feed both take turns in a wave, and two waves to a SIMD overlap part of it.  At 256 positions of 256 heads (50 MB) 16 us or
-// 3.2 TB/s: start, first loads and stores of one round of workgroups.  One sequence of 256 positions, 12 heads of 64 channels, fp32: 10.2 us.
+// Two products of 2 * hd operations for each allowed pair, three where weights are pairs.  What bounds it: at 4096 positions of 16 heads, 128
+// channels, bfloat16, 133 to 142 us or 500 TFLOP/s of the two, the walk of the last block over its 64 tiles, 2.1 us each: products (34 cycles for
+// 32 x 32 x 16), exponentials, the weights' second halves and the reads of LDS that feed all take turns in a wave, and two waves to a SIMD
+// overlap part of it.  At 256 positions of 256 heads (50 MB) 18 us or 2.8 TB/s: start, first loads and stores of one round of workgroups.
+// One sequence of 256 positions, 12 heads of 64 channels, fp32: 10.4 us.
 // A panel has 64 keys (32 in fp32) and is fetched while the one before is used; four waves of 32 queries share it.
 constexpr float FAR = 16777216.f;           // 2^24
 

@@ -456,10 +456,11 @@ __device__ __forceinline__ void product_unit(const Work &w, int unit, char *lds)
     }
 }
 
-// What bounds it: 256 x 256 tiles, 32000 x 4096 results of 768 terms 275 us, 730 TFLOP/s (a library product of that size 205): a tile takes
-// 26 us of which 18 are the sum's products at 1.5 times what the matrix cores alone need, 7.3 the way of its 128 KB of results to memory,
-// and its successor starts 3.5 later, with nobody else on the compute unit.  128 x 128 tiles: 1024 x 4096 results of 2048 terms with the
-// residual 23 to 25 us, 690 TFLOP/s (the library's product alone 24.5).  Both gradients of that layer 66 us, 520 TFLOP/s, of which 57 for the products.
+// What bounds it: 256 x 256 tiles, 32000 x 4096 results of 768 terms 270 to 290 us, 720 TFLOP/s (a library product of that size 205 to 208; in a
+// kernel trace, whose calls follow one another less closely, 278 to 354): a tile takes 26 us of which 18 are the sum's products at 1.5
+// times what the matrix cores alone need, 7.3 the way of its 128 KB of results to memory, and its successor starts 3.5 later, with nobody
+// else on the compute unit.  128 x 128 tiles: 1024 x 4096 results of 2048 terms with the residual 25 to 29 us from one card to another, 640
+// TFLOP/s (the library's product alone 24.6).  Both gradients of that layer 53 to 62 us, 600 TFLOP/s, of which 9 for the slices and row sums.
 // The units of one or two products, a workgroup to each, neighbours on one XCD (xcd_remap).  (As many workgroups as run
 // at once, each with several units: 278 -> 297 us for 32000 x 4096 results.  A unit's first loads then come behind the stores of the one
 // before, and so does the wait for them.)
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(BM / WM *BN / WN * 64) void linear_kernel(Work w0, 
     }
 }
 
-// (8 rows of 197 positions x 768 channels: 4 to 5 us, of 21 for the whole call; read from there as often as tiles need it.)
+// (8 rows of 197 positions x 768 channels: 4 to 6 us, of 21.4 for the whole call; read from there as often as tiles need it.)
 // A tensor whose rows begin at any value, as one of [rows][cols8] whose rows begin at multiples of eight: zeros from its last column on.
 __global__ __launch_bounds__(256) void repack_kernel(bf16_t *__restrict__ out, Mat a, int cols8) {
     const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(256) void gemv_kernel(const bf16_t *__restrict__ w,
     }
 }
 
-// dpre may be dy: a thread loads what it writes before it does.
+// dpre may be dy: a thread loads what it writes before it does.  Three tensors once: 2^20 values 3.7 us, 2^25 33.5 or 6.0 TB/s, 2^27 125 or 6.5.
 __global__ __launch_bounds__(256) void act_bwd_kernel(bf16_t *dpre, const bf16_t *dy, const bf16_t *__restrict__ pre, float alpha, int act, size_t n) {
     const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (i + 8 <= n) {
