@@ -109,3 +109,16 @@ def test_gradients_in_every_tile(br, i):
         close(db.numpy(), want, E32 * (n + 6) * np.abs(G).sum(1) + 2 * E32 * (np.abs(want) + np.abs(db0)))
     else:
         assert np.array_equal(db.numpy(), db0)
+
+
+@pytest.mark.parametrize("M,K,S,B", [(300, 200, 1, 2), (130, 96, 75, 3), (1500, 72, 197, 11), (1500, 136, 200, 17), (4300, 24, 197, 39), (77, 4096, 40, 1), (2050, 2048, 1, 4)])
+def test_residual_in_place_in_every_tile(br, M, K, S, B):
+    """y may be res: the same bits as into another tensor, by rows, in every tile and by way of slices; pre beside it."""
+    rng = np.random.default_rng(M)
+    x, w = to_bf16(rng.standard_normal((B, K, S), np.float32)), to_bf16(rng.standard_normal((M, K), np.float32) / np.float32(np.sqrt(K)))
+    res = to_bf16(rng.standard_normal((B, M, S), np.float32))
+    want, wpre = run_forward(br, x, w, None, SILU, res, -0.25)
+    D = br.DevArray.from_numpy
+    y, xd, wd, pre = D(res), D(x), D(w), br.DevArray((B, M, S), np.uint16)
+    br.check(br.lib.mi355_linear_fwd_bf16_dev(y.ptr, pre.ptr, xd.ptr, wd.ptr, None, SILU, y.ptr, -0.25, M, K, S, B))
+    assert np.array_equal(y.numpy(), want) and np.array_equal(pre.numpy(), wpre)
