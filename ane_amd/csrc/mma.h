@@ -223,8 +223,8 @@ __device__ __forceinline__ unsigned lds_place(const char *array) {
 // The compiler does not look into the asm, so its wait states are here: five between a vector instruction that writes a scalar register
 // (readfirstlane, where the compiler does not see by itself that a value is the same in all lanes) and a load that reads it, one between m0 and
 // a load into LDS.  (tests/test_wait_states.py looks the library's code over for both.  They are in every load, where the values are known to be
-// the same too: that costs up to
-// 1 %: gradients of 4096 positions 398 -> 401 us, 32000 x 4096 results of 768 terms 282 -> 285, the others of ten cases no difference.)
+// the same too, at up to 1 %: gradients of 4096 positions 398 -> 401 us, 32000 x 4096 results of 768 terms 282 -> 285, the others of ten cases
+// no difference.)
 __device__ __forceinline__ void load_to_lds(rsrc_t r, unsigned voffset, unsigned soffset, unsigned place) {
     auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };        // (nothing, where the compiler sees it by itself)
     const rsrc_t u = {uni(r[0]), uni(r[1]), uni(r[2]), uni(r[3])};

@@ -180,8 +180,8 @@ int mi355_act_bwd_bf16_dev(uint16_t *dpre, const uint16_t *dy, const uint16_t *p
  * position's on what later ones hold, infinities and NaNs included (a row whose own values hold one is what the formula gives).
  * Sums and the softmax are fp32; with bfloat16 storage p and the score gradients are multiplied again to 2^-15 of themselves, so a result
  * is as exact as its type lets it be.  A backward call's delta is of o as stored (bfloat16 sequences of a few positions: dq and dk are off
- * by up to twice the rounding of their type), and its p is as exact as lse is, which is off by up to
- * 2^-21 of itself beside what its scores' sums are.
+ * by up to twice the rounding of their type), and its p is as exact as lse is, which is off by up to 2^-21 of itself beside what its
+ * scores' sums are.
  * Outputs must not overlap inputs.  Deterministic: no atomics. */
 int mi355_attn_fwd_dev(float *o, float *lse, const float *q, const float *k, const float *v, const int32_t *bounds, int heads,
                        int kv_heads, int hd, int S, int batch, float scale);
