@@ -39,6 +39,12 @@ class CkptHdr(C.Structure):
                 [(n, C.c_int) for n in ("cum_steps", "cum_batches", "adam_t", "kv_heads", "head_dim", "q_dim")])
 
 
+class KvCache(C.Structure):
+    """A layer's paged cache (``mi355_kv_cache``): device addresses and sizes."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pages", C.c_void_p)] + [
+        (n, C.c_int) for n in ("n_pages", "page", "n_seqs", "max_pages", "kv_heads", "hd")]
+
+
 CK_TENSORS = ("WQ", "WK", "WV", "WO", "W1", "W2", "W3", "RMS_ATT", "RMS_FFN", "RMS_FINAL", "EMBED")
 
 # name -> (restype, argtypes); every symbol include/mi355_bridge.h declares
@@ -131,6 +137,14 @@ SIGNATURES = {
     "mi355_attn_fwd_bf16_dev": (_i, [_p] * 6 + [_i] * 5 + [_f]),
     "mi355_attn_bwd_dev": (_i, [_p] * 10 + [_i] * 5 + [_f]),
     "mi355_attn_bwd_bf16_dev": (_i, [_p] * 10 + [_i] * 5 + [_f]),
+    "mi355_kv_append_dev": (_i, [C.POINTER(KvCache)] + [_p] * 8 + [_i] * 3 + [_p, _p, _i, _f]),
+    "mi355_kv_append_bf16_dev": (_i, [C.POINTER(KvCache)] + [_p] * 8 + [_i] * 3 + [_p, _p, _i, _f]),
+    "mi355_attn_paged_dev": (_i, [C.POINTER(KvCache)] + [_p] * 5 + [_i] * 3 + [_f]),
+    "mi355_attn_paged_bf16_dev": (_i, [C.POINTER(KvCache)] + [_p] * 5 + [_i] * 3 + [_f]),
+    "mi355_beam_step_dev": (_i, [_p] * 7 + [_i] * 6),
+    "mi355_beam_step_bf16_dev": (_i, [_p] * 7 + [_i] * 6),
+    "mi355_kv_reorder_dev": (_i, [C.POINTER(KvCache), _i] + [_p] * 6 + [_i]),
+    "mi355_kv_reorder_bf16_dev": (_i, [C.POINTER(KvCache), _i] + [_p] * 6 + [_i]),
     "mi355_workspace_size": (_z, []),
     "mi355_graph_begin": (_i, []),
     "mi355_graph_end": (_p, []),

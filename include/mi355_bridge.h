@@ -202,6 +202,72 @@ int mi355_attn_bwd_bf16_dev(uint16_t *dq, uint16_t *dk, uint16_t *dv, const uint
  * {0, length}, n_seqs = 1).  bounds: [batch][2][S].  batch at most 65535, S and n_seqs at most 2^30. */
 int mi355_attn_plan_dev(int32_t *bounds, const int32_t *cu, int n_seqs, int S, int batch);
 
+/* Generating text: a paged cache of keys and values, attention of new tokens over it, and beam search.  No counterpart in the reference, whose
+ * loops train.  Columns as everywhere: column n = b * S + s of [batch][channels][S] is one token, so a step of N sequences is S = N, batch = 1
+ * (as mi355_linear_fwd_bf16_dev takes its columns best) or S = 1, batch = N, and a prompt is S positions of one sequence.
+ *
+ * The cache of a layer is k and v, [n_pages][kv_heads][page][hd] each, fp32 or bfloat16, allocated by the caller at a multiple of 16 bytes;
+ * pages[n_seqs][max_pages] (device memory) names the pages of each sequence in order: position p of sequence i is row p % page of page
+ * pages[i][p / page].  page: a multiple of 16, at most 65536; hd: a multiple of 8, at most 128.  One table serves all layers.  Entries
+ * behind a sequence's last page are not read; an entry outside [0, n_pages) is no page: nothing is written there, and attention leaves its
+ * positions out.  The struct is read during the call only. */
+typedef struct mi355_kv_cache {
+    void *k, *v;                /* device memory */
+    const int32_t *pages;       /* device memory */
+    int n_pages, page, n_seqs, max_pages, kv_heads, hd;
+} mi355_kv_cache;
+/* Appends the keys and values of new tokens, through the per-head norm and the rotation of mi355_qknorm_rope_fwd_dev at each token's own
+ * position.  Column n is position pos[n] of sequence seq[n] (seq NULL: of sequence n).
+ *   q_out = rotate(norm(q, wq), pos), the cache's k = rotate(norm(k, wk), pos), its v = v
+ * q, q_out: [batch][heads*hd][S] (both NULL and heads = 0: keys and values only; q_out may be q); k, v: [batch][kv_heads*hd][S]; wq, wk: [hd]
+ * fp32, NULL for no norm; cos, sin: [hd/2][table], as mi355_rope_tables_dev(.., table, hd, theta) gives them, both NULL for no rotation.
+ * A column whose sequence is not in [0, n_seqs), whose position is negative, behind max_pages * page or behind the table of angles, or whose page
+ * is none, is no token: nothing of it is written.  Of two columns with one place either may stay.  batch * S at most 2^22, heads at most 2^14,
+ * kv_heads at most 4096. */
+int mi355_kv_append_dev(const mi355_kv_cache *cache, float *q_out, const float *q, const float *k, const float *v, const float *wq,
+                        const float *wk, const int32_t *seq, const int32_t *pos, int heads, int S, int batch, const float *cos_dev,
+                        const float *sin_dev, int table, float eps);
+int mi355_kv_append_bf16_dev(const mi355_kv_cache *cache, uint16_t *q_out, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                             const float *wq, const float *wk, const int32_t *seq, const int32_t *pos, int heads, int S, int batch,
+                             const float *cos_dev, const float *sin_dev, int table, float eps);
+/* Attention of each column over positions 0 .. pos[n] of sequence seq[n] (seq NULL: of sequence n), its own, which is in the cache, among them:
+ *   p_t = exp(scale q.k_t - lse), o = sum_t p_t v_t, lse = log sum_t exp(scale q.k_t)
+ * q, o: [batch][heads*hd][S], heads a multiple of kv_heads (query heads as in mi355_attn_fwd_dev); lse: [batch][heads][S] fp32, may be NULL.
+ * 0 < scale <= 2.3e38.  Columns may share a sequence (several new tokens of one, each at its position) and sequences pages.  A column that is
+ * no token (as above), or that has no page at all, is not written.  What lies in a page behind a column's position has no influence,
+ * infinities and NaNs included.  Sums and the softmax are fp32.  Deterministic.  o must not overlap q.  The workspace holds the partial sums of
+ * sequences that several workgroups share. */
+int mi355_attn_paged_dev(const mi355_kv_cache *cache, float *o, float *lse, const float *q, const int32_t *seq, const int32_t *pos, int heads,
+                         int S, int batch, float scale);
+int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *lse, const uint16_t *q, const int32_t *seq, const int32_t *pos,
+                              int heads, int S, int batch, float scale);
+/* A step of beam search.  logits: [batch][V][S], column n = b * S + s the next token's logits of beam n; groups of `beams` consecutive columns
+ * (batch * S a multiple of it) are the beams of a prompt.  score[batch*S]: log probabilities so far; done[batch*S]: beams that have ended
+ * (nonzero; NULL: none).
+ *   candidate (n, v) = score[n] + (logits[v] - log sum_u exp(logits[u])); of an ended beam score[n] for v = pad and -inf for every other v
+ * The `beams` largest candidates of a group, equal ones in the order of (n, v), become its new beams, best first: score_out, token = v, parent = n
+ * (a column's number), done_out (may be NULL) = done[n] or v == eos (eos < 0: no token ends a beam).  A candidate that is NaN counts as -inf.
+ * A greedy step is beams = 1; a group's first step has scores 0, -inf, -inf, ...
+ * Exponentials and blocks' sums are fp32, sums over the vocabulary and candidates fp64, so that equal candidates stay equal.  Outputs must not
+ * overlap inputs.  beams at most 64, batch * S at most 2^22, V * beams below 2^31.  Deterministic; the workspace holds partial sums. */
+int mi355_beam_step_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const float *logits, const float *score,
+                        const int32_t *done, int V, int S, int batch, int beams, int eos, int pad);
+int mi355_beam_step_bf16_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const uint16_t *logits, const float *score,
+                             const int32_t *done, int V, int S, int batch, int beams, int eos, int pad);
+/* The cache follows the beams: sequence n becomes its parent, in the `count` caches (host array; the layers of a model, of one shape and table) at
+ * once.  pos[n_seqs]: each sequence's last position; a sequence and its parent are at the same one (one that is not, or is given a parent
+ * outside [0, n_seqs), stays as it is).  pages_out[n_seqs][max_pages], the new table: pages before the one that holds pos are the parent's; pages
+ * behind it stay n's own; the one that holds it is the parent's where that is n itself or where the page is full, else spare[n], into
+ * which the parent's rows are copied.  spare_out[n] is then n's former page, else spare[n].  pos_out (may be NULL) = pos + advance (a negative
+ * pos, nothing held, stays).
+ * With pages of its own for all its positions and one spare page for each sequence at the start, every page that is written to has one owner, and
+ * no page is freed or allocated in between.  pages_out, pos_out and spare_out must not overlap the tables they come from; the
+ * next calls use pages_out.  n_seqs * kv_heads below 2^24. */
+int mi355_kv_reorder_dev(const mi355_kv_cache *caches, int count, int32_t *pages_out, int32_t *pos_out, int32_t *spare_out,
+                         const int32_t *parent, const int32_t *pos, const int32_t *spare, int advance);
+int mi355_kv_reorder_bf16_dev(const mi355_kv_cache *caches, int count, int32_t *pages_out, int32_t *pos_out, int32_t *spare_out,
+                              const int32_t *parent, const int32_t *pos, const int32_t *spare, int advance);
+
 /* Graphs: record a launch-bound sequence of device-resident ops once, replay it as one submission.  No
  * counterpart in the reference (its ops are synchronous CPU calls).  Between begin and end the *_dev ops are
  * recorded instead of run; calls that allocate, wait or touch the host (buf_alloc/free/read/write, sync,
