@@ -1,54 +1,570 @@
 // attn_paged.hip — attention of one new token over a paged cache of keys and values.
 //   p_t = exp(scale q.k_t - lse) for 0 <= t <= pos,  o = sum_t p_t v_t,  lse = log sum_t exp(scale q.k_t)
+//
+// Every key and value is read once for the query heads that share it, and little is computed with it: the time is that of reading the cache.
+// So a wave takes tiles of 32 positions (fp32: 16), 16 KB of keys and values at 128 channels, straight into registers, the next tile under way
+// while one is used, with nothing shared between waves and no barrier on the way: eight waves to a compute unit keep 128 KB in flight.
+//
+// Both products run on the matrix cores, with up to 16 query heads of a KV head for their columns (a group of two leaves 14 of them empty, and the
+// products still take a tenth of the time that the reading does):
+//   scores[position][head] = K q:  a lane's operand is 16 bytes of a row of the cache, position lane % 16, as it lies in memory;
+//   o[channel][head] += V' p:      p is taken from the registers that the scores are in: register r of lane l is position 4 (l / 16) + r, so the
+//                                  lane reads the values of just these positions.  In bfloat16 an operand is eight positions of a
+//                                  channel: the lane holds eight rows of 8 (4) channels and exchanges halves of words between them.
+// The running maximum is brought up to date only when a score passes it, which is rare after the first tiles, so lanes hardly ever talk.
 #include "kv_cache.h"
+#include "mma.h"
 
 #include <math.h>
 
 namespace {
 
 constexpr float LOG2E = 1.44269502162933349609375f, LN2 = 0.693147182464599609375f;
+constexpr float FAR = 16777216.f;           // 2^24
+constexpr int HEADS = 16;                   // query heads of one product
+constexpr int WAVES = 4;
+constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
 __device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// A wave to a head of a column; two channels to a lane.
-template <typename T>
-__global__ __launch_bounds__(64) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q, mi355_kv_cache c,
-                                                        const int *__restrict__ seqs, const int *__restrict__ pos, int heads, int S, float scale2) {
-    const int lane = threadIdx.x, hd = c.hd;
-    const size_t unit = blockIdx.x, col = unit / heads;
-    const int head = (int)(unit - col * heads), kvh = head / (heads / c.kv_heads), b = (int)(col / S), s = (int)(col - (size_t)b * S), at = pos[col];
-    const int seq = seqs ? seqs[col] : (int)col;
-    if (paged_entry(seq, at, c.n_seqs, c.max_pages, c.page) < 0) return;
-    const bool mine0 = lane < hd, mine1 = lane + 64 < hd;
-    const T *qp = q + ((size_t)b * heads + head) * hd * S + s;
-    const float q0 = mine0 ? load_one(qp + (size_t)lane * S) : 0.f, q1 = mine1 ? load_one(qp + (size_t)(lane + 64) * S) : 0.f;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    bool any = false;
-    for (int t = 0; t <= at; t++) {
-        const int id = c.pages[paged_entry(seq, t, c.n_seqs, c.max_pages, c.page)];
-        if (!paged_id_ok(id, c.n_pages)) continue;
-        any = true;
-        const size_t row = paged_row(id, kvh, t % c.page, c.kv_heads, c.page, hd);
-        const T *k = (const T *)c.k + row, *v = (const T *)c.v + row;
-        float z = mine0 ? q0 * load_one(k + lane) : 0.f;
-        if (mine1) z += q1 * load_one(k + lane + 64);
-        z = wave_sum_stride<1>(z) * scale2;
-        const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(z - base);
-        m = top;
-        l = l * f + p;
-        o0 = o0 * f + (mine0 ? p * load_one(v + lane) : 0.f);
-        o1 = o1 * f + (mine1 ? p * load_one(v + lane + 64) : 0.f);
+struct PagedArgs {
+    mi355_kv_cache c;
+    const int *seq, *pos;
+    int heads, S, cols, group;      // group: query heads of a KV head
+    float scale2;
+    float *slots;                   // partial results: two for each workgroup
+    unsigned *arrived;
+};
+
+// ---- the parts of a tile that depend on the type ----
+
+template <typename T, int HDB> struct Tile;
+
+template <int HDB> struct Tile<bf16_t, HDB> {
+    static constexpr int PIECES = 2, POSITIONS = 32;            // pieces of 16 positions, each in one page
+    static constexpr int VC = HDB > 2 ? 8 : 4, ACC = VC;        // channels of V to a lane; products of 16 channels each
+    typedef unsigned Vec __attribute__((ext_vector_type(VC / 2), aligned(VC * 2)));
+    typedef bf16x8 Q;
+    static constexpr int QS = HDB;
+    v4u k[PIECES][HDB];
+    Vec v[8];
+    static __device__ __forceinline__ int channel(int acc, int r, int g) { return VC * (4 * g + r) + acc; }
+    static __device__ __forceinline__ Q query(const float *row, int s) {        // LDS: fp32 values of a head
+        const float *p = row + 32 * s + 8 * ((threadIdx.x & 63) >> 4);
+        const v4u w = {f2_to_bf2(p[0], p[1]), f2_to_bf2(p[2], p[3]), f2_to_bf2(p[4], p[5]), f2_to_bf2(p[6], p[7])};
+        return __builtin_bit_cast(Q, w);
     }
-    if (!any) return;
-    T *op = o + ((size_t)b * heads + head) * hd * S + s;
-    if (mine0) store_one(op + (size_t)lane * S, o0 / l);
-    if (mine1) store_one(op + (size_t)(lane + 64) * S, o1 / l);
-    if (lse && lane == 0) lse[((size_t)b * heads + head) * S + s] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    // Bytes from the first of a piece's 16 rows to what the lane reads of them (channels behind the last: other ones in their place).
+    struct Offsets { unsigned k, k_last, v, v_row; };
+    static __device__ __forceinline__ Offsets offsets(int hd) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 8 * g;
+        return {(unsigned)(i * hd + 8 * g) * 2, (unsigned)(i * hd + (tail < hd ? tail : 0)) * 2, (unsigned)(4 * g * hd + (VC * i < hd ? VC * i : 0)) * 2, (unsigned)hd * 2};
+    }
+    __device__ __forceinline__ void load(const char *kp, const char *vp, int piece, const Offsets &o) {
+#pragma unroll
+        for (int s = 0; s < HDB; s++) k[piece][s] = *reinterpret_cast<const v4u *>(kp + (s < HDB - 1 ? o.k + 64 * s : o.k_last));
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[4 * piece + r] = *reinterpret_cast<const Vec *>(vp + r * o.v_row + o.v);
+    }
+    // channels behind the last count as zero; q has zeros there, but what was read in their place may be no number
+    __device__ __forceinline__ void trim(int hd) {
+        if ((hd & 31) == 0) return;
+        const bool in = 32 * (HDB - 1) + 8 * ((threadIdx.x & 63) >> 4) < hd;
+#pragma unroll
+        for (int p = 0; p < PIECES; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) k[p][HDB - 1][e] = in ? k[p][HDB - 1][e] : 0u;
+    }
+    __device__ __forceinline__ v4f scores(const Q (&q)[QS], int piece) const {
+        v4f s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < HDB; j++) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[piece][j]), q[j], s, 0, 0, 0);
+        return s;
+    }
+    __device__ __forceinline__ void hide(int piece, int r) { v[4 * piece + r] = Vec(0u); }
+    // acc += V' p.  A weight is a pair of bfloat16 values, its upper half and what that leaves of it: off by 2^-15 of it, where one value
+    // alone is off by as much as the rounding of the result (2^-8).  ODD: infinities and NaNs among the values count as zero.
+    template <bool ODD>
+    __device__ __forceinline__ void weigh(v4f (&acc)[ACC], const v4f (&p)[PIECES]) const {
+        v4u hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = p[i >> 1][2 * (i & 1)], y = p[i >> 1][2 * (i & 1) + 1];
+            const unsigned a = __float_as_uint(x), b = __float_as_uint(y);
+            hi[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            float ra = x - __uint_as_float(a & 0xffff0000u), rb = y - __uint_as_float(b & 0xffff0000u);
+            lo[i] = f2_to_bf2(ra, rb);
+        }
+#pragma unroll
+        for (int c = 0; c < VC; c++) {
+            v4u w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_perm(v[2 * i + 1][c >> 1], v[2 * i][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+            if (ODD) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+                    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+                }
+            }
+            const bf16x8 a = __builtin_bit_cast(bf16x8, w);
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, lo), acc[c], 0, 0, 0);
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, hi), acc[c], 0, 0, 0);
+        }
+    }
+};
+
+template <int HDB> struct Tile<float, HDB> {
+    static constexpr int PIECES = 1, POSITIONS = 16;
+    static constexpr int WIDE = HDB > 2 ? 2 : 1, ACC = 4 * WIDE;        // 16 lanes read 64 channels of a row at a time
+    typedef v4f Q;
+    static constexpr int QS = 2 * HDB;
+    v4f k[2 * HDB], v[4][WIDE];
+    static __device__ __forceinline__ int channel(int acc, int r, int g) { return 64 * (acc >> 2) + 4 * (4 * g + r) + (acc & 3); }
+    static __device__ __forceinline__ Q query(const float *row, int s) { return *reinterpret_cast<const v4f *>(row + 16 * s + 4 * ((threadIdx.x & 63) >> 4)); }
+    struct Offsets { unsigned k, k_tail[2], v, v_last, v_row; };
+    static __device__ __forceinline__ Offsets offsets(int hd) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 4 * g, last = 64 * (WIDE - 1) + 4 * i;
+        return {(unsigned)(i * hd + 4 * g) * 4, {(unsigned)(i * hd + (tail < hd ? tail : 0)) * 4, (unsigned)(i * hd + (tail + 16 < hd ? tail + 16 : 0)) * 4},
+                (unsigned)(4 * g * hd + 4 * i) * 4, (unsigned)(4 * g * hd + (last < hd ? last : 0)) * 4, (unsigned)hd * 4};
+    }
+    __device__ __forceinline__ void load(const char *kp, const char *vp, int, const Offsets &o) {
+#pragma unroll
+        for (int s = 0; s < 2 * HDB; s++) k[s] = *reinterpret_cast<const v4f *>(kp + (s < 2 * HDB - 2 ? o.k + 64 * s : o.k_tail[s & 1]));
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int w = 0; w < WIDE; w++) v[r][w] = *reinterpret_cast<const v4f *>(vp + r * o.v_row + (w < WIDE - 1 ? o.v : o.v_last));
+    }
+    __device__ __forceinline__ void trim(int hd) {
+        if ((hd & 31) == 0) return;
+#pragma unroll
+        for (int s = 2 * HDB - 2; s < 2 * HDB; s++) {
+            const bool in = 16 * s + 4 * ((threadIdx.x & 63) >> 4) < hd;
+#pragma unroll
+            for (int e = 0; e < 4; e++) k[s][e] = in ? k[s][e] : 0.f;
+        }
+    }
+    __device__ __forceinline__ v4f scores(const Q (&q)[QS], int) const {
+        v4f s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2 * HDB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], q[j][e], s, 0, 0, 0);
+        return s;
+    }
+    __device__ __forceinline__ void hide(int, int r) {
+#pragma unroll
+        for (int w = 0; w < WIDE; w++) v[r][w] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    template <bool ODD>
+    __device__ __forceinline__ void weigh(v4f (&acc)[ACC], const v4f (&p)[PIECES]) const {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int w = 0; w < WIDE; w++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][w][e], p[0][r], acc[4 * w + e], 0, 0, 0);
+    }
+};
+
+// ---- a walk over tiles of one sequence and KV head ----
+
+// Where a wave's pieces lie: piece number, and its page's place in the table.  Each step goes WAVES tiles on.
+struct Pieces {
+    const int *table;       // of the sequence
+    int per_page, n_pages, end;         // pieces of a page; pieces that hold positions
+    int piece, at, off, step_at, step_off;
+    __device__ __forceinline__ void begin(const int *t, int p, int pages, int last, int first, int step) {
+        table = t; per_page = p; n_pages = pages; end = last; piece = first;
+        at = first / p; off = first - at * p;
+        step_at = step / p; step_off = step - step_at * p;
+    }
+    // The page of piece + i (0 or 1), -1 behind the last one.
+    __device__ __forceinline__ int page(int i) const { return piece + i < end ? table[off + i >= per_page ? at + 1 : at] : -1; }
+    __device__ __forceinline__ int slot(int i) const { return off + i >= per_page ? off + i - per_page : off + i; }      // (in pieces)
+    __device__ __forceinline__ void next(int step) {
+        piece += step;
+        at += step_at;
+        off += step_off;
+        if (off >= per_page) { off -= per_page; at++; }
+    }
+};
+
+template <typename T, int HDB>
+struct Walk {
+    typedef Tile<T, HDB> Tl;
+    v4f acc[Tl::ACC];
+    float m, l;
+    bool seen;
+
+    struct Place { int id[Tl::PIECES], slot[Tl::PIECES]; };
+    static __device__ __forceinline__ Place places(const Pieces &at) {
+        Place p;
+#pragma unroll
+        for (int i = 0; i < Tl::PIECES; i++) { p.id[i] = uniform(at.page(i)); p.slot[i] = at.slot(i); }
+        return p;
+    }
+
+    // tile: its number; ids: its pages
+    template <bool ODD>
+    __device__ __forceinline__ void use(Tl &t, const Place &p, const typename Tl::Q (&q)[Tl::QS], int tile, int len, int n_pages, int hd, float scale2,
+                                        const T *v, size_t page_stride) {
+        const int g = (threadIdx.x & 63) >> 4;
+        bool whole = (tile + 1) * Tl::POSITIONS <= len;
+#pragma unroll
+        for (int i = 0; i < Tl::PIECES; i++) {
+            const bool ok = paged_id_ok(p.id[i], n_pages);
+            whole &= ok;
+            seen |= ok;
+        }
+        t.trim(hd);
+        v4f s[Tl::PIECES];
+#pragma unroll
+        for (int i = 0; i < Tl::PIECES; i++) s[i] = t.scores(q, i);
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < Tl::PIECES; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (!(paged_id_ok(p.id[i], n_pages) && tile * Tl::POSITIONS + 16 * i + 4 * g + r < len)) {
+                        s[i][r] = -INFINITY;
+                        t.hide(i, r);
+                    }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < Tl::PIECES; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[i][r]);
+        mx *= scale2;
+        if (__any(mx > m)) {        // the running maximum moves: what is there is brought to the new one
+            mx = fmaxf(mx, lane_xor<16>(mx));
+            mx = fmaxf(mx, lane_xor<32>(mx));
+            const float to = fmaxf(m, mx), f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+            l *= f;
+#pragma unroll
+            for (int a = 0; a < Tl::ACC; a++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[a][r] *= f;
+            m = to;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        // m is rounded and the fused product is not: their difference, up to 2^-24 m, is in every weight and in their sum alike, until it is
+        // beyond what an exponential holds.  From FAR on products are rounded as m is, and the largest is exactly 0 off.
+        float by = scale2;
+        if (__any(fabsf(base) > FAR)) {
+            const bool far = fabsf(base) > FAR;
+#pragma unroll
+            for (int i = 0; i < Tl::PIECES; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[i][r] = far ? s[i][r] * scale2 : s[i][r];
+            by = far ? 1.f : scale2;
+        }
+#pragma unroll
+        for (int i = 0; i < Tl::PIECES; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], by, -base));
+                l += s[i][r];
+            }
+        t.template weigh<ODD>(acc, s);
+        if constexpr (ODD) {
+            // the infinities and NaNs that were left out of the product, one position after the other
+#pragma unroll 1
+            for (int x = 0; x < Tl::POSITIONS; x++) {
+                const int i = x >> 4, r = x & 3;
+                const float w0 = i ? s[Tl::PIECES - 1][0] : s[0][0], w1 = i ? s[Tl::PIECES - 1][1] : s[0][1], w2 = i ? s[Tl::PIECES - 1][2] : s[0][2],
+                            w3 = i ? s[Tl::PIECES - 1][3] : s[0][3];
+                const float w = __shfl(r == 0 ? w0 : r == 1 ? w1 : r == 2 ? w2 : w3, (threadIdx.x & 15) + ((x >> 2 & 3) << 4), 64);
+                const int id = i ? p.id[Tl::PIECES - 1] : p.id[0], slot = i ? p.slot[Tl::PIECES - 1] : p.slot[0];
+                if (!paged_id_ok(id, n_pages) || tile * Tl::POSITIONS + x >= len) continue;
+                const T *row = v + id * page_stride + (size_t)(slot * 16 + (x & 15)) * hd;
+#pragma unroll
+                for (int a = 0; a < Tl::ACC; a++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int ch = Tl::channel(a, e, g);
+                        const float y = ch < hd ? load_one(row + ch) : 0.f;
+                        if (!is_finite(y)) acc[a][e] += w * y;
+                    }
+            }
+        }
+    }
+
+    // Tiles first, first + WAVES, ... below last.  k, v: the KV head's rows of page 0.
+    template <bool ODD>
+    __device__ __forceinline__ void run(const typename Tl::Q (&q)[Tl::QS], const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages,
+                                        int hd, int first, int last, int len, float scale2) {
+        m = -INFINITY;
+        l = 0.f;
+        seen = false;
+#pragma unroll
+        for (int a = 0; a < Tl::ACC; a++) acc[a] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (first >= last) return;
+        constexpr int STEP = WAVES * Tl::PIECES;
+        Pieces at;
+        at.begin(table, page / 16, n_pages, (len + 15) / 16, first * Tl::PIECES, STEP);
+        const typename Tl::Offsets offsets = Tl::offsets(hd);
+        auto load = [&](Tl &t, const Place &p) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < Tl::PIECES; i++) {
+                // a piece of no page is read from page 0, and hidden
+                const size_t o = (size_t)(paged_id_ok(p.id[i], n_pages) ? p.id[i] : 0) * page_stride + (size_t)(p.slot[i] * 16) * hd;
+                t.load((const char *)(k + o), (const char *)(v + o), i, offsets);
+            }
+        };
+        Tl a, b;
+        Place pa = places(at), pb;
+        load(a, pa);
+        at.next(STEP);
+        pb = places(at);
+        int tile = first;
+        while (true) {
+            if (tile + WAVES < last) load(b, pb);
+            at.next(STEP);
+            Place pc = places(at);
+            use<ODD>(a, pa, q, tile, len, n_pages, hd, scale2, v, page_stride);
+            tile += WAVES;
+            if (tile >= last) break;
+            if (tile + WAVES < last) load(a, pc);
+            at.next(STEP);
+            pa = pc;
+            pc = places(at);
+            use<ODD>(b, pb, q, tile, len, n_pages, hd, scale2, v, page_stride);
+            tile += WAVES;
+            if (tile >= last) break;
+            pb = pc;
+        }
+        l += lane_xor<16>(l);
+        l += lane_xor<32>(l);
+    }
+};
+
+// What the waves of a workgroup leave one another of the unit at hand.
+template <int HDB>
+struct Shared {
+    static constexpr int ROW = HDB * 32 + 4;
+    float q[HEADS * ROW], o[WAVES * HEADS * ROW];       // the queries as fp32 values; each wave's o
+    float m[WAVES * HEADS], l[WAVES * HEADS];
+    int seen[WAVES];
+    __device__ __forceinline__ float sum_at(int h, int ch) const {
+        const float *p = o + h * ROW + ch;
+        return ((p[0] + p[HEADS * ROW]) + p[2 * HEADS * ROW]) + p[3 * HEADS * ROW];
+    }
+    __device__ __forceinline__ void stats(int h, float &top, float &sum) const {
+        top = fmaxf(fmaxf(m[h], m[HEADS + h]), fmaxf(m[2 * HEADS + h], m[3 * HEADS + h]));
+        const float base = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) sum += l[i * HEADS + h] * __builtin_amdgcn_exp2f(m[i * HEADS + h] - base);
+    }
+};
+template <int HDB> using shared_ptr = __attribute__((address_space(3))) Shared<HDB> *;
+
+// Tiles t0 .. t1 - 1 of a sequence and KV head: the waves' shares, brought to the largest of their maxima, are in LDS at the end.
+template <typename T, int HDB, bool ODD>
+__device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages, int hd, int heads,
+                                          int t0, int t1, int len, float scale2) {
+    typedef Tile<T, HDB> Tl;
+    Shared<HDB> &lds = *(Shared<HDB> *)lds_;
+    constexpr int ROW = Shared<HDB>::ROW;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, head = lane & 15;
+    typename Tl::Q q[Tl::QS];
+#pragma unroll
+    for (int i = 0; i < Tl::QS; i++) q[i] = Tl::query(lds.q + head * ROW, i);
+    Walk<T, HDB> walk;
+    walk.template run<ODD>(q, k, v, page_stride, table, page, n_pages, hd, t0 + wave, t1, len, scale2);
+    if (g == 0) {
+        lds.m[wave * HEADS + head] = walk.m;
+        lds.l[wave * HEADS + head] = walk.l;
+    }
+    if (lane == 0) lds.seen[wave] = walk.seen;
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) top = fmaxf(top, lds.m[i * HEADS + head]);
+    const float f = __builtin_amdgcn_exp2f(walk.m - (top == -INFINITY ? 0.f : top));
+    if (head < heads) {
+#pragma unroll
+        for (int x = 0; x < Tl::ACC; x += 4)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int ch = Tl::channel(x, r, g);            // and the three behind it
+                if (ch < HDB * 32)
+                    *reinterpret_cast<v4f *>(lds.o + (wave * HEADS + head) * ROW + ch) =
+                        v4f{walk.acc[x][r] * f, walk.acc[x + 1][r] * f, walk.acc[x + 2][r] * f, walk.acc[x + 3][r] * f};
+            }
+    }
+    __syncthreads();
 }
+// The same with infinities and NaNs among the values taken one by one; a function of its own, for its registers not to be the kernel's.
+template <typename T, int HDB>
+__device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages,
+                                                          int hd, int heads, int t0, int t1, int len, float scale2) {
+    share_out<T, HDB, true>(lds, k, v, page_stride, table, page, n_pages, hd, heads, t0, t1, len, scale2);
+}
+
+// The tiles of all columns, KV heads and parts of a group of query heads, one after the other, are dealt out evenly: workgroup w has tiles
+// w T / W .. (w + 1) T / W - 1, whatever sequences they belong to.  (Lengths are in device memory: the host cannot deal them out, and a batch's
+// longest sequence would otherwise decide when it ends.)  A column's tiles of one KV head that lie in several workgroups are a split unit; each of
+// these leaves its maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.
+template <typename T, int HDB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
+                                                                                                  PagedArgs a) {
+    typedef Tile<T, HDB> Tl;
+    constexpr int ROW = Shared<HDB>::ROW;
+    __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
+    __shared__ long long sums[256];
+    __shared__ int ticket;
+    const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
+    const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts;      // units of a column
+    auto length = [&](int col) __attribute__((always_inline)) {
+        const int p = a.pos[col];
+        return paged_entry(a.seq ? a.seq[col] : col, p, a.c.n_seqs, a.c.max_pages, page) < 0 ? 0 : p + 1;
+    };
+    auto tiles_of = [&](int col) __attribute__((always_inline)) { return (length(col) + Tl::POSITIONS - 1) / Tl::POSITIONS; };
+
+    // where this workgroup's tiles begin and end
+    const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
+    long long mine = 0;
+    for (int c = c0; c < c1; c++) mine += tiles_of(c);
+    sums[tid] = mine;
+    __syncthreads();
+    for (int d = 1; d < 256; d <<= 1) {
+        const long long v = tid >= d ? sums[tid - d] : 0;
+        __syncthreads();
+        sums[tid] += v;
+        __syncthreads();
+    }
+    const long long total = sums[255] * units;
+    const long long wanted = (total + 2 * WAVES - 1) / (2 * WAVES);
+    const int groups = (int)(wanted < gridDim.x ? wanted : gridDim.x), w = blockIdx.x;
+    if (w >= groups) return;
+    auto bound = [&](long long i) __attribute__((always_inline)) { return total * i / groups; };
+    long long lo = bound(w);
+    const long long hi = bound(w + 1);
+    // the column of tile lo: the thread whose columns have it walks over them
+    {
+        const long long before = sums[tid] - mine;
+        __syncthreads();
+        if (lo >= before * units && lo < (before + mine) * units) {
+            long long b = before * units;
+            int c = c0;
+            while (lo >= b + (long long)tiles_of(c) * units) { b += (long long)tiles_of(c) * units; c++; }
+            sums[0] = c;
+            sums[1] = b;
+        }
+        __syncthreads();
+    }
+    int col = uniform((int)sums[0]);
+    long long start = ((long long)uniform((int)(sums[1] >> 32)) << 32) | (unsigned)uniform((int)sums[1]);       // of the column's first tile
+    const size_t page_stride = (size_t)a.c.kv_heads * page * hd;
+
+    while (lo < hi) {
+        const int len = uniform(length(col)), n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
+        if (n == 0 || lo >= start + (long long)n * units) {
+            start += (long long)n * units;
+            col++;
+            continue;
+        }
+        const int unit = (int)((lo - start) / n), part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads;
+        const long long unit_lo = start + (long long)unit * n;
+        const int t0 = (int)(lo - unit_lo), t1 = (int)(min(hi, unit_lo + n) - unit_lo);
+        const int heads = min(a.group - part * HEADS, HEADS), head0 = kvh * a.group + part * HEADS;
+        const int b = col / a.S, s = col - b * a.S, seq = uniform(a.seq ? a.seq[col] : col);
+        // the queries, as fp32 values
+        for (int i = tid; i < HEADS * HDB * 32; i += 256) {
+            const int h = i / (HDB * 32), ch = i - h * (HDB * 32);
+            lds.q[h * ROW + ch] = h < heads && ch < hd ? load_one(q + (((size_t)b * a.heads + head0 + h) * hd + ch) * a.S + s) : 0.f;
+        }
+        __syncthreads();
+        const T *k = (const T *)a.c.k + (size_t)kvh * page * hd, *v = (const T *)a.c.v + (size_t)kvh * page * hd;
+        const int *table = a.c.pages + (size_t)seq * a.c.max_pages;
+        share_out<T, HDB, false>((shared_ptr<HDB>)&lds, k, v, page_stride, table, page, a.c.n_pages, hd, heads, t0, t1, len, a.scale2);
+        if constexpr (sizeof(T) == 2) {
+            // An infinity times the half of a weight that is zero is NaN: such sums are formed again.
+            bool odd = false;
+            for (int i = tid; i < heads * hd; i += 256) {
+                const float x = lds.sum_at(i / hd, i % hd);
+                odd |= x != x;
+            }
+            if (__syncthreads_or(odd))
+                share_out_again<T, HDB>((shared_ptr<HDB>)&lds, k, v, page_stride, table, page, a.c.n_pages, hd, heads, t0, t1, len, a.scale2);
+        }
+        const bool any = lds.seen[0] | lds.seen[1] | lds.seen[2] | lds.seen[3];
+        auto write = [&](int h, int ch, float val) __attribute__((always_inline)) { store_one(o + (((size_t)b * a.heads + head0 + h) * hd + ch) * a.S + s, val); };
+        auto write_lse = [&](int h, float top, float sum) __attribute__((always_inline)) {
+            if (lse) lse[((size_t)b * a.heads + head0 + h) * a.S + s] = (top + __builtin_amdgcn_logf(sum)) * LN2;
+        };
+        if (t0 == 0 && t1 == n) {
+            if (any)
+                for (int i = tid; i < heads * hd; i += 256) {
+                    const int h = i / hd, ch = i - h * hd;
+                    float top, sum;
+                    lds.stats(h, top, sum);
+                    write(h, ch, lds.sum_at(h, ch) / sum);
+                    if (ch == 0) write_lse(h, top, sum);
+                }
+        } else {
+            // a slot: [head][maximum, sum, whether anything was seen, -, channels]
+            const int row = hd + 4;
+            const size_t slot_size = (size_t)HEADS * (HDB * 32 + 4);
+            float *slot = a.slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;       // (of the two units that a workgroup may share, the one that begins in it second)
+            for (int i = tid; i < heads * row; i += 256) {
+                const int h = i / row, x = i - h * row;
+                float top, sum;
+                lds.stats(h, top, sum);
+                const float val = x == 0 ? top : x == 1 ? sum : x == 2 ? (any ? 1.f : 0.f) : x == 3 ? 0.f : lds.sum_at(h, x - 4);
+                __hip_atomic_store(slot + i, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            // the workgroups that have tiles of the unit
+            auto owner = [&](long long tile) __attribute__((always_inline)) {
+                long long i = tile * groups / total;
+                while (bound(i + 1) <= tile) i++;
+                while (bound(i) > tile) i--;
+                return (int)i;
+            };
+            const int first = owner(unit_lo), last = owner(unit_lo + n - 1);
+            __syncthreads();
+            if (tid == 0) ticket = (int)__hip_atomic_fetch_add(a.arrived + first, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (ticket == last - first) {
+                if (tid == 0) __hip_atomic_store(a.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                auto from = [&](int i) __attribute__((always_inline)) { return a.slots + ((size_t)i * 2 + (i == first)) * slot_size; };
+                auto get = [&](const float *p) __attribute__((always_inline)) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                for (int i = tid; i < heads * hd; i += 256) {
+                    const int h = i / hd, ch = i - h * hd;
+                    float top = -INFINITY, sum = 0.f, val = 0.f, some = 0.f;
+                    for (int j = first; j <= last; j++) {
+                        const float *p = from(j) + h * row;
+                        top = fmaxf(top, get(p));
+                        some += get(p + 2);
+                    }
+                    if (some == 0.f) continue;
+                    const float base = top == -INFINITY ? 0.f : top;
+                    for (int j = first; j <= last; j++) {
+                        const float *p = from(j) + h * row;
+                        const float f = __builtin_amdgcn_exp2f(get(p) - base);
+                        sum += get(p + 1) * f;
+                        val += get(p + 4 + ch) * f;
+                    }
+                    write(h, ch, val / sum);
+                    if (ch == 0) write_lse(h, top, sum);
+                }
+            }
+        }
+        __syncthreads();
+        lo = unit_lo + t1;
+    }
+}
+
+// Counts of workgroups that have left a slot; every launch leaves zeros.  (Launches follow one another on the library's stream.)
+__device__ unsigned g_arrived[MAX_GROUPS];
 
 template <typename T>
 int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const T *q, const int32_t *seq, const int32_t *pos, int heads, int S, int batch,
@@ -61,9 +577,22 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     const size_t units = (size_t)S * batch * heads;
     if (units > 0xffffff) return mi355_fail("%s: %zu heads of columns (at most 2^24 - 1)", who, units);
     if (!mi355_ready(who)) return -1;
-    attn_paged_kernel<T><<<(unsigned)units, 64, 0, g_ctx.stream>>>(o, lse, q, *c, seq, pos, heads, S, scale * LOG2E);
-    LAUNCH_OK(who);
-    return 0;
+    static unsigned *arrived = nullptr;
+    if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
+    const int groups = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
+    auto go = [&](auto blocks) {
+        constexpr int HDB = decltype(blocks)::value;
+        float *slots = (float *)mi355_ws((size_t)groups * 2 * HEADS * (HDB * 32 + 4) * sizeof(float));
+        if (!slots) return -1;
+        const PagedArgs a = {*c, seq, pos, heads, S, S * batch, heads / c->kv_heads, scale * LOG2E, slots, arrived};
+        attn_paged_kernel<T, HDB><<<(unsigned)groups, 256, 0, g_ctx.stream>>>(o, lse, q, a);
+        LAUNCH_OK(who);
+        return 0;
+    };
+    if (c->hd <= 32) return go(std::integral_constant<int, 1>());
+    if (c->hd <= 64) return go(std::integral_constant<int, 2>());
+    if (c->hd <= 96) return go(std::integral_constant<int, 3>());
+    return go(std::integral_constant<int, 4>());
 }
 
 }  // namespace

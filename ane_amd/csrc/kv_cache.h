@@ -12,6 +12,10 @@ static inline bool kv_cache_ok(const char *who, const mi355_kv_cache *c) {
     }
     if (c->page % 16 || c->page > 1 << 16) { mi355_fail("%s: pages of %d positions (a multiple of 16, at most 65536)", who, c->page); return false; }
     if (c->hd % 8 || c->hd > 128) { mi355_fail("%s: head size %d (a multiple of 8, at most 128)", who, c->hd); return false; }
+    if ((double)c->max_pages * c->page > 1 << 30) {
+        mi355_fail("%s: max_pages * page = %.0f positions (at most 2^30)", who, (double)c->max_pages * c->page);
+        return false;
+    }
     if (c->kv_heads > 1 << 12) { mi355_fail("%s: kv_heads=%d (at most 4096)", who, c->kv_heads); return false; }
     if (!aligned16(c->k) || !aligned16(c->v)) { mi355_fail("%s: k and v of a cache begin at multiples of 16 bytes", who); return false; }
     return true;

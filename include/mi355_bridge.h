@@ -208,7 +208,7 @@ int mi355_attn_plan_dev(int32_t *bounds, const int32_t *cu, int n_seqs, int S, i
  *
  * The cache of a layer is k and v, [n_pages][kv_heads][page][hd] each, fp32 or bfloat16, allocated by the caller at a multiple of 16 bytes;
  * pages[n_seqs][max_pages] (device memory) names the pages of each sequence in order: position p of sequence i is row p % page of page
- * pages[i][p / page].  page: a multiple of 16, at most 65536; hd: a multiple of 8, at most 128.  One table serves all layers.  Entries
+ * pages[i][p / page].  page: a multiple of 16, at most 65536; hd: a multiple of 8, at most 128; max_pages * page at most 2^30.  One table serves all layers.  Entries
  * behind a sequence's last page are not read; an entry outside [0, n_pages) is no page: nothing is written there, and attention leaves its
  * positions out.  The struct is read during the call only. */
 typedef struct mi355_kv_cache {

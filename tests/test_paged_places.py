@@ -71,7 +71,7 @@ def cache(**over):
 
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(pages=None), dict(n_pages=0), dict(page=0), dict(page=8), dict(page=24), dict(page=1 << 17), dict(page=-16),
-              dict(n_seqs=0), dict(max_pages=0), dict(max_pages=-3), dict(kv_heads=0), dict(kv_heads=5000), dict(hd=0), dict(hd=4), dict(hd=60),
+              dict(n_seqs=0), dict(max_pages=0), dict(max_pages=-3), dict(max_pages=(1 << 26) + 1), dict(max_pages=2 ** 31 - 1), dict(kv_heads=0), dict(kv_heads=5000), dict(hd=0), dict(hd=4), dict(hd=60),
               dict(hd=136), dict(hd=-8), dict(k=P + 4), dict(v=P + 8)]
 
 
