@@ -24,12 +24,14 @@ constexpr float FAR = 16777216.f;           // 2^24
 constexpr int HEADS = 16;                   // query heads of one product
 constexpr int WAVES = 4;
 constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
+constexpr int GRAIN = 2 * WAVES;            // tiles that a workgroup should have at least
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
 __device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long uniform(long long v) { return (long long)uniform((int)(v >> 32)) << 32 | (unsigned)uniform((int)v); }
 
 struct PagedArgs {
     mi355_kv_cache c;
@@ -58,26 +60,20 @@ template <int HDB> struct Tile<bf16_t, HDB> {
         const v4u w = {f2_to_bf2(p[0], p[1]), f2_to_bf2(p[2], p[3]), f2_to_bf2(p[4], p[5]), f2_to_bf2(p[6], p[7])};
         return __builtin_bit_cast(Q, w);
     }
-    // Bytes from the first of a piece's 16 rows to what the lane reads of them (channels behind the last: other ones in their place).
-    struct Offsets { unsigned k, k_last, v, v_row; };
+    // Bytes from the first of a piece's 16 rows to what the lane reads of them; channels behind the last are read as zero.
+    struct Offsets { unsigned k, k_last, v, row; };
     static __device__ __forceinline__ Offsets offsets(int hd) {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 8 * g;
-        return {(unsigned)(i * hd + 8 * g) * 2, (unsigned)(i * hd + (tail < hd ? tail : 0)) * 2, (unsigned)(4 * g * hd + (VC * i < hd ? VC * i : 0)) * 2, (unsigned)hd * 2};
+        return {(unsigned)(i * hd + 8 * g) * 2, tail < hd ? (unsigned)(i * hd + tail) * 2 : OUTSIDE, VC * i < hd ? (unsigned)(4 * g * hd + VC * i) * 2 : OUTSIDE, (unsigned)hd * 2};
     }
-    __device__ __forceinline__ void load(const char *kp, const char *vp, int piece, const Offsets &o) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, int piece, const Offsets &o) {
 #pragma unroll
-        for (int s = 0; s < HDB; s++) k[piece][s] = *reinterpret_cast<const v4u *>(kp + (s < HDB - 1 ? o.k + 64 * s : o.k_last));
+        for (int s = 0; s < HDB; s++) k[piece][s] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(s < HDB - 1 ? o.k + 64 * s : o.k_last), 0, 0));
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[4 * piece + r] = *reinterpret_cast<const Vec *>(vp + r * o.v_row + o.v);
-    }
-    // channels behind the last count as zero; q has zeros there, but what was read in their place may be no number
-    __device__ __forceinline__ void trim(int hd) {
-        if ((hd & 31) == 0) return;
-        const bool in = 32 * (HDB - 1) + 8 * ((threadIdx.x & 63) >> 4) < hd;
-#pragma unroll
-        for (int p = 0; p < PIECES; p++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) k[p][HDB - 1][e] = in ? k[p][HDB - 1][e] : 0u;
+        for (int r = 0; r < 4; r++) {
+            if constexpr (VC == 8) v[4 * piece + r] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)o.v, (int)(r * o.row), 0));
+            else v[4 * piece + r] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b64(vr, (int)o.v, (int)(r * o.row), 0));
+        }
     }
     __device__ __forceinline__ v4f scores(const Q (&q)[QS], int piece) const {
         v4f s = {0.f, 0.f, 0.f, 0.f};
@@ -126,28 +122,20 @@ template <int HDB> struct Tile<float, HDB> {
     v4f k[2 * HDB], v[4][WIDE];
     static __device__ __forceinline__ int channel(int acc, int r, int g) { return 64 * (acc >> 2) + 4 * (4 * g + r) + (acc & 3); }
     static __device__ __forceinline__ Q query(const float *row, int s) { return *reinterpret_cast<const v4f *>(row + 16 * s + 4 * ((threadIdx.x & 63) >> 4)); }
-    struct Offsets { unsigned k, k_tail[2], v, v_last, v_row; };
+    struct Offsets { unsigned k, k_tail[2], v, v_last, row; };
     static __device__ __forceinline__ Offsets offsets(int hd) {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 4 * g, last = 64 * (WIDE - 1) + 4 * i;
-        return {(unsigned)(i * hd + 4 * g) * 4, {(unsigned)(i * hd + (tail < hd ? tail : 0)) * 4, (unsigned)(i * hd + (tail + 16 < hd ? tail + 16 : 0)) * 4},
-                (unsigned)(4 * g * hd + 4 * i) * 4, (unsigned)(4 * g * hd + (last < hd ? last : 0)) * 4, (unsigned)hd * 4};
+        return {(unsigned)(i * hd + 4 * g) * 4, {tail < hd ? (unsigned)(i * hd + tail) * 4 : OUTSIDE, tail + 16 < hd ? (unsigned)(i * hd + tail + 16) * 4 : OUTSIDE},
+                (unsigned)(4 * g * hd + 4 * i) * 4, last < hd ? (unsigned)(4 * g * hd + last) * 4 : OUTSIDE, (unsigned)hd * 4};
     }
-    __device__ __forceinline__ void load(const char *kp, const char *vp, int, const Offsets &o) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, int, const Offsets &o) {
 #pragma unroll
-        for (int s = 0; s < 2 * HDB; s++) k[s] = *reinterpret_cast<const v4f *>(kp + (s < 2 * HDB - 2 ? o.k + 64 * s : o.k_tail[s & 1]));
+        for (int s = 0; s < 2 * HDB; s++)
+            k[s] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(s < 2 * HDB - 2 ? o.k + 64 * s : o.k_tail[s & 1]), 0, 0));
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int w = 0; w < WIDE; w++) v[r][w] = *reinterpret_cast<const v4f *>(vp + r * o.v_row + (w < WIDE - 1 ? o.v : o.v_last));
-    }
-    __device__ __forceinline__ void trim(int hd) {
-        if ((hd & 31) == 0) return;
-#pragma unroll
-        for (int s = 2 * HDB - 2; s < 2 * HDB; s++) {
-            const bool in = 16 * s + 4 * ((threadIdx.x & 63) >> 4) < hd;
-#pragma unroll
-            for (int e = 0; e < 4; e++) k[s][e] = in ? k[s][e] : 0.f;
-        }
+            for (int w = 0; w < WIDE; w++) v[r][w] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)(w < WIDE - 1 ? o.v : o.v_last), (int)(r * o.row), 0));
     }
     __device__ __forceinline__ v4f scores(const Q (&q)[QS], int) const {
         v4f s = {0.f, 0.f, 0.f, 0.f};
@@ -174,24 +162,19 @@ template <int HDB> struct Tile<float, HDB> {
 
 // ---- a walk over tiles of one sequence and KV head ----
 
-// Where a wave's pieces lie: piece number, and its page's place in the table.  Each step goes WAVES tiles on.
+// Where a wave's pieces lie: lane j has the page and the place in it of the j-th of 64 of them (-1 behind the sequence's end).  A wave
+// looks 64 up at once, long before it needs them: waiting for one number of the table would wait for all loads of keys and values before it.
 struct Pieces {
-    const int *table;       // of the sequence
-    int per_page, n_pages, end;         // pieces of a page; pieces that hold positions
-    int piece, at, off, step_at, step_off;
-    __device__ __forceinline__ void begin(const int *t, int p, int pages, int last, int first, int step) {
-        table = t; per_page = p; n_pages = pages; end = last; piece = first;
-        at = first / p; off = first - at * p;
-        step_at = step / p; step_off = step - step_at * p;
-    }
-    // The page of piece + i (0 or 1), -1 behind the last one.
-    __device__ __forceinline__ int page(int i) const { return piece + i < end ? table[off + i >= per_page ? at + 1 : at] : -1; }
-    __device__ __forceinline__ int slot(int i) const { return off + i >= per_page ? off + i - per_page : off + i; }      // (in pieces)
-    __device__ __forceinline__ void next(int step) {
-        piece += step;
-        at += step_at;
-        off += step_off;
-        if (off >= per_page) { off -= per_page; at++; }
+    int id, slot;
+    // PIECES of tile first, of tile first + WAVES, ...
+    template <int PIECES>
+    __device__ __forceinline__ void look_up(const int *table, int page, int len, int first) {
+        const int j = threadIdx.x & 63, per_page = page >> 4;
+        const int piece = (first + j / PIECES * WAVES) * PIECES + j % PIECES;
+        const unsigned at = (unsigned)piece / (unsigned)per_page;
+        slot = piece - (int)at * per_page;
+        id = -1;
+        if (piece < (len + 15) >> 4) id = table[at];        // (looked at when it is needed: see places())
     }
 };
 
@@ -203,26 +186,30 @@ struct Walk {
     bool seen;
 
     struct Place { int id[Tl::PIECES], slot[Tl::PIECES]; };
-    static __device__ __forceinline__ Place places(const Pieces &at) {
+    static constexpr int BATCH = 64 / Tl::PIECES;           // tiles whose pages are looked up at once
+    static __device__ __forceinline__ Place places(const Pieces &in, int i, int n_pages) {
         Place p;
 #pragma unroll
-        for (int i = 0; i < Tl::PIECES; i++) { p.id[i] = uniform(at.page(i)); p.slot[i] = at.slot(i); }
+        for (int j = 0; j < Tl::PIECES; j++) {
+            const int id = __builtin_amdgcn_readlane(in.id, (i % BATCH) * Tl::PIECES + j);
+            p.id[j] = paged_id_ok(id, n_pages) ? id : -1;
+            p.slot[j] = __builtin_amdgcn_readlane(in.slot, (i % BATCH) * Tl::PIECES + j);
+        }
         return p;
     }
 
     // tile: its number; ids: its pages
     template <bool ODD>
-    __device__ __forceinline__ void use(Tl &t, const Place &p, const typename Tl::Q (&q)[Tl::QS], int tile, int len, int n_pages, int hd, float scale2,
-                                        const T *v, size_t page_stride) {
+    __device__ __forceinline__ void use(Tl &t, const Place &p, const typename Tl::Q (&q)[Tl::QS], int tile, int len, int hd, float scale2, const T *v,
+                                        size_t page_stride) {
         const int g = (threadIdx.x & 63) >> 4;
         bool whole = (tile + 1) * Tl::POSITIONS <= len;
 #pragma unroll
         for (int i = 0; i < Tl::PIECES; i++) {
-            const bool ok = paged_id_ok(p.id[i], n_pages);
+            const bool ok = p.id[i] >= 0;
             whole &= ok;
             seen |= ok;
         }
-        t.trim(hd);
         v4f s[Tl::PIECES];
 #pragma unroll
         for (int i = 0; i < Tl::PIECES; i++) s[i] = t.scores(q, i);
@@ -231,7 +218,7 @@ struct Walk {
             for (int i = 0; i < Tl::PIECES; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    if (!(paged_id_ok(p.id[i], n_pages) && tile * Tl::POSITIONS + 16 * i + 4 * g + r < len)) {
+                    if (!(p.id[i] >= 0 && tile * Tl::POSITIONS + 16 * i + 4 * g + r < len)) {
                         s[i][r] = -INFINITY;
                         t.hide(i, r);
                     }
@@ -282,7 +269,7 @@ struct Walk {
                             w3 = i ? s[Tl::PIECES - 1][3] : s[0][3];
                 const float w = __shfl(r == 0 ? w0 : r == 1 ? w1 : r == 2 ? w2 : w3, (threadIdx.x & 15) + ((x >> 2 & 3) << 4), 64);
                 const int id = i ? p.id[Tl::PIECES - 1] : p.id[0], slot = i ? p.slot[Tl::PIECES - 1] : p.slot[0];
-                if (!paged_id_ok(id, n_pages) || tile * Tl::POSITIONS + x >= len) continue;
+                if (id < 0 || tile * Tl::POSITIONS + x >= len) continue;
                 const T *row = v + id * page_stride + (size_t)(slot * 16 + (x & 15)) * hd;
 #pragma unroll
                 for (int a = 0; a < Tl::ACC; a++)
@@ -306,39 +293,43 @@ struct Walk {
 #pragma unroll
         for (int a = 0; a < Tl::ACC; a++) acc[a] = v4f{0.f, 0.f, 0.f, 0.f};
         if (first >= last) return;
-        constexpr int STEP = WAVES * Tl::PIECES;
-        Pieces at;
-        at.begin(table, page / 16, n_pages, (len + 15) / 16, first * Tl::PIECES, STEP);
         const typename Tl::Offsets offsets = Tl::offsets(hd);
         auto load = [&](Tl &t, const Place &p) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < Tl::PIECES; i++) {
-                // a piece of no page is read from page 0, and hidden
-                const size_t o = (size_t)(paged_id_ok(p.id[i], n_pages) ? p.id[i] : 0) * page_stride + (size_t)(p.slot[i] * 16) * hd;
-                t.load((const char *)(k + o), (const char *)(v + o), i, offsets);
+                const size_t o = (size_t)max(p.id[i], 0) * page_stride + (size_t)(p.slot[i] * 16) * hd;
+                const int bytes = p.id[i] < 0 ? 0 : 16 * hd * (int)sizeof(T);      // a piece of no page is read as zeros
+                t.load(__builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(k + o), 0, bytes, 0x00027000),
+                       __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(v + o), 0, bytes, 0x00027000), i, offsets);
             }
         };
+        Pieces now, then;
+        now.look_up<Tl::PIECES>(table, page, len, first);
         Tl a, b;
-        Place pa = places(at), pb;
+        Place pa = places(now, 0, n_pages), pb;
         load(a, pa);
-        at.next(STEP);
-        pb = places(at);
-        int tile = first;
-        while (true) {
-            if (tile + WAVES < last) load(b, pb);
-            at.next(STEP);
-            Place pc = places(at);
-            use<ODD>(a, pa, q, tile, len, n_pages, hd, scale2, v, page_stride);
-            tile += WAVES;
-            if (tile >= last) break;
-            if (tile + WAVES < last) load(a, pc);
-            at.next(STEP);
-            pa = pc;
-            pc = places(at);
-            use<ODD>(b, pb, q, tile, len, n_pages, hd, scale2, v, page_stride);
-            tile += WAVES;
-            if (tile >= last) break;
-            pb = pc;
+        then.look_up<Tl::PIECES>(table, page, len, first + BATCH * WAVES);
+        // tile i is used while tile i + 1 is under way
+        auto ahead = [&](Tl &t, Place &p, int i) __attribute__((always_inline)) {
+            if (i % BATCH == 0) {
+                now = then;
+                then.look_up<Tl::PIECES>(table, page, len, first + (i + BATCH) * WAVES);
+            }
+            p = places(now, i, n_pages);
+            // (behind the last one nothing; but a load behind a condition would have the compiler wait for all of them)
+            if (first + i * WAVES >= last) {
+#pragma unroll
+                for (int j = 0; j < Tl::PIECES; j++) p.id[j] = -1;
+            }
+            load(t, p);
+        };
+        for (int i = 0;; i += 2) {
+            ahead(b, pb, i + 1);
+            use<ODD>(a, pa, q, first + i * WAVES, len, hd, scale2, v, page_stride);
+            if (first + (i + 1) * WAVES >= last) break;
+            ahead(a, pa, i + 2);
+            use<ODD>(b, pb, q, first + (i + 1) * WAVES, len, hd, scale2, v, page_stride);
+            if (first + (i + 2) * WAVES >= last) break;
         }
         l += lane_xor<16>(l);
         l += lane_xor<32>(l);
@@ -373,7 +364,7 @@ __device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, const T *k, cons
     typedef Tile<T, HDB> Tl;
     Shared<HDB> &lds = *(Shared<HDB> *)lds_;
     constexpr int ROW = Shared<HDB>::ROW;
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, head = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), g = lane >> 4, head = lane & 15;
     typename Tl::Q q[Tl::QS];
 #pragma unroll
     for (int i = 0; i < Tl::QS; i++) q[i] = Tl::query(lds.q + head * ROW, i);
@@ -409,6 +400,17 @@ __device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, c
     share_out<T, HDB, true>(lds, k, v, page_stride, table, page, n_pages, hd, heads, t0, t1, len, scale2);
 }
 
+// Two values of a slot.  Slots pass from one workgroup to another inside a launch without fences, which would write back and invalidate whole L2s:
+// such stores go through to memory and such loads do not stop at the L2, and the count of those that have arrived goes up when the stores of a
+// workgroup have ended.
+__device__ __forceinline__ void slot_put(float *p, float x, float y) {
+    __hip_atomic_store((unsigned long long *)p, (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ v2f slot_get(const float *p) {
+    const unsigned long long v = __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return v2f{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
+}
+
 // The tiles of all columns, KV heads and parts of a group of query heads, one after the other, are dealt out evenly: workgroup w has tiles
 // w T / W .. (w + 1) T / W - 1, whatever sequences they belong to.  (Lengths are in device memory: the host cannot deal them out, and a batch's
 // longest sequence would otherwise decide when it ends.)  A column's tiles of one KV head that lie in several workgroups are a split unit; each of
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     typedef Tile<T, HDB> Tl;
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
-    __shared__ long long sums[256];
+    __shared__ long long sums[WAVES + 2];
     __shared__ int ticket;
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
     const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts;      // units of a column
@@ -433,36 +435,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
     long long mine = 0;
     for (int c = c0; c < c1; c++) mine += tiles_of(c);
-    sums[tid] = mine;
-    __syncthreads();
-    for (int d = 1; d < 256; d <<= 1) {
-        const long long v = tid >= d ? sums[tid - d] : 0;
-        __syncthreads();
-        sums[tid] += v;
-        __syncthreads();
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long x = __shfl_up(upto, d, 64);
+        if ((tid & 63) >= d) upto += x;
     }
-    const long long total = sums[255] * units;
-    const long long wanted = (total + 2 * WAVES - 1) / (2 * WAVES);
+    if ((tid & 63) == 63) sums[tid >> 6] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        if (i < tid >> 6) upto += sums[i];
+        total += sums[i];
+    }
+    total = uniform(total * units);
+    const long long wanted = (total + GRAIN - 1) / GRAIN;
     const int groups = (int)(wanted < gridDim.x ? wanted : gridDim.x), w = blockIdx.x;
     if (w >= groups) return;
-    auto bound = [&](long long i) __attribute__((always_inline)) { return total * i / groups; };
+    const long long share = total / groups, more = total - share * groups;          // the first `more` workgroups have one tile more
+    auto bound = [&](int i) __attribute__((always_inline)) { return i * share + min((long long)i, more); };
     long long lo = bound(w);
     const long long hi = bound(w + 1);
     // the column of tile lo: the thread whose columns have it walks over them
-    {
-        const long long before = sums[tid] - mine;
-        __syncthreads();
-        if (lo >= before * units && lo < (before + mine) * units) {
-            long long b = before * units;
-            int c = c0;
-            while (lo >= b + (long long)tiles_of(c) * units) { b += (long long)tiles_of(c) * units; c++; }
-            sums[0] = c;
-            sums[1] = b;
+    if (lo >= (upto - mine) * units && lo < upto * units) {
+        long long b = (upto - mine) * units;
+        int c = c0;
+        while (true) {
+            const long long n = (long long)tiles_of(c) * units;
+            if (lo < b + n) break;
+            b += n;
+            c++;
         }
-        __syncthreads();
+        sums[WAVES] = c;
+        sums[WAVES + 1] = b;
     }
-    int col = uniform((int)sums[0]);
-    long long start = ((long long)uniform((int)(sums[1] >> 32)) << 32) | (unsigned)uniform((int)sums[1]);       // of the column's first tile
+    __syncthreads();
+    int col = uniform((int)sums[WAVES]);
+    long long start = uniform(sums[WAVES + 1]);         // the first tile of the column
     const size_t page_stride = (size_t)a.c.kv_heads * page * hd;
 
     while (lo < hi) {
@@ -515,47 +525,91 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             const int row = hd + 4;
             const size_t slot_size = (size_t)HEADS * (HDB * 32 + 4);
             float *slot = a.slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;       // (of the two units that a workgroup may share, the one that begins in it second)
-            for (int i = tid; i < heads * row; i += 256) {
+            for (int i = 2 * tid; i < heads * row; i += 512) {
                 const int h = i / row, x = i - h * row;
-                float top, sum;
-                lds.stats(h, top, sum);
-                const float val = x == 0 ? top : x == 1 ? sum : x == 2 ? (any ? 1.f : 0.f) : x == 3 ? 0.f : lds.sum_at(h, x - 4);
-                __hip_atomic_store(slot + i, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                float first_of, second;
+                if (x == 0) lds.stats(h, first_of, second);
+                else if (x == 2) first_of = any ? 1.f : 0.f, second = 0.f;
+                else first_of = lds.sum_at(h, x - 4), second = lds.sum_at(h, x - 3);
+                slot_put(slot + i, first_of, second);
             }
             // the workgroups that have tiles of the unit
             auto owner = [&](long long tile) __attribute__((always_inline)) {
-                long long i = tile * groups / total;
-                while (bound(i + 1) <= tile) i++;
-                while (bound(i) > tile) i--;
-                return (int)i;
+                const long long longer = more * (share + 1);
+                return (int)(tile < longer ? tile / (share + 1) : more + (tile - longer) / share);
             };
             const int first = owner(unit_lo), last = owner(unit_lo + n - 1);
-            __syncthreads();
-            if (tid == 0) ticket = (int)__hip_atomic_fetch_add(a.arrived + first, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // this wave's part of the slot is in memory,
+            __syncthreads();                                        // everybody's is
+            if (tid == 0) ticket = (int)__hip_atomic_fetch_add(a.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (ticket == last - first) {
+                // Everybody's slots are in memory.  Maxima and sums first, 16 threads to a head; then the channels, two to a thread and the
+                // slots in turns where there are threads to spare.
                 if (tid == 0) __hip_atomic_store(a.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                auto from = [&](int i) __attribute__((always_inline)) { return a.slots + ((size_t)i * 2 + (i == first)) * slot_size; };
-                auto get = [&](const float *p) __attribute__((always_inline)) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                for (int i = tid; i < heads * hd; i += 256) {
-                    const int h = i / hd, ch = i - h * hd;
-                    float top = -INFINITY, sum = 0.f, val = 0.f, some = 0.f;
-                    for (int j = first; j <= last; j++) {
-                        const float *p = from(j) + h * row;
-                        top = fmaxf(top, get(p));
-                        some += get(p + 2);
+                const int count = last - first + 1;
+                auto from = [&](int j) __attribute__((always_inline)) { return a.slots + ((size_t)(first + j) * 2 + (j == 0)) * slot_size; };
+                {
+                    const int h = tid >> 4;
+                    float top = -INFINITY, some = 0.f, sum = 0.f;
+                    if (h < heads) {
+                        for (int j = tid & 15; j < count; j += 16) {
+                            const v2f x = slot_get(from(j) + h * row);
+                            some += slot_get(from(j) + h * row + 2)[0];
+                            const float to = fmaxf(top, x[0]), base = to == -INFINITY ? 0.f : to;
+                            sum = sum * __builtin_amdgcn_exp2f(top - base) + x[1] * __builtin_amdgcn_exp2f(x[0] - base);
+                            top = to;
+                        }
+#pragma unroll
+                        for (int d = 1; d < 16; d <<= 1) {
+                            const float t2 = __shfl_xor(top, d, 64), s2 = __shfl_xor(sum, d, 64);
+                            const float to = fmaxf(top, t2), base = to == -INFINITY ? 0.f : to;
+                            sum = sum * __builtin_amdgcn_exp2f(top - base) + s2 * __builtin_amdgcn_exp2f(t2 - base);
+                            top = to;
+                            some += __shfl_xor(some, d, 64);
+                        }
+                        if ((tid & 15) == 0) {
+                            lds.m[h] = top;
+                            lds.l[h] = sum;
+                            lds.m[HEADS + h] = some;
+                        }
                     }
-                    if (some == 0.f) continue;
-                    const float base = top == -INFINITY ? 0.f : top;
-                    for (int j = first; j <= last; j++) {
-                        const float *p = from(j) + h * row;
-                        const float f = __builtin_amdgcn_exp2f(get(p) - base);
-                        sum += get(p + 1) * f;
-                        val += get(p + 4 + ch) * f;
-                    }
-                    write(h, ch, val / sum);
-                    if (ch == 0) write_lse(h, top, sum);
                 }
+                __syncthreads();
+                const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
+                for (int i = tid; i < pairs * turns; i += 256) {
+                    const int turn = i / pairs, x = i - turn * pairs, h = 2 * x / hd, ch = 2 * x - h * hd;
+                    const float base = lds.m[h] == -INFINITY ? 0.f : lds.m[h];
+                    float v0 = 0.f, v1 = 0.f;
+                    // eight at a time on their way (the last one again behind the end, and not added)
+                    for (int j = turn; j < count; j += 8 * turns) {
+                        v2f m[8], y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float *p = from(min(j + e * turns, count - 1)) + h * row;
+                            m[e] = slot_get(p);
+                            y[e] = slot_get(p + 4 + ch);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            if (j + e * turns >= count) break;
+                            const float f = __builtin_amdgcn_exp2f(m[e][0] - base);
+                            v0 += y[e][0] * f;
+                            v1 += y[e][1] * f;
+                        }
+                    }
+                    lds.o[2 * i] = v0;
+                    lds.o[2 * i + 1] = v1;
+                }
+                __syncthreads();
+                if (lds.m[HEADS] != 0.f)
+                    for (int i = tid; i < heads * hd; i += 256) {
+                        float val = 0.f;
+                        for (int turn = 0; turn < turns; turn++) val += lds.o[turn * heads * hd + i];
+                        const int h = i / hd, ch = i - h * hd;
+                        write(h, ch, val / lds.l[h]);
+                        if (ch == 0) write_lse(h, lds.m[h], lds.l[h]);
+                    }
             }
         }
         __syncthreads();
