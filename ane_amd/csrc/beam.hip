@@ -1,83 +1,375 @@
 // beam.hip — a step of beam search: the best continuations of each group of beams.
 //   candidate (n, v) = score[n] + (x[v][n] - log sum_u exp x[u][n]);  a finished beam has (n, pad) = score[n], and -inf for every other token.
 // The `beams` largest of a group, equal ones in the order of (n, v); a NaN counts as -inf.
+//
+// Two launches.  The first reads the logits once, at the rate of memory, and leaves for every block of rows of a column its largest logit and the
+// sum of exponentials.  The second has a workgroup for each group: log sums; the `beams` best blocks by their largest candidates; and
+// the best of these blocks' elements, which are read again.  The best `beams` elements lie in the best `beams` blocks, with equal ones in the
+// order of their indices in both: each block before another has an element before all of the other's.
 #include "tile.h"
 
 #include <math.h>
 
 namespace {
 
+constexpr int SELECT = 1024;        // threads of a group's workgroup
+constexpr int LIST = 1024;          // candidates that it ranks
+constexpr int MOST = 64;            // beams
+
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
-
-// A workgroup to a column: max and log of the sum of exponentials.
-template <typename T>
-__global__ __launch_bounds__(256) void beam_lse_kernel(double *__restrict__ lse, const T *__restrict__ logits, int V, int S) {
-    __shared__ float ms[4];
-    __shared__ double ls[4];
-    const size_t col = blockIdx.x, b = col / S;
-    const T *x = logits + b * V * S + (col - b * S);
-    float m = -INFINITY;
-    for (int v = threadIdx.x; v < V; v += 256) m = __builtin_elementwise_maximum(m, load_one(x + (size_t)v * S));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, d, 64));
-    if ((threadIdx.x & 63) == 0) ms[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(ms[0], ms[1]), __builtin_elementwise_maximum(ms[2], ms[3]));
-    double l = 0.0;
-    for (int v = threadIdx.x; v < V; v += 256) l += exp_neg(load_one(x + (size_t)v * S) - m);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    if ((threadIdx.x & 63) == 0) ls[threadIdx.x >> 6] = l;
-    __syncthreads();
-    if (threadIdx.x == 0) lse[col] = (double)m + log(ls[0] + ls[1] + ls[2] + ls[3]);
+template <int VEC> __device__ __forceinline__ void load_vec(float (&r)[VEC], const float *p) {
+    if constexpr (VEC == 1) r[0] = __builtin_nontemporal_load(p);
+    else ldv_nt<VEC>(r, p);
+}
+template <int VEC> __device__ __forceinline__ void load_vec(float (&r)[VEC], const bf16_t *p) {
+    if constexpr (VEC == 1) r[0] = bf_to_f(__builtin_nontemporal_load(p));
+    else ldb<VEC, true>(r, p);
 }
 
-// A candidate in the order of the search: larger values first, then lower indices.
-struct Candidate { double value; int index; };
-__device__ __forceinline__ bool before(const Candidate &a, const Candidate &b) { return a.value > b.value || (a.value == b.value && a.index < b.index); }
+// {largest, sum of exp(x - largest)} of two parts; -inf with a sum of 0: nothing.
+__device__ __forceinline__ void join(float &m, float &l, float m2, float l2) {
+    const float to = fmaxf(m, m2), base = to == -INFINITY ? 0.f : to;
+    l = l * exp_neg_fast(m - base) + l2 * exp_neg_fast(m2 - base);
+    m = to;
+}
+// The values of N rows at once.  (fmaxf passes NaNs over; the sum does not, and with it all candidates of the column are NaN.)
+template <int N>
+__device__ __forceinline__ void take(float &m, float &l, const float (&x)[N]) {
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < N; i++) top = fmaxf(top, x[i]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) sum += exp_neg_fast(x[i] - base);
+    l = l * exp_neg_fast(m - base) + sum;
+    m = top;
+}
 
-// A workgroup to a group: one walk over its candidates for each of the beams.
-template <typename T>
-__global__ __launch_bounds__(256) void beam_select_kernel(float *__restrict__ score_out, int *__restrict__ token, int *__restrict__ parent,
-                                                          int *__restrict__ done_out, const T *__restrict__ logits, const float *__restrict__ score,
-                                                          const int *__restrict__ done, const double *__restrict__ lse, int V, int S, int beams, int eos,
-                                                          int pad) {
-    __shared__ Candidate best[4];
-    const int first = blockIdx.x * beams;
-    Candidate last = {INFINITY, -1};
-    for (int i = 0; i < beams; i++) {
-        Candidate mine = {-INFINITY, 0x7fffffff};
-        for (int j = threadIdx.x; j < beams * V; j += 256) {
-            const int n = first + j / V, v = j % V;
-            const size_t b = n / S;
-            double c = (double)score[n];
-            if (done && done[n]) c = v == pad ? c : -INFINITY;
-            else c = c + ((double)load_one(logits + (b * V + v) * S + (n - b * S)) - lse[n]);
-            if (c != c) c = -INFINITY;
-            const Candidate it = {c, j};
-            if (before(last, it) && before(it, mine)) mine = it;
-        }
+// Several columns: threads side by side take VEC columns of a row each (the last ones of a row its last VEC, some of them twice), `across` threads
+// to a row; a thread takes every (256 / across)-th of the block's rows, ROWS at a time.  part[block][column].
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void beam_columns_kernel(float2 *__restrict__ part, const T *__restrict__ logits, int V, int S, int columns, int across, int rows) {
+    constexpr int ROWS = 8;
+    __shared__ float ms[256 * VEC], ls[256 * VEC];
+    const int down = 256 / across, r = threadIdx.x / across, c = threadIdx.x - r * across;
+    const int first = blockIdx.x * rows, last = min(first + rows, V);
+    const size_t b = blockIdx.z;
+    const int col = min(((int)blockIdx.y * across + c) * VEC, S - VEC);
+    float m[VEC], l[VEC];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const Candidate o = {__shfl_xor(mine.value, d, 64), __shfl_xor(mine.index, d, 64)};
-            if (before(o, mine)) mine = o;
-        }
-        if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
-        __syncthreads();
-        last = best[0];
+    for (int e = 0; e < VEC; e++) { m[e] = -INFINITY; l[e] = 0.f; }
+    if (r < down) {
+        const T *x = logits + b * V * S + col;
+        for (int v = first + r; v < last; v += ROWS * down) {
+            float in[ROWS][VEC];
 #pragma unroll
-        for (int w = 1; w < 4; w++)
-            if (before(best[w], last)) last = best[w];
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const int n = first + last.index / V, v = last.index % V;
-            score_out[first + i] = (float)last.value;
-            token[first + i] = v;
-            parent[first + i] = n;
-            if (done_out) done_out[first + i] = (done && done[n]) || v == eos;
+            for (int i = 0; i < ROWS; i++) load_vec<VEC>(in[i], x + (size_t)min(v + i * down, last - 1) * S);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                float of[ROWS];
+#pragma unroll
+                for (int i = 0; i < ROWS; i++) of[i] = v + i * down < last ? in[i][e] : -INFINITY;
+                take(m[e], l[e], of);
+            }
         }
     }
+#pragma unroll
+    for (int e = 0; e < VEC; e++) { ms[threadIdx.x * VEC + e] = m[e]; ls[threadIdx.x * VEC + e] = l[e]; }
+    // the threads of a column in halves
+    for (int n = down; n > 1;) {
+        const int half = (n + 1) / 2;
+        __syncthreads();
+        if (r < n - half) {
+            const int at = threadIdx.x * VEC, of = at + half * across * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                join(m[e], l[e], ms[of + e], ls[of + e]);
+                ms[at + e] = m[e];
+                ls[at + e] = l[e];
+            }
+        }
+        n = half;
+    }
+    if (r == 0)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) part[(size_t)blockIdx.x * columns + b * S + col + e] = make_float2(m[e], l[e]);
+}
+
+// Columns whose logits lie one after the other (S = 1): a wave to a block of 64 * VEC * N rows.
+template <typename T, int VEC, int N>
+__global__ __launch_bounds__(256) void beam_rows_kernel(float2 *__restrict__ part, const T *__restrict__ logits, int V, int columns, int blocks) {
+    constexpr int ROWS = 64 * VEC * N;
+    const int block = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (block >= blocks) return;
+    const size_t col = blockIdx.y;
+    const T *x = logits + col * V;
+    float in[N * VEC];
+    const int first = block * ROWS;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int v = first + (i * 64 + lane) * VEC;
+        float r[VEC];
+        if (v + VEC <= V) load_vec<VEC>(r, x + v);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) r[e] = v + e < V ? load_one(x + v + e) : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) in[i * VEC + e] = r[e];
+    }
+    float m = -INFINITY, l = 0.f;
+    take(m, l, in);
+    const float top = wave_max(m);
+    l = wave_sum_stride<1>(l * exp_neg_fast(m - (top == -INFINITY ? 0.f : top)));
+    if (lane == 0) part[(size_t)block * columns + col] = make_float2(top, l);
+}
+
+struct SelectLds {
+    double lse[MOST], value[LIST], out_value[MOST], wave_value[SELECT / 64];
+    int key[LIST], out_key[MOST], wave_key[SELECT / 64], count;
+    float tops[64], tau;
+    float m[SELECT];
+    double l[SELECT];
+};
+__device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
+
+// The `want` first of all threads' items, larger values first, equal ones by their keys: out_value, out_key in order.  own: the largest of the
+// thread's items as a float (rounding keeps the order); walk(f) calls f(value, key) for each of them.
+// Of 64 parts of the threads the largest ones are compared; what is not below the `want`-th of these goes into a list, in which every item counts
+// those before it.  Few threads have any of those, and only they walk.
+template <typename F>
+__device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F walk) {
+    constexpr int PART = SELECT / 64;
+    const int tid = threadIdx.x;
+    float best = own;
+    if constexpr (PART >= 2) best = fmaxf(best, lane_xor<1>(best));
+    if constexpr (PART >= 4) best = fmaxf(best, lane_xor<2>(best));
+    if constexpr (PART >= 8) best = fmaxf(best, dpp_half_mirror(best));
+    if constexpr (PART >= 16) best = fmaxf(best, dpp_row_mirror(best));
+    if (tid % PART == 0) lds.tops[tid / PART] = best;
+    if (tid == 0) lds.count = 0;
+    __syncthreads();
+    {
+        const float mine = lds.tops[tid / PART];
+        float rank = 0.f;
+#pragma unroll
+        for (int i = 0; i < 64 / PART; i++) {
+            const int j = tid % PART * (64 / PART) + i;
+            const float t = lds.tops[j];
+            rank += t > mine || (t == mine && j < tid / PART) ? 1.f : 0.f;
+        }
+        if ((int)group_sum<PART>(rank) == want - 1) lds.tau = mine;
+    }
+    __syncthreads();
+    const float tau = lds.tau;
+    if (own >= tau) {
+        auto put = [&](double v, int k) __attribute__((always_inline)) {
+            if ((float)v < tau) return;
+            const int at = atomicAdd(&lds.count, 1);
+            if (at < LIST) { lds.value[at] = v; lds.key[at] = k; }
+        };
+        walk(put);
+    }
+    __syncthreads();
+    const int count = lds.count;
+    if (count <= LIST) {
+        for (int i = tid >> 4; i < count; i += SELECT / 16) {       // 16 threads to an item
+            const double v = lds.value[i];
+            const int k = lds.key[i];
+            float rank = 0.f;
+            for (int j = tid & 15; j < count; j += 16) rank += before(lds.value[j], lds.key[j], v, k) ? 1.f : 0.f;
+            const int r = (int)group_sum<16>(rank);
+            if (r < want && (tid & 15) == 0) { lds.out_value[r] = v; lds.out_key[r] = k; }
+        }
+    } else {            // too many equal ones (or nothing but -inf): one walk over all items for each
+        double last = INFINITY;
+        int last_key = -1;
+        for (int r = 0; r < want; r++) {
+            double v = -INFINITY;
+            int k = 0x7fffffff;
+            auto least = [&](double x, int y) __attribute__((always_inline)) {
+                if (before(last, last_key, x, y) && before(x, y, v, k)) { v = x; k = y; }
+            };
+            walk(least);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double v2 = __shfl_xor(v, d, 64);
+                const int k2 = __shfl_xor(k, d, 64);
+                if (before(v2, k2, v, k)) { v = v2; k = k2; }
+            }
+            if ((tid & 63) == 0) { lds.wave_value[tid >> 6] = v; lds.wave_key[tid >> 6] = k; }
+            __syncthreads();
+            last = lds.wave_value[0];
+            last_key = lds.wave_key[0];
+            for (int w = 1; w < SELECT / 64; w++)
+                if (before(lds.wave_value[w], lds.wave_key[w], last, last_key)) { last = lds.wave_value[w]; last_key = lds.wave_key[w]; }
+            if (tid == 0) { lds.out_value[r] = last; lds.out_key[r] = last_key; }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T>
+__global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__ score_out, int *__restrict__ token, int *__restrict__ parent,
+                                                             int *__restrict__ done_out, const T *__restrict__ logits, const float *__restrict__ score,
+                                                             const int *__restrict__ done, const float2 *__restrict__ part, int blocks, int rows, int V, int S,
+                                                             int columns, int beams, int eos, int pad) {
+    __shared__ SelectLds lds;
+    __shared__ float scores[MOST];
+    __shared__ int ended[MOST], chosen[MOST];
+    const int tid = threadIdx.x, first = blockIdx.x * beams;
+    if (tid < beams) {
+        scores[tid] = score[first + tid];
+        ended[tid] = done ? done[first + tid] : 0;
+    }
+    // A thread keeps to one beam: every (SELECT / beams)-th of its blocks.
+    const int side = SELECT / beams, beam = tid % beams, step = tid / beams;
+    float m = -INFINITY, tops[8];       // tops: of its first eight
+    double l = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) tops[i] = -INFINITY;
+    if (step < side)
+        for (int b = step; b < blocks; b += 8 * side) {
+            float2 p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] = part[(size_t)min(b + i * side, blocks - 1) * columns + first + beam];
+            if (b == step)
+#pragma unroll
+                for (int i = 0; i < 8; i++) tops[i] = p[i].x;
+            float to = m;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (b + i * side < blocks) to = fmaxf(to, p[i].x);
+            const float base = to == -INFINITY ? 0.f : to;
+            l *= (double)exp_neg_fast(m - base);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (b + i * side < blocks) l += (double)p[i].y * (double)exp_neg(p[i].x - base);
+            m = to;
+        }
+    lds.m[tid] = m;
+    lds.l[tid] = l;
+    __syncthreads();
+    for (int n = tid >> 6; n < beams; n += SELECT / 64) {
+        float top = -INFINITY;
+        double sum = 0.0;
+        for (int i = tid & 63; i < side; i += 64) top = fmaxf(top, lds.m[i * beams + n]);
+        top = wave_max(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int i = tid & 63; i < side; i += 64) sum += lds.l[i * beams + n] * (double)exp_neg(lds.m[i * beams + n] - base);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+        if ((tid & 63) == 0) lds.lse[n] = (double)top + log(sum);
+    }
+    __syncthreads();
+    auto candidate = [&](int n, float x, bool is_pad) __attribute__((always_inline)) {
+        const double s = scores[n];
+        double c = ended[n] ? (is_pad ? s : -INFINITY) : s + ((double)x - lds.lse[n]);
+        return c == c ? c : -INFINITY;
+    };
+    // the best blocks; of a beam's candidates the one with the largest logit is the largest, but an ended beam has only one
+    const int pad_block = pad / rows, best_blocks = (int)min((long long)beams, (long long)beams * blocks);
+    float own = -INFINITY;
+    if (step < side && (!ended[beam] || pad_block % side == step)) own = (float)candidate(beam, m, true);
+    first_of(lds, best_blocks, own, [&](auto f) __attribute__((always_inline)) {
+        if (step >= side) return;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i * side < blocks && step + i * side < blocks) f(candidate(beam, tops[i], step + i * side == pad_block), beam * blocks + step + i * side);
+        for (int b = step + 8 * side; b < blocks; b += side)
+            f(candidate(beam, part[(size_t)b * columns + first + beam].x, b == pad_block), beam * blocks + b);
+    });
+    if (tid < best_blocks) chosen[tid] = lds.out_key[tid];
+    __syncthreads();
+    // the best of their elements
+    {
+        constexpr int N = 4;
+        const int n_elements = best_blocks * rows;
+        double value[N];
+        int key[N];
+        auto element = [&](int i, double &v, int &k) __attribute__((always_inline)) {
+            const int at = min(i, n_elements - 1), j = at / rows, n = chosen[j] / blocks, row = (chosen[j] - n * blocks) * rows + (at - j * rows);
+            const int col = first + n, b = col / S;
+            v = candidate(n, load_one(logits + ((size_t)b * V + min(row, V - 1)) * S + (col - b * S)), row == pad);
+            k = i < n_elements && row < V ? n * V + row : -1;
+        };
+        own = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            key[i] = -1;
+            if (i * SELECT < n_elements) element(tid + i * SELECT, value[i], key[i]);
+            if (key[i] >= 0) own = fmaxf(own, (float)value[i]);
+        }
+        auto rest = [&](auto f) __attribute__((always_inline)) {
+            for (int i = tid + N * SELECT; i < n_elements; i += SELECT) {
+                double v;
+                int k;
+                element(i, v, k);
+                if (k >= 0) f(v, k);
+            }
+        };
+        rest([&](double v, int) __attribute__((always_inline)) { own = fmaxf(own, (float)v); });
+        first_of(lds, beams, own, [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i * SELECT < n_elements && key[i] >= 0) f(value[i], key[i]);
+            rest(f);
+        });
+    }
+    if (tid < beams) {
+        const int n = lds.out_key[tid] / V, v = lds.out_key[tid] - n * V;
+        score_out[first + tid] = (float)lds.out_value[tid];
+        token[first + tid] = v;
+        parent[first + tid] = first + n;
+        if (done_out) done_out[first + tid] = ended[n] || v == eos;
+    }
+}
+
+// Rows to a block, and the first launch.
+template <typename T>
+int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T *logits, int V, int S, int batch) {
+    constexpr int WIDE = 16 / (int)sizeof(T);
+    const size_t columns = (size_t)S * batch;
+    if (S == 1) {
+        auto go = [&](auto loads) {
+            constexpr int N = decltype(loads)::value;
+            *rows = 64 * WIDE * N;
+            *blocks = (int)ceil_div(V, *rows);
+            *part = (float2 *)mi355_ws(*blocks * columns * sizeof(float2));
+            if (!*part) return -1;
+            for (size_t c = 0; c < columns; c += 65535) {
+                const unsigned n = (unsigned)(columns - c < 65535 ? columns - c : 65535);
+                beam_rows_kernel<T, WIDE, N><<<dim3((unsigned)ceil_div(*blocks, 4), n), 256, 0, g_ctx.stream>>>(*part + c, logits + c * V, V, (int)columns, *blocks);
+                LAUNCH_OK(who);
+            }
+            return 0;
+        };
+        // a launch of eight workgroups and more to a compute unit can have longer blocks
+        const size_t waves = columns * ceil_div(V, 64 * WIDE);
+        if (waves >= 4 * 16 * (size_t)g_ctx.num_cu) return go(std::integral_constant<int, 2>());
+        return go(std::integral_constant<int, 1>());
+    }
+    auto go = [&](auto vec) {
+        constexpr int VEC = decltype(vec)::value;
+        const int threads = (int)ceil_div(S, VEC), across = threads < 64 ? threads : 64, strips = (int)ceil_div(threads, across), down = 256 / across;
+        // rows to a thread: eight at a time, more where there are workgroups enough
+        const size_t steps = ceil_div(V, down), each = steps * strips * batch / (4 * (size_t)g_ctx.num_cu);
+        *rows = down * (each >= 32 && down <= 8 ? 64 : each >= 32 ? 32 : each >= 16 ? 16 : each >= 8 ? 8 : each >= 4 ? 4 : each >= 2 ? 2 : 1);
+        *blocks = (int)ceil_div(V, *rows);
+        *part = (float2 *)mi355_ws(*blocks * columns * sizeof(float2));
+        if (!*part) return -1;
+        for (int b = 0; b < batch; b += 65535) {
+            const unsigned n = (unsigned)(batch - b < 65535 ? batch - b : 65535);
+            beam_columns_kernel<T, VEC><<<dim3((unsigned)*blocks, (unsigned)strips, n), 256, 0, g_ctx.stream>>>(*part + (size_t)b * S, logits + (size_t)b * V * S, V, S,
+                                                                                                                 (int)columns, across, *rows);
+            LAUNCH_OK(who);
+        }
+        return 0;
+    };
+    if (S >= WIDE) return go(std::integral_constant<int, WIDE>());
+    return go(std::integral_constant<int, 1>());
 }
 
 template <typename T>
@@ -91,11 +383,11 @@ int beam_step(const char *who, float *score_out, int32_t *token, int32_t *parent
     if (score_out == score || (done_out && done_out == done)) return mi355_fail("%s: the new scores and marks must not be the old ones", who);
     if (!mi355_ready(who)) return -1;
     const size_t n = (size_t)S * batch;
-    double *lse = (double *)mi355_ws(n * sizeof(double));
-    if (!lse) return -1;
-    beam_lse_kernel<T><<<(unsigned)n, 256, 0, g_ctx.stream>>>(lse, logits, V, S);
-    LAUNCH_OK(who);
-    beam_select_kernel<T><<<(unsigned)(n / beams), 256, 0, g_ctx.stream>>>(score_out, token, parent, done_out, logits, score, done, lse, V, S, beams, eos, pad);
+    float2 *part;
+    int blocks, rows;
+    if (beam_blocks(who, &part, &blocks, &rows, logits, V, S, batch)) return -1;
+    beam_select_kernel<T><<<(unsigned)(n / beams), SELECT, 0, g_ctx.stream>>>(score_out, token, parent, done_out, logits, score, done, part, blocks, rows, V, S,
+                                                                             (int)n, beams, eos, pad);
     LAUNCH_OK(who);
     return 0;
 }
