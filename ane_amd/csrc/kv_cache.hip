@@ -10,61 +10,272 @@ __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p);
 __device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
 
-struct AppendArgs {
-    mi355_kv_cache c;
-    const float *wq, *wk, *cos_t, *sin_t;
-    const int *seq, *pos;
-    int heads, S, batch, table;
-    float eps;
-};
+// 16 bytes of a row, and their values
+__device__ __forceinline__ v4f raw_cols(const float *p) { return ld4(p); }
+__device__ __forceinline__ v4u raw_cols(const bf16_t *p) { return *reinterpret_cast<const v4u_any *>(p); }
+__device__ __forceinline__ void widen(float (&r)[4], v4f w) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) r[j] = w[j];
+}
+__device__ __forceinline__ void widen(float (&r)[8], v4u w) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) { r[2 * j] = bf_to_f(w[j] & 0xffffu); r[2 * j + 1] = bf_to_f(w[j] >> 16); }
+}
+template <int VEC> __device__ __forceinline__ void store_cols(float *p, const float (&r)[VEC]) { stv<VEC>(p, r); }
+template <int VEC> __device__ __forceinline__ void store_cols(bf16_t *p, const float (&r)[VEC]) { stb<VEC>(p, r); }
+typedef unsigned bf_pair __attribute__((ext_vector_type(1)));
+typedef unsigned f_pair __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ bf_pair pair_of(float a, float b, bf16_t *) { return bf_pair(f2_to_bf2(a, b)); }
+__device__ __forceinline__ f_pair pair_of(float a, float b, float *) { return f_pair{__float_as_uint(a), __float_as_uint(b)}; }
+
+// What a column is a token of: the row of its page and of head 0, -1 if it is none.
+__device__ __forceinline__ long long token_row(const int *seq, const int *pages, size_t col, int pos, int n_pages, int page, int n_seqs, int max_pages, int kv_heads,
+                                               int positions) {
+    const long long entry = paged_entry(seq ? seq[col] : (int)col, pos, n_seqs, max_pages, page);
+    if (entry < 0 || pos >= positions) return -1;
+    const int id = pages[entry];
+    return paged_id_ok(id, n_pages) ? (long long)paged_row(id, 0, pos % page, kv_heads, page, 1) : -1;
+}
 
 // A wave to a head of a column, a pair of channels to a lane.
 template <typename T>
-__global__ __launch_bounds__(256) void kv_append_kernel(T *q_out, const T *q, const T *__restrict__ k, const T *__restrict__ v, AppendArgs a) {
-    const int lane = threadIdx.x & 63, slabs = a.heads + 2 * a.c.kv_heads, hd = a.c.hd, half = hd / 2;
+__global__ __launch_bounds__(256) void kv_append_kernel(
+    T *q_out, const T *q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ k_cache, T *__restrict__ v_cache,
+    const int *__restrict__ pages, const int *__restrict__ seq, const int *__restrict__ pos_of, const float *__restrict__ wq, const float *__restrict__ wk,
+    const float *__restrict__ cos_t, const float *__restrict__ sin_t, int n_pages, int page, int n_seqs, int max_pages, int kv_heads, int hd, int heads, int S,
+    int table, float eps, int columns) {
+    const int lane = threadIdx.x & 63, slabs = heads + 2 * kv_heads, half = hd / 2;
     const size_t unit = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const size_t col = unit / slabs;
-    const int slab = (int)(unit - col * slabs);
-    if (col >= (size_t)a.S * a.batch) return;
-    const int b = (int)(col / a.S), s = (int)(col - (size_t)b * a.S), pos = a.pos[col];
-    const long long entry = paged_entry(a.seq ? a.seq[col] : (int)col, pos, a.c.n_seqs, a.c.max_pages, a.c.page);
-    if (entry < 0 || (a.cos_t && pos >= a.table)) return;
-    const int id = a.c.pages[entry];
-    if (!paged_id_ok(id, a.c.n_pages)) return;
-    const bool is_q = slab < a.heads, is_k = !is_q && slab < a.heads + a.c.kv_heads;
-    const int head = is_q ? slab : is_k ? slab - a.heads : slab - a.heads - a.c.kv_heads;
-    const T *in = (is_q ? q : is_k ? k : v) + ((size_t)b * (is_q ? a.heads : a.c.kv_heads) + head) * hd * a.S + s;
-    const float *w = is_q ? a.wq : is_k ? a.wk : nullptr;
+    const int col = (int)(unit / slabs), slab = (int)(unit - (size_t)col * slabs);
+    if (col >= columns) return;
+    const int b = col / S, s = col - b * S, pos = pos_of[col];
+    const long long place = token_row(seq, pages, col, pos, n_pages, page, n_seqs, max_pages, kv_heads, cos_t ? table : 0x7fffffff);
+    if (place < 0) return;
+    const bool is_q = slab < heads, is_k = !is_q && slab < heads + kv_heads;
+    const int head = is_q ? slab : is_k ? slab - heads : slab - heads - kv_heads;
+    const T *in = (is_q ? q : is_k ? k : v) + ((size_t)b * (is_q ? heads : kv_heads) + head) * hd * S + s;
+    const float *w = is_q ? wq : is_k ? wk : nullptr;
     const bool mine = lane < half;
     float x0 = 0.f, x1 = 0.f;
     if (mine) {
-        x0 = load_one(in + (size_t)(2 * lane) * a.S);
-        x1 = load_one(in + (size_t)(2 * lane + 1) * a.S);
+        x0 = load_one(in + (size_t)(2 * lane) * S);
+        x1 = load_one(in + (size_t)(2 * lane + 1) * S);
     }
     if (w) {
-        const float rr = 1.f / sqrtf(wave_sum_stride<1>(x0 * x0 + x1 * x1) * (1.f / hd) + a.eps);
+        const float rr = 1.f / sqrtf(wave_sum_stride<1>(x0 * x0 + x1 * x1) * (1.f / hd) + eps);
         if (mine) {
             x0 = (x0 * rr) * w[2 * lane];
             x1 = (x1 * rr) * w[2 * lane + 1];
         }
     }
     if (!mine) return;
-    if ((is_q || is_k) && a.cos_t) {
-        const float cs = a.cos_t[(size_t)lane * a.table + pos], sn = a.sin_t[(size_t)lane * a.table + pos];
+    if ((is_q || is_k) && cos_t) {
+        const float cs = cos_t[(size_t)lane * table + pos], sn = sin_t[(size_t)lane * table + pos];
         const float y0 = x0 * cs - x1 * sn, y1 = x0 * sn + x1 * cs;
         x0 = y0;
         x1 = y1;
     }
     if (is_q) {
-        T *out = q_out + ((size_t)b * a.heads + head) * hd * a.S + s;
-        store_one(out + (size_t)(2 * lane) * a.S, x0);
-        store_one(out + (size_t)(2 * lane + 1) * a.S, x1);
+        T *out = q_out + ((size_t)b * heads + head) * hd * S + s;
+        store_one(out + (size_t)(2 * lane) * S, x0);
+        store_one(out + (size_t)(2 * lane + 1) * S, x1);
     } else {
-        T *out = (T *)(is_k ? a.c.k : a.c.v) + paged_row(id, head, pos % a.c.page, a.c.kv_heads, a.c.page, hd);
+        T *out = (is_k ? k_cache : v_cache) + (size_t)(place + head * page) * hd;
         store_one(out + 2 * lane, x0);
         store_one(out + 2 * lane + 1, x1);
     }
 }
+
+// Columns side by side: a workgroup has 64 of them and some of the heads.  As in qknorm_rope.hip a thread has whole row pairs of VEC columns, so the
+// rotation needs no other lane; the angles of its pairs and columns stay in registers for all the heads.  Rotated queries go back as they came.
+// A key or value is a row of the cache: 64 x hd values are turned round in LDS, 16 bytes of a row to a lane on the way out.  Chunks of 4 (fp32) or 8
+// pairs of a row are exchanged by the group of columns, so that neither side meets a bank twice.
+template <typename P>
+__device__ __forceinline__ P of_kind(bool is_q, bool is_k, P q, P k, P v) { return is_q ? q : is_k ? k : v; }
+// A head of the queries, the keys or the values, one after the other.
+template <typename T> struct Slab { bool is_q, is_k; int head, heads; const T *in; };
+template <typename T>
+__device__ __forceinline__ Slab<T> slab_of(int i, int heads, int kv_heads, const T *q, const T *k, const T *v) {
+    Slab<T> s;
+    s.is_q = i < heads;
+    s.is_k = !s.is_q && i < heads + kv_heads;
+    s.head = i - (s.is_q ? 0 : s.is_k ? heads : heads + kv_heads);
+    s.heads = s.is_q ? heads : kv_heads;
+    s.in = of_kind(s.is_q, s.is_k, q, k, v);
+    return s;
+}
+template <typename T, int CAP, int PPS, typename Raw>
+__device__ __forceinline__ void load_slab(Raw (&r0)[CAP], Raw (&r1)[CAP], const Slab<T> s, int b, int hd, int S, int col, int p0, bool ok) {
+    const T *in = s.in + ((size_t)b * s.heads + s.head) * hd * S + col;
+#pragma unroll
+    for (int kk = 0; kk < CAP; kk++) {
+        const int rp = p0 + kk * PPS;
+        r0[kk] = r1[kk] = Raw(0);
+        if (2 * rp < hd && ok) {
+            r0[kk] = raw_cols(in + (size_t)(2 * rp) * S);
+            r1[kk] = raw_cols(in + (size_t)(2 * rp + 1) * S);
+        }
+    }
+}
+template <typename T> constexpr int PAIRS_AT_ONCE = 256 * 16 / (int)sizeof(T) / 64;
+
+template <typename T, int CAP>
+__global__ __launch_bounds__(256) void kv_append_tile_kernel(
+    T *q_out, const T *q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ k_cache, T *__restrict__ v_cache,
+    const int *__restrict__ pages, const int *__restrict__ seq, const int *__restrict__ pos_of, const float *__restrict__ wq, const float *__restrict__ wk,
+    const float *__restrict__ cos_t, const float *__restrict__ sin_t, int n_pages, int page, int n_seqs, int max_pages, int kv_heads, int hd, int heads, int S,
+    int table, float eps, int tiles, int slabs_each) {
+    constexpr int VEC = 16 / (int)sizeof(T), LPR = 64 / VEC, PPS = 256 / LPR, ROW = 64;        // row pairs: of a step, of a column in LDS
+    typedef unsigned pair_t __attribute__((ext_vector_type(sizeof(T) / 2)));                  // a column's values of a row pair
+    __shared__ __attribute__((aligned(16))) pair_t turned[64 * ROW];
+    __shared__ float sums[4 * LPR * VEC];
+    __shared__ long long place[64];         // row of head 0, -1: no token
+    __shared__ int at[64];
+    const int tid = threadIdx.x, half = hd / 2;
+    const int b = blockIdx.x / tiles, s0 = (blockIdx.x - b * tiles) * 64;
+    bool some = false;
+    if (tid < 64) {
+        long long p = -1;
+        int pos = 0;
+        if (s0 + tid < S) {
+            const size_t col = (size_t)b * S + s0 + tid;
+            pos = pos_of[col];
+            p = token_row(seq, pages, col, pos, n_pages, page, n_seqs, max_pages, kv_heads, cos_t ? table : 0x7fffffff);
+        }
+        place[tid] = p;
+        at[tid] = p < 0 ? 0 : pos;
+        some = p >= 0;
+    }
+    if (!__syncthreads_or(some)) return;        // (the end of a padded prompt)
+    const int lc = tid % LPR, p0 = tid / LPR;
+    const LaneCols mine = lane_cols<VEC>(s0 + lc * VEC, S);
+    // the lane's columns that are its own, and tokens
+    bool own[VEC], all = true, in_a_row = true;
+    int pos[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+        const int c = mine.col + j - s0;
+        own[j] = mine.ok && j >= mine.dup && place[max(c, 0)] >= 0;
+        pos[j] = own[j] ? at[c] : 0;
+        all &= own[j];
+        in_a_row &= pos[j] == pos[0] + j;
+    }
+    float cs[CAP][VEC], sn[CAP][VEC];
+    if (cos_t) {
+#pragma unroll
+        for (int kk = 0; kk < CAP; kk++) {
+            const int rp = min(p0 + kk * PPS, half - 1);
+            const float *pc = cos_t + (size_t)rp * table, *ps = sin_t + (size_t)rp * table;
+            if (in_a_row) {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) {
+                    const v4f x = ld4(pc + pos[0] + j), y = ld4(ps + pos[0] + j);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { cs[kk][j + e] = x[e]; sn[kk][j + e] = y[e]; }
+                }
+            } else
+#pragma unroll
+                for (int j = 0; j < VEC; j++) { cs[kk][j] = pc[pos[j]]; sn[kk][j] = ps[pos[j]]; }
+        }
+    }
+    const int slabs = heads + 2 * kv_heads, first = blockIdx.y * slabs_each, last = min(first + slabs_each, slabs);
+    // the next head's values are under way while one is worked on
+    typedef decltype(raw_cols((const T *)nullptr)) Raw;
+    Raw r0[CAP], r1[CAP];
+    load_slab<T, CAP, PPS>(r0, r1, slab_of(first, heads, kv_heads, q, k, v), b, hd, S, mine.col, p0, mine.ok);
+    for (int slab = first; slab < last; slab++) {
+        const Slab<T> now = slab_of(slab, heads, kv_heads, q, k, v);
+        const bool is_q = now.is_q, is_k = now.is_k;
+        const int head = now.head;
+        const float *w = of_kind(is_q, is_k, wq, wk, (const float *)nullptr);
+        float x0[CAP][VEC], x1[CAP][VEC];
+#pragma unroll
+        for (int kk = 0; kk < CAP; kk++) { widen(x0[kk], r0[kk]); widen(x1[kk], r1[kk]); }
+        if (slab + 1 < last) load_slab<T, CAP, PPS>(r0, r1, slab_of(slab + 1, heads, kv_heads, q, k, v), b, hd, S, mine.col, p0, mine.ok);
+        __syncthreads();            // (everybody is done with LDS)
+        if (w) {
+            float acc[1][VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                acc[0][j] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < CAP; kk++) { acc[0][j] += x0[kk][j] * x0[kk][j]; acc[0][j] += x1[kk][j] * x1[kk][j]; }
+            }
+            // the column's sum: over the wave's lanes, then over the waves by one thread to a column, which takes the root for all
+#pragma unroll
+            for (int j = 0; j < VEC; j++) acc[0][j] = wave_sum_stride<LPR>(acc[0][j]);
+            if ((tid & 63) < LPR)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) sums[(tid >> 6) * 64 + lc * VEC + j] = acc[0][j];
+            __syncthreads();
+            if (tid < 64) sums[tid] = 1.f / sqrtf((((sums[tid] + sums[64 + tid]) + sums[128 + tid]) + sums[192 + tid]) * (1.f / hd) + eps);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < VEC; j++) acc[0][j] = sums[lc * VEC + j];
+#pragma unroll
+            for (int kk = 0; kk < CAP; kk++) {
+                const int rp = min(p0 + kk * PPS, half - 1);
+                const float w0 = w[2 * rp], w1 = w[2 * rp + 1];
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    x0[kk][j] = (x0[kk][j] * acc[0][j]) * w0;
+                    x1[kk][j] = (x1[kk][j] * acc[0][j]) * w1;
+                }
+            }
+        }
+        if ((is_q || is_k) && cos_t) {
+#pragma unroll
+            for (int kk = 0; kk < CAP; kk++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const float y0 = x0[kk][j] * cs[kk][j] - x1[kk][j] * sn[kk][j];
+                    x1[kk][j] = x0[kk][j] * sn[kk][j] + x1[kk][j] * cs[kk][j];
+                    x0[kk][j] = y0;
+                }
+        }
+        if (is_q) {
+#pragma unroll
+            for (int kk = 0; kk < CAP; kk++) {
+                const int rp = p0 + kk * PPS;
+                if (rp >= half) continue;
+                T *out = q_out + (((size_t)b * heads + head) * hd + 2 * rp) * S + mine.col;
+                if (all) {
+                    store_cols<VEC>(out, x0[kk]);
+                    store_cols<VEC>(out + S, x1[kk]);
+                } else
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        if (own[j]) {
+                            store_one(out + j, x0[kk][j]);
+                            store_one(out + S + j, x1[kk][j]);
+                        }
+            }
+            continue;
+        }
+        constexpr int XOR = 64 / LPR;           // pairs that a wave has of a column; the lanes of a column take other places in its row
+#pragma unroll
+        for (int kk = 0; kk < CAP; kk++) {
+            const int rp = p0 + kk * PPS;
+            if (rp >= half) continue;
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (own[j]) turned[(mine.col + j - s0) * ROW + (rp ^ ((mine.col + j - s0) / VEC * XOR & (ROW - 1)))] = pair_of(x0[kk][j], x1[kk][j], (T *)nullptr);
+        }
+        __syncthreads();
+        T *out = of_kind(false, is_k, k_cache, k_cache, v_cache) + (size_t)head * page * hd;
+        const int chunks = hd / VEC;            // of 16 bytes
+        constexpr int PER = VEC / 2;            // pairs of a chunk
+        for (int i = tid; i < 64 * chunks; i += 256) {
+            const int c = i / chunks, x = i - c * chunks;
+            if (place[c] < 0) continue;
+            *reinterpret_cast<v4u *>(out + (size_t)place[c] * hd + x * VEC) = *reinterpret_cast<const v4u *>(turned + c * ROW + (x * PER ^ (c / VEC * XOR & (ROW - 1))));
+        }
+    }
+}
+
+// Heads of columns from which tiles pay, where rows have 16 columns at least.  us, a wave to a head of a column / tiles, 16 + 8 + 8 heads of 128, bfloat16:
+// one row of 128 new tokens 7.5 / 9.3, of 256 (8192 heads) 12.5 / 10.9, 16 rows of 16 positions 8.4 / 9.0, 32 of 32 17.6 / 13.9, 16 of 256 62 / 21.
+constexpr size_t TILE_FROM = 8192;
 
 template <typename T>
 int kv_append(const char *who, const mi355_kv_cache *c, T *q_out, const T *q, const T *k, const T *v, const float *wq, const float *wk,
@@ -78,10 +289,23 @@ int kv_append(const char *who, const mi355_kv_cache *c, T *q_out, const T *q, co
     const size_t units = (size_t)S * batch * (heads + 2 * c->kv_heads);
     if (ceil_div(units, 4) > 0xffffff) return mi355_fail("%s: %zu heads of columns (at most 2^26 - 4)", who, units);
     if (!mi355_ready(who)) return -1;
-    const AppendArgs a = {*c, wq, wk, cos_dev, sin_dev, seq, pos, heads, S, batch, table, eps};
-    kv_append_kernel<T><<<(unsigned)ceil_div(units, 4), 256, 0, g_ctx.stream>>>(q_out, q, k, v, a);
-    LAUNCH_OK(who);
-    return 0;
+    auto go = [&](auto kernel, dim3 grid, auto... more) {
+        kernel<<<grid, 256, 0, g_ctx.stream>>>(q_out, q, k, v, (T *)c->k, (T *)c->v, c->pages, seq, pos, wq, wk, cos_dev, sin_dev, c->n_pages, c->page, c->n_seqs,
+                                               c->max_pages, c->kv_heads, c->hd, heads, S, table, eps, more...);
+        LAUNCH_OK(who);
+        return 0;
+    };
+    if (S >= 16 && units >= TILE_FROM) {
+        const int slabs = heads + 2 * c->kv_heads, tiles = (int)ceil_div(S, 64);
+        // two workgroups to a compute unit; what is beyond that goes to more heads for each, up to eight
+        const size_t all = (size_t)tiles * batch * slabs, rounds = all / (2 * (size_t)g_ctx.num_cu);
+        const int each = rounds >= 8 ? 8 : rounds >= 4 ? 4 : rounds >= 2 ? 2 : 1;
+        const dim3 grid((unsigned)(tiles * batch), (unsigned)ceil_div(slabs, each));
+        constexpr int PPS = PAIRS_AT_ONCE<T>;
+        if (c->hd / 2 <= 32) return go(kv_append_tile_kernel<T, 32 / PPS>, grid, tiles, each);
+        return go(kv_append_tile_kernel<T, 64 / PPS>, grid, tiles, each);
+    }
+    return go(kv_append_kernel<T>, dim3((unsigned)ceil_div(units, 4)), S * batch);
 }
 
 // ---- rows that follow their parents ----------------------------------------------------------------------------------------------

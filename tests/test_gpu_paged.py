@@ -311,6 +311,10 @@ APPENDS = [
     (16, 8, 128, 16, 2, 256, [256, 100], True, True), (2, 1, 64, 32, 1, 197, [197], True, True), (3, 3, 40, 16, 3, 33, [33, 1, 0], False, True),
     (12, 12, 64, 16, 1, 1030, [1030], False, True), (8, 2, 120, 16, 2, 65, [64, 65], True, False), (0, 2, 128, 16, 2, 40, [40, 17], True, True),
     (40, 2, 128, 256, 1, 300, [300], True, True), (4, 4, 16, 16, 5, 15, [15, 3, 16 - 1, 8, 2], True, True), (2, 2, 88, 16, 1, 130, [129], True, True),
+    # enough columns for tiles: rows of odd lengths, sizes of heads that fill no tile, the last columns of a row short, columns of different sequences
+    (8, 2, 120, 16, 2, 345, [345, 65], True, True), (3, 3, 40, 32, 5, 211, [211, 0, 64, 65, 128], False, True), (6, 1, 88, 48, 3, 449, [449, 448, 3], True, False),
+    (16, 8, 8, 16, 1, 515, [515], True, True), (5, 5, 72, 16, 40, 19, None, True, True), (16, 8, 128, 16, 1, 300, None, True, True),
+    (0, 4, 64, 64, 4, 260, [260, 100, 259, 1], True, True), (16, 8, 24, 16, 16, 16, [16] * 15 + [7], True, True),
 ]
 
 
@@ -359,7 +363,7 @@ def test_append(br, i, storage):
 
 
 @pytest.mark.parametrize("storage", ["f32", "bf16"])
-@pytest.mark.parametrize("S", [4, 70])
+@pytest.mark.parametrize("S", [4, 70, 403])
 def test_append_of_columns_that_are_no_token(br, storage, S):
     """Sequences, positions, pages and angles that are none: nothing is written for them, everything for the others."""
     cache = Cache(storage, 2, 64, 16, [200, 200, 90], seed=80, values=False)
@@ -368,7 +372,7 @@ def test_append_of_columns_that_are_no_token(br, storage, S):
     q, k, v = (stored(storage, rng.standard_normal((3, h * 64, S))) for h in (4, 2, 2))
     seq = np.array([0, 1, 1, 5, -1, 2, 0, 2 ** 31 - 1, -2 ** 31, 1], np.int64)
     pos = np.array([199, 37, 70, 0, 3, 13 * 16, 2 ** 31 - 1, 5, 5, -2 ** 31], np.int64)
-    places = [(0, 100 + j) for j in range(60)] + [(2, j) for j in range(50)] + [(1, 80 + j) for j in range(90)]       # of the others, each its own
+    places = [(0, 100 + j) for j in range(60)] + [(2, j) for j in range(50)] + [(1, 80 + j) for j in range(90)] + [(0, j) for j in range(99)]     # of the others, each its own
     seqs, poss = np.empty(3 * S, np.int32), np.empty(3 * S, np.int32)
     good = np.zeros(3 * S, bool)
     for n in range(3 * S):
@@ -389,7 +393,7 @@ def test_append_of_columns_that_are_no_token(br, storage, S):
         page, slot = cache.row(seqs[b, s], poss[b, s])
         want_k[page, :, slot], off_k[page, :, slot] = val[b, :, s].reshape(2, 64), bound[b, :, s].reshape(2, 64)
         want_v[page, :, slot] = v[b, :, s].reshape(2, 64)
-    assert good.sum() > S // 2 and np.all(np.abs(f64(got_k) - want_k) <= off_k) and np.array_equal(got_v, want_v)
+    assert good.sum() > min(S // 2, 100) and np.all(np.abs(f64(got_k) - want_k) <= off_k) and np.array_equal(got_v, want_v)
 
 
 @pytest.mark.parametrize("storage", ["f32", "bf16"])
