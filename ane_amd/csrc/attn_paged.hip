@@ -25,18 +25,18 @@ constexpr int HEADS = 16;                   // query heads of one product
 constexpr int WAVES = 4;
 constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
 constexpr int GRAIN = 2 * WAVES;            // tiles that a workgroup should have at least
+constexpr int JOIN = 16;                    // slots whose values a thread has on their way at once
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
 __device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ long long uniform(long long v) { return (long long)uniform((int)(v >> 32)) << 32 | (unsigned)uniform((int)v); }
 
 struct PagedArgs {
     mi355_kv_cache c;
     const int *seq, *pos;
-    int heads, S, cols, group;      // group: query heads of a KV head
+    int heads, S, col0, cols, group, positions;     // columns col0 .. col0 + cols - 1; group: query heads of a KV head; positions of a row of the table
     float scale2;
     float *slots;                   // partial results: two for each workgroup
     unsigned *arrived;
@@ -411,86 +411,88 @@ __device__ __forceinline__ v2f slot_get(const float *p) {
     return v2f{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
 }
 
-// The tiles of all columns, KV heads and parts of a group of query heads, one after the other, are dealt out evenly: workgroup w has tiles
-// w T / W .. (w + 1) T / W - 1, whatever sequences they belong to.  (Lengths are in device memory: the host cannot deal them out, and a batch's
-// longest sequence would otherwise decide when it ends.)  A column's tiles of one KV head that lie in several workgroups are a split unit; each of
-// these leaves its maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.
+// A unit is the tiles of a column and KV head (of 16 of its query heads); those of all columns, one after the other, are dealt out evenly:
+// workgroup w of W has T / W neighbouring tiles, whatever sequences they belong to.  (Lengths are in device memory: the host cannot deal them out,
+// and a batch's longest sequence would otherwise decide when it ends.)  A unit whose tiles lie in several workgroups is split: each of these leaves its
+// maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.  A workgroup has two such units at most, the
+// one that it begins with and the one that it ends with, and looks after both when it is done with its tiles.
 template <typename T, int HDB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
                                                                                                   PagedArgs a) {
     typedef Tile<T, HDB> Tl;
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
-    __shared__ long long sums[WAVES + 2];
-    __shared__ int ticket;
+    __shared__ int sums[WAVES + 2], ticket[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
     const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts;      // units of a column
     auto length = [&](int col) __attribute__((always_inline)) {
-        const int p = a.pos[col];
-        return paged_entry(a.seq ? a.seq[col] : col, p, a.c.n_seqs, a.c.max_pages, page) < 0 ? 0 : p + 1;
+        const int p = a.pos[col], seq = a.seq ? a.seq[col] : col;
+        return seq < 0 || seq >= a.c.n_seqs || p < 0 || p >= a.positions ? 0 : p + 1;
     };
     auto tiles_of = [&](int col) __attribute__((always_inline)) { return (length(col) + Tl::POSITIONS - 1) / Tl::POSITIONS; };
 
     // where this workgroup's tiles begin and end
     const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
-    long long mine = 0;
-    for (int c = c0; c < c1; c++) mine += tiles_of(c);
-    long long upto = mine;
+    int mine = 0;
+    for (int c = c0; c < c1; c++) mine += tiles_of(a.col0 + c);
+    for (int i = tid; i < HEADS * ROW; i += 256) lds.q[i] = 0.f;           // (heads that there are not)
+    int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const long long x = __shfl_up(upto, d, 64);
+        const int x = __shfl_up(upto, d, 64);
         if ((tid & 63) >= d) upto += x;
     }
     if ((tid & 63) == 63) sums[tid >> 6] = upto;
     __syncthreads();
-    long long total = 0;
+    int total = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; i++) {
         if (i < tid >> 6) upto += sums[i];
         total += sums[i];
     }
     total = uniform(total * units);
-    const long long wanted = (total + GRAIN - 1) / GRAIN;
-    const int groups = (int)(wanted < gridDim.x ? wanted : gridDim.x), w = blockIdx.x;
+    const int w = blockIdx.x, groups = min((total + GRAIN - 1) / GRAIN, (int)gridDim.x);
     if (w >= groups) return;
-    const long long share = total / groups, more = total - share * groups;          // the first `more` workgroups have one tile more
-    auto bound = [&](int i) __attribute__((always_inline)) { return i * share + min((long long)i, more); };
-    long long lo = bound(w);
-    const long long hi = bound(w + 1);
+    const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one tile more
+    int lo = w * share + min(w, more);
+    const int hi = lo + share + (w < more);
     // the column of tile lo: the thread whose columns have it walks over them
     if (lo >= (upto - mine) * units && lo < upto * units) {
-        long long b = (upto - mine) * units;
-        int c = c0;
+        int b = (upto - mine) * units, c = c0;
         while (true) {
-            const long long n = (long long)tiles_of(c) * units;
+            const int n = tiles_of(a.col0 + c) * units;
             if (lo < b + n) break;
             b += n;
             c++;
         }
-        sums[WAVES] = c;
+        sums[WAVES] = a.col0 + c;
         sums[WAVES + 1] = b;
     }
     __syncthreads();
-    int col = uniform((int)sums[WAVES]);
-    long long start = uniform(sums[WAVES + 1]);         // the first tile of the column
-    const size_t page_stride = (size_t)a.c.kv_heads * page * hd;
+    int col = uniform(sums[WAVES]), start = uniform(sums[WAVES + 1]);       // start: the first tile of the column
+    const size_t page_stride = (size_t)a.c.kv_heads * page * hd, slot_size = (size_t)HEADS * (HDB * 32 + 2);
+    const int row = hd + 2;             // of a slot: a head's maximum, its sum (-1: no position seen), its channels
+    struct Split { int col, part, kvh, first, last; } split[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};      // the unit that began before, the one that ends behind
+    auto out_of = [&](int col, int head0, size_t channels) __attribute__((always_inline)) {
+        const int b = col / a.S, s = col - b * a.S;
+        return ((size_t)b * a.heads + head0) * channels * a.S + s;
+    };
 
     while (lo < hi) {
         const int len = uniform(length(col)), n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
-        if (n == 0 || lo >= start + (long long)n * units) {
-            start += (long long)n * units;
+        if (lo >= start + n * units) {
+            start += n * units;
             col++;
             continue;
         }
-        const int unit = (int)((lo - start) / n), part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads;
-        const long long unit_lo = start + (long long)unit * n;
-        const int t0 = (int)(lo - unit_lo), t1 = (int)(min(hi, unit_lo + n) - unit_lo);
-        const int heads = min(a.group - part * HEADS, HEADS), head0 = kvh * a.group + part * HEADS;
-        const int b = col / a.S, s = col - b * a.S, seq = uniform(a.seq ? a.seq[col] : col);
+        const int unit = (lo - start) / n, part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads;
+        const int unit_lo = start + unit * n, t0 = lo - unit_lo, t1 = min(hi, unit_lo + n) - unit_lo;
+        const int heads = min(a.group - part * HEADS, HEADS), head0 = kvh * a.group + part * HEADS, seq = uniform(a.seq ? a.seq[col] : col);
+        const T *qp = q + out_of(col, head0, hd);
         // the queries, as fp32 values
-        for (int i = tid; i < HEADS * HDB * 32; i += 256) {
-            const int h = i / (HDB * 32), ch = i - h * (HDB * 32);
-            lds.q[h * ROW + ch] = h < heads && ch < hd ? load_one(q + (((size_t)b * a.heads + head0 + h) * hd + ch) * a.S + s) : 0.f;
+        for (int i = tid; i < heads * hd; i += 256) {
+            const int h = i / hd;
+            lds.q[h * ROW + i - h * hd] = load_one(qp + (size_t)i * a.S);
         }
         __syncthreads();
         const T *k = (const T *)a.c.k + (size_t)kvh * page * hd, *v = (const T *)a.c.v + (size_t)kvh * page * hd;
@@ -500,120 +502,115 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             // An infinity times the half of a weight that is zero is NaN: such sums are formed again.
             bool odd = false;
             for (int i = tid; i < heads * hd; i += 256) {
-                const float x = lds.sum_at(i / hd, i % hd);
+                const int h = i / hd;
+                const float x = lds.sum_at(h, i - h * hd);
                 odd |= x != x;
             }
             if (__syncthreads_or(odd))
                 share_out_again<T, HDB>((shared_ptr<HDB>)&lds, k, v, page_stride, table, page, a.c.n_pages, hd, heads, t0, t1, len, a.scale2);
         }
         const bool any = lds.seen[0] | lds.seen[1] | lds.seen[2] | lds.seen[3];
-        auto write = [&](int h, int ch, float val) __attribute__((always_inline)) { store_one(o + (((size_t)b * a.heads + head0 + h) * hd + ch) * a.S + s, val); };
-        auto write_lse = [&](int h, float top, float sum) __attribute__((always_inline)) {
-            if (lse) lse[((size_t)b * a.heads + head0 + h) * a.S + s] = (top + __builtin_amdgcn_logf(sum)) * LN2;
-        };
         if (t0 == 0 && t1 == n) {
+            T *op = o + out_of(col, head0, hd);
             if (any)
                 for (int i = tid; i < heads * hd; i += 256) {
-                    const int h = i / hd, ch = i - h * hd;
+                    const int h = i / hd;
                     float top, sum;
                     lds.stats(h, top, sum);
-                    write(h, ch, lds.sum_at(h, ch) / sum);
-                    if (ch == 0) write_lse(h, top, sum);
+                    store_one(op + (size_t)i * a.S, lds.sum_at(h, i - h * hd) / sum);
+                    if (lse && i == h * hd) lse[out_of(col, head0 + h, 1)] = (top + __builtin_amdgcn_logf(sum)) * LN2;
                 }
         } else {
-            // a slot: [head][maximum, sum, whether anything was seen, -, channels]
-            const int row = hd + 4;
-            const size_t slot_size = (size_t)HEADS * (HDB * 32 + 4);
-            float *slot = a.slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;       // (of the two units that a workgroup may share, the one that begins in it second)
+            float *slot = a.slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;
             for (int i = 2 * tid; i < heads * row; i += 512) {
                 const int h = i / row, x = i - h * row;
-                float first_of, second;
-                if (x == 0) lds.stats(h, first_of, second);
-                else if (x == 2) first_of = any ? 1.f : 0.f, second = 0.f;
-                else first_of = lds.sum_at(h, x - 4), second = lds.sum_at(h, x - 3);
-                slot_put(slot + i, first_of, second);
+                float v0, v1;
+                if (x == 0) {
+                    lds.stats(h, v0, v1);
+                    v1 = any ? v1 : -1.f;
+                } else v0 = lds.sum_at(h, x - 2), v1 = lds.sum_at(h, x - 1);
+                slot_put(slot + i, v0, v1);
             }
             // the workgroups that have tiles of the unit
-            auto owner = [&](long long tile) __attribute__((always_inline)) {
-                const long long longer = more * (share + 1);
-                return (int)(tile < longer ? tile / (share + 1) : more + (tile - longer) / share);
+            auto owner = [&](int tile) __attribute__((always_inline)) {
+                const int longer = more * (share + 1);
+                return tile < longer ? tile / (share + 1) : more + (tile - longer) / share;
             };
-            const int first = owner(unit_lo), last = owner(unit_lo + n - 1);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // this wave's part of the slot is in memory,
-            __syncthreads();                                        // everybody's is
-            if (tid == 0) ticket = (int)__hip_atomic_fetch_add(a.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (ticket == last - first) {
-                // Everybody's slots are in memory.  Maxima and sums first, 16 threads to a head; then the channels, two to a thread and the
-                // slots in turns where there are threads to spare.
-                if (tid == 0) __hip_atomic_store(a.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const int count = last - first + 1;
-                auto from = [&](int j) __attribute__((always_inline)) { return a.slots + ((size_t)(first + j) * 2 + (j == 0)) * slot_size; };
-                {
-                    const int h = tid >> 4;
-                    float top = -INFINITY, some = 0.f, sum = 0.f;
-                    if (h < heads) {
-                        for (int j = tid & 15; j < count; j += 16) {
-                            const v2f x = slot_get(from(j) + h * row);
-                            some += slot_get(from(j) + h * row + 2)[0];
-                            const float to = fmaxf(top, x[0]), base = to == -INFINITY ? 0.f : to;
-                            sum = sum * __builtin_amdgcn_exp2f(top - base) + x[1] * __builtin_amdgcn_exp2f(x[0] - base);
-                            top = to;
-                        }
-#pragma unroll
-                        for (int d = 1; d < 16; d <<= 1) {
-                            const float t2 = __shfl_xor(top, d, 64), s2 = __shfl_xor(sum, d, 64);
-                            const float to = fmaxf(top, t2), base = to == -INFINITY ? 0.f : to;
-                            sum = sum * __builtin_amdgcn_exp2f(top - base) + s2 * __builtin_amdgcn_exp2f(t2 - base);
-                            top = to;
-                            some += __shfl_xor(some, d, 64);
-                        }
-                        if ((tid & 15) == 0) {
-                            lds.m[h] = top;
-                            lds.l[h] = sum;
-                            lds.m[HEADS + h] = some;
-                        }
-                    }
-                }
-                __syncthreads();
-                const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
-                for (int i = tid; i < pairs * turns; i += 256) {
-                    const int turn = i / pairs, x = i - turn * pairs, h = 2 * x / hd, ch = 2 * x - h * hd;
-                    const float base = lds.m[h] == -INFINITY ? 0.f : lds.m[h];
-                    float v0 = 0.f, v1 = 0.f;
-                    // eight at a time on their way (the last one again behind the end, and not added)
-                    for (int j = turn; j < count; j += 8 * turns) {
-                        v2f m[8], y[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float *p = from(min(j + e * turns, count - 1)) + h * row;
-                            m[e] = slot_get(p);
-                            y[e] = slot_get(p + 4 + ch);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            if (j + e * turns >= count) break;
-                            const float f = __builtin_amdgcn_exp2f(m[e][0] - base);
-                            v0 += y[e][0] * f;
-                            v1 += y[e][1] * f;
-                        }
-                    }
-                    lds.o[2 * i] = v0;
-                    lds.o[2 * i + 1] = v1;
-                }
-                __syncthreads();
-                if (lds.m[HEADS] != 0.f)
-                    for (int i = tid; i < heads * hd; i += 256) {
-                        float val = 0.f;
-                        for (int turn = 0; turn < turns; turn++) val += lds.o[turn * heads * hd + i];
-                        const int h = i / hd, ch = i - h * hd;
-                        write(h, ch, val / lds.l[h]);
-                        if (ch == 0) write_lse(h, lds.m[h], lds.l[h]);
-                    }
-            }
+            split[t0 == 0] = {col, part, kvh, owner(unit_lo), owner(unit_lo + n - 1)};
         }
         __syncthreads();
         lo = unit_lo + t1;
+    }
+
+    if (split[0].col < 0 && split[1].col < 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // this wave's parts of the slots are in memory,
+    __syncthreads();                                        // everybody's are
+    if (tid < 2 && (tid ? split[1].col : split[0].col) >= 0)
+        ticket[tid] = (int)__hip_atomic_fetch_add(a.arrived + (tid ? split[1].first : split[0].first), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+        const Split u = i ? split[1] : split[0];
+        if (u.col < 0 || ticket[i] != u.last - u.first) continue;
+        // The last to arrive: everybody's slots are in memory.
+        if (tid == 0) __hip_atomic_store(a.arrived + u.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int heads = min(a.group - u.part * HEADS, HEADS), head0 = u.kvh * a.group + u.part * HEADS, count = u.last - u.first + 1;
+        T *op = o + out_of(u.col, head0, hd);
+        // two channels to a thread, and the slots in turns where there are threads to spare
+        const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
+        for (int x0 = 0; x0 < pairs * turns; x0 += 256) {
+            const int x = x0 + tid, turn = x / pairs, pair = x - turn * pairs, h = 2 * pair / hd, ch = 2 * pair - h * hd;
+            const bool in = x < pairs * turns;
+            const float *mine = a.slots + ((size_t)u.first * 2) * slot_size + h * row;
+            float top = -INFINITY, sum = -1.f, v0 = 0.f, v1 = 0.f;
+            for (int j = in ? turn : count; j < count; j += JOIN * turns) {
+                v2f st[JOIN], y[JOIN];
+                // all on their way at once (the last one again behind the end, and not added)
+#pragma unroll
+                for (int e = 0; e < JOIN; e++) {
+                    const int at = min(j + e * turns, count - 1);
+                    const float *p = mine + (size_t)(2 * at + (at == 0)) * slot_size;
+                    st[e] = slot_get(p);
+                    y[e] = slot_get(p + 2 + ch);
+                }
+                float to = top;
+#pragma unroll
+                for (int e = 0; e < JOIN; e++) to = fmaxf(to, st[e][0]);
+                const float base = to == -INFINITY ? 0.f : to, old = __builtin_amdgcn_exp2f(top - base);
+                sum = sum < 0.f ? sum : sum * old;
+                v0 *= old;
+                v1 *= old;
+                top = to;
+#pragma unroll
+                for (int e = 0; e < JOIN; e++) {
+                    if (j + e * turns >= count) break;
+                    const float f = __builtin_amdgcn_exp2f(st[e][0] - base);
+                    if (!(st[e][1] < 0.f)) sum = (sum < 0.f ? 0.f : sum) + st[e][1] * f;
+                    v0 += y[e][0] * f;
+                    v1 += y[e][1] * f;
+                }
+            }
+            if (turns > 1) {                // (one round then)
+                float *p = lds.o + 5 * tid;
+                p[0] = top; p[1] = sum; p[2] = v0; p[3] = v1;
+                __syncthreads();
+            }
+            if (turn > 0 || !in) continue;
+            for (int t = 1; t < turns; t++) {
+                const float *p = lds.o + 5 * (tid + t * pairs);
+                const float to = fmaxf(top, p[0]), base = to == -INFINITY ? 0.f : to, f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(p[0] - base);
+                if (!(p[1] < 0.f)) sum = (sum < 0.f ? 0.f : sum * f0) + p[1] * f1;
+                else if (!(sum < 0.f)) sum *= f0;
+                v0 = v0 * f0 + p[2] * f1;
+                v1 = v1 * f0 + p[3] * f1;
+                top = to;
+            }
+            if (sum < 0.f) continue;
+            store_one(op + (size_t)(2 * pair) * a.S, v0 / sum);
+            store_one(op + (size_t)(2 * pair + 1) * a.S, v1 / sum);
+            if (lse && ch == 0) lse[out_of(u.col, head0 + h, 1)] = (top + __builtin_amdgcn_logf(sum)) * LN2;
+        }
+        __syncthreads();
     }
 }
 
@@ -633,14 +630,21 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
     if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
-    const int groups = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
+    const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
     auto go = [&](auto blocks) {
         constexpr int HDB = decltype(blocks)::value;
-        float *slots = (float *)mi355_ws((size_t)groups * 2 * HEADS * (HDB * 32 + 4) * sizeof(float));
+        // tiles are counted in 32 bits: columns that could have more go in several launches
+        const size_t column = ceil_div((size_t)c->max_pages * c->page, Tile<T, HDB>::POSITIONS) * c->kv_heads * parts;
+        if (column > 0x7fffffff) return mi355_fail("%s: %zu tiles of positions and heads of a column (at most 2^31 - 1)", who, column);
+        const size_t at_once = 0x7fffffff / column;
+        float *slots = (float *)mi355_ws((size_t)most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));
         if (!slots) return -1;
-        const PagedArgs a = {*c, seq, pos, heads, S, S * batch, heads / c->kv_heads, scale * LOG2E, slots, arrived};
-        attn_paged_kernel<T, HDB><<<(unsigned)groups, 256, 0, g_ctx.stream>>>(o, lse, q, a);
-        LAUNCH_OK(who);
+        for (size_t c0 = 0; c0 < (size_t)S * batch; c0 += at_once) {
+            const size_t cols = (size_t)S * batch - c0 < at_once ? (size_t)S * batch - c0 : at_once, grid = ceil_div(cols * column, GRAIN);
+            const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)cols, group, c->max_pages * c->page, scale * LOG2E, slots, arrived};
+            attn_paged_kernel<T, HDB><<<(unsigned)(grid < (size_t)most ? grid : most), 256, 0, g_ctx.stream>>>(o, lse, q, a);
+            LAUNCH_OK(who);
+        }
         return 0;
     };
     if (c->hd <= 32) return go(std::integral_constant<int, 1>());

@@ -316,32 +316,31 @@ __device__ __forceinline__ int parent_of(int n, const int *parents, const int *p
     return p >= 0 && p < rows && pos[p] == pos[n] ? p : n;
 }
 
-// A workgroup to a row.
-__global__ __launch_bounds__(256) void kv_table_kernel(int *__restrict__ pages_out, int *__restrict__ pos_out, int *__restrict__ spare_out,
-                                                       const int *__restrict__ pages, const int *__restrict__ parents, const int *__restrict__ pos,
-                                                       const int *__restrict__ spare, int rows, int max_pages, int page, int advance) {
-    const int n = blockIdx.x, at = pos[n], parent = parent_of(n, parents, pos, rows);
-    const PagedMove m = paged_move(n, parent, at, page);
-    const bool moves = m.moves && m.tail < max_pages;
-    const int *from = pages + (size_t)parent * max_pages, *mine = pages + (size_t)n * max_pages;
-    for (int j = threadIdx.x; j < max_pages; j += 256)
-        pages_out[(size_t)n * max_pages + j] = j > m.tail ? mine[j] : j == m.tail && moves ? spare[n] : from[j];
-    if (threadIdx.x == 0) {
-        if (pos_out) pos_out[n] = at < 0 ? at : at + advance;
-        spare_out[n] = moves ? mine[m.tail] : spare[n];
-    }
-}
-
 constexpr int MOVE_LAYERS = 64;
 struct MoveArgs { void *cache[2 * MOVE_LAYERS]; };
 
-// The tails: a workgroup to a head of a row and a tensor of a layer; `words` 16-byte words to a position.
-__global__ __launch_bounds__(256) void kv_move_kernel(MoveArgs t, const int *__restrict__ pages, const int *__restrict__ parents,
-                                                      const int *__restrict__ pos, const int *__restrict__ spare, int rows, int max_pages, int page,
-                                                      int n_pages, int kv_heads, int words) {
-    const int n = blockIdx.x / kv_heads, head = blockIdx.x - n * kv_heads, parent = parent_of(n, parents, pos, rows);
-    const PagedMove m = paged_move(n, parent, pos[n], page);
-    if (!m.moves || m.tail >= max_pages) return;
+// A workgroup to a row's head, in y to a tensor of a layer: its part of the tail, `words` 16-byte words to a position.  Behind the last tensor (in the first
+// of several launches) the new table, a workgroup to a row; it is read by none of the copies.
+// Rows that stay, and full pages, are not touched: 256 beams of 28 layers move 787 MB in 148 us, which is what a copy of as much takes.
+__global__ __launch_bounds__(256) void kv_reorder_kernel(MoveArgs t, int tensors, int *__restrict__ pages_out, int *__restrict__ pos_out, int *__restrict__ spare_out,
+                                                         const int *__restrict__ pages, const int *__restrict__ parents, const int *__restrict__ pos,
+                                                         const int *__restrict__ spare, int rows, int max_pages, int page, int n_pages, int kv_heads, int words,
+                                                         int advance) {
+    const int n = blockIdx.x / kv_heads, head = blockIdx.x - n * kv_heads, at = pos[n], parent = parent_of(n, parents, pos, rows);
+    const PagedMove m = paged_move(n, parent, at, page);
+    const bool moves = m.moves && m.tail < max_pages;
+    if ((int)blockIdx.y == tensors) {
+        if (head != 0) return;
+        const int *from = pages + (size_t)parent * max_pages, *mine = pages + (size_t)n * max_pages;
+        for (int j = threadIdx.x; j < max_pages; j += 256)
+            pages_out[(size_t)n * max_pages + j] = j > m.tail ? mine[j] : j == m.tail && moves ? spare[n] : from[j];
+        if (threadIdx.x == 0) {
+            if (pos_out) pos_out[n] = at < 0 ? at : at + advance;
+            spare_out[n] = moves ? mine[m.tail] : spare[n];
+        }
+        return;
+    }
+    if (!moves) return;
     const int from = pages[(size_t)parent * max_pages + m.tail], to = spare[n];
     if (!paged_id_ok(from, n_pages) || !paged_id_ok(to, n_pages)) return;
     v4i *base = (v4i *)t.cache[blockIdx.y];
@@ -368,19 +367,16 @@ int kv_reorder(const char *who, int size, const mi355_kv_cache *caches, int coun
     if ((double)c.n_seqs * c.kv_heads > (1 << 24) - 1) return mi355_fail("%s: n_seqs * kv_heads = %.0f (at most 2^24 - 1)", who, (double)c.n_seqs * c.kv_heads);
     if (!mi355_ready(who)) return -1;
     for (int i = 0; i < count; i += MOVE_LAYERS) {
-        MoveArgs t;
+        MoveArgs t = {};
         const int n = count - i < MOVE_LAYERS ? count - i : MOVE_LAYERS;
         for (int j = 0; j < n; j++) {
             t.cache[2 * j] = caches[i + j].k;
             t.cache[2 * j + 1] = caches[i + j].v;
         }
-        kv_move_kernel<<<dim3((unsigned)(c.n_seqs * c.kv_heads), 2 * n), 256, 0, g_ctx.stream>>>(t, c.pages, parent, pos, spare, c.n_seqs, c.max_pages,
-                                                                                               c.page, c.n_pages, c.kv_heads, c.hd * size / 16);
+        kv_reorder_kernel<<<dim3((unsigned)(c.n_seqs * c.kv_heads), 2 * n + (i == 0)), 256, 0, g_ctx.stream>>>(
+            t, 2 * n, pages_out, pos_out, spare_out, c.pages, parent, pos, spare, c.n_seqs, c.max_pages, c.page, c.n_pages, c.kv_heads, c.hd * size / 16, advance);
         LAUNCH_OK(who);
     }
-    kv_table_kernel<<<(unsigned)c.n_seqs, 256, 0, g_ctx.stream>>>(pages_out, pos_out, spare_out, c.pages, parent, pos, spare, c.n_seqs, c.max_pages,
-                                                                  c.page, advance);
-    LAUNCH_OK(who);
     return 0;
 }
 
