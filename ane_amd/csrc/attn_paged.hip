@@ -24,7 +24,11 @@ constexpr float FAR = 16777216.f;           // 2^24
 constexpr int HEADS = 16;                   // query heads of one product
 constexpr int WAVES = 4;
 constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
-constexpr int GRAIN = 2 * WAVES;            // tiles that a workgroup should have at least
+// In tiles, of which a workgroup's waves have one each at a time (1 us for four): what beginning another unit takes (3.6 us), what a workgroup should have
+// at least, and what is not cut off a unit (joining parts takes 3 us).  us, workgroups of at least 8 / 16 / 32 tiles, by tiles alone: one sequence of 256
+// positions, 12 heads of 64 fp32 10.2 / 8.2 / 13.1, 8 heads of 128 bfloat16 8.8 / 14.4 / 25.5, of 2048 positions 11.8 / 13.6 / 17.8, 64 of up to 200
+// 36.6 / 67.7 / 101, of up to 4096 95 / 95 / 95.
+constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
 constexpr int JOIN = 16;                    // slots whose values a thread has on their way at once
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
@@ -411,18 +415,20 @@ __device__ __forceinline__ v2f slot_get(const float *p) {
     return v2f{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
 }
 
-// A unit is the tiles of a column and KV head (of 16 of its query heads); those of all columns, one after the other, are dealt out evenly:
-// workgroup w of W has T / W neighbouring tiles, whatever sequences they belong to.  (Lengths are in device memory: the host cannot deal them out,
-// and a batch's longest sequence would otherwise decide when it ends.)  A unit whose tiles lie in several workgroups is split: each of these leaves its
-// maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.  A workgroup has two such units at most, the
-// one that it begins with and the one that it ends with, and looks after both when it is done with its tiles.
+// A unit is the tiles of a column and KV head (of 16 of its query heads).  Those of all columns, one after the other, are dealt out evenly, a unit
+// counted as its tiles and BEGIN more for what it takes to begin one: workgroup w of W has T / W of that line, whatever sequences they belong to.
+// (Lengths are in device memory: the host cannot deal them out, and a batch's longest sequence would otherwise decide when it ends.)  A border that
+// would cut off fewer than SHORT tiles is moved to the unit's end or beginning.  A unit with borders inside is split: each of its workgroups
+// leaves its maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.  A workgroup has two such units at
+// most, the one that it begins with and the one that it ends with, and looks after both when it is done with its tiles.
 template <typename T, int HDB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
                                                                                                   PagedArgs a) {
     typedef Tile<T, HDB> Tl;
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
-    __shared__ int sums[WAVES + 2], ticket[2];
+    __shared__ int sums[WAVES], ticket[2];
+    __shared__ struct { int col, unit, tile, start; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
     const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts;      // units of a column
     auto length = [&](int col) __attribute__((always_inline)) {
@@ -430,11 +436,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         return seq < 0 || seq >= a.c.n_seqs || p < 0 || p >= a.positions ? 0 : p + 1;
     };
     auto tiles_of = [&](int col) __attribute__((always_inline)) { return (length(col) + Tl::POSITIONS - 1) / Tl::POSITIONS; };
+    auto weight_of = [&](int col) __attribute__((always_inline)) {
+        const int n = tiles_of(col);
+        return n ? (n + BEGIN) * units : 0;
+    };
 
     // where this workgroup's tiles begin and end
     const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
     int mine = 0;
-    for (int c = c0; c < c1; c++) mine += tiles_of(a.col0 + c);
+    for (int c = c0; c < c1; c++) mine += weight_of(a.col0 + c);
     for (int i = tid; i < HEADS * ROW; i += 256) lds.q[i] = 0.f;           // (heads that there are not)
     int upto = mine;
 #pragma unroll
@@ -450,26 +460,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (i < tid >> 6) upto += sums[i];
         total += sums[i];
     }
-    total = uniform(total * units);
+    total = uniform(total);
     const int w = blockIdx.x, groups = min((total + GRAIN - 1) / GRAIN, (int)gridDim.x);
     if (w >= groups) return;
-    const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one tile more
-    int lo = w * share + min(w, more);
-    const int hi = lo + share + (w < more);
-    // the column of tile lo: the thread whose columns have it walks over them
-    if (lo >= (upto - mine) * units && lo < upto * units) {
-        int b = (upto - mine) * units, c = c0;
-        while (true) {
-            const int n = tiles_of(a.col0 + c) * units;
-            if (lo < b + n) break;
-            b += n;
-            c++;
+    const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one more
+    auto border = [&](int i) __attribute__((always_inline)) { return i * share + min(i, more); };
+    // the last border that is not behind x
+    auto border_at = [&](int x) __attribute__((always_inline)) {
+        const int longer = more * (share + 1);
+        return x < longer ? x / (share + 1) : more + (x - longer) / share;
+    };
+    // The column, unit and tile of a border: the thread whose columns have it walks over them.
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int x = border(w + i);
+        if (x >= upto - mine && x < upto) {
+            int b = upto - mine, c = a.col0 + c0;
+            while (x >= b + weight_of(c)) b += weight_of(c++);
+            const int n = tiles_of(c);
+            int unit = (x - b) / (n + BEGIN), tile = x - b - unit * (n + BEGIN) - BEGIN;
+            if (tile < SHORT || n - tile < SHORT) {
+                unit += tile >= n - tile;
+                tile = 0;
+            }
+            ends[i].col = c;
+            ends[i].unit = unit;
+            ends[i].tile = tile;
+            ends[i].start = b;
         }
-        sums[WAVES] = a.col0 + c;
-        sums[WAVES + 1] = b;
+        if (x == total && tid == 0) ends[i] = {a.col0 + a.cols, 0, 0, total};
     }
     __syncthreads();
-    int col = uniform(sums[WAVES]), start = uniform(sums[WAVES + 1]);       // start: the first tile of the column
+    int col = uniform(ends[0].col), unit = uniform(ends[0].unit), tile = uniform(ends[0].tile), start = uniform(ends[0].start);       // start: of the column
+    const int end_col = uniform(ends[1].col), end_unit = uniform(ends[1].unit), end_tile = uniform(ends[1].tile);
     const size_t page_stride = (size_t)a.c.kv_heads * page * hd, slot_size = (size_t)HEADS * (HDB * 32 + 2);
     const int row = hd + 2;             // of a slot: a head's maximum, its sum (-1: no position seen), its channels
     struct Split { int col, part, kvh, first, last; } split[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};      // the unit that began before, the one that ends behind
@@ -478,15 +501,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         return ((size_t)b * a.heads + head0) * channels * a.S + s;
     };
 
-    while (lo < hi) {
+    while (col < end_col || (col == end_col && (unit < end_unit || (unit == end_unit && tile < end_tile)))) {
         const int len = uniform(length(col)), n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
-        if (lo >= start + n * units) {
-            start += n * units;
+        if (n == 0 || unit == units) {
+            if (n) start += (n + BEGIN) * units;
             col++;
+            unit = tile = 0;
             continue;
         }
-        const int unit = (lo - start) / n, part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads;
-        const int unit_lo = start + unit * n, t0 = lo - unit_lo, t1 = min(hi, unit_lo + n) - unit_lo;
+        const int part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
         const int heads = min(a.group - part * HEADS, HEADS), head0 = kvh * a.group + part * HEADS, seq = uniform(a.seq ? a.seq[col] : col);
         const T *qp = q + out_of(col, head0, hd);
         // the queries, as fp32 values
@@ -531,15 +554,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 } else v0 = lds.sum_at(h, x - 2), v1 = lds.sum_at(h, x - 1);
                 slot_put(slot + i, v0, v1);
             }
-            // the workgroups that have tiles of the unit
-            auto owner = [&](int tile) __attribute__((always_inline)) {
-                const int longer = more * (share + 1);
-                return tile < longer ? tile / (share + 1) : more + (tile - longer) / share;
-            };
-            split[t0 == 0] = {col, part, kvh, owner(unit_lo), owner(unit_lo + n - 1)};
+            // the workgroups that have tiles of the unit: those before the first and behind the last border inside it
+            const int first_tile = start + unit * (n + BEGIN) + BEGIN;
+            split[t0 == 0] = {col, part, kvh, border_at(first_tile + SHORT - 1), border_at(first_tile + n - SHORT)};
         }
         __syncthreads();
-        lo = unit_lo + t1;
+        unit++;
+        tile = 0;
     }
 
     if (split[0].col < 0 && split[1].col < 0) return;
@@ -563,15 +584,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             const bool in = x < pairs * turns;
             const float *mine = a.slots + ((size_t)u.first * 2) * slot_size + h * row;
             float top = -INFINITY, sum = -1.f, v0 = 0.f, v1 = 0.f;
-            for (int j = in ? turn : count; j < count; j += JOIN * turns) {
+            for (int j = 0; j < count; j += JOIN * turns) {
                 v2f st[JOIN], y[JOIN];
-                // all on their way at once (the last one again behind the end, and not added)
+                // all on their way at once
 #pragma unroll
                 for (int e = 0; e < JOIN; e++) {
-                    const int at = min(j + e * turns, count - 1);
-                    const float *p = mine + (size_t)(2 * at + (at == 0)) * slot_size;
-                    st[e] = slot_get(p);
-                    y[e] = slot_get(p + 2 + ch);
+                    st[e] = v2f{-INFINITY, -1.f};
+                    y[e] = v2f{0.f, 0.f};
+                    const int at = j + e * turns + turn;
+                    if (in && at < count) {
+                        const float *p = mine + (size_t)(2 * at + (at == 0)) * slot_size;
+                        st[e] = slot_get(p);
+                        y[e] = slot_get(p + 2 + ch);
+                    }
                 }
                 float to = top;
 #pragma unroll
@@ -634,7 +659,7 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     auto go = [&](auto blocks) {
         constexpr int HDB = decltype(blocks)::value;
         // tiles are counted in 32 bits: columns that could have more go in several launches
-        const size_t column = ceil_div((size_t)c->max_pages * c->page, Tile<T, HDB>::POSITIONS) * c->kv_heads * parts;
+        const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, HDB>::POSITIONS) + BEGIN) * c->kv_heads * parts;
         if (column > 0x7fffffff) return mi355_fail("%s: %zu tiles of positions and heads of a column (at most 2^31 - 1)", who, column);
         const size_t at_once = 0x7fffffff / column;
         float *slots = (float *)mi355_ws((size_t)most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));
