@@ -652,22 +652,22 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     if (!(scale > 0.f) || !isfinite(scale * LOG2E)) return mi355_fail("%s: scale must be positive, and finite times log2(e)", who);
     const size_t units = (size_t)S * batch * heads;
     if (units > 0xffffff) return mi355_fail("%s: %zu heads of columns (at most 2^24 - 1)", who, units);
+    // tiles are counted in 32 bits: columns that could have more go in several launches
+    const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), cols = S * batch;
+    const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads * parts;
+    if (column > 0x7fffffff) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 1", who, (double)c->max_pages * c->page * c->kv_heads);
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
     if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
-    const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
+    const size_t at_once = 0x7fffffff / column, most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
     auto go = [&](auto blocks) {
         constexpr int HDB = decltype(blocks)::value;
-        // tiles are counted in 32 bits: columns that could have more go in several launches
-        const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, HDB>::POSITIONS) + BEGIN) * c->kv_heads * parts;
-        if (column > 0x7fffffff) return mi355_fail("%s: %zu tiles of positions and heads of a column (at most 2^31 - 1)", who, column);
-        const size_t at_once = 0x7fffffff / column;
-        float *slots = (float *)mi355_ws((size_t)most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));
+        float *slots = (float *)mi355_ws(most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));
         if (!slots) return -1;
-        for (size_t c0 = 0; c0 < (size_t)S * batch; c0 += at_once) {
-            const size_t cols = (size_t)S * batch - c0 < at_once ? (size_t)S * batch - c0 : at_once, grid = ceil_div(cols * column, GRAIN);
-            const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)cols, group, c->max_pages * c->page, scale * LOG2E, slots, arrived};
-            attn_paged_kernel<T, HDB><<<(unsigned)(grid < (size_t)most ? grid : most), 256, 0, g_ctx.stream>>>(o, lse, q, a);
+        for (size_t c0 = 0; c0 < (size_t)cols; c0 += at_once) {
+            const size_t n = cols - c0 < at_once ? cols - c0 : at_once, grid = ceil_div(n * column, GRAIN);
+            const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, scale * LOG2E, slots, arrived};
+            attn_paged_kernel<T, HDB><<<(unsigned)(grid < most ? grid : most), 256, 0, g_ctx.stream>>>(o, lse, q, a);
             LAUNCH_OK(who);
         }
         return 0;

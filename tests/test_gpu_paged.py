@@ -265,6 +265,70 @@ def test_cache_of_more_than_four_gigabytes(br, storage):
         a.free()
 
 
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_a_table_of_a_billion_positions(br, storage):
+    """Columns go in several launches where their tiles could be more than 32 bits count: 20 of them, 16 heads, 2^30 positions to a row of the table."""
+    kv, hd, page = 16, 8, 1 << 16
+    lengths = [300, 66000, 1, 131073]
+    small = Cache(storage, kv, hd, 16, lengths, seed=55)                # the oracle's own
+    ids, table = iter(range(100)), np.full((4, 1 << 14), -1, np.int32)
+    shape = (8, kv, page, hd)
+    k, v = np.zeros(shape, small.k.dtype), np.zeros(shape, small.k.dtype)
+    for i, n in enumerate(lengths):
+        for j in range(-(-n // page)):
+            table[i, j] = next(ids)
+        at = np.arange(n)
+        old = small.pages[i, at // 16]
+        for new, src in ((k, small.k), (v, small.v)):
+            new[table[i, at // page], :, at % page] = src[old, :, at % 16]
+    seq = np.array([0, 1, 2, 3] * 5, np.int32)
+    pos = np.array([n - 1 for n in lengths] * 5, np.int32)
+    pos[4:8], pos[-1] = [150, 65535, 0, 65536], 17
+    q = stored(storage, np.random.default_rng(56).standard_normal((1, kv * hd, 20)))
+    D = br.DevArray.from_numpy
+    kd, vd, td, qd, sd, pd, o, l = D(k), D(v), D(table), D(q), D(seq), D(pos), D(np.zeros_like(q)), br.DevArray((1, kv, 20))
+    c = br.KvCache(kd.ptr, vd.ptr, td.ptr, 8, page, 4, 1 << 14, kv, hd)
+    br.check(fn(br, "attn_paged", storage)(C.byref(c), o.ptr, l.ptr, qd.ptr, sd.ptr, pd.ptr, kv, 20, 1, 0.35))
+    check((o.numpy(), l.numpy()), expected(small, q, seq, pos, kv, 0.35))
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("S", [5, 333])
+def test_a_prompt_through_the_cache(br, storage, S):
+    """A prompt appended, and each of its positions attending over the cache, gives what mi355_qknorm_rope_fwd_dev and mi355_attn_fwd_dev give: the
+    same values but for the order of sums and their rounding (twice, where a rounded k is multiplied again)."""
+    heads, kv, hd, end = 8, 4, 64, "_dev" if storage == "f32" else "_bf16_dev"
+    rng = np.random.default_rng(57)
+    q, k, v = (stored(storage, rng.standard_normal((1, h * hd, S))) for h in (heads, kv, kv))
+    wq, wk = ((1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2))
+    D = br.DevArray.from_numpy
+    cos, sin = br.rope_tables_dev(S, hd, 10000.0)
+    qd, kd, vd, wqd, wkd = D(q), D(k), D(v), D(wq), D(wk)
+    qr, kr, o, l = D(np.zeros_like(q)), D(np.zeros_like(k)), D(np.zeros_like(q)), br.DevArray((1, heads, S))
+    br.check(getattr(br.lib, "mi355_qknorm_rope_fwd" + end)(qr.ptr, kr.ptr, qd.ptr, kd.ptr, wqd.ptr, wkd.ptr, heads, kv, hd, S, 1, cos, sin, 1e-5))
+    br.check(getattr(br.lib, "mi355_attn_fwd" + end)(o.ptr, l.ptr, qr.ptr, kr.ptr, vd.ptr, None, heads, kv, hd, S, 1, 0.125))
+    cache = Cache(storage, kv, hd, 16, [S], seed=58, values=False)
+    c, seq, pos = cache.to(br), D(np.zeros((1, S), np.int32)), D(np.arange(S, dtype=np.int32)[None])
+    q2, o2, l2 = D(np.zeros_like(q)), D(np.zeros_like(q)), br.DevArray((1, heads, S))
+    br.check(fn(br, "kv_append", storage)(C.byref(c), q2.ptr, qd.ptr, kd.ptr, vd.ptr, wqd.ptr, wkd.ptr, seq.ptr, pos.ptr, heads, S, 1, cos, sin, S, 1e-5))
+    br.check(fn(br, "attn_paged", storage)(C.byref(c), o2.ptr, l2.ptr, q2.ptr, seq.ptr, pos.ptr, heads, S, 1, 0.125))
+    cache.k, cache.v = cache.kd.numpy(), cache.vd.numpy()
+    step = STEP[storage]
+    a, b = f64(qr.numpy()), f64(q2.numpy())
+    off = 2.1 * step * np.abs(a) + E32 * (hd + 16) * 8          # (values are below 8)
+    assert np.all(np.abs(a - b) <= off)
+    want = expected(cache, q2.numpy(), np.zeros(S, int), np.arange(S), heads, 0.125)
+    check((o2.numpy(), l2.numpy()), want)
+    # against the other path: scores differ by what their rounded q and k do, 2 * 2.1 steps of the sum of magnitudes
+    K = np.abs(f64(kr.numpy()).reshape(kv, hd, S))
+    for h in range(heads):
+        A = np.abs(a[0, h * hd:(h + 1) * hd])
+        dz = 0.125 * (A.T @ K[h // 2]).max(1) * 4.3 * (step + E32 * hd)
+        V = np.abs(f64(v).reshape(kv, hd, S)[h // 2]).max()
+        assert np.all(np.abs(f64(o.numpy())[0, h * hd:(h + 1) * hd] - f64(o2.numpy())[0, h * hd:(h + 1) * hd]).max(0) <= V * (2.2 * dz + 3 * step + E32 * S))
+        assert np.all(np.abs(l.numpy()[0, h] - l2.numpy()[0, h]) <= dz + E32 * (S + 64))
+
+
 # ---- appending -------------------------------------------------------------------------------------------------------------------
 
 def append(br, cache, q, k, v, wq, wk, seq, pos, heads, cos, sin, eps, fill=5.0, inplace=False):

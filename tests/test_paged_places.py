@@ -124,6 +124,7 @@ def test_attention_refuses(fn):
         call(_9=scale)
     call(_4=None, _7=5)
     call(_1=P, _3=P, _6=1 << 14, _7=1 << 11)
+    call(_0=cache(page=1 << 16, max_pages=1 << 14, kv_heads=128), _6=128)       # more tiles than 32 bits count
 
 
 @pytest.mark.parametrize("fn", names("beam_step"))
