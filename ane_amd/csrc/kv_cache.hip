@@ -90,6 +90,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(
 // rotation needs no other lane; the angles of its pairs and columns stay in registers for all the heads.  Rotated queries go back as they came.
 // A key or value is a row of the cache: 64 x hd values are turned round in LDS, 16 bytes of a row to a lane on the way out.  Chunks of 4 (fp32) or 8
 // pairs of a row are exchanged by the group of columns, so that neither side meets a bank twice.
+// 16 padded prompts of 256 positions, 16 + 8 + 8 heads of 128, bfloat16: 19.7 us (25 MB); one of 8191, 12 + 12 + 12 heads of 64, fp32: 40 us (153 MB, 3.8
+// TB/s).  What bounds it is the work of a wave on a head, some 900 instructions or 2.3 us alone on its SIMD, and 4 us until it has its angles.
+// (With 16 columns to a wave, each by itself and without barriers: as long for these, four prompts of 4096 60 us for 39, since a wave's loads are then
+// of 32 bytes of each row.)
 template <typename P>
 __device__ __forceinline__ P of_kind(bool is_q, bool is_k, P q, P k, P v) { return is_q ? q : is_k ? k : v; }
 // A head of the queries, the keys or the values, one after the other.
@@ -297,9 +301,9 @@ int kv_append(const char *who, const mi355_kv_cache *c, T *q_out, const T *q, co
     };
     if (S >= 16 && units >= TILE_FROM) {
         const int slabs = heads + 2 * c->kv_heads, tiles = (int)ceil_div(S, 64);
-        // two workgroups to a compute unit; what is beyond that goes to more heads for each, up to eight
-        const size_t all = (size_t)tiles * batch * slabs, rounds = all / (2 * (size_t)g_ctx.num_cu);
-        const int each = rounds >= 8 ? 8 : rounds >= 4 ? 4 : rounds >= 2 ? 2 : 1;
+        // Two heads to a workgroup, whose angles are then fetched once, where that leaves each compute unit two workgroups.  us, one / two / four / eight
+        // heads: 256 columns 11 / 12 / 11 / 26, 16 padded prompts of 256 26 / 19.7 / 19.8 / 26, four of 4096 - / 39 / 43 / -.
+        const int each = (size_t)tiles * batch * slabs >= 4 * (size_t)g_ctx.num_cu ? 2 : 1;
         const dim3 grid((unsigned)(tiles * batch), (unsigned)ceil_div(slabs, each));
         constexpr int PPS = PAIRS_AT_ONCE<T>;
         if (c->hd / 2 <= 32) return go(kv_append_tile_kernel<T, 32 / PPS>, grid, tiles, each);
