@@ -29,6 +29,10 @@ constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
 // positions, 12 heads of 64 fp32 10.2 / 8.2 / 13.1, 8 heads of 128 bfloat16 8.8 / 14.4 / 25.5, of 2048 positions 11.8 / 13.6 / 17.8, 64 of up to 200
 // 36.6 / 67.7 / 101, of up to 4096 95 / 95 / 95.
 constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
+// Joining costs by the heads: 40 heads on two KV heads, 9 sequences of up to 7892 positions, 10 heads to a unit, GRAIN / twice that 33 / 26, 64 heads on one,
+// 16 of up to 4000, 33 / 27; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
+constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRAIN : GRAIN; }
+__device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
 constexpr int JOIN = 16;                    // slots whose values a thread has on their way at once
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int sums[WAVES], ticket[2];
     __shared__ struct { int col, unit, tile, start; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
-    const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts;      // units of a column
+    const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts, part_heads = (a.group + parts - 1) / parts;      // units of a column; heads of one
     auto length = [&](int col) __attribute__((always_inline)) {
         const int p = a.pos[col], seq = a.seq ? a.seq[col] : col;
         return seq < 0 || seq >= a.c.n_seqs || p < 0 || p >= a.positions ? 0 : p + 1;
@@ -461,7 +465,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         total += sums[i];
     }
     total = uniform(total);
-    const int w = blockIdx.x, groups = min((total + GRAIN - 1) / GRAIN, (int)gridDim.x);
+    const int w = blockIdx.x, groups = min(ceil_of(total, grain(part_heads)), (int)gridDim.x);
     if (w >= groups) return;
     const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one more
     auto border = [&](int i) __attribute__((always_inline)) { return i * share + min(i, more); };
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             continue;
         }
         const int part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
-        const int heads = min(a.group - part * HEADS, HEADS), head0 = kvh * a.group + part * HEADS, seq = uniform(a.seq ? a.seq[col] : col);
+        const int heads = min(a.group - part * part_heads, part_heads), head0 = kvh * a.group + part * part_heads, seq = uniform(a.seq ? a.seq[col] : col);
         const T *qp = q + out_of(col, head0, hd);
         // the queries, as fp32 values
         for (int i = tid; i < heads * hd; i += 256) {
@@ -575,7 +579,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (u.col < 0 || ticket[i] != u.last - u.first) continue;
         // The last to arrive: everybody's slots are in memory.
         if (tid == 0) __hip_atomic_store(a.arrived + u.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int heads = min(a.group - u.part * HEADS, HEADS), head0 = u.kvh * a.group + u.part * HEADS, count = u.last - u.first + 1;
+        const int heads = min(a.group - u.part * part_heads, part_heads), head0 = u.kvh * a.group + u.part * part_heads, count = u.last - u.first + 1;
         T *op = o + out_of(u.col, head0, hd);
         // two channels to a thread, and the slots in turns where there are threads to spare
         const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
