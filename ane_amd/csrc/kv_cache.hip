@@ -90,9 +90,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(
 // rotation needs no other lane; the angles of its pairs and columns stay in registers for all the heads.  Rotated queries go back as they came.
 // A key or value is a row of the cache: 64 x hd values are turned round in LDS, 16 bytes of a row to a lane on the way out.  Chunks of 4 (fp32) or 8
 // pairs of a row are exchanged by the group of columns, so that neither side meets a bank twice.
-// 16 padded prompts of 256 positions, 16 + 8 + 8 heads of 128, bfloat16: 19.7 us (25 MB); one of 8191, 12 + 12 + 12 heads of 64, fp32: 40 us (153 MB, 3.8
-// TB/s).  What bounds it is the work of a wave on a head, some 900 instructions or 2.3 us alone on its SIMD, and 4 us until it has its angles.
-// (With 16 columns to a wave, each by itself and without barriers: as long for these, four prompts of 4096 60 us for 39, since a wave's loads are then
+// 16 padded prompts of 256 positions, 16 + 8 + 8 heads of 128, bfloat16: 15 us (25 MB); one of 8191, 12 + 12 + 12 heads of 64, fp32: 40 us (153 MB, 3.8
+// TB/s).  What bounds it is the work of a wave on a head, 2.3 us alone on its SIMD, and 4 us until it has its angles.
+// (With 16 columns to a wave, each by itself and without barriers: as long for these, four prompts of 4096 60 us for 40, since a wave's loads are then
 // of 32 bytes of each row.)
 template <typename P>
 __device__ __forceinline__ P of_kind(bool is_q, bool is_k, P q, P k, P v) { return is_q ? q : is_k ? k : v; }
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
     T *q_out, const T *q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ k_cache, T *__restrict__ v_cache,
     const int *__restrict__ pages, const int *__restrict__ seq, const int *__restrict__ pos_of, const float *__restrict__ wq, const float *__restrict__ wk,
     const float *__restrict__ cos_t, const float *__restrict__ sin_t, int n_pages, int page, int n_seqs, int max_pages, int kv_heads, int hd, int heads, int S,
-    int table, float eps, int tiles, int slabs_each) {
+    int table, float eps, int tiles, int slabs_each, int all_tiles) {
     constexpr int VEC = 16 / (int)sizeof(T), LPR = 64 / VEC, PPS = 256 / LPR, ROW = 64;        // row pairs: of a step, of a column in LDS
     typedef unsigned pair_t __attribute__((ext_vector_type(sizeof(T) / 2)));                  // a column's values of a row pair
     __shared__ __attribute__((aligned(16))) pair_t turned[64 * ROW];
@@ -136,7 +136,10 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
     __shared__ long long place[64];         // row of head 0, -1: no token
     __shared__ int at[64];
     const int tid = threadIdx.x, half = hd / 2;
-    const int b = blockIdx.x / tiles, s0 = (blockIdx.x - b * tiles) * 64;
+    // Neighbours in a row of the batch follow one another, but begin elsewhere for each group of heads: where tiles are a multiple of 8, the tiles that
+    // padding leaves empty would else be those of the same XCDs for all of them.
+    const int group = blockIdx.x / all_tiles, turn = blockIdx.x - group * all_tiles + group % all_tiles, tile = turn >= all_tiles ? turn - all_tiles : turn;
+    const int b = tile / tiles, s0 = (tile - b * tiles) * 64;
     bool some = false;
     if (tid < 64) {
         long long p = -1;
@@ -182,7 +185,17 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
                 for (int j = 0; j < VEC; j++) { cs[kk][j] = pc[pos[j]]; sn[kk][j] = ps[pos[j]]; }
         }
     }
-    const int slabs = heads + 2 * kv_heads, first = blockIdx.y * slabs_each, last = min(first + slabs_each, slabs);
+    const int slabs = heads + 2 * kv_heads, first = group * slabs_each, last = min(first + slabs_each, slabs);
+    // (weights from memory inside the loop would have it wait for the next head's values too, which are asked for before them)
+    float gq[2 * CAP], gk[2 * CAP];
+#pragma unroll
+    for (int kk = 0; kk < CAP; kk++) {
+        const int rp = min(p0 + kk * PPS, half - 1);
+        gq[2 * kk] = wq ? wq[2 * rp] : 0.f;
+        gq[2 * kk + 1] = wq ? wq[2 * rp + 1] : 0.f;
+        gk[2 * kk] = wk ? wk[2 * rp] : 0.f;
+        gk[2 * kk + 1] = wk ? wk[2 * rp + 1] : 0.f;
+    }
     // the next head's values are under way while one is worked on
     typedef decltype(raw_cols((const T *)nullptr)) Raw;
     Raw r0[CAP], r1[CAP];
@@ -191,13 +204,13 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
         const Slab<T> now = slab_of(slab, heads, kv_heads, q, k, v);
         const bool is_q = now.is_q, is_k = now.is_k;
         const int head = now.head;
-        const float *w = of_kind(is_q, is_k, wq, wk, (const float *)nullptr);
+        const bool norm = is_q ? wq != nullptr : is_k && wk != nullptr;
         float x0[CAP][VEC], x1[CAP][VEC];
 #pragma unroll
         for (int kk = 0; kk < CAP; kk++) { widen(x0[kk], r0[kk]); widen(x1[kk], r1[kk]); }
         if (slab + 1 < last) load_slab<T, CAP, PPS>(r0, r1, slab_of(slab + 1, heads, kv_heads, q, k, v), b, hd, S, mine.col, p0, mine.ok);
         __syncthreads();            // (everybody is done with LDS)
-        if (w) {
+        if (norm) {
             float acc[1][VEC];
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
@@ -218,8 +231,7 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
             for (int j = 0; j < VEC; j++) acc[0][j] = sums[lc * VEC + j];
 #pragma unroll
             for (int kk = 0; kk < CAP; kk++) {
-                const int rp = min(p0 + kk * PPS, half - 1);
-                const float w0 = w[2 * rp], w1 = w[2 * rp + 1];
+                const float w0 = is_q ? gq[2 * kk] : gk[2 * kk], w1 = is_q ? gq[2 * kk + 1] : gk[2 * kk + 1];
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
                     x0[kk][j] = (x0[kk][j] * acc[0][j]) * w0;
@@ -301,13 +313,14 @@ int kv_append(const char *who, const mi355_kv_cache *c, T *q_out, const T *q, co
     };
     if (S >= 16 && units >= TILE_FROM) {
         const int slabs = heads + 2 * c->kv_heads, tiles = (int)ceil_div(S, 64);
-        // Two heads to a workgroup, whose angles are then fetched once, where that leaves each compute unit two workgroups.  us, one / two / four / eight
-        // heads: 256 columns 11 / 12 / 11 / 26, 16 padded prompts of 256 26 / 19.7 / 19.8 / 26, four of 4096 - / 39 / 43 / -.
-        const int each = (size_t)tiles * batch * slabs >= 4 * (size_t)g_ctx.num_cu ? 2 : 1;
-        const dim3 grid((unsigned)(tiles * batch), (unsigned)ceil_div(slabs, each));
+        // Heads to a workgroup, whose angles are then fetched once, by how many each compute unit gets.  us, one / two / four heads: 16 padded prompts of 256
+        // (8 to a compute unit) 15.7 / 15.3 / 18.8, 32 of 32 14.7 / 13.2 / 15.6, one of 8191 in fp32 (18) 44 / 40 / 38, four of 4096 (32) 52 / 42 / 36.
+        const size_t heads_each = (size_t)tiles * batch * slabs / g_ctx.num_cu;
+        const int each = heads_each >= 16 ? 4 : heads_each >= 4 ? 2 : 1;
+        const dim3 grid((unsigned)((size_t)tiles * batch * ceil_div(slabs, each)));
         constexpr int PPS = PAIRS_AT_ONCE<T>;
-        if (c->hd / 2 <= 32) return go(kv_append_tile_kernel<T, 32 / PPS>, grid, tiles, each);
-        return go(kv_append_tile_kernel<T, 64 / PPS>, grid, tiles, each);
+        if (c->hd / 2 <= 32) return go(kv_append_tile_kernel<T, 32 / PPS>, grid, tiles, each, tiles * batch);
+        return go(kv_append_tile_kernel<T, 64 / PPS>, grid, tiles, each, tiles * batch);
     }
     return go(kv_append_kernel<T>, dim3((unsigned)ceil_div(units, 4)), S * batch);
 }

@@ -222,8 +222,8 @@ typedef struct mi355_kv_cache {
  * q, q_out: [batch][heads*hd][S] (both NULL and heads = 0: keys and values only; q_out may be q); k, v: [batch][kv_heads*hd][S]; wq, wk: [hd]
  * fp32, NULL for no norm; cos, sin: [hd/2][table], as mi355_rope_tables_dev(.., table, hd, theta) gives them, both NULL for no rotation.
  * A column whose sequence is not in [0, n_seqs), whose position is negative, behind max_pages * page or behind the table of angles, or whose page
- * is none, is no token: nothing of it is written.  Of two columns with one place either may stay.  batch * S at most 2^22, heads at most 2^14,
- * kv_heads at most 4096. */
+ * is none, is no token: nothing of it is written.  Of two columns with one place either may stay.  Outputs must not overlap inputs otherwise.
+ * batch * S at most 2^22, heads at most 2^14, kv_heads at most 4096, batch * S * (heads + 2 kv_heads) below 2^26 - 3. */
 int mi355_kv_append_dev(const mi355_kv_cache *cache, float *q_out, const float *q, const float *k, const float *v, const float *wq,
                         const float *wk, const int32_t *seq, const int32_t *pos, int heads, int S, int batch, const float *cos_dev,
                         const float *sin_dev, int table, float eps);
@@ -235,8 +235,10 @@ int mi355_kv_append_bf16_dev(const mi355_kv_cache *cache, uint16_t *q_out, const
  * q, o: [batch][heads*hd][S], heads a multiple of kv_heads (query heads as in mi355_attn_fwd_dev); lse: [batch][heads][S] fp32, may be NULL.
  * 0 < scale <= 2.3e38.  Columns may share a sequence (several new tokens of one, each at its position) and sequences pages.  A column that is
  * no token (as above), or that has no page at all, is not written.  What lies in a page behind a column's position has no influence,
- * infinities and NaNs included.  Sums and the softmax are fp32.  Deterministic.  o must not overlap q.  The workspace holds the partial sums of
- * sequences that several workgroups share. */
+ * infinities and NaNs included.  Sums and the softmax are fp32, weights are multiplied again to 2^-15 of themselves.  Deterministic.  Outputs must not
+ * overlap inputs.  batch * S * heads below 2^24.  The workspace holds the partial sums of sequences that several workgroups share, which these hand over
+ * inside the launch: calls that overlap on one GPU (two streams, two threads) race.  Each workgroup looks at all columns' lengths: meant for
+ * some thousands of columns at most. */
 int mi355_attn_paged_dev(const mi355_kv_cache *cache, float *o, float *lse, const float *q, const int32_t *seq, const int32_t *pos, int heads,
                          int S, int batch, float scale);
 int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *lse, const uint16_t *q, const int32_t *seq, const int32_t *pos,
@@ -249,7 +251,7 @@ int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *l
  * (a column's number), done_out (may be NULL) = done[n] or v == eos (eos < 0: no token ends a beam).  A candidate that is NaN counts as -inf.
  * A greedy step is beams = 1; a group's first step has scores 0, -inf, -inf, ...
  * Exponentials and blocks' sums are fp32, sums over the vocabulary and candidates fp64, so that equal candidates stay equal.  Outputs must not
- * overlap inputs.  beams at most 64, batch * S at most 2^22, V * beams below 2^31.  Deterministic; the workspace holds partial sums. */
+ * overlap inputs.  beams at most 64, batch * S below 2^22, V * beams below 2^31.  Deterministic; the workspace holds partial sums. */
 int mi355_beam_step_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const float *logits, const float *score,
                         const int32_t *done, int V, int S, int batch, int beams, int eos, int pad);
 int mi355_beam_step_bf16_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const uint16_t *logits, const float *score,

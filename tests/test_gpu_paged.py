@@ -235,6 +235,43 @@ def test_scores_of_any_size(br, storage):
 
 
 @pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_scores_beyond_what_fp32_tells_apart(br, storage):
+    """Scores of 2^24 to 2^34: the largest one of a row takes all where it is ahead of the others by more than the rounding of its sum; equal ones share."""
+    cache = Cache(storage, 1, 64, 16, [500, 40, 33], seed=59, spread=4e4)
+    q = stored(storage, 4e4 * np.random.default_rng(60).standard_normal((1, 2 * 64, 3)))
+    page, slot = cache.row(1, 7)
+    page2, slot2 = cache.row(1, 30)
+    cache.k[page2, 0, slot2] = cache.k[page, 0, slot]
+    o, l = attend(br, cache, q, None, [499, 39, 32], 2, 0.125)
+    assert np.all(np.isfinite(f64(o))) and np.all(np.isfinite(l))
+    told = 0
+    for i, n in enumerate(cache.lengths):
+        K, V = cache.rows(cache.k, i, n)[0], cache.rows(cache.v, i, n)[0]
+        for h in range(2):
+            Q = f64(q)[0, h * 64:(h + 1) * 64, i]
+            z, off = 0.125 * (K @ Q), 0.125 * (np.abs(K) @ np.abs(Q)).max() * E32 * 80
+            ahead = np.flatnonzero(z >= z.max() - 2 * off - 40)
+            if len({tuple(K[a]) for a in ahead}) > 1:
+                continue
+            told += 1
+            want = V[ahead].mean(0)
+            assert np.all(np.abs(f64(o)[0, h * 64:(h + 1) * 64, i] - want) <= (1.01 * STEP[storage] + 2.0 ** -14) * np.abs(V[ahead]).max(0) + 1e-12)
+            assert abs(l[0, h, i] - z.max()) <= off + 2 * E32 * abs(z.max()) + 1
+    assert told >= 4
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_nothing_but_columns_of_no_token(br, storage):
+    cache = Cache(storage, 2, 64, 16, [20, 30], seed=61)
+    q = stored(storage, np.ones((1, 4 * 64, 300)))
+    for seq, pos in ((np.full(300, -1), np.zeros(300)), (np.zeros(300), np.full(300, -1))):
+        o, l = attend(br, cache, q, seq.astype(np.int32), pos.astype(np.int32), 4, 0.1)
+        assert np.all(f64(o) == 7.0) and np.all(l == 7.0)
+        got = append(br, cache, q, q[:, :128], q[:, 128:], None, None, seq.astype(np.int32), pos.astype(np.int32), 4, None, None, 0.0)
+        assert np.all(f64(got[0]) == 5.0) and np.array_equal(got[1], cache.k) and np.array_equal(got[2], cache.v)
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
 def test_cache_of_more_than_four_gigabytes(br, storage):
     """The last pages of a cache whose values pass 2^31 and whose bytes pass 2^32; all other pages are never touched."""
     kv, hd, page, n = 8, 128, 64, 150
@@ -516,3 +553,34 @@ def test_graphs_that_share_the_workspace(br, storage):
         attend(br, other, stored(storage, np.ones((1, 64, 1))), None, [2499], 1, 0.125)
     for s in steps:
         br.lib.mi355_graph_free(s[2])
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_another_stream(br, storage):
+    """Append, attention, a beam's step and the rows that follow, on a stream of the caller's."""
+    hip, stream = br.lib, C.c_void_p()          # (the runtime that the library itself has loaded)
+    cache = Cache(storage, 2, 64, 16, [700, 9], seed=95)
+    rng = np.random.default_rng(96)
+    q, k, v = (stored(storage, rng.standard_normal((1, h * 64, 2))) for h in (4, 2, 2))
+    pos = np.array([699, 8], np.int32)
+
+    def all_four():
+        new = append(br, cache, q, k, v, None, None, None, pos, 4, None, None, 0.0)
+        out = attend(br, cache, new[0], None, pos, 4, 0.125)
+        D = br.DevArray.from_numpy
+        x, s = D(q.reshape(1, 256, 2)), D(np.zeros(2, np.float32))
+        o = [br.DevArray(2)] + [br.DevArray(2, np.int32) for _ in range(3)]
+        br.check(fn(br, "beam_step", storage)(*[a.ptr for a in o], x.ptr, s.ptr, None, 256, 2, 1, 2, 3, 0))
+        c, par, po, sp, t = cache.to(br), D(np.array([1, 1], np.int32)), D(np.array([8, 8], np.int32)), D(np.array([0, 1], np.int32)), [D(np.zeros((2, cache.max_pages), np.int32)), D(np.zeros(2, np.int32)), D(np.zeros(2, np.int32))]
+        br.check(fn(br, "kv_reorder", storage)(C.byref(c), 1, t[0].ptr, t[1].ptr, t[2].ptr, par.ptr, po.ptr, sp.ptr, 1))
+        return list(new) + list(out) + [a.numpy() for a in o + t] + [cache.kd.numpy()]
+
+    want = all_four()
+    assert hip.hipStreamCreate(C.byref(stream)) == 0
+    br.check(br.lib.mi355_set_stream(stream))
+    try:
+        got = all_four()
+    finally:
+        br.check(br.lib.mi355_set_stream(None))         # (waits for the other one)
+        assert hip.hipStreamDestroy(stream) == 0
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
