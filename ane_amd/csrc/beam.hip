@@ -217,8 +217,8 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
                                                              const int *__restrict__ done, const float2 *__restrict__ part, int blocks, int rows, int V, int S,
                                                              int columns, int beams, int eos, int pad) {
     __shared__ SelectLds lds;
-    __shared__ float scores[MOST];
-    __shared__ int ended[MOST], chosen[MOST];
+    __shared__ float scores[MOST], tops_of[MOST];
+    __shared__ int ended[MOST], beam_of[MOST], row_of[MOST];       // the last two: of the best blocks, whose beams and where they begin
     const int tid = threadIdx.x, first = blockIdx.x * beams;
     if (tid < beams) {
         scores[tid] = score[first + tid];
@@ -261,8 +261,10 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         for (int i = tid & 63; i < side; i += 64) sum += lds.l[i * beams + n] * (double)exp_neg(lds.m[i * beams + n] - base);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        if ((tid & 63) == 0) lds.lse[n] = (double)top + log(sum);
+        if ((tid & 63) == 0) { lds.value[n] = sum; tops_of[n] = top; }
     }
+    __syncthreads();
+    if (tid < beams) lds.lse[tid] = (double)tops_of[tid] + log(lds.value[tid]);        // (one wave's work, for all beams)
     __syncthreads();
     auto candidate = [&](int n, float x, bool is_pad) __attribute__((always_inline)) {
         const double s = scores[n];
@@ -281,17 +283,25 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         for (int b = step + 8 * side; b < blocks; b += side)
             f(candidate(beam, part[(size_t)b * columns + first + beam].x, b == pad_block), beam * blocks + b);
     });
-    if (tid < best_blocks) chosen[tid] = lds.out_key[tid];
+    if (tid < best_blocks) {
+        const int n = lds.out_key[tid] / blocks;
+        beam_of[tid] = n;
+        row_of[tid] = (lds.out_key[tid] - n * blocks) * rows;
+    }
     __syncthreads();
     // the best of their elements
     {
         constexpr int N = 4;
-        const int n_elements = best_blocks * rows;
+        const int n_elements = best_blocks * rows;          // (at most 2^19: 64 blocks of 8192 rows)
+        const float per_row = 1.f / rows;
         double value[N];
         int key[N];
         auto element = [&](int i, double &v, int &k) __attribute__((always_inline)) {
-            const int at = min(i, n_elements - 1), j = at / rows, n = chosen[j] / blocks, row = (chosen[j] - n * blocks) * rows + (at - j * rows);
-            const int col = first + n, b = col / S;
+            const int at = min(i, n_elements - 1);
+            int j = (int)((float)at * per_row);             // at / rows, or one off
+            j -= j * rows > at;
+            j += (j + 1) * rows <= at;
+            const int n = beam_of[j], row = row_of[j] + (at - j * rows), col = first + n, b = S == 1 ? col : col / S;
             v = candidate(n, load_one(logits + ((size_t)b * V + min(row, V - 1)) * S + (col - b * S)), row == pad);
             k = i < n_elements && row < V ? n * V + row : -1;
         };
