@@ -292,9 +292,10 @@ struct Walk {
     }
 
     // Tiles first, first + WAVES, ... below last.  k, v: the KV head's rows of page 0.
+    // now: the pages of the first 64 pieces.
     template <bool ODD>
-    __device__ __forceinline__ void run(const typename Tl::Q (&q)[Tl::QS], const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages,
-                                        int hd, int first, int last, int len, float scale2) {
+    __device__ __forceinline__ void run(const typename Tl::Q (&q)[Tl::QS], Pieces now, const T *k, const T *v, size_t page_stride, const int *table, int page,
+                                        int n_pages, int hd, int first, int last, int len, float scale2) {
         m = -INFINITY;
         l = 0.f;
         seen = false;
@@ -311,8 +312,7 @@ struct Walk {
                        __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(v + o), 0, bytes, 0x00027000), i, offsets);
             }
         };
-        Pieces now, then;
-        now.look_up<Tl::PIECES>(table, page, len, first);
+        Pieces then;
         Tl a, b;
         Place pa = places(now, 0, n_pages), pb;
         load(a, pa);
@@ -367,7 +367,7 @@ template <int HDB> using shared_ptr = __attribute__((address_space(3))) Shared<H
 
 // Tiles t0 .. t1 - 1 of a sequence and KV head: the waves' shares, brought to the largest of their maxima, are in LDS at the end.
 template <typename T, int HDB, bool ODD>
-__device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages, int hd, int heads,
+__device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, Pieces now, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages, int hd, int heads,
                                           int t0, int t1, int len, float scale2) {
     typedef Tile<T, HDB> Tl;
     Shared<HDB> &lds = *(Shared<HDB> *)lds_;
@@ -377,7 +377,7 @@ __device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, const T *k, cons
 #pragma unroll
     for (int i = 0; i < Tl::QS; i++) q[i] = Tl::query(lds.q + head * ROW, i);
     Walk<T, HDB> walk;
-    walk.template run<ODD>(q, k, v, page_stride, table, page, n_pages, hd, t0 + wave, t1, len, scale2);
+    walk.template run<ODD>(q, now, k, v, page_stride, table, page, n_pages, hd, t0 + wave, t1, len, scale2);
     if (g == 0) {
         lds.m[wave * HEADS + head] = walk.m;
         lds.l[wave * HEADS + head] = walk.l;
@@ -405,7 +405,9 @@ __device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, const T *k, cons
 template <typename T, int HDB>
 __device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages,
                                                           int hd, int heads, int t0, int t1, int len, float scale2) {
-    share_out<T, HDB, true>(lds, k, v, page_stride, table, page, n_pages, hd, heads, t0, t1, len, scale2);
+    Pieces now;
+    now.look_up<Tile<T, HDB>::PIECES>(table, page, len, t0 + uniform((int)threadIdx.x >> 6));
+    share_out<T, HDB, true>(lds, now, k, v, page_stride, table, page, n_pages, hd, heads, t0, t1, len, scale2);
 }
 
 // Two values of a slot.  Slots pass from one workgroup to another inside a launch without fences, which would write back and invalidate whole L2s:
@@ -515,6 +517,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         const int part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
         const int heads = min(a.group - part * part_heads, part_heads), head0 = kvh * a.group + part * part_heads, seq = uniform(a.seq ? a.seq[col] : col);
+        const T *k = (const T *)a.c.k + (size_t)kvh * page * hd, *v = (const T *)a.c.v + (size_t)kvh * page * hd;
+        const int *table = a.c.pages + (size_t)seq * a.c.max_pages;
+        Pieces now;
+        now.look_up<Tl::PIECES>(table, page, len, t0 + uniform(tid >> 6));
         const T *qp = q + out_of(col, head0, hd);
         // the queries, as fp32 values
         for (int i = tid; i < heads * hd; i += 256) {
@@ -522,9 +528,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             lds.q[h * ROW + i - h * hd] = load_one(qp + (size_t)i * a.S);
         }
         __syncthreads();
-        const T *k = (const T *)a.c.k + (size_t)kvh * page * hd, *v = (const T *)a.c.v + (size_t)kvh * page * hd;
-        const int *table = a.c.pages + (size_t)seq * a.c.max_pages;
-        share_out<T, HDB, false>((shared_ptr<HDB>)&lds, k, v, page_stride, table, page, a.c.n_pages, hd, heads, t0, t1, len, a.scale2);
+        share_out<T, HDB, false>((shared_ptr<HDB>)&lds, now, k, v, page_stride, table, page, a.c.n_pages, hd, heads, t0, t1, len, a.scale2);
         if constexpr (sizeof(T) == 2) {
             // An infinity times the half of a weight that is zero is NaN: such sums are formed again.
             bool odd = false;
