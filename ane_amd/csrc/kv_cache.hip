@@ -136,10 +136,10 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
     __shared__ long long place[64];         // row of head 0, -1: no token
     __shared__ int at[64];
     const int tid = threadIdx.x, half = hd / 2;
-    // Neighbours in a row of the batch follow one another, but begin elsewhere for each group of heads: where tiles are a multiple of 8, the tiles that
-    // padding leaves empty would else be those of the same XCDs for all of them.
-    const int group = blockIdx.x / all_tiles, turn = blockIdx.x - group * all_tiles + group % all_tiles, tile = turn >= all_tiles ? turn - all_tiles : turn;
-    const int b = tile / tiles, s0 = (tile - b * tiles) * 64;
+    // The last tiles of padded prompts are empty, and should not be those of the same XCDs for every group of heads: in a batch each group begins at another
+    // tile (16 prompts of 256 positions 20 -> 15 us).  A single row does not: an XCD then has its own tiles' angles only (one of 8191 42.7 -> 40).
+    const int group = blockIdx.x / all_tiles, turn = blockIdx.x - group * all_tiles + (all_tiles > tiles ? group % all_tiles : 0);
+    const int tile = turn >= all_tiles ? turn - all_tiles : turn, b = tile / tiles, s0 = (tile - b * tiles) * 64;
     bool some = false;
     if (tid < 64) {
         long long p = -1;
@@ -314,9 +314,9 @@ int kv_append(const char *who, const mi355_kv_cache *c, T *q_out, const T *q, co
     if (S >= 16 && units >= TILE_FROM) {
         const int slabs = heads + 2 * c->kv_heads, tiles = (int)ceil_div(S, 64);
         // Heads to a workgroup, whose angles are then fetched once, by how many each compute unit gets.  us, one / two / four heads: 16 padded prompts of 256
-        // (8 to a compute unit) 15.7 / 15.3 / 18.8, 32 of 32 14.7 / 13.2 / 15.6, one of 8191 in fp32 (18) 44 / 40 / 38, four of 4096 (32) 52 / 42 / 36.
+        // (8 to a compute unit) 15.7 / 15.3 / 18.8, 32 of 32 14.7 / 13.2 / 15.6, one of 8191 in fp32 (18) 44 / 40 / 41, four of 4096 (32) 52 / 42 / 36.
         const size_t heads_each = (size_t)tiles * batch * slabs / g_ctx.num_cu;
-        const int each = heads_each >= 16 ? 4 : heads_each >= 4 ? 2 : 1;
+        const int each = heads_each >= 24 ? 4 : heads_each >= 4 ? 2 : 1;
         const dim3 grid((unsigned)((size_t)tiles * batch * ceil_div(slabs, each)));
         constexpr int PPS = PAIRS_AT_ONCE<T>;
         if (c->hd / 2 <= 32) return go(kv_append_tile_kernel<T, 32 / PPS>, grid, tiles, each, tiles * batch);
