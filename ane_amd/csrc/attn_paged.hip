@@ -663,11 +663,12 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     // tiles are counted in 32 bits: columns that could have more go in several launches
     const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), cols = S * batch;
     const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads * parts;
-    if (column > 0x7fffffff) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 1", who, (double)c->max_pages * c->page * c->kv_heads);
+    constexpr size_t COUNT = 0x7fffff00;           // (and a grain more is still counted)
+    if (column > COUNT) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 256", who, (double)c->max_pages * c->page * c->kv_heads);
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
     if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
-    const size_t at_once = 0x7fffffff / column, most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
+    const size_t at_once = COUNT / column, most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
     auto go = [&](auto blocks) {
         constexpr int HDB = decltype(blocks)::value;
         float *slots = (float *)mi355_ws(most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));

@@ -345,7 +345,8 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(MoveArgs t, int tensors
                                                          int advance) {
     const int n = blockIdx.x / kv_heads, head = blockIdx.x - n * kv_heads, at = pos[n], parent = parent_of(n, parents, pos, rows);
     const PagedMove m = paged_move(n, parent, at, page);
-    const bool moves = m.moves && m.tail < max_pages;
+    // (a page that is none is passed on as it is)
+    const bool moves = m.moves && m.tail < max_pages && paged_id_ok(pages[(size_t)parent * max_pages + m.tail], n_pages);
     if ((int)blockIdx.y == tensors) {
         if (head != 0) return;
         const int *from = pages + (size_t)parent * max_pages, *mine = pages + (size_t)n * max_pages;
@@ -359,7 +360,7 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(MoveArgs t, int tensors
     }
     if (!moves) return;
     const int from = pages[(size_t)parent * max_pages + m.tail], to = spare[n];
-    if (!paged_id_ok(from, n_pages) || !paged_id_ok(to, n_pages)) return;
+    if (!paged_id_ok(to, n_pages)) return;
     v4i *base = (v4i *)t.cache[blockIdx.y];
     const v4i *src = base + paged_row(from, head, 0, kv_heads, page, words);
     v4i *dst = base + paged_row(to, head, 0, kv_heads, page, words);

@@ -260,7 +260,7 @@ int mi355_beam_step_bf16_dev(float *score_out, int32_t *token, int32_t *parent, 
  * once.  pos[n_seqs]: each sequence's last position; a sequence and its parent are at the same one (one that is not, or is given a parent
  * outside [0, n_seqs), stays as it is).  pages_out[n_seqs][max_pages], the new table: pages before the one that holds pos are the parent's; pages
  * behind it stay n's own; the one that holds it is the parent's where that is n itself or where the page is full, else spare[n], into
- * which the parent's rows are copied.  spare_out[n] is then n's former page, else spare[n].  pos_out (may be NULL) = pos + advance (a negative
+ * which the parent's rows are copied (an entry that is no page is passed on as it is).  spare_out[n] is then n's former page, else spare[n].  pos_out (may be NULL) = pos + advance (a negative
  * pos, nothing held, stays).
  * With pages of its own for all its positions and one spare page for each sequence at the start, every page that is written to has one owner, and
  * no page is freed or allocated in between.  pages_out, pos_out and spare_out must not overlap the tables they come from; the

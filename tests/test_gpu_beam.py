@@ -206,9 +206,9 @@ def follow(caches, parent, pos, spare, advance=1):
             continue
         tail, filled = pos[i] // page, pos[i] % page + 1
         pages[i, :tail + 1] = c0.pages[p, :tail + 1]
-        if p != i and filled < page and tail < c0.max_pages:
+        if p != i and filled < page and tail < c0.max_pages and 0 <= c0.pages[p, tail] < c0.n_pages:
             pages[i, tail], spare_out[i] = spare[i], c0.pages[i, tail]
-            if 0 <= spare[i] < c0.n_pages and 0 <= c0.pages[p, tail] < c0.n_pages:
+            if 0 <= spare[i] < c0.n_pages:
                 for c, (k, v) in zip(caches, after):
                     k[spare[i], :, :filled] = c.k[c0.pages[p, tail], :, :filled]
                     v[spare[i], :, :filled] = c.v[c0.pages[p, tail], :, :filled]
@@ -249,9 +249,11 @@ def test_rows_without_a_place(br, storage):
     pos = np.array([35, 35, 35, 35, -1, -1, 20, 35, 700, 700])
     parent = np.array([-1, 10, 2 ** 31 - 1, 6, 0, 5, 3, 1, 9, 8])
     spare = np.array([int(cache.n_pages) - 1, -1, 3, 4, 5, 6, 7, -5, 8, 9])
+    cache.pages[7, 2], parent[1], pos[1] = -3, 7, 35               # a tail that is no page
     got, want = reorder(br, [cache], parent, pos, spare), follow([cache], parent, pos, spare)
     for a, b in zip(got[:3], want[:3]):
         assert np.array_equal(a, b)
+    assert got[0][1, 2] == -3 and got[2][1] == -1
     assert np.array_equal(got[3][0][0], want[3][0][0]) and np.array_equal(got[3][0][1], want[3][0][1])
 
 

@@ -120,7 +120,7 @@ SHAPES = [
     (2, 2, 128, 64, [3000], True), (16, 8, 128, 16, [2048, 5, 900], False), (8, 2, 120, 32, [1, 1, 1, 5000], False),
     (2, 1, 64, 16, [1 + 37 * (i % 11) for i in range(300)], False), (1, 1, 16, 16, list(range(1, 66)), True), (130, 130, 24, 16, [70, 20], False),
     (70, 1, 64, 16, [100, 400], True), (130, 2, 32, 16, [33, 500, 1500], False), (48, 1, 128, 16, [700, 64], True), (65, 1, 96, 48, [2000], True),
-    (40, 2, 128, 16, [3000, 17, 450], False),
+    (40, 2, 128, 16, [3000, 17, 450], False), (1, 1, 16, 16, [1 + i % 19 for i in range(1500)], False),
 ]
 
 
