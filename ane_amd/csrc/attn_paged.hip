@@ -12,6 +12,11 @@
 //                                  lane reads the values of just these positions.  In bfloat16 an operand is eight positions of a
 //                                  channel: the lane holds eight rows of 8 (4) channels and exchanges halves of words between them.
 // The running maximum is brought up to date only when a score passes it, which is rare after the first tiles, so lanes hardly ever talk.
+//
+// Measured: 64 sequences of up to 4096 positions, 16 heads on 8 KV heads of 128, bfloat16, 93 us, 4.55 TB/s; one of 131071, 107.6 us, 4.99 TB/s, where a
+// copy of 1 GiB reaches 5.12: bound by HBM.  Groups of 2 / 8 waves instead of 4: the long one 125 / 102, the 64 93.5 -> 92.4 with 8, small calls worse with both
+// (one of 256 positions 9.3, 64 of up to 200 46 instead of 38 with 8).  One sequence of 256, 12 heads of 64, fp32, 8.2 us: bound by one load after the other (positions, a
+// page, a tile, 3 us of joining).
 #include "kv_cache.h"
 #include "mma.h"
 
@@ -434,7 +439,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
     __shared__ int sums[WAVES], ticket[2];
-    __shared__ struct { int col, unit, tile, start; } ends[2];
+    __shared__ struct { int col, unit, tile, start, len; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
     const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts, part_heads = (a.group + parts - 1) / parts;      // units of a column; heads of one
     auto length = [&](int col) __attribute__((always_inline)) {
@@ -449,8 +454,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // where this workgroup's tiles begin and end
     const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
-    int mine = 0;
-    for (int c = c0; c < c1; c++) mine += weight_of(a.col0 + c);
+    // (Up to 256 columns a thread has one, whose length it keeps: looked up again it is waited for three times more, and calls of 8 to 65 us take 0.4 us longer.)
+    const int len0 = c0 < c1 ? length(a.col0 + c0) : 0, n0 = (len0 + Tl::POSITIONS - 1) / Tl::POSITIONS;
+    int mine = n0 ? (n0 + BEGIN) * units : 0;
+    for (int c = c0 + 1; c < c1; c++) mine += weight_of(a.col0 + c);
     for (int i = tid; i < HEADS * ROW; i += 256) lds.q[i] = 0.f;           // (heads that there are not)
     int upto = mine;
 #pragma unroll
@@ -481,9 +488,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int i = 0; i < 2; i++) {
         const int x = border(w + i);
         if (x >= upto - mine && x < upto) {
-            int b = upto - mine, c = a.col0 + c0;
-            while (x >= b + weight_of(c)) b += weight_of(c++);
-            const int n = tiles_of(c);
+            int b = upto - mine, c = a.col0 + c0, len = len0;
+            if (each > 1) {
+                while (x >= b + weight_of(c)) b += weight_of(c++);
+                len = length(c);
+            }
+            const int n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
             int unit = (x - b) / (n + BEGIN), tile = x - b - unit * (n + BEGIN) - BEGIN;
             if (tile < SHORT || n - tile < SHORT) {
                 unit += tile >= n - tile;
@@ -493,11 +503,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             ends[i].unit = unit;
             ends[i].tile = tile;
             ends[i].start = b;
+            ends[i].len = len;
         }
-        if (x == total && tid == 0) ends[i] = {a.col0 + a.cols, 0, 0, total};
+        if (x == total && tid == 0) ends[i] = {a.col0 + a.cols, 0, 0, total, 0};
     }
     __syncthreads();
     int col = uniform(ends[0].col), unit = uniform(ends[0].unit), tile = uniform(ends[0].tile), start = uniform(ends[0].start);       // start: of the column
+    int len = uniform(ends[0].len);
     const int end_col = uniform(ends[1].col), end_unit = uniform(ends[1].unit), end_tile = uniform(ends[1].tile);
     const size_t page_stride = (size_t)a.c.kv_heads * page * hd, slot_size = (size_t)HEADS * (HDB * 32 + 2);
     const int row = hd + 2;             // of a slot: a head's maximum, its sum (-1: no position seen), its channels
@@ -508,11 +520,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
 
     while (col < end_col || (col == end_col && (unit < end_unit || (unit == end_unit && tile < end_tile)))) {
-        const int len = uniform(length(col)), n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
+        const int n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
         if (n == 0 || unit == units) {
             if (n) start += (n + BEGIN) * units;
             col++;
             unit = tile = 0;
+            if (col < a.col0 + a.cols) len = uniform(length(col));
             continue;
         }
         const int part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
