@@ -386,8 +386,8 @@ template <typename T>
 int beam_step(const char *who, float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const T *logits, const float *score,
               const int32_t *done, int V, int S, int batch, int beams, int eos, int pad) {
     if (!score_out || !token || !parent || !logits || !score) return mi355_fail("%s: NULL pointer", who);
-    if (V <= 0 || S <= 0 || batch <= 0 || beams <= 0 || beams > MOST || (double)S * batch >= 1 << 22 || (double)V * beams >= 2147483648.0)
-        return mi355_fail("%s: bad shape V=%d S=%d batch=%d beams=%d (at most 64; batch * S below 2^22, V * beams below 2^31)", who, V, S, batch, beams);
+    if (V <= 0 || S <= 0 || batch <= 0 || beams <= 0 || beams > MOST || (double)S * batch >= 1 << 22 || (double)V * beams > 1 << 30)
+        return mi355_fail("%s: bad shape V=%d S=%d batch=%d beams=%d (at most 64; batch * S below 2^22, V * beams at most 2^30)", who, V, S, batch, beams);
     if (S * batch % beams) return mi355_fail("%s: %d columns are no multiple of beams=%d", who, S * batch, beams);
     if (pad < 0 || pad >= V || eos >= V) return mi355_fail("%s: pad=%d or eos=%d is no token of %d", who, pad, eos, V);
     if (score_out == score || (done_out && done_out == done)) return mi355_fail("%s: the new scores and marks must not be the old ones", who);

@@ -16,7 +16,8 @@ constexpr __attribute__((always_inline)) size_t paged_row(int id, int head, int 
     return (((size_t)id * kv_heads + head) * page + slot) * hd;
 }
 
-// What happens to row n of the table when it becomes the row of its parent, which is at the same position `pos`, on page `tail`: pages before the tail are the parent's, pages behind it stay n's own, and the tail itself is
+// What happens to row n of the table when it becomes the row of its parent, which is at the same position `pos`, on page `tail`: pages before the
+// tail are the parent's, pages behind it stay n's own, and the tail itself is
 //   the parent's page where parent == n or the page is full (nobody writes to a full page, so it is shared),
 //   else n's spare page, into which the parent's rows are copied, while n's former tail, which nobody else has, becomes its spare.
 struct PagedMove { bool moves; int tail, filled; };        // filled: rows of the tail that hold positions

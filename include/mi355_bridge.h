@@ -251,7 +251,7 @@ int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *l
  * (a column's number), done_out (may be NULL) = done[n] or v == eos (eos < 0: no token ends a beam).  A candidate that is NaN counts as -inf.
  * A greedy step is beams = 1; a group's first step has scores 0, -inf, -inf, ...
  * Exponentials and blocks' sums are fp32, sums over the vocabulary and candidates fp64, so that equal candidates stay equal.  Outputs must not
- * overlap inputs.  beams at most 64, batch * S below 2^22, V * beams below 2^31.  Deterministic; the workspace holds partial sums. */
+ * overlap inputs.  beams at most 64, batch * S below 2^22, V * beams at most 2^30.  Deterministic; the workspace holds partial sums. */
 int mi355_beam_step_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const float *logits, const float *score,
                         const int32_t *done, int V, int S, int batch, int beams, int eos, int pad);
 int mi355_beam_step_bf16_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const uint16_t *logits, const float *score,

@@ -140,6 +140,7 @@ def test_beam_refuses(fn):
         call(**{"_%d" % i: None})
     call(_7=0), call(_8=0), call(_9=0), call(_10=0), call(_10=65, _8=65), call(_10=3), call(_8=1 << 22), call(_8=1 << 22, _9=1, _10=1), call(_7=1 << 30)
     call(_12=-1), call(_12=100), call(_11=100)
+    call(_7=2**31 - 1, _10=1), call(_7=2**30 + 1, _10=1), call(_7=2**28 + 1)        # rows near 2^31: the places behind the last one would not fit 32 bits
     call(_0=q), call(_3=q)
 
 
