@@ -13,7 +13,8 @@
 namespace {
 
 constexpr int SELECT = 1024;        // threads of a group's workgroup
-constexpr int LIST = 1024;          // candidates that it ranks
+constexpr int LIST = 512;           // candidates that it ranks
+constexpr int NONE = 0x7fffffff;    // no candidate's key
 constexpr int MOST = 64;            // beams
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
@@ -126,20 +127,31 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(float2 *__restrict__ par
 }
 
 struct SelectLds {
-    double lse[MOST], value[LIST], out_value[MOST], wave_value[SELECT / 64];
-    int key[LIST], out_key[MOST], wave_key[SELECT / 64], count;
+    double lse[MOST], value[SELECT], out_value[MOST];
+    int key[SELECT], out_key[MOST], count;
     float tops[64], tau;
     float m[SELECT];
     double l[SELECT];
 };
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
 
+// All of these are loaded here.  (Else each load is moved to where its value is used, behind a condition, and waited for there.)
+__device__ __forceinline__ void loaded(float (&x)[4]) { asm("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3])); }
+
+// Of this lane's item and that of lane ^ d the lower lane keeps the first, or (back) the last.
+__device__ __forceinline__ void first_of_two(double &v, int &k, int d, bool back) {
+    const double x = __shfl_xor(v, d, 64);
+    const int y = __shfl_xor(k, d, 64);
+    if (before(v, k, x, y) != (((threadIdx.x & d) == 0) != back)) { v = x; k = y; }
+}
+
 // The `want` first of all threads' items, larger values first, equal ones by their keys: out_value, out_key in order.  own: the largest of the
-// thread's items as a float (rounding keeps the order); walk(f) calls f(value, key) for each of them.
+// thread's items as a float (rounding keeps the order); walk(f) calls f(value, key) for each of them, item(i, load(i), value, key) has the i-th of `items`, key -1:
+// none (nor is there one behind the last).
 // Of 64 parts of the threads the largest ones are compared; what is not below the `want`-th of these goes into a list, in which every item counts
-// those before it.  Few threads have any of those, and only they walk.
-template <typename F>
-__device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F walk) {
+// those before it.  Few threads have any of those, and only they walk.  (512 at most: 1000 of them take 60 us.)
+template <typename F, typename G, typename H>
+__device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F walk, int items, G load, H item) {
     constexpr int PART = SELECT / 64;
     const int tid = threadIdx.x;
     float best = own;
@@ -182,30 +194,76 @@ __device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F 
             const int r = (int)group_sum<16>(rank);
             if (r < want && (tid & 15) == 0) { lds.out_value[r] = v; lds.out_key[r] = k; }
         }
-    } else {            // too many equal ones (or nothing but -inf): one walk over all items for each
-        double last = INFINITY;
-        int last_key = -1;
-        for (int r = 0; r < want; r++) {
-            double v = -INFINITY;
-            int k = 0x7fffffff;
-            auto least = [&](double x, int y) __attribute__((always_inline)) {
-                if (before(last, last_key, x, y) && before(x, y, v, k)) { v = x; k = y; }
-            };
-            walk(least);
+    } else {
+        // Too many equal ones, or so many of one part's: a wave has the `want` first of its threads' items in order, one to a lane, and brings in those
+        // that are before the last of them, few of them one by one; then each counts those before it in all waves' lists.
+        const int lane = tid & 63;
+        // (The compiler sets a pair of scalar registers to the double -inf with an instruction that holds only 32 bits of it, and they are 0 then: here it
+        // does not see the constant.)
+        float lowest = -INFINITY;
+        asm("" : "+v"(lowest));
+        double held = lowest, last = lowest;
+        int held_key = NONE, last_key = NONE;
+        auto of_lane = [](double x, int from) __attribute__((always_inline)) {
+            const long long b = __double_as_longlong(x);
+            return __longlong_as_double((long long)(unsigned)__builtin_amdgcn_readlane((int)b, from) | (long long)__builtin_amdgcn_readlane((int)(b >> 32), from) << 32);
+        };
+        constexpr int AT_ONCE = 4;          // items on their way
+        for (int i0 = 0; i0 < items; i0 += AT_ONCE) {
+            float x[AT_ONCE];
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double v2 = __shfl_xor(v, d, 64);
-                const int k2 = __shfl_xor(k, d, 64);
-                if (before(v2, k2, v, k)) { v = v2; k = k2; }
+            for (int i = 0; i < AT_ONCE; i++) x[i] = load(i0 + i);
+            loaded(x);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++) {
+                double v;
+                int k;
+                item(i0 + i, x[i], v, k);
+                const bool in = k >= 0 && before(v, k, last, last_key);
+                unsigned long long more = __ballot(in);
+                if (__popcll(more) > 8) {
+                    v = in ? v : -INFINITY;
+                    k = in ? k : NONE;
+#pragma unroll 1
+                    for (int size = 2; size <= 64; size *= 2)
+#pragma unroll 1
+                        for (int d = size / 2; d; d /= 2) first_of_two(v, k, d, (lane & size) != 0);
+                    const double x = __shfl(v, 63 - lane, 64);
+                    const int y = __shfl(k, 63 - lane, 64);
+                    if (before(x, y, held, held_key)) { held = x; held_key = y; }
+#pragma unroll 1
+                    for (int d = 32; d; d /= 2) first_of_two(held, held_key, d, false);
+                    more = 0;
+                    last = of_lane(held, want - 1);
+                    last_key = __builtin_amdgcn_readlane(held_key, want - 1);
+                }
+                while (more) {
+                    const int from = __builtin_ctzll(more);
+                    const double x = of_lane(v, from), above = __shfl_up(held, 1, 64);
+                    const int y = __builtin_amdgcn_readlane(k, from), key_above = __shfl_up(held_key, 1, 64);
+                    const int rank = __popcll(__ballot(before(held, held_key, x, y)));
+                    held = lane > rank ? above : lane == rank ? x : held;
+                    held_key = lane > rank ? key_above : lane == rank ? y : held_key;
+                    last = of_lane(held, want - 1);
+                    last_key = __builtin_amdgcn_readlane(held_key, want - 1);
+                    more &= more - 1;
+                    more &= __ballot(before(v, k, last, last_key));
+                }
             }
-            if ((tid & 63) == 0) { lds.wave_value[tid >> 6] = v; lds.wave_key[tid >> 6] = k; }
-            __syncthreads();
-            last = lds.wave_value[0];
-            last_key = lds.wave_key[0];
-            for (int w = 1; w < SELECT / 64; w++)
-                if (before(lds.wave_value[w], lds.wave_key[w], last, last_key)) { last = lds.wave_value[w]; last_key = lds.wave_key[w]; }
-            if (tid == 0) { lds.out_value[r] = last; lds.out_key[r] = last_key; }
-            __syncthreads();
+        }
+        lds.value[tid] = held;
+        lds.key[tid] = held_key;
+        __syncthreads();
+        if (lane < want && held_key != NONE) {
+            int rank = 0;
+            for (int list = 0; list < SELECT; list += 64) {
+                int n = 0;          // of the list, before this one
+#pragma unroll
+                for (int step = 64; step; step >>= 1)
+                    if (n + step <= 64 && before(lds.value[list + n + step - 1], lds.key[list + n + step - 1], held, held_key)) n += step;
+                rank += n;
+            }
+            if (rank < want) { lds.out_value[rank] = held; lds.out_key[rank] = held_key; }
         }
     }
     __syncthreads();
@@ -282,6 +340,12 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
             if (i * side < blocks && step + i * side < blocks) f(candidate(beam, tops[i], step + i * side == pad_block), beam * blocks + step + i * side);
         for (int b = step + 8 * side; b < blocks; b += side)
             f(candidate(beam, part[(size_t)b * columns + first + beam].x, b == pad_block), beam * blocks + b);
+    }, (blocks + side - 1) / side,
+    [&](int i) __attribute__((always_inline)) { return part[(size_t)min(step + i * side, blocks - 1) * columns + first + beam].x; },
+    [&](int i, float x, double &v, int &k) __attribute__((always_inline)) {
+        const int b = step + i * side;
+        v = candidate(beam, x, b == pad_block);
+        k = step < side && b < blocks ? beam * blocks + b : -1;
     });
     if (tid < best_blocks) {
         const int n = lds.out_key[tid] / blocks;
@@ -296,37 +360,69 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         const float per_row = 1.f / rows;
         double value[N];
         int key[N];
-        auto element = [&](int i, double &v, int &k) __attribute__((always_inline)) {
+        auto place = [&](int i, int &n, int &row) __attribute__((always_inline)) {
             const int at = min(i, n_elements - 1);
             int j = (int)((float)at * per_row);             // at / rows, or one off
             j -= j * rows > at;
             j += (j + 1) * rows <= at;
-            const int n = beam_of[j], row = row_of[j] + (at - j * rows), col = first + n, b = S == 1 ? col : col / S;
-            v = candidate(n, load_one(logits + ((size_t)b * V + min(row, V - 1)) * S + (col - b * S)), row == pad);
-            k = i < n_elements && row < V ? n * V + row : -1;
+            n = beam_of[j];
+            row = row_of[j] + (at - j * rows);
         };
+        auto load_from = [&](int n, int row) __attribute__((always_inline)) {
+            const int col = first + n, b = S == 1 ? col : col / S;
+            return load_one(logits + ((size_t)b * V + min(row, V - 1)) * S + (col - b * S));
+        };
+        auto element_of = [&](int i, int n, int row, float x, double &v, int &k) __attribute__((always_inline)) {
+            v = candidate(n, x, row == pad);
+            k = tid + i * SELECT < n_elements && row < V ? n * V + row : -1;
+        };
+        auto load = [&](int i) __attribute__((always_inline)) {
+            int n, row;
+            place(tid + i * SELECT, n, row);
+            return load_from(n, row);
+        };
+        auto element = [&](int i, float x, double &v, int &k) __attribute__((always_inline)) {
+            int n, row;
+            place(tid + i * SELECT, n, row);
+            element_of(i, n, row, x, v, k);
+        };
+        const int items = (n_elements + SELECT - 1) / SELECT;
+        float x[N];
+        int n[N], row[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i < items) place(tid + i * SELECT, n[i], row[i]);
+            x[i] = i < items ? load_from(n[i], row[i]) : 0.f;
+        }
         own = -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             key[i] = -1;
-            if (i * SELECT < n_elements) element(tid + i * SELECT, value[i], key[i]);
+            if (i < items) element_of(i, n[i], row[i], x[i], value[i], key[i]);
             if (key[i] >= 0) own = fmaxf(own, (float)value[i]);
         }
         auto rest = [&](auto f) __attribute__((always_inline)) {
-            for (int i = tid + N * SELECT; i < n_elements; i += SELECT) {
-                double v;
-                int k;
-                element(i, v, k);
-                if (k >= 0) f(v, k);
+            for (int i0 = N; i0 < items; i0 += N) {
+                float x[N];
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] = load(i0 + i);
+                loaded(x);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    double v;
+                    int k;
+                    element(i0 + i, x[i], v, k);
+                    if (k >= 0) f(v, k);
+                }
             }
         };
         rest([&](double v, int) __attribute__((always_inline)) { own = fmaxf(own, (float)v); });
         first_of(lds, beams, own, [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (i * SELECT < n_elements && key[i] >= 0) f(value[i], key[i]);
+                if (i < items && key[i] >= 0) f(value[i], key[i]);
             rest(f);
-        });
+        }, items, load, element);
     }
     if (tid < beams) {
         const int n = lds.out_key[tid] / V, v = lds.out_key[tid] - n * V;
@@ -339,7 +435,7 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
 
 // Rows to a block, and the first launch.
 template <typename T>
-int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T *logits, int V, int S, int batch) {
+int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T *logits, int V, int S, int batch, int beams) {
     constexpr int WIDE = 16 / (int)sizeof(T);
     const size_t columns = (size_t)S * batch;
     if (S == 1) {
@@ -367,6 +463,9 @@ int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T 
         // rows to a thread: eight at a time, more where there are workgroups enough
         const size_t steps = ceil_div(V, down), each = steps * strips * batch / (4 * (size_t)g_ctx.num_cu);
         *rows = down * (each >= 32 && down <= 8 ? 64 : each >= 32 ? 32 : each >= 16 ? 16 : each >= 8 ? 8 : each >= 4 ? 4 : each >= 2 ? 2 : 1);
+        // The second launch looks at all blocks of a group, and then at as many blocks' rows as it has beams.  us, 4 / 1 blocks to a row at most / any number:
+        // 32000 tokens, 64 beams 48 / 69 / 75, 50257, 32 beams 25 / 27 / 43, 16 beams 16.8 / 16.8 / 20.7, 151936, 64 beams 77 / 129 / 75, four beams 12.2 / - / 13.0.
+        while (beams >= 4 && ceil_div(V, *rows) > 4 * (size_t)*rows) *rows *= 2;
         *blocks = (int)ceil_div(V, *rows);
         *part = (float2 *)mi355_ws(*blocks * columns * sizeof(float2));
         if (!*part) return -1;
@@ -395,7 +494,7 @@ int beam_step(const char *who, float *score_out, int32_t *token, int32_t *parent
     const size_t n = (size_t)S * batch;
     float2 *part;
     int blocks, rows;
-    if (beam_blocks(who, &part, &blocks, &rows, logits, V, S, batch)) return -1;
+    if (beam_blocks(who, &part, &blocks, &rows, logits, V, S, batch, beams)) return -1;
     beam_select_kernel<T><<<(unsigned)(n / beams), SELECT, 0, g_ctx.stream>>>(score_out, token, parent, done_out, logits, score, done, part, blocks, rows, V, S,
                                                                              (int)n, beams, eos, pad);
     LAUNCH_OK(who);

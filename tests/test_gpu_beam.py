@@ -127,6 +127,33 @@ def test_first_step_of_equal_beams(br, storage, shape):
 
 
 @pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["first", "first of equal", "equal", "three allowed", "one allowed", "rising", "falling"])
+@pytest.mark.parametrize("shape", [(1, 70, 64, 64), (1, 1000, 64, 64), (64, 1000, 1, 64), (2, 9000, 48, 48), (1, 9000, 63, 63), (16, 2000, 1, 16)])
+def test_many_candidates_at_the_border(br, storage, kind, shape):
+    """Many beams of which one counts, masked vocabularies, equal logits: more candidates at the last new beam's than a short list holds."""
+    B, V, S, beams = shape
+    N = B * S
+    rng = np.random.default_rng(140 + V + beams)
+    logits, score = apart(rng, storage, B, V, S)
+    if not kind.endswith("allowed"):
+        score = np.repeat(score[:N // beams], beams)
+    if kind.startswith("first"):
+        score = np.where(np.arange(N) % beams == 0, 0.0, -np.inf)
+    if kind.endswith("equal"):
+        logits = stored(storage, np.full((B, V, S), -0.5))
+    elif kind.endswith("allowed"):
+        keep = rng.choice(V, 3 if kind[0] == "t" else 1, replace=False)
+        masked = stored(storage, np.full((B, V, S), -np.inf))
+        masked[:, keep] = logits[:, keep]
+        logits = masked
+    elif kind in ("rising", "falling"):
+        rows = np.sort(np.round(rng.uniform(-15.9, 15.9, V) * 8) / 8)
+        logits = stored(storage, np.tile((rows if kind == "rising" else rows[::-1])[None, :, None], (B, 1, S)))
+    assert gap(logits, score, None, beams, 0) > 4 * OFF
+    check(step(br, storage, logits, score, None, beams), definition(logits, score, None, beams, -1, 0))
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
 @pytest.mark.parametrize("shape", [(1, 3000, 8), (8, 3000, 1), (2, 30, 4)])
 def test_logits_that_are_no_numbers(br, storage, shape):
     """Masked vocabularies, by -inf and by the type's lowest value, columns of nothing else, infinities and NaNs."""
