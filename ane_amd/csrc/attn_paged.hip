@@ -38,7 +38,9 @@ constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
 // 16 of up to 4000, 33 / 27; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
 constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRAIN : GRAIN; }
 __device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
-constexpr int JOIN = 16;                    // slots whose values a thread has on their way at once
+// Slots whose values a thread has on their way at once.  us, 4 / 8 / 12 / 16 / 24: one sequence of 131071 positions 109.5 / 106.9 / 105.5 / 107.7 / 105.6, 6 of up to
+// 46491, 40 heads on two 74 / 66.3 / 64.7 / 65.4 / 63.6, 16 of up to 4000, 64 heads on one 27.3 / 25.3 / 25.4 / 27.2 / 27, one of 256 8.4 / 8.2 / 8.35 / 8.25 / 8.5.
+constexpr int JOIN = 12;
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
