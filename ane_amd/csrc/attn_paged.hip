@@ -52,6 +52,7 @@ struct PagedArgs {
     mi355_kv_cache c;
     const int *seq, *pos;
     int heads, S, col0, cols, group, positions;     // columns col0 .. col0 + cols - 1; group: query heads of a KV head; positions of a row of the table
+    int part0, parts;               // which parts of the groups this launch has
     float scale2;
     float *slots;                   // partial results: two for each workgroup
     unsigned *arrived;
@@ -428,12 +429,15 @@ __device__ __forceinline__ v2f slot_get(const float *p) {
     return v2f{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
 }
 
-// A unit is the tiles of a column and KV head (of 16 of its query heads).  Those of all columns, one after the other, are dealt out evenly, a unit
+// A unit is the tiles of a column and KV head.  Those of all columns, one after the other, are dealt out evenly, a unit
 // counted as its tiles and BEGIN more for what it takes to begin one: workgroup w of W has T / W of that line, whatever sequences they belong to.
 // (Lengths are in device memory: the host cannot deal them out, and a batch's longest sequence would otherwise decide when it ends.)  A border that
 // would cut off fewer than SHORT tiles is moved to the unit's end or beginning.  A unit with borders inside is split: each of its workgroups
 // leaves its maxima, sums and unnormalised o in a slot, and the last one to arrive joins them in their order.  A workgroup has two such units at
 // most, the one that it begins with and the one that it ends with, and looks after both when it is done with its tiles.
+// More than 16 query heads to a KV head go in parts, each with workgroups, slots and counts of its own.  Those with the same tiles lie 8 apart in the grid:
+// they begin together on one XCD, and what the first one reads the others find in its L2.  (40 heads on two KV heads, 6 sequences of up to 46491 positions
+// 64.5 -> 54.2 us, 16 of up to 8000 37.3 -> 32.4, against parts that followed one another on one line.)
 template <typename T, int HDB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
                                                                                                   PagedArgs a) {
@@ -443,7 +447,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int sums[WAVES], ticket[2];
     __shared__ struct { int col, unit, tile, start, len; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
-    const int parts = (a.group + HEADS - 1) / HEADS, units = a.c.kv_heads * parts, part_heads = (a.group + parts - 1) / parts;      // units of a column; heads of one
+    const int all_parts = (a.group + HEADS - 1) / HEADS, part_heads = (a.group + all_parts - 1) / all_parts, units = a.c.kv_heads;  // units: of a column
+    const int turn = blockIdx.x / (8 * a.parts), rest = blockIdx.x - turn * 8 * a.parts, part = a.part0 + (rest >> 3), w = turn * 8 + (rest & 7);
+    const int heads = min(a.group - part * part_heads, part_heads), most = gridDim.x / a.parts;
     auto length = [&](int col) __attribute__((always_inline)) {
         const int p = a.pos[col], seq = a.seq ? a.seq[col] : col;
         return seq < 0 || seq >= a.c.n_seqs || p < 0 || p >= a.positions ? 0 : p + 1;
@@ -476,7 +482,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         total += sums[i];
     }
     total = uniform(total);
-    const int w = blockIdx.x, groups = min(ceil_of(total, grain(part_heads)), (int)gridDim.x);
+    const int groups = min(ceil_of(total, grain(part_heads)), most);
     if (w >= groups) return;
     const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one more
     auto border = [&](int i) __attribute__((always_inline)) { return i * share + min(i, more); };
@@ -515,7 +521,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int end_col = uniform(ends[1].col), end_unit = uniform(ends[1].unit), end_tile = uniform(ends[1].tile);
     const size_t page_stride = (size_t)a.c.kv_heads * page * hd, slot_size = (size_t)HEADS * (HDB * 32 + 2);
     const int row = hd + 2;             // of a slot: a head's maximum, its sum (-1: no position seen), its channels
-    struct Split { int col, part, kvh, first, last; } split[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};      // the unit that began before, the one that ends behind
+    float *const slots = a.slots + (size_t)(part - a.part0) * most * 2 * slot_size;
+    unsigned *const arrived = a.arrived + (part - a.part0) * most;
+    struct Split { int col, kvh, first, last; } split[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};      // the unit that began before, the one that ends behind
     auto out_of = [&](int col, int head0, size_t channels) __attribute__((always_inline)) {
         const int b = col / a.S, s = col - b * a.S;
         return ((size_t)b * a.heads + head0) * channels * a.S + s;
@@ -530,8 +538,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             if (col < a.col0 + a.cols) len = uniform(length(col));
             continue;
         }
-        const int part = unit / a.c.kv_heads, kvh = unit - part * a.c.kv_heads, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
-        const int heads = min(a.group - part * part_heads, part_heads), head0 = kvh * a.group + part * part_heads, seq = uniform(a.seq ? a.seq[col] : col);
+        const int kvh = unit, t0 = tile, t1 = col == end_col && unit == end_unit ? end_tile : n;
+        const int head0 = kvh * a.group + part * part_heads, seq = uniform(a.seq ? a.seq[col] : col);
         const T *k = (const T *)a.c.k + (size_t)kvh * page * hd, *v = (const T *)a.c.v + (size_t)kvh * page * hd;
         const int *table = a.c.pages + (size_t)seq * a.c.max_pages;
         Pieces now;
@@ -567,7 +575,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     if (lse && i == h * hd) lse[out_of(col, head0 + h, 1)] = (top + __builtin_amdgcn_logf(sum)) * LN2;
                 }
         } else {
-            float *slot = a.slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;
+            float *slot = slots + ((size_t)w * 2 + (t0 == 0)) * slot_size;
             for (int i = 2 * tid; i < heads * row; i += 512) {
                 const int h = i / row, x = i - h * row;
                 float v0, v1;
@@ -579,7 +587,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             // the workgroups that have tiles of the unit: those before the first and behind the last border inside it
             const int first_tile = start + unit * (n + BEGIN) + BEGIN;
-            split[t0 == 0] = {col, part, kvh, border_at(first_tile + SHORT - 1), border_at(first_tile + n - SHORT)};
+            split[t0 == 0] = {col, kvh, border_at(first_tile + SHORT - 1), border_at(first_tile + n - SHORT)};
         }
         __syncthreads();
         unit++;
@@ -590,22 +598,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // this wave's parts of the slots are in memory,
     __syncthreads();                                        // everybody's are
     if (tid < 2 && (tid ? split[1].col : split[0].col) >= 0)
-        ticket[tid] = (int)__hip_atomic_fetch_add(a.arrived + (tid ? split[1].first : split[0].first), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        ticket[tid] = (int)__hip_atomic_fetch_add(arrived + (tid ? split[1].first : split[0].first), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
 #pragma unroll 1
     for (int i = 0; i < 2; i++) {
         const Split u = i ? split[1] : split[0];
         if (u.col < 0 || ticket[i] != u.last - u.first) continue;
         // The last to arrive: everybody's slots are in memory.
-        if (tid == 0) __hip_atomic_store(a.arrived + u.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int heads = min(a.group - u.part * part_heads, part_heads), head0 = u.kvh * a.group + u.part * part_heads, count = u.last - u.first + 1;
+        if (tid == 0) __hip_atomic_store(arrived + u.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int head0 = u.kvh * a.group + part * part_heads, count = u.last - u.first + 1;
         T *op = o + out_of(u.col, head0, hd);
         // two channels to a thread, and the slots in turns where there are threads to spare
         const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
         for (int x0 = 0; x0 < pairs * turns; x0 += 256) {
             const int x = x0 + tid, turn = x / pairs, pair = x - turn * pairs, h = 2 * pair / hd, ch = 2 * pair - h * hd;
             const bool in = x < pairs * turns;
-            const float *mine = a.slots + ((size_t)u.first * 2) * slot_size + h * row;
+            const float *mine = slots + ((size_t)u.first * 2) * slot_size + h * row;
             float top = -INFINITY, sum = -1.f, v0 = 0.f, v1 = 0.f;
             for (int j = 0; j < count; j += JOIN * turns) {
                 v2f st[JOIN], y[JOIN];
@@ -677,7 +685,7 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     if (units > 0xffffff) return mi355_fail("%s: %zu heads of columns (at most 2^24 - 1)", who, units);
     // tiles are counted in 32 bits: columns that could have more go in several launches
     const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), cols = S * batch;
-    const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads * parts;
+    const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads;
     constexpr size_t COUNT = 0x7fffff00;           // (and a grain more is still counted)
     if (column > COUNT) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 256", who, (double)c->max_pages * c->page * c->kv_heads);
     if (!mi355_ready(who)) return -1;
@@ -688,12 +696,16 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
         constexpr int HDB = decltype(blocks)::value;
         float *slots = (float *)mi355_ws(most * 2 * HEADS * (HDB * 32 + 2) * sizeof(float));
         if (!slots) return -1;
-        for (size_t c0 = 0; c0 < (size_t)cols; c0 += at_once) {
-            const size_t n = cols - c0 < at_once ? cols - c0 : at_once, grid = ceil_div(n * column, GRAIN);
-            const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, scale * LOG2E, slots, arrived};
-            attn_paged_kernel<T, HDB><<<(unsigned)(grid < most ? grid : most), 256, 0, g_ctx.stream>>>(o, lse, q, a);
-            LAUNCH_OK(who);
-        }
+        for (size_t c0 = 0; c0 < (size_t)cols; c0 += at_once)
+            for (int p0 = 0; p0 < parts; p0 += most / 8) {
+                const size_t n = cols - c0 < at_once ? cols - c0 : at_once, useful = ceil_div(n * column, GRAIN);
+                const int now = parts - p0 < (int)most / 8 ? parts - p0 : (int)most / 8;
+                // workgroups of a part: of several, a multiple of 8
+                const size_t room = now == 1 ? most : most / (8 * now) * 8, each = useful < room ? (now == 1 ? useful : ceil_div(useful, 8) * 8) : room;
+                const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, p0, now, scale * LOG2E, slots, arrived};
+                attn_paged_kernel<T, HDB><<<(unsigned)(each * now), 256, 0, g_ctx.stream>>>(o, lse, q, a);
+                LAUNCH_OK(who);
+            }
         return 0;
     };
     if (c->hd <= 32) return go(std::integral_constant<int, 1>());
