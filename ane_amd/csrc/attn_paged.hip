@@ -34,12 +34,12 @@ constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
 // positions, 12 heads of 64 fp32 10.2 / 8.2 / 13.1, 8 heads of 128 bfloat16 8.8 / 14.4 / 25.5, of 2048 positions 11.8 / 13.6 / 17.8, 64 of up to 200
 // 36.6 / 67.7 / 101, of up to 4096 95 / 95 / 95.
 constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
-// Joining costs by the heads: 40 heads on two KV heads, 9 sequences of up to 7892 positions, 10 heads to a unit, GRAIN / twice that 33 / 26, 64 heads on one,
-// 16 of up to 4000, 33 / 27; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
+// Joining costs by the heads: 40 heads on two KV heads, 9 sequences of up to 7892 positions, 10 heads to a unit, GRAIN / twice that 27.8 / 22.7, 64 heads on
+// one, 16 of up to 4000, 27.3 / 23, but 3 of up to 449 in fp32 15.2 / 17.2; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
 constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRAIN : GRAIN; }
 __device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
-// Slots whose values a thread has on their way at once.  us, 4 / 8 / 12 / 16 / 24: one sequence of 131071 positions 109.5 / 106.9 / 105.5 / 107.7 / 105.6, 6 of up to
-// 46491, 40 heads on two 74 / 66.3 / 64.7 / 65.4 / 63.6, 16 of up to 4000, 64 heads on one 27.3 / 25.3 / 25.4 / 27.2 / 27, one of 256 8.4 / 8.2 / 8.35 / 8.25 / 8.5.
+// Slots whose values a thread has on their way at once.  us, 6 / 8 / 12: one sequence of 131071 positions 105.7 / 106 / 105.5, 6 of up to 46491, 40 heads on two
+// 53.4 / 52.3 / 51.4, 16 of up to 8000 31.5 / 30.5 / 30.3, 64 heads on one, 16 of up to 4000, 23.6 / 23.2 / 23.1, one of 256 8.25 / 8.2 / 8.25.
 constexpr int JOIN = 12;
 
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
@@ -437,7 +437,7 @@ __device__ __forceinline__ v2f slot_get(const float *p) {
 // most, the one that it begins with and the one that it ends with, and looks after both when it is done with its tiles.
 // More than 16 query heads to a KV head go in parts, each with workgroups, slots and counts of its own.  Those with the same tiles lie 8 apart in the grid:
 // they begin together on one XCD, and what the first one reads the others find in its L2.  (40 heads on two KV heads, 6 sequences of up to 46491 positions
-// 64.5 -> 54.2 us, 16 of up to 8000 37.3 -> 32.4, against parts that followed one another on one line.)
+// 64.5 -> 54.2 us, 16 of up to 8000 37.3 -> 32.4, where parts followed one another on one line.)
 template <typename T, int HDB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
                                                                                                   PagedArgs a) {
@@ -608,25 +608,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (tid == 0) __hip_atomic_store(arrived + u.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const int head0 = u.kvh * a.group + part * part_heads, count = u.last - u.first + 1;
         T *op = o + out_of(u.col, head0, hd);
-        // two channels to a thread, and the slots in turns where there are threads to spare
-        const int pairs = heads * hd / 2, turns = max(1, 256 / pairs);
-        for (int x0 = 0; x0 < pairs * turns; x0 += 256) {
-            const int x = x0 + tid, turn = x / pairs, pair = x - turn * pairs, h = 2 * pair / hd, ch = 2 * pair - h * hd;
-            const bool in = x < pairs * turns;
+        // four channels to a thread (two: 5 to 7 % longer with ten heads and more), and the slots in turns where there are threads to spare
+        const int quads = heads * hd / 4, turns = min(max(1, 256 / quads), (count + 1) / 2);
+        for (int x0 = 0; x0 < quads * turns; x0 += 256) {
+            const int x = x0 + tid, turn = x / quads, quad = x - turn * quads, h = 4 * quad / hd, ch = 4 * quad - h * hd;
+            const bool in = x < quads * turns;
             const float *mine = slots + ((size_t)u.first * 2) * slot_size + h * row;
-            float top = -INFINITY, sum = -1.f, v0 = 0.f, v1 = 0.f;
+            float top = -INFINITY, sum = -1.f;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
             for (int j = 0; j < count; j += JOIN * turns) {
-                v2f st[JOIN], y[JOIN];
+                v2f st[JOIN], y[JOIN][2];
                 // all on their way at once
 #pragma unroll
                 for (int e = 0; e < JOIN; e++) {
                     st[e] = v2f{-INFINITY, -1.f};
-                    y[e] = v2f{0.f, 0.f};
+                    y[e][0] = y[e][1] = v2f{0.f, 0.f};
                     const int at = j + e * turns + turn;
                     if (in && at < count) {
                         const float *p = mine + (size_t)(2 * at + (at == 0)) * slot_size;
                         st[e] = slot_get(p);
-                        y[e] = slot_get(p + 2 + ch);
+                        y[e][0] = slot_get(p + 2 + ch);
+                        y[e][1] = slot_get(p + 4 + ch);
                     }
                 }
                 float to = top;
@@ -634,36 +636,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int e = 0; e < JOIN; e++) to = fmaxf(to, st[e][0]);
                 const float base = to == -INFINITY ? 0.f : to, old = __builtin_amdgcn_exp2f(top - base);
                 sum = sum < 0.f ? sum : sum * old;
-                v0 *= old;
-                v1 *= old;
+                v *= old;
                 top = to;
 #pragma unroll
                 for (int e = 0; e < JOIN; e++) {
                     if (j + e * turns >= count) break;
                     const float f = __builtin_amdgcn_exp2f(st[e][0] - base);
                     if (!(st[e][1] < 0.f)) sum = (sum < 0.f ? 0.f : sum) + st[e][1] * f;
-                    v0 += y[e][0] * f;
-                    v1 += y[e][1] * f;
+                    v += v4f{y[e][0][0], y[e][0][1], y[e][1][0], y[e][1][1]} * f;
                 }
             }
             if (turns > 1) {                // (one round then)
-                float *p = lds.o + 5 * tid;
-                p[0] = top; p[1] = sum; p[2] = v0; p[3] = v1;
+                float *p = lds.o + 8 * tid;
+                p[0] = top; p[1] = sum;
+                *reinterpret_cast<v4f *>(p + 4) = v;
                 __syncthreads();
             }
             if (turn > 0 || !in) continue;
             for (int t = 1; t < turns; t++) {
-                const float *p = lds.o + 5 * (tid + t * pairs);
+                const float *p = lds.o + 8 * (tid + t * quads);
                 const float to = fmaxf(top, p[0]), base = to == -INFINITY ? 0.f : to, f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(p[0] - base);
                 if (!(p[1] < 0.f)) sum = (sum < 0.f ? 0.f : sum * f0) + p[1] * f1;
                 else if (!(sum < 0.f)) sum *= f0;
-                v0 = v0 * f0 + p[2] * f1;
-                v1 = v1 * f0 + p[3] * f1;
+                v = v * f0 + *reinterpret_cast<const v4f *>(p + 4) * f1;
                 top = to;
             }
             if (sum < 0.f) continue;
-            store_one(op + (size_t)(2 * pair) * a.S, v0 / sum);
-            store_one(op + (size_t)(2 * pair + 1) * a.S, v1 / sum);
+#pragma unroll
+            for (int e = 0; e < 4; e++) store_one(op + (size_t)(4 * quad + e) * a.S, v[e] / sum);
             if (lse && ch == 0) lse[out_of(u.col, head0 + h, 1)] = (top + __builtin_amdgcn_logf(sum)) * LN2;
         }
         __syncthreads();
