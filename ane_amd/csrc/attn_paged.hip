@@ -37,6 +37,11 @@ constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
 // Joining costs by the heads: 40 heads on two KV heads, 9 sequences of up to 7892 positions, 10 heads to a unit, GRAIN / twice that 27.8 / 22.7, 64 heads on
 // one, 16 of up to 4000, 27.3 / 23, but 3 of up to 449 in fp32 15.2 / 17.2; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
 constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRAIN : GRAIN; }
+// Few units of many tiles should not be cut into as many pieces as there are workgroups: a piece takes as long as it has tiles, the join as long as there are
+// pieces and heads, and both together least at pieces of about sqrt(tiles heads) / 3.  us, without / with that, one sequence of 65536 positions: 6 heads of 96 on one,
+// fp32, 94 / 35, 40 of 128 on two, bfloat16, 67 / 39, 64 on one 65 / 42; of 131071, 8 heads on one 62 / 39.  Not where it leaves more than one workgroup to a
+// compute unit but fewer than two: those take as long as two each (6 of up to 46491, 40 heads on two, 62 instead of 51).
+constexpr float PIECE = 1.f / 3;
 __device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
 // Slots whose values a thread has on their way at once.  us, 6 / 8 / 12: one sequence of 131071 positions 105.7 / 106 / 105.5, 6 of up to 46491, 40 heads on two
 // 53.4 / 52.3 / 51.4, 16 of up to 8000 31.5 / 30.5 / 30.3, 64 heads on one, 16 of up to 4000, 23.6 / 23.2 / 23.1, one of 256 8.25 / 8.2 / 8.25.
@@ -52,7 +57,7 @@ struct PagedArgs {
     mi355_kv_cache c;
     const int *seq, *pos;
     int heads, S, col0, cols, group, positions;     // columns col0 .. col0 + cols - 1; group: query heads of a KV head; positions of a row of the table
-    int part0, parts;               // which parts of the groups this launch has
+    int part0, parts, units;        // which parts of the groups this launch has; compute units, 0 where units are not long enough for PIECE to matter
     float scale2;
     float *slots;                   // partial results: two for each workgroup
     unsigned *arrived;
@@ -445,6 +450,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
     __shared__ int sums[WAVES], ticket[2];
+    __shared__ float tops[WAVES];
     __shared__ struct { int col, unit, tile, start, len; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
     const int all_parts = (a.group + HEADS - 1) / HEADS, part_heads = (a.group + all_parts - 1) / all_parts, units = a.c.kv_heads;  // units: of a column
@@ -465,7 +471,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // (Up to 256 columns a thread has one, whose length it keeps: looked up again it is waited for three times more, and calls of 8 to 65 us take 0.4 us longer.)
     const int len0 = c0 < c1 ? length(a.col0 + c0) : 0, n0 = (len0 + Tl::POSITIONS - 1) / Tl::POSITIONS;
     int mine = n0 ? (n0 + BEGIN) * units : 0;
-    for (int c = c0 + 1; c < c1; c++) mine += weight_of(a.col0 + c);
+    float longest = n0;
+    for (int c = c0 + 1; c < c1; c++) {
+        const int n = tiles_of(a.col0 + c);
+        mine += n ? (n + BEGIN) * units : 0;
+        longest = fmaxf(longest, n);
+    }
+    if (a.units) longest = wave_max(longest);
     for (int i = tid; i < HEADS * ROW; i += 256) lds.q[i] = 0.f;           // (heads that there are not)
     int upto = mine;
 #pragma unroll
@@ -473,16 +485,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int x = __shfl_up(upto, d, 64);
         if ((tid & 63) >= d) upto += x;
     }
-    if ((tid & 63) == 63) sums[tid >> 6] = upto;
+    if ((tid & 63) == 63) {
+        sums[tid >> 6] = upto;
+        tops[tid >> 6] = longest;
+    }
     __syncthreads();
     int total = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; i++) {
         if (i < tid >> 6) upto += sums[i];
         total += sums[i];
+        longest = fmaxf(longest, tops[i]);
     }
     total = uniform(total);
-    const int groups = min(ceil_of(total, grain(part_heads)), most);
+    int groups = min(ceil_of(total, grain(part_heads)), most);
+    if (a.units) {
+        // (a multiple of the units: a workgroup that ends one and begins another is often the last of both, and joins one after the other)
+        const int few = ceil_of(ceil_of(total, max(1, uniform((int)(sqrtf(longest * part_heads) * PIECE)))), units) * units;
+        if (few <= a.units / a.parts) groups = min(groups, few);
+    }
     if (w >= groups) return;
     const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one more
     auto border = [&](int i) __attribute__((always_inline)) { return i * share + min(i, more); };
@@ -691,6 +712,8 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
     if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
+    const int heads_of = (int)ceil_div(group, parts);
+    const bool lengthy = sqrt((double)c->max_pages * c->page / Tile<T, 1>::POSITIONS * heads_of) * PIECE > grain(heads_of);
     const size_t at_once = COUNT / column, most = 2 * g_ctx.num_cu < MAX_GROUPS ? 2 * g_ctx.num_cu : MAX_GROUPS;
     auto go = [&](auto blocks) {
         constexpr int HDB = decltype(blocks)::value;
@@ -702,7 +725,7 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
                 const int now = parts - p0 < (int)most / 8 ? parts - p0 : (int)most / 8;
                 // workgroups of a part: of several, a multiple of 8
                 const size_t room = now == 1 ? most : most / (8 * now) * 8, each = useful < room ? (now == 1 ? useful : ceil_div(useful, 8) * 8) : room;
-                const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, p0, now, scale * LOG2E, slots, arrived};
+                const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, p0, now, lengthy ? g_ctx.num_cu : 0, scale * LOG2E, slots, arrived};
                 attn_paged_kernel<T, HDB><<<(unsigned)(each * now), 256, 0, g_ctx.stream>>>(o, lse, q, a);
                 LAUNCH_OK(who);
             }

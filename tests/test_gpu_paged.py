@@ -141,6 +141,23 @@ def test_attention(br, i, storage):
 
 
 @pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(8, 1, 64, 16, [40000]), (6, 1, 96, 48, [20001, 3, 700]), (40, 2, 64, 64, [30000]), (48, 1, 32, 16, [40000, 39000, 1]),
+                                   (1, 1, 32, 256, [200000]), (15, 5, 40, 32, [33333, 40]), (20, 1, 128, 16, [25000, 0, 11])])
+def test_units_of_many_tiles(br, storage, shape):
+    """Few sequences, long ones: cut into fewer pieces than there are workgroups; a length of 0 is a column of no token."""
+    heads, kv, hd, page, lengths = shape
+    cache = Cache(storage, kv, hd, page, [max(n, 1) for n in lengths], seed=sum(lengths))
+    N, scale = len(lengths), float(np.float32(1.0 / np.sqrt(hd)))
+    q = stored(storage, np.random.default_rng(N + heads).standard_normal((1, heads * hd, N)))
+    pos = np.array(lengths) - 1
+    want = expected(cache, q, None, pos, heads, scale)
+    got = attend(br, cache, q, None, pos, heads, scale)
+    check(got, want)
+    again = attend(br, cache, q, None, pos, heads, scale)
+    assert np.array_equal(again[0], got[0]) and np.array_equal(again[1], got[1])
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
 def test_columns_of_no_token_and_several_of_one_sequence(br, storage):
     """[3][C][4]: padded columns, positions in the middle of a sequence, one sequence many times, sequences and positions that are none."""
     cache = Cache(storage, 2, 64, 16, [70, 33, 200], seed=40, room=1)
