@@ -13,7 +13,7 @@
 //                                  channel: the lane holds eight rows of 8 (4) channels and exchanges halves of words between them.
 // The running maximum is brought up to date only when a score passes it, which is rare after the first tiles, so lanes hardly ever talk.
 //
-// Measured: 64 sequences of up to 4096 positions, 16 heads on 8 KV heads of 128, bfloat16, 93 us, 4.55 TB/s; one of 131071, 107.6 us, 4.99 TB/s, where a
+// Measured: 64 sequences of up to 4096 positions, 16 heads on 8 KV heads of 128, bfloat16, 91 us, 4.6 TB/s; one of 131071, 106 us, 5.05 TB/s, where a
 // copy of 1 GiB reaches 5.12: bound by HBM.  Workgroups of 2 waves instead of 4: the long one 125; of 8: 102, but one of 256 positions 9.3 and 64 of up to
 // 200 46 instead of 38.  One sequence of 256, 12 heads of 64, fp32, 8.2 us: bound by one load after the other (positions, a
 // page, a tile, 3 us of joining).
