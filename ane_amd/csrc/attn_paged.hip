@@ -17,6 +17,7 @@
 // copy of 1 GiB reaches 5.12: bound by HBM.  Workgroups of 2 waves instead of 4: the long one 125; of 8: 102, but one of 256 positions 9.3 and 64 of up to
 // 200 46 instead of 38.  One sequence of 256, 12 heads of 64, fp32, 8.2 us: bound by one load after the other (positions, a
 // page, a tile, 3 us of joining).
+#include "deal.h"
 #include "kv_cache.h"
 #include "mma.h"
 
@@ -42,7 +43,6 @@ constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRA
 // fp32, 94 / 35, 40 of 128 on two, bfloat16, 67 / 39, 64 on one 65 / 42; of 131071, 8 heads on one 62 / 39.  Not where it leaves more than one workgroup to a
 // compute unit but fewer than two: those take as long as two each (6 of up to 46491, 40 heads on two, 62 instead of 51).
 constexpr float PIECE = 1.f / 3;
-__device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
 // Slots whose values a thread has on their way at once.  us, 6 / 8 / 12: one sequence of 131071 positions 105.7 / 106 / 105.5, 6 of up to 46491, 40 heads on two
 // 53.4 / 52.3 / 51.4, 16 of up to 8000 31.5 / 30.5 / 30.3, 64 heads on one, 16 of up to 4000, 23.6 / 23.2 / 23.1, one of 256 8.25 / 8.2 / 8.25.
 constexpr int JOIN = 12;
@@ -498,24 +498,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         longest = fmaxf(longest, tops[i]);
     }
     total = uniform(total);
-    int groups = min(ceil_of(total, grain(part_heads)), most);
-    if (a.units) {
-        // (a multiple of the units: a workgroup that ends one and begins another is often the last of both, and joins one after the other)
-        const int few = ceil_of(ceil_of(total, max(1, uniform((int)(sqrtf(longest * part_heads) * PIECE)))), units) * units;
-        if (few <= a.units / a.parts) groups = min(groups, few);
-    }
+    int groups = deal_groups(total, most, grain(part_heads));
+    // (a multiple of the units: a workgroup that ends one and begins another is often the last of both, and joins one after the other)
+    if (a.units) groups = deal_fewer(groups, total, max(1, uniform((int)(sqrtf(longest * part_heads) * PIECE))), units, a.units / a.parts);
     if (w >= groups) return;
-    const int share = total / groups, more = total - share * groups;          // the first `more` workgroups have one more
-    auto border = [&](int i) __attribute__((always_inline)) { return i * share + min(i, more); };
-    // the last border that is not behind x
-    auto border_at = [&](int x) __attribute__((always_inline)) {
-        const int longer = more * (share + 1);
-        return x < longer ? x / (share + 1) : more + (x - longer) / share;
-    };
+    const Deal deal = deal_out(total, groups);
     // The column, unit and tile of a border: the thread whose columns have it walks over them.
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const int x = border(w + i);
+        const int x = deal.border(w + i);
         if (x >= upto - mine && x < upto) {
             int b = upto - mine, c = a.col0 + c0, len = len0;
             if (each > 1) {
@@ -523,14 +514,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 len = length(c);
             }
             const int n = (len + Tl::POSITIONS - 1) / Tl::POSITIONS;
-            int unit = (x - b) / (n + BEGIN), tile = x - b - unit * (n + BEGIN) - BEGIN;
-            if (tile < SHORT || n - tile < SHORT) {
-                unit += tile >= n - tile;
-                tile = 0;
-            }
+            const DealPlace at = deal_place(x - b, n, BEGIN, SHORT);
             ends[i].col = c;
-            ends[i].unit = unit;
-            ends[i].tile = tile;
+            ends[i].unit = at.unit;
+            ends[i].tile = at.tile;
             ends[i].start = b;
             ends[i].len = len;
         }
@@ -606,9 +593,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 } else v0 = lds.sum_at(h, x - 2), v1 = lds.sum_at(h, x - 1);
                 slot_put(slot + i, v0, v1);
             }
-            // the workgroups that have tiles of the unit: those before the first and behind the last border inside it
-            const int first_tile = start + unit * (n + BEGIN) + BEGIN;
-            split[t0 == 0] = {col, kvh, border_at(first_tile + SHORT - 1), border_at(first_tile + n - SHORT)};
+            const DealShared shared = deal_shared(deal, start + unit * (n + BEGIN), n, BEGIN, SHORT);
+            split[t0 == 0] = {col, kvh, shared.first, shared.last};
         }
         __syncthreads();
         unit++;
@@ -707,7 +693,7 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     // tiles are counted in 32 bits: columns that could have more go in several launches
     const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), cols = S * batch;
     const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads;
-    constexpr size_t COUNT = 0x7fffff00;           // (and a grain more is still counted)
+    constexpr size_t COUNT = 0x7fffff00;
     if (column > COUNT) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 256", who, (double)c->max_pages * c->page * c->kv_heads);
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
