@@ -137,6 +137,14 @@ struct SelectLds {
 };
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
 
+// -inf.  (The compiler has set a pair of scalar registers to this double with an instruction that holds only 32 bits of it, and they were 0 then; here it
+// does not see the constant.)
+__device__ __forceinline__ double lowest() {
+    float x = -INFINITY;
+    asm("" : "+v"(x));
+    return x;
+}
+
 // All of these are loaded here.  (Else each load is moved to where its value is used, behind a condition, and waited for there.)
 __device__ __forceinline__ void loaded(float (&x)[4]) { asm("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3])); }
 
@@ -200,11 +208,8 @@ __device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F 
         // Too many equal ones, or so many of one part's: a wave has the `want` first of its threads' items in order, one to a lane, and brings in those
         // that are before the last of them, few of them one by one; then each counts those before it in all waves' lists.
         const int lane = tid & 63;
-        // (The compiler sets a pair of scalar registers to the double -inf with an instruction that holds only 32 bits of it, and they are 0 then: here it
-        // does not see the constant.)
-        float lowest = -INFINITY;
-        asm("" : "+v"(lowest));
-        double held = lowest, last = lowest;
+        const double low = lowest();
+        double held = low, last = low;
         int held_key = NONE, last_key = NONE;
         auto of_lane = [](double x, int from) __attribute__((always_inline)) {
             const long long b = __double_as_longlong(x);
@@ -224,7 +229,7 @@ __device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F 
                 const bool in = k >= 0 && before(v, k, last, last_key);
                 unsigned long long more = __ballot(in);
                 if (__popcll(more) > 8) {
-                    v = in ? v : -INFINITY;
+                    v = in ? v : low;
                     k = in ? k : NONE;
 #pragma unroll 1
                     for (int size = 2; size <= 64; size *= 2)
@@ -326,10 +331,11 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
     __syncthreads();
     if (tid < beams) lds.lse[tid] = (double)tops_of[tid] + log(lds.value[tid]);        // (one wave's work, for all beams)
     __syncthreads();
+    const double none = lowest();
     auto candidate = [&](int n, float x, bool is_pad) __attribute__((always_inline)) {
         const double s = scores[n];
-        double c = ended[n] ? (is_pad ? s : -INFINITY) : s + ((double)x - lds.lse[n]);
-        return c == c ? c : -INFINITY;
+        double c = ended[n] ? (is_pad ? s : none) : s + ((double)x - lds.lse[n]);
+        return c == c ? c : none;
     };
     // the best blocks; of a beam's candidates the one with the largest logit is the largest, but an ended beam has only one
     const int pad_block = pad / rows, best_blocks = (int)min((long long)beams, (long long)beams * blocks);
