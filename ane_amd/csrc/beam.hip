@@ -337,11 +337,12 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         double c = ended[n] ? (is_pad ? s : none) : s + ((double)x - lds.lse[n]);
         return c == c ? c : none;
     };
-    // the best blocks; of a beam's candidates the one with the largest logit is the largest, but an ended beam has only one
-    const int pad_block = pad / rows, best_blocks = (int)min((long long)beams, (long long)beams * blocks);
+    // the best blocks, as many as beams (each beam has one at least); of a beam's candidates the one with the largest logit is the largest, but an ended
+    // beam has only one
+    const int pad_block = pad / rows;
     float own = -INFINITY;
     if (step < side && (!ended[beam] || pad_block % side == step)) own = (float)candidate(beam, m, true);
-    first_of(lds, best_blocks, own, [&](auto f) __attribute__((always_inline)) {
+    first_of(lds, beams, own, [&](auto f) __attribute__((always_inline)) {
         if (step >= side) return;
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         v = candidate(beam, x, b == pad_block);
         k = step < side && b < blocks ? beam * blocks + b : -1;
     });
-    if (tid < best_blocks) {
+    if (tid < beams) {
         const int n = lds.out_key[tid] / blocks;
         beam_of[tid] = n;
         row_of[tid] = (lds.out_key[tid] - n * blocks) * rows;
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
     // the best of their elements
     {
         constexpr int N = 4;
-        const int n_elements = best_blocks * rows;          // (at most 2^19: 64 blocks of 8192 rows)
+        const int n_elements = beams * rows;          // (at most 2^19: 64 blocks of 8192 rows)
         const float per_row = 1.f / rows;
         double value[N];
         int key[N];
