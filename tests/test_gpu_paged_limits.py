@@ -1,11 +1,11 @@
-"""Attention over a paged cache at the ends of what its entry point takes."""
+"""A paged cache at the ends of what its entry points take."""
 import ctypes as C
 
 import numpy as np
 import pytest
 
 from test_gpu_attention import E32, STEP
-from test_gpu_paged import f64, fn, stored
+from test_gpu_paged import Cache, attend, f64, fn, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,42 @@ def test_as_many_tiles_as_a_launch_counts(br, storage, kv, max_pages):
     assert np.all(np.abs(f64(o.numpy()).reshape(kv, hd) - want) <= bound)
     want_lse = z.max(1) + np.log(e.sum(1))
     assert np.all(np.abs(lse.numpy().reshape(kv) - want_lse) <= row + 4 * E32 * (1 + np.abs(want_lse)))
+
+
+def definition(K, V, Q, scale, storage):
+    """(o, bound of o, lse, bound of lse) of one head: K, V [n][hd], Q [hd]; bounds as in test_gpu_paged."""
+    n, hd = K.shape
+    z = scale * (K @ Q)
+    w = np.exp(z - z.max())
+    lse = z.max() + np.log(w.sum())
+    w /= w.sum()
+    row = 2 * E32 * (hd + 6) * scale * (np.abs(K) @ np.abs(Q)).max() + E32 * (n + 32 + 2 * np.abs(z).max())
+    o = w @ V
+    extra = 2.0 ** -15 if storage == "bf16" else 0.0
+    return o, 1.01 * (w @ np.abs(V)) * (2 * row + E32 * (n + 16) + extra) + 1.01 * STEP[storage] * np.abs(o), lse, row + 4 * E32 * (1 + abs(lse))
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 40, 700, 9000])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_a_key_of_infinity(br, storage, n, value):
+    """A score of +inf leaves NaN in all of its head, one of -inf takes its position out and no more, one of 0 * inf is NaN."""
+    hd, heads, at = 64, 4, n // 2
+    cache = Cache(storage, 1, hd, 16, [n], seed=70)
+    q = stored(storage, np.random.default_rng(71).standard_normal((1, heads * hd, 1)))
+    sign = np.array([1.0, -1.0, 0.0, -0.25])                    # of each head's query in that channel, 5
+    q[0, 5::hd, 0] = stored(storage, sign)
+    page, slot = cache.row(0, at)
+    cache.k[page, 0, slot, 5] = stored(storage, np.full(1, value))[0]
+    o, lse = attend(br, cache, q, None, [n - 1], heads, 0.125)
+    o, lse = f64(o)[0, :, 0].reshape(heads, hd), lse[0, :, 0].astype(np.float64)
+    K, V = cache.rows(cache.k, 0, n)[0], cache.rows(cache.v, 0, n)[0]
+    others = np.arange(n) != at
+    for h in range(heads):
+        if sign[h] == 0 or sign[h] * value > 0:
+            assert np.all(np.isnan(o[h])) and not np.isfinite(lse[h]), h
+        elif n == 1:
+            assert np.all(np.isnan(o[h])) and lse[h] == -np.inf, h      # nothing is left: 0 / 0
+        else:
+            want, bound, want_lse, bound_lse = definition(K[others], V[others], f64(q)[0, h * hd:(h + 1) * hd, 0], 0.125, storage)
+            assert np.all(np.abs(o[h] - want) <= bound) and abs(lse[h] - want_lse) <= bound_lse, h
