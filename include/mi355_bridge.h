@@ -222,7 +222,8 @@ typedef struct mi355_kv_cache {
  * q, q_out: [batch][heads*hd][S] (both NULL and heads = 0: keys and values only; q_out may be q); k, v: [batch][kv_heads*hd][S]; wq, wk: [hd]
  * fp32, NULL for no norm; cos, sin: [hd/2][table], as mi355_rope_tables_dev(.., table, hd, theta) gives them, both NULL for no rotation.
  * A column whose sequence is not in [0, n_seqs), whose position is negative, behind max_pages * page or behind the table of angles, or whose page
- * is none, is no token: nothing of it is written.  Of two columns with one place either may stay.  Outputs must not overlap inputs otherwise.
+ * is none, is no token: nothing of it is written.  A place should be named by one column: where several name it, each of its values is that of one
+ * of them, and of which is not defined (a row may be made up of both).  Outputs must not overlap inputs otherwise.
  * batch * S at most 2^22, heads at most 2^14, kv_heads at most 4096, batch * S * (heads + 2 kv_heads) below 2^26 - 3. */
 int mi355_kv_append_dev(const mi355_kv_cache *cache, float *q_out, const float *q, const float *k, const float *v, const float *wq,
                         const float *wk, const int32_t *seq, const int32_t *pos, int heads, int S, int batch, const float *cos_dev,

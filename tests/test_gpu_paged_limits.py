@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from test_gpu_attention import E32, STEP
-from test_gpu_paged import Cache, attend, f64, fn, stored
+from test_gpu_paged import Cache, append, attend, f64, fn, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,28 @@ def test_a_key_of_infinity(br, storage, n, value):
         else:
             want, bound, want_lse, bound_lse = definition(K[others], V[others], f64(q)[0, h * hd:(h + 1) * hd, 0], 0.125, storage)
             assert np.all(np.abs(o[h] - want) <= bound) and abs(lse[h] - want_lse) <= bound_lse, h
+
+
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("S", [6, 40, 700])
+def test_two_columns_at_one_place(br, storage, S):
+    """Every value of a row is that of a column that names it, also where two do; rows that none names, and all columns' queries, are as they should be."""
+    heads, kv, hd = 8, 4, 64
+    cache = Cache(storage, kv, hd, 16, [S], seed=72, values=False)
+    rng = np.random.default_rng(73)
+    q, k, v = (stored(storage, rng.standard_normal((1, h * hd, S))) for h in (heads, kv, kv))
+    pos = np.arange(S, dtype=np.int32)[None]
+    twice = [(0, 1), (2, S - 1), (S // 2, S // 2 - 1)]          # side by side, far apart
+    for a, b in twice:
+        pos[0, b] = pos[0, a]
+    got_q, got_k, got_v = append(br, cache, q, k, v, None, None, np.zeros((1, S), np.int32), pos, heads, None, None, 0.0)
+    assert np.array_equal(got_q, q)
+    for got, new, old in ((got_k, k, cache.k), (got_v, v, cache.v)):
+        new = new.reshape(kv, hd, S)
+        want = old.copy()
+        for place in np.unique(pos):
+            page, slot = cache.row(0, place)
+            row = got[page, :, slot]
+            assert np.all((row[:, :, None] == new[:, :, pos[0] == place]).any(2)), place
+            want[page, :, slot] = row
+        assert np.array_equal(got, want)
