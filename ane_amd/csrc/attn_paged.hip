@@ -47,16 +47,13 @@ constexpr float PIECE = 1.f / 3;
 // 53.4 / 52.3 / 51.4, 16 of up to 8000 31.5 / 30.5 / 30.3, 64 heads on one, 16 of up to 4000, 23.6 / 23.2 / 23.1, one of 256 8.25 / 8.2 / 8.25.
 constexpr int JOIN = 12;
 
-__device__ __forceinline__ float load_one(const float *p) { return *p; }
-__device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
-__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
-__device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 struct PagedArgs {
     mi355_kv_cache c;
     const int *seq, *pos;
-    int heads, S, col0, cols, group, positions;     // columns col0 .. col0 + cols - 1; group: query heads of a KV head; positions of a row of the table
+    int heads, S, col0, cols;       // columns col0 .. col0 + cols - 1
+    int group, positions;           // query heads of a KV head; positions of a row of the table
     int part0, parts, units;        // which parts of the groups this launch has; compute units, 0 where units are not long enough for PIECE to matter
     float scale2;
     float *slots;                   // partial results: two for each workgroup
@@ -64,6 +61,12 @@ struct PagedArgs {
 };
 
 // ---- the parts of a tile that depend on the type ----
+
+// 16 bytes at `at` of the lane and `row` of the wave
+template <typename V>
+__device__ __forceinline__ V load16(__amdgpu_buffer_rsrc_t from, unsigned at, unsigned row) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, (int)row, 0));
+}
 
 template <typename T, int HDB> struct Tile;
 
@@ -85,14 +88,15 @@ template <int HDB> struct Tile<bf16_t, HDB> {
     struct Offsets { unsigned k, k_last, v, row; };
     static __device__ __forceinline__ Offsets offsets(int hd) {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 8 * g;
-        return {(unsigned)(i * hd + 8 * g) * 2, tail < hd ? (unsigned)(i * hd + tail) * 2 : OUTSIDE, VC * i < hd ? (unsigned)(4 * g * hd + VC * i) * 2 : OUTSIDE, (unsigned)hd * 2};
+        return {(unsigned)(i * hd + 8 * g) * 2, tail < hd ? (unsigned)(i * hd + tail) * 2 : OUTSIDE,
+                VC * i < hd ? (unsigned)(4 * g * hd + VC * i) * 2 : OUTSIDE, (unsigned)hd * 2};
     }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, int piece, const Offsets &o) {
 #pragma unroll
-        for (int s = 0; s < HDB; s++) k[piece][s] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(s < HDB - 1 ? o.k + 64 * s : o.k_last), 0, 0));
+        for (int s = 0; s < HDB; s++) k[piece][s] = load16<v4u>(kr, s < HDB - 1 ? o.k + 64 * s : o.k_last, 0);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            if constexpr (VC == 8) v[4 * piece + r] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)o.v, (int)(r * o.row), 0));
+            if constexpr (VC == 8) v[4 * piece + r] = load16<Vec>(vr, o.v, r * o.row);
             else v[4 * piece + r] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b64(vr, (int)o.v, (int)(r * o.row), 0));
         }
     }
@@ -142,21 +146,24 @@ template <int HDB> struct Tile<float, HDB> {
     static constexpr int QS = 2 * HDB;
     v4f k[2 * HDB], v[4][WIDE];
     static __device__ __forceinline__ int channel(int acc, int r, int g) { return 64 * (acc >> 2) + 4 * (4 * g + r) + (acc & 3); }
-    static __device__ __forceinline__ Q query(const float *row, int s) { return *reinterpret_cast<const v4f *>(row + 16 * s + 4 * ((threadIdx.x & 63) >> 4)); }
+    static __device__ __forceinline__ Q query(const float *row, int s) {
+        return *reinterpret_cast<const v4f *>(row + 16 * s + 4 * ((threadIdx.x & 63) >> 4));
+    }
     struct Offsets { unsigned k, k_tail[2], v, v_last, row; };
     static __device__ __forceinline__ Offsets offsets(int hd) {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, tail = 32 * (HDB - 1) + 4 * g, last = 64 * (WIDE - 1) + 4 * i;
-        return {(unsigned)(i * hd + 4 * g) * 4, {tail < hd ? (unsigned)(i * hd + tail) * 4 : OUTSIDE, tail + 16 < hd ? (unsigned)(i * hd + tail + 16) * 4 : OUTSIDE},
+        return {(unsigned)(i * hd + 4 * g) * 4,
+                {tail < hd ? (unsigned)(i * hd + tail) * 4 : OUTSIDE, tail + 16 < hd ? (unsigned)(i * hd + tail + 16) * 4 : OUTSIDE},
                 (unsigned)(4 * g * hd + 4 * i) * 4, last < hd ? (unsigned)(4 * g * hd + last) * 4 : OUTSIDE, (unsigned)hd * 4};
     }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, int, const Offsets &o) {
 #pragma unroll
         for (int s = 0; s < 2 * HDB; s++)
-            k[s] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(s < 2 * HDB - 2 ? o.k + 64 * s : o.k_tail[s & 1]), 0, 0));
+            k[s] = load16<v4f>(kr, s < 2 * HDB - 2 ? o.k + 64 * s : o.k_tail[s & 1], 0);
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int w = 0; w < WIDE; w++) v[r][w] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)(w < WIDE - 1 ? o.v : o.v_last), (int)(r * o.row), 0));
+            for (int w = 0; w < WIDE; w++) v[r][w] = load16<v4f>(vr, w < WIDE - 1 ? o.v : o.v_last, r * o.row);
     }
     __device__ __forceinline__ v4f scores(const Q (&q)[QS], int) const {
         v4f s = {0.f, 0.f, 0.f, 0.f};
@@ -307,8 +314,8 @@ struct Walk {
     // Tiles first, first + WAVES, ... below last.  k, v: the KV head's rows of page 0.
     // now: the pages of the first 64 pieces.
     template <bool ODD>
-    __device__ __forceinline__ void run(const typename Tl::Q (&q)[Tl::QS], Pieces now, const T *k, const T *v, size_t page_stride, const int *table, int page,
-                                        int n_pages, int hd, int first, int last, int len, float scale2) {
+    __device__ __forceinline__ void run(const typename Tl::Q (&q)[Tl::QS], Pieces now, const T *k, const T *v, size_t page_stride, const int *table,
+                                        int page, int n_pages, int hd, int first, int last, int len, float scale2) {
         m = -INFINITY;
         l = 0.f;
         seen = false;
@@ -380,8 +387,8 @@ template <int HDB> using shared_ptr = __attribute__((address_space(3))) Shared<H
 
 // Tiles t0 .. t1 - 1 of a sequence and KV head: the waves' shares, brought to the largest of their maxima, are in LDS at the end.
 template <typename T, int HDB, bool ODD>
-__device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, Pieces now, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages, int hd, int heads,
-                                          int t0, int t1, int len, float scale2) {
+__device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, Pieces now, const T *k, const T *v, size_t page_stride, const int *table, int page,
+                                          int n_pages, int hd, int heads, int t0, int t1, int len, float scale2) {
     typedef Tile<T, HDB> Tl;
     Shared<HDB> &lds = *(Shared<HDB> *)lds_;
     constexpr int ROW = Shared<HDB>::ROW;
@@ -416,8 +423,8 @@ __device__ __forceinline__ void share_out(shared_ptr<HDB> lds_, Pieces now, cons
 }
 // The same with infinities and NaNs among the values taken one by one; a function of its own, for its registers not to be the kernel's.
 template <typename T, int HDB>
-__device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, const T *k, const T *v, size_t page_stride, const int *table, int page, int n_pages,
-                                                          int hd, int heads, int t0, int t1, int len, float scale2) {
+__device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, const T *k, const T *v, size_t page_stride, const int *table, int page,
+                                                          int n_pages, int hd, int heads, int t0, int t1, int len, float scale2) {
     Pieces now;
     now.look_up<Tile<T, HDB>::PIECES>(table, page, len, t0 + uniform((int)threadIdx.x >> 6));
     share_out<T, HDB, true>(lds, now, k, v, page_stride, table, page, n_pages, hd, heads, t0, t1, len, scale2);
@@ -427,7 +434,8 @@ __device__ __attribute__((noinline)) void share_out_again(shared_ptr<HDB> lds, c
 // such stores go through to memory and such loads do not stop at the L2, and the count of those that have arrived goes up when the stores of a
 // workgroup have ended.
 __device__ __forceinline__ void slot_put(float *p, float x, float y) {
-    __hip_atomic_store((unsigned long long *)p, (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+    __hip_atomic_store((unsigned long long *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ v2f slot_get(const float *p) {
     const unsigned long long v = __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -444,8 +452,8 @@ __device__ __forceinline__ v2f slot_get(const float *p) {
 // they begin together on one XCD, and what the first one reads the others find in its L2.  (40 heads on two KV heads, 6 sequences of up to 46491 positions
 // 64.5 -> 54.2 us, 16 of up to 8000 37.3 -> 32.4, where parts followed one another on one line.)
 template <typename T, int HDB>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q,
-                                                                                                  PagedArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void attn_paged_kernel(T *__restrict__ o, float *__restrict__ lse, const T *__restrict__ q, PagedArgs a) {
     typedef Tile<T, HDB> Tl;
     constexpr int ROW = Shared<HDB>::ROW;
     __shared__ __attribute__((aligned(16))) Shared<HDB> lds;
@@ -453,7 +461,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ float tops[WAVES];
     __shared__ struct { int col, unit, tile, start, len; } ends[2];
     const int tid = threadIdx.x, hd = a.c.hd, page = a.c.page;
-    const int all_parts = (a.group + HEADS - 1) / HEADS, part_heads = (a.group + all_parts - 1) / all_parts, units = a.c.kv_heads;  // units: of a column
+    const int all_parts = (a.group + HEADS - 1) / HEADS, part_heads = (a.group + all_parts - 1) / all_parts;
+    const int units = a.c.kv_heads;         // of a column
     const int turn = blockIdx.x / (8 * a.parts), rest = blockIdx.x - turn * 8 * a.parts, part = a.part0 + (rest >> 3), w = turn * 8 + (rest & 7);
     const int heads = min(a.group - part * part_heads, part_heads), most = gridDim.x / a.parts;
     auto length = [&](int col) __attribute__((always_inline)) {
@@ -468,7 +477,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // where this workgroup's tiles begin and end
     const int each = (a.cols + 255) / 256, c0 = min(tid * each, a.cols), c1 = min(c0 + each, a.cols);
-    // (Up to 256 columns a thread has one, whose length it keeps: looked up again it is waited for three times more, and calls of 8 to 65 us take 0.4 us longer.)
+    // (Up to 256 columns a thread has one, whose length it keeps: looked up again it is waited for three times more, and calls of 8 to 65 us take
+    // 0.4 us longer.)
     const int len0 = c0 < c1 ? length(a.col0 + c0) : 0, n0 = (len0 + Tl::POSITIONS - 1) / Tl::POSITIONS;
     int mine = n0 ? (n0 + BEGIN) * units : 0;
     float longest = n0;
@@ -524,14 +534,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (x == total && tid == 0) ends[i] = {a.col0 + a.cols, 0, 0, total, 0};
     }
     __syncthreads();
-    int col = uniform(ends[0].col), unit = uniform(ends[0].unit), tile = uniform(ends[0].tile), start = uniform(ends[0].start);       // start: of the column
-    int len = uniform(ends[0].len);
+    int col = uniform(ends[0].col), unit = uniform(ends[0].unit), tile = uniform(ends[0].tile);
+    int start = uniform(ends[0].start), len = uniform(ends[0].len);         // of the column
     const int end_col = uniform(ends[1].col), end_unit = uniform(ends[1].unit), end_tile = uniform(ends[1].tile);
     const size_t page_stride = (size_t)a.c.kv_heads * page * hd, slot_size = (size_t)HEADS * (HDB * 32 + 2);
     const int row = hd + 2;             // of a slot: a head's maximum, its sum (-1: no position seen), its channels
     float *const slots = a.slots + (size_t)(part - a.part0) * most * 2 * slot_size;
     unsigned *const arrived = a.arrived + (part - a.part0) * most;
-    struct Split { int col, kvh, first, last; } split[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};      // the unit that began before, the one that ends behind
+    // the unit that began before, the one that ends behind
+    struct Split { int col, kvh, first, last; } split[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
     auto out_of = [&](int col, int head0, size_t channels) __attribute__((always_inline)) {
         const int b = col / a.S, s = col - b * a.S;
         return ((size_t)b * a.heads + head0) * channels * a.S + s;
@@ -662,7 +673,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             if (turn > 0 || !in) continue;
             for (int t = 1; t < turns; t++) {
                 const float *p = lds.o + 8 * (tid + t * quads);
-                const float to = fmaxf(top, p[0]), base = to == -INFINITY ? 0.f : to, f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(p[0] - base);
+                const float to = fmaxf(top, p[0]), base = to == -INFINITY ? 0.f : to;
+                const float f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(p[0] - base);
                 if (!(p[1] < 0.f)) sum = (sum < 0.f ? 0.f : sum * f0) + p[1] * f1;
                 else if (!(sum < 0.f)) sum *= f0;
                 v = v * f0 + *reinterpret_cast<const v4f *>(p + 4) * f1;
@@ -681,8 +693,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 __device__ unsigned g_arrived[MAX_GROUPS];
 
 template <typename T>
-int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const T *q, const int32_t *seq, const int32_t *pos, int heads, int S, int batch,
-               float scale) {
+int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const T *q, const int32_t *seq, const int32_t *pos, int heads, int S,
+               int batch, float scale) {
     if (!kv_cache_ok(who, c)) return -1;
     if (!o || !q || !pos) return mi355_fail("%s: NULL pointer", who);
     if (heads == 0) return mi355_fail("%s: no heads", who);
@@ -694,7 +706,8 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
     const int group = heads / c->kv_heads, parts = (int)ceil_div(group, HEADS), cols = S * batch;
     const size_t column = (ceil_div((size_t)c->max_pages * c->page, Tile<T, 1>::POSITIONS) + BEGIN) * c->kv_heads;
     constexpr size_t COUNT = 0x7fffff00;
-    if (column > COUNT) return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 256", who, (double)c->max_pages * c->page * c->kv_heads);
+    if (column > COUNT)
+        return mi355_fail("%s: max_pages * page * kv_heads = %.0f is more tiles than 2^31 - 256", who, (double)c->max_pages * c->page * c->kv_heads);
     if (!mi355_ready(who)) return -1;
     static unsigned *arrived = nullptr;
     if (!arrived) HIP_OK(hipGetSymbolAddress((void **)&arrived, HIP_SYMBOL(g_arrived)));
@@ -710,8 +723,10 @@ int attn_paged(const char *who, const mi355_kv_cache *c, T *o, float *lse, const
                 const size_t n = cols - c0 < at_once ? cols - c0 : at_once, useful = ceil_div(n * column, GRAIN);
                 const int now = parts - p0 < (int)most / 8 ? parts - p0 : (int)most / 8;
                 // workgroups of a part: of several, a multiple of 8
-                const size_t room = now == 1 ? most : most / (8 * now) * 8, each = useful < room ? (now == 1 ? useful : ceil_div(useful, 8) * 8) : room;
-                const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, p0, now, lengthy ? g_ctx.num_cu : 0, scale * LOG2E, slots, arrived};
+                const size_t room = now == 1 ? most : most / (8 * now) * 8;
+                const size_t each = useful < room ? (now == 1 ? useful : ceil_div(useful, 8) * 8) : room;
+                const PagedArgs a = {*c, seq, pos, heads, S, (int)c0, (int)n, group, c->max_pages * c->page, p0, now, lengthy ? g_ctx.num_cu : 0,
+                                     scale * LOG2E, slots, arrived};
                 attn_paged_kernel<T, HDB><<<(unsigned)(each * now), 256, 0, g_ctx.stream>>>(o, lse, q, a);
                 LAUNCH_OK(who);
             }

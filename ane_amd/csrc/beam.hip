@@ -19,8 +19,6 @@ constexpr int LIST = 512;           // candidates that it ranks
 constexpr int NONE = 0x7fffffff;    // no candidate's key
 constexpr int MOST = 64;            // beams
 
-__device__ __forceinline__ float load_one(const float *p) { return *p; }
-__device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
 template <int VEC> __device__ __forceinline__ void load_vec(float (&r)[VEC], const float *p) {
     if constexpr (VEC == 1) r[0] = __builtin_nontemporal_load(p);
     else ldv_nt<VEC>(r, p);
@@ -53,7 +51,8 @@ __device__ __forceinline__ void take(float &m, float &l, const float (&x)[N]) {
 // Several columns: threads side by side take VEC columns of a row each (the last ones of a row its last VEC, some of them twice), `across` threads
 // to a row; a thread takes every (256 / across)-th of the block's rows, ROWS at a time.  part[block][column].
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void beam_columns_kernel(float2 *__restrict__ part, const T *__restrict__ logits, int V, int S, int columns, int across, int rows) {
+__global__ __launch_bounds__(256) void beam_columns_kernel(float2 *__restrict__ part, const T *__restrict__ logits, int V, int S, int columns,
+                                                           int across, int rows) {
     constexpr int ROWS = 8;
     __shared__ float ms[256 * VEC], ls[256 * VEC];
     const int down = 256 / across, r = threadIdx.x / across, c = threadIdx.x - r * across;
@@ -137,8 +136,8 @@ struct SelectLds {
 };
 __device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
 
-// -inf.  (The compiler has set a pair of scalar registers to this double with an instruction that holds only 32 bits of it, and they were 0 then; here it
-// does not see the constant.)
+// -inf.  (The compiler has set a pair of scalar registers to this double with an instruction that holds only 32 bits of it, and they were 0 then;
+// here it does not see the constant.)
 __device__ __forceinline__ double lowest() {
     float x = -INFINITY;
     asm("" : "+v"(x));
@@ -156,8 +155,8 @@ __device__ __forceinline__ void first_of_two(double &v, int &k, int d, bool back
 }
 
 // The `want` first of all threads' items, larger values first, equal ones by their keys: out_value, out_key in order.  own: the largest of the
-// thread's items as a float (rounding keeps the order); walk(f) calls f(value, key) for each of them, item(i, load(i), value, key) has the i-th of `items`, key -1:
-// none (nor is there one behind the last).
+// thread's items as a float (rounding keeps the order); walk(f) calls f(value, key) for each of them, item(i, load(i), value, key) has the i-th of
+// `items`, key -1: none (nor is there one behind the last).
 // Of 64 parts of the threads the largest ones are compared; what is not below the `want`-th of these goes into a list, in which every item counts
 // those before it.  Few threads have any of those, and only they walk.  (512 at most: 1000 of them take 60 us.)
 template <typename F, typename G, typename H>
@@ -213,7 +212,8 @@ __device__ __forceinline__ void first_of(SelectLds &lds, int want, float own, F 
         int held_key = NONE, last_key = NONE;
         auto of_lane = [](double x, int from) __attribute__((always_inline)) {
             const long long b = __double_as_longlong(x);
-            return __longlong_as_double((long long)(unsigned)__builtin_amdgcn_readlane((int)b, from) | (long long)__builtin_amdgcn_readlane((int)(b >> 32), from) << 32);
+            const unsigned low_half = __builtin_amdgcn_readlane((int)b, from);
+            return __longlong_as_double((long long)low_half | (long long)__builtin_amdgcn_readlane((int)(b >> 32), from) << 32);
         };
         constexpr int AT_ONCE = 4;          // items on their way
         for (int i0 = 0; i0 < items; i0 += AT_ONCE) {
@@ -337,8 +337,8 @@ __global__ __launch_bounds__(SELECT) void beam_select_kernel(float *__restrict__
         double c = ended[n] ? (is_pad ? s : none) : s + ((double)x - lds.lse[n]);
         return c == c ? c : none;
     };
-    // the best blocks, as many as beams (each beam has one at least); of a beam's candidates the one with the largest logit is the largest, but an ended
-    // beam has only one
+    // the best blocks, as many as beams (each beam has one at least); of a beam's candidates the one with the largest logit is the largest, but an
+    // ended beam has only one
     const int pad_block = pad / rows;
     float own = -INFINITY;
     if (step < side && (!ended[beam] || pad_block % side == step)) own = (float)candidate(beam, m, true);
@@ -456,7 +456,8 @@ int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T 
             if (!*part) return -1;
             for (size_t c = 0; c < columns; c += 65535) {
                 const unsigned n = (unsigned)(columns - c < 65535 ? columns - c : 65535);
-                beam_rows_kernel<T, WIDE, N><<<dim3((unsigned)ceil_div(*blocks, 4), n), 256, 0, g_ctx.stream>>>(*part + c, logits + c * V, V, (int)columns, *blocks);
+                beam_rows_kernel<T, WIDE, N><<<dim3((unsigned)ceil_div(*blocks, 4), n), 256, 0, g_ctx.stream>>>(*part + c, logits + c * V, V, (int)columns,
+                                                                                                                      *blocks);
                 LAUNCH_OK(who);
             }
             return 0;
@@ -480,8 +481,8 @@ int beam_blocks(const char *who, float2 **part, int *blocks, int *rows, const T 
         if (!*part) return -1;
         for (int b = 0; b < batch; b += 65535) {
             const unsigned n = (unsigned)(batch - b < 65535 ? batch - b : 65535);
-            beam_columns_kernel<T, VEC><<<dim3((unsigned)*blocks, (unsigned)strips, n), 256, 0, g_ctx.stream>>>(*part + (size_t)b * S, logits + (size_t)b * V * S, V, S,
-                                                                                                                 (int)columns, across, *rows);
+            beam_columns_kernel<T, VEC><<<dim3((unsigned)*blocks, (unsigned)strips, n), 256, 0, g_ctx.stream>>>(
+                *part + (size_t)b * S, logits + (size_t)b * V * S, V, S, (int)columns, across, *rows);
             LAUNCH_OK(who);
         }
         return 0;

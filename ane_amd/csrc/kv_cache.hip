@@ -5,11 +5,6 @@
 
 namespace {
 
-__device__ __forceinline__ float load_one(const float *p) { return *p; }
-__device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
-__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
-__device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
-
 // 16 bytes of a row, and their values
 __device__ __forceinline__ v4f raw_cols(const float *p) { return ld4(p); }
 __device__ __forceinline__ v4u raw_cols(const bf16_t *p) { return *reinterpret_cast<const v4u_any *>(p); }
@@ -29,8 +24,8 @@ __device__ __forceinline__ bf_pair pair_of(float a, float b, bf16_t *) { return 
 __device__ __forceinline__ f_pair pair_of(float a, float b, float *) { return f_pair{__float_as_uint(a), __float_as_uint(b)}; }
 
 // What a column is a token of: the row of its page and of head 0, -1 if it is none.
-__device__ __forceinline__ long long token_row(const int *seq, const int *pages, size_t col, int pos, int n_pages, int page, int n_seqs, int max_pages, int kv_heads,
-                                               int positions) {
+__device__ __forceinline__ long long token_row(const int *seq, const int *pages, size_t col, int pos, int n_pages, int page, int n_seqs, int max_pages,
+                                               int kv_heads, int positions) {
     const long long entry = paged_entry(seq ? seq[col] : (int)col, pos, n_seqs, max_pages, page);
     if (entry < 0 || pos >= positions) return -1;
     const int id = pages[entry];
@@ -275,7 +270,10 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
             if (rp >= half) continue;
 #pragma unroll
             for (int j = 0; j < VEC; j++)
-                if (own[j]) turned[(mine.col + j - s0) * ROW + (rp ^ ((mine.col + j - s0) / VEC * XOR & (ROW - 1)))] = pair_of(x0[kk][j], x1[kk][j], (T *)nullptr);
+                if (own[j]) {
+                    const int c = mine.col + j - s0;
+                    turned[c * ROW + (rp ^ (c / VEC * XOR & (ROW - 1)))] = pair_of(x0[kk][j], x1[kk][j], (T *)nullptr);
+                }
         }
         __syncthreads();
         T *out = of_kind(false, is_k, k_cache, k_cache, v_cache) + (size_t)head * page * hd;
@@ -284,7 +282,8 @@ __global__ __launch_bounds__(256) void kv_append_tile_kernel(
         for (int i = tid; i < 64 * chunks; i += 256) {
             const int c = i / chunks, x = i - c * chunks;
             if (place[c] < 0) continue;
-            *reinterpret_cast<v4u *>(out + (size_t)place[c] * hd + x * VEC) = *reinterpret_cast<const v4u *>(turned + c * ROW + (x * PER ^ (c / VEC * XOR & (ROW - 1))));
+            const pair_t *chunk = turned + c * ROW + (x * PER ^ (c / VEC * XOR & (ROW - 1)));
+            *reinterpret_cast<v4u *>(out + (size_t)place[c] * hd + x * VEC) = *reinterpret_cast<const v4u *>(chunk);
         }
     }
 }
@@ -339,10 +338,10 @@ struct MoveArgs { void *cache[2 * MOVE_LAYERS]; };
 // A workgroup to a row's head, in y to a tensor of a layer: its part of the tail, `words` 16-byte words to a position.  Behind the last tensor (in the first
 // of several launches) the new table, a workgroup to a row; it is read by none of the copies.
 // Rows that stay, and full pages, are not touched: 256 beams of 28 layers move 787 MB in 148 us, which is what a copy of as much takes.
-__global__ __launch_bounds__(256) void kv_reorder_kernel(MoveArgs t, int tensors, int *__restrict__ pages_out, int *__restrict__ pos_out, int *__restrict__ spare_out,
-                                                         const int *__restrict__ pages, const int *__restrict__ parents, const int *__restrict__ pos,
-                                                         const int *__restrict__ spare, int rows, int max_pages, int page, int n_pages, int kv_heads, int words,
-                                                         int advance) {
+__global__ __launch_bounds__(256) void kv_reorder_kernel(MoveArgs t, int tensors, int *__restrict__ pages_out, int *__restrict__ pos_out,
+                                                         int *__restrict__ spare_out, const int *__restrict__ pages, const int *__restrict__ parents, const int *__restrict__ pos,
+                                                         const int *__restrict__ spare, int rows, int max_pages, int page, int n_pages, int kv_heads,
+                                                         int words, int advance) {
     const int n = blockIdx.x / kv_heads, head = blockIdx.x - n * kv_heads, at = pos[n], parent = parent_of(n, parents, pos, rows);
     const PagedMove m = paged_move(n, parent, at, page);
     // (a page that is none is passed on as it is)
@@ -382,7 +381,8 @@ int kv_reorder(const char *who, int size, const mi355_kv_cache *caches, int coun
         return mi355_fail("%s: the new table, positions and spare pages must not be the old ones", who);
     if (advance < 0) return mi355_fail("%s: advance must not be negative", who);
     const mi355_kv_cache &c = *caches;
-    if ((double)c.n_seqs * c.kv_heads > (1 << 24) - 1) return mi355_fail("%s: n_seqs * kv_heads = %.0f (at most 2^24 - 1)", who, (double)c.n_seqs * c.kv_heads);
+    if ((double)c.n_seqs * c.kv_heads > (1 << 24) - 1)
+        return mi355_fail("%s: n_seqs * kv_heads = %.0f (at most 2^24 - 1)", who, (double)c.n_seqs * c.kv_heads);
     if (!mi355_ready(who)) return -1;
     for (int i = 0; i < count; i += MOVE_LAYERS) {
         MoveArgs t = {};
@@ -392,7 +392,8 @@ int kv_reorder(const char *who, int size, const mi355_kv_cache *caches, int coun
             t.cache[2 * j + 1] = caches[i + j].v;
         }
         kv_reorder_kernel<<<dim3((unsigned)(c.n_seqs * c.kv_heads), 2 * n + (i == 0)), 256, 0, g_ctx.stream>>>(
-            t, 2 * n, pages_out, pos_out, spare_out, c.pages, parent, pos, spare, c.n_seqs, c.max_pages, c.page, c.n_pages, c.kv_heads, c.hd * size / 16, advance);
+            t, 2 * n, pages_out, pos_out, spare_out, c.pages, parent, pos, spare, c.n_seqs, c.max_pages, c.page, c.n_pages, c.kv_heads, c.hd * size / 16,
+            advance);
         LAUNCH_OK(who);
     }
     return 0;

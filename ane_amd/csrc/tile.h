@@ -157,6 +157,12 @@ __device__ __forceinline__ void stb(bf16_t *p, const float (&r)[VEC]) {
     }
 }
 
+// One value of either storage.
+__device__ __forceinline__ float load_one(const float *p) { return *p; }
+__device__ __forceinline__ float load_one(const bf16_t *p) { return bf_to_f(*p); }
+__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)f_to_bf(v); }
+
 // Register tiles keep the bf16 words packed (half the registers of an fp32 tile) and widen them at each use.
 template <int VEC> struct RawT { typedef unsigned type; };
 template <> struct RawT<8> { typedef v4u type; };
