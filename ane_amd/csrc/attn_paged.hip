@@ -13,10 +13,14 @@
 //                                  channel: the lane holds eight rows of 8 (4) channels and exchanges halves of words between them.
 // The running maximum is brought up to date only when a score passes it, which is rare after the first tiles, so lanes hardly ever talk.
 //
-// Measured: 64 sequences of up to 4096 positions, 16 heads on 8 KV heads of 128, bfloat16, 91 us, 4.6 TB/s; one of 131071, 106 us, 5.05 TB/s, where a
-// copy of 1 GiB reaches 5.12: bound by HBM.  Workgroups of 2 waves instead of 4: the long one 125; of 8: 102, but one of 256 positions 9.3 and 64 of up to
-// 200 46 instead of 38.  One sequence of 256, 12 heads of 64, fp32, 8.2 us: bound by one load after the other (positions, a
-// page, a tile, 3 us of joining).
+// Measured, pages of 16: 64 sequences of up to 4096 positions, 16 heads on 8 KV heads of 128, bfloat16, 91.7 us for 421 MB, 4.6 TB/s; one of 131071
+// (pages of 64) 107 us, 5.0 TB/s, where a copy of 1 GiB reaches 5.1: bound by HBM.  64 of up to 200 14.4 us, one of 256 8.7; 12 heads of 64, fp32,
+// 8.3: bound by one load after the other (positions, a page, a tile, the parts of a result).  (Workgroups of 2 waves instead of 4 took 125 us for the
+// long one when that took 108, of 8 102, but one of 256 9.3 instead of 8.7.)
+//
+// Two waves to a SIMD, with half of its registers each.  In fp32 a wave takes 136 to 247 vector registers, by the head's size, and 45 to 53 scalar
+// ones are kept in lanes of vector registers.  In bfloat16 it is 248 to 256 for any size, 105 to 123 and 56 to 448 bytes of private memory: the rare
+// second pass (share_out_again) is a call, and what is alive across it is kept as its convention has it.
 #include "deal.h"
 #include "kv_cache.h"
 #include "mma.h"
@@ -30,21 +34,28 @@ constexpr float FAR = 16777216.f;           // 2^24
 constexpr int HEADS = 16;                   // query heads of one product
 constexpr int WAVES = 4;
 constexpr int MAX_GROUPS = 1024;            // workgroups of a launch
-// In tiles, of which a workgroup's waves have one each at a time (1 us for four): what beginning another unit takes (3.6 us), what a workgroup should have
-// at least, and what is not cut off a unit (joining parts takes 3 us).  us, workgroups of at least 8 / 16 / 32 tiles, by tiles alone: one sequence of 256
-// positions, 12 heads of 64 fp32 10.2 / 8.2 / 13.1, 8 heads of 128 bfloat16 8.8 / 14.4 / 25.5, of 2048 positions 11.8 / 13.6 / 17.8, 64 of up to 200
-// 36.6 / 67.7 / 101, of up to 4096 95 / 95 / 95.
+// In tiles, of which a workgroup's waves have one each at a time: what beginning another unit takes, what a workgroup should have at least, and what is
+// not cut off a unit.  us, pages of 16, bfloat16, 16 heads on 8 KV heads of 128, unless said otherwise:
+//                                              as it is   GRAIN 16 / 32    BEGIN 1   SHORT 1
+//   one sequence of 256, 12 heads of 64, fp32      8.3       8.3 / 12.9       8.4       9.2
+//   one of 256                                     8.7       8.8 / 13.9       8.8       8.7
+//   one of 2048                                   13.6      15.6 / 19.6      13.4      11.6
+//   64 of up to 200                               14.5      17.2 / 19.7      19.3      17.5
+//   64 of up to 4096                              91.7      91.7 / 91.9      91.6      90.5
+//   9 of up to 7892, 40 heads on two, pages of 64 23.3      27.8 / 35.6      23.4      25.7
+//   16 of up to 8000, 40 heads on two, the same   31.0      31.4 / 38.4      30.7      36.3
 constexpr int BEGIN = 8, GRAIN = 8, SHORT = 9;
-// Joining costs by the heads: 40 heads on two KV heads, 9 sequences of up to 7892 positions, 10 heads to a unit, GRAIN / twice that 27.8 / 22.7, 64 heads on
-// one, 16 of up to 4000, 27.3 / 23, but 3 of up to 449 in fp32 15.2 / 17.2; (two heads to a unit, 8 of up to 1000) 14.7 / 16.3.
+// Joining costs by the heads.  us, GRAIN / twice that for all: 64 heads on one KV head, 16 of up to 4000, 27.8 / 23.0, 8 of up to 1000, 16 heads on 8,
+// 13.6 / 15.6, but 3 of up to 449, 40 heads on two, fp32, 15.4 / 17.0.
 constexpr __host__ __device__ int grain(int heads) { return heads >= 8 ? 2 * GRAIN : GRAIN; }
-// Few units of many tiles should not be cut into as many pieces as there are workgroups: a piece takes as long as it has tiles, the join as long as there are
-// pieces and heads, and both together least at pieces of about sqrt(tiles heads) / 3.  us, without / with that, one sequence of 65536 positions: 6 heads of 96 on one,
-// fp32, 94 / 35, 40 of 128 on two, bfloat16, 67 / 39, 64 on one 65 / 42; of 131071, 8 heads on one 62 / 39.  Not where it leaves more than one workgroup to a
-// compute unit but fewer than two: those take as long as two each (6 of up to 46491, 40 heads on two, 62 instead of 51).
+// Few units of many tiles should not be cut into as many pieces as there are workgroups: a piece takes as long as it has tiles, the join as long as
+// there are pieces and heads, and both together least at pieces of about sqrt(tiles heads) / 3.  us, without / with that, one sequence of 65536
+// positions: 6 heads of 96 on one, fp32, 94.6 / 35.0, 40 of 128 on two, bfloat16, 66.9 / 38.8, 64 on one 65.4 / 41.7; of 131071, 8 heads on one
+// 61.9 / 39.1.  Not where it leaves more than one workgroup to a compute unit but fewer than two: those take as long as two each (6 of up to 46491, 40
+// heads on two, 62 instead of 51).
 constexpr float PIECE = 1.f / 3;
-// Slots whose values a thread has on their way at once.  us, 6 / 8 / 12: one sequence of 131071 positions 105.7 / 106 / 105.5, 6 of up to 46491, 40 heads on two
-// 53.4 / 52.3 / 51.4, 16 of up to 8000 31.5 / 30.5 / 30.3, 64 heads on one, 16 of up to 4000, 23.6 / 23.2 / 23.1, one of 256 8.25 / 8.2 / 8.25.
+// Slots whose values a thread has on their way at once.  us, 6 / 8 / 12: one sequence of 65536 positions, 6 heads on one KV head, fp32, 38.9 / 36.8 /
+// 35.0, 40 on two 42.5 / 40.8 / 38.8, 6 of up to 46491 53.8 / 52.8 / 51.7, 64 heads on one, 16 of up to 4000, 23.9 / 23.2 / 23.2, one of 256 8.7 / 8.7 / 8.7.
 constexpr int JOIN = 12;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -109,6 +120,9 @@ template <int HDB> struct Tile<bf16_t, HDB> {
     __device__ __forceinline__ void hide(int piece, int r) { v[4 * piece + r] = Vec(0u); }
     // acc += V' p.  A weight is a pair of bfloat16 values, its upper half and what that leaves of it: off by 2^-15 of it, where one value
     // alone is off by as much as the rounding of the result (2^-8).  ODD: infinities and NaNs among the values count as zero.
+    // (A third value would leave nothing out.  Relative error of o, 64 sequences of up to 4096 positions: 0.00166210 with two, 0.00166209 with three or
+    // fp32 weights, all of it the rounding of o, of which 0.36 % and 0.05 % come out as the neighbouring value.  us, two / three: that call 91.4 / 91.7,
+    // one of 65536, 40 heads on two, 39.2 / 44.7, 64 on one 41.8 / 46.2, 6 of up to 46491, 40 on two, 51.7 / 55.0.)
     template <bool ODD>
     __device__ __forceinline__ void weigh(v4f (&acc)[ACC], const v4f (&p)[PIECES]) const {
         v4u hi, lo;

@@ -236,10 +236,13 @@ int mi355_kv_append_bf16_dev(const mi355_kv_cache *cache, uint16_t *q_out, const
  * q, o: [batch][heads*hd][S], heads a multiple of kv_heads (query heads as in mi355_attn_fwd_dev); lse: [batch][heads][S] fp32, may be NULL.
  * 0 < scale <= 2.3e38.  Columns may share a sequence (several new tokens of one, each at its position) and sequences pages.  A column that is
  * no token (as above), or that has no page at all, is not written.  What lies in a page behind a column's position has no influence,
- * infinities and NaNs included.  Sums and the softmax are fp32, weights are multiplied again to 2^-15 of themselves.  Deterministic.  Outputs must not
- * overlap inputs.  batch * S * heads below 2^24.  The workspace holds the partial sums of sequences that several workgroups share, which these hand over
- * inside the launch: calls that overlap on one GPU (two streams, two threads) race.  Each workgroup looks at all columns' lengths: meant for
- * some thousands of columns at most. */
+ * infinities and NaNs included.  Sums and the softmax are fp32, on bfloat16 storage weights are multiplied again to 2^-15 of themselves.
+ * Deterministic.  Outputs must not overlap inputs.  batch * S * heads below 2^24; (max_pages * page / 16 + 8) * kv_heads, on bfloat16 storage
+ * (max_pages * page / 32, rounded up, + 8) * kv_heads, at most 2^31 - 256.  The workspace holds the partial sums of sequences that several workgroups share, which
+ * these hand over inside the launch: calls that overlap on one GPU (two streams, two threads) race.
+ * Meant for new tokens.  A column's positions are read for it alone, also where columns share a sequence or pages, so a prompt with nothing before it is
+ * better given to mi355_attn_fwd_dev, from some 32 positions on (16 heads on 8 KV heads of 128, bfloat16, 64 positions 12 us against 8, 256 33 against 9,
+ * 2048 759 against 51).  And each workgroup looks at all columns' lengths: 4096 columns of one position take 42 us, 16384 182. */
 int mi355_attn_paged_dev(const mi355_kv_cache *cache, float *o, float *lse, const float *q, const int32_t *seq, const int32_t *pos, int heads,
                          int S, int batch, float scale);
 int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *lse, const uint16_t *q, const int32_t *seq, const int32_t *pos,
@@ -251,8 +254,9 @@ int mi355_attn_paged_bf16_dev(const mi355_kv_cache *cache, uint16_t *o, float *l
  * The `beams` largest candidates of a group, equal ones in the order of (n, v), become its new beams, best first: score_out, token = v, parent = n
  * (a column's number), done_out (may be NULL) = done[n] or v == eos (eos < 0: no token ends a beam).  A candidate that is NaN counts as -inf.
  * A greedy step is beams = 1; a group's first step has scores 0, -inf, -inf, ...
- * Exponentials and blocks' sums are fp32, sums over the vocabulary and candidates fp64, so that equal candidates stay equal.  Outputs must not
- * overlap inputs.  beams at most 64, batch * S below 2^22, V * beams at most 2^30.  Deterministic; the workspace holds partial sums. */
+ * Exponentials and blocks' sums are fp32, sums over the vocabulary and candidates fp64, so that equal candidates stay equal.  A log sum is off by
+ * some 2^-20 at most: candidates of beams with different logits that are closer than that may change places.  Outputs must not overlap inputs.
+ * beams at most 64, batch * S below 2^22, V * beams at most 2^30.  Deterministic; the workspace holds partial sums. */
 int mi355_beam_step_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const float *logits, const float *score,
                         const int32_t *done, int V, int S, int batch, int beams, int eos, int pad);
 int mi355_beam_step_bf16_dev(float *score_out, int32_t *token, int32_t *parent, int32_t *done_out, const uint16_t *logits, const float *score,
